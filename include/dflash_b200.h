@@ -333,6 +333,92 @@ int dflash_lm_head_argmax(const uint16_t* hn, const uint16_t* E, int batch, int 
                           int32_t* correction, void* workspace, size_t workspace_bytes,
                           void* stream);
 
+/* ---- paged 4-bit K/V cache ------------------------------------------------
+ * A cache shared by many requests, for the target model's K/V (or a draft's)
+ * where the f16 rings above would reserve every request's longest length.  It
+ * has no counterpart in the reference, whose caches hold one request
+ * (mirror_sd/dflash.py:139-212; the target's quantised cache,
+ * mirror_sd/turboquant.py:21-51, is an external package's).
+ *
+ * Pages of page_size rows (16, 32, 64, 128 or 256) live in one pool per layer;
+ * a block table names each request's pages.  Lengths, tables and the free list
+ * stay on the device: a step needs no host round trip after acceptance.  One
+ * step is
+ *   dflash_paged_reserve   pages and slots for the rows that each request brings
+ *   dflash_q4_append       K and V of those rows into their slots (per layer)
+ *   dflash_q4_attention    the query rows over everything cached (per layer)
+ *   dflash_paged_release   pages beyond the rows that each request keeps
+ *
+ * 16 channels of a row share a scale s with 5 exponent and 3 mantissa bits,
+ * the smallest >= max|x| / 7.5 within [2^-17, 9216], and are stored as whole
+ * numbers x / s rounded half away from zero, within [-7, 7]: 4.5 bits a
+ * channel.  NaN is stored as 0; infinities and larger values saturate.
+ * head_dim is 128.  A pool is num_pages * dflash_q4_page_bytes() bytes,
+ * 16-byte aligned.
+ *
+ * Every array below is a device array.  `status` (one int32, or NULL)
+ * accumulates the DFLASH_PAGED_* bits.  Requests per call: at most
+ * DFLASH_PAGED_MAX_SEQS.  The calls allocate nothing and do not synchronise. */
+#define DFLASH_PAGED_MAX_SEQS 2048
+#define DFLASH_Q4_MAX_ROWS 65536       /* query rows of one request */
+#define DFLASH_PAGED_DRY 1             /* too few free pages for a request */
+#define DFLASH_PAGED_LONG 2            /* a request outgrew its row of the table */
+#define DFLASH_PAGED_SLOTS 4           /* more new rows than num_slots */
+#define DFLASH_PAGED_CORRUPT 8         /* more pages came back than were lent */
+#define DFLASH_PAGED_NONFINITE 16      /* a NaN or an infinity was appended */
+#define DFLASH_PAGED_TIMEOUT 32        /* a bounded device-side wait expired */
+
+/* Request i holds lens[i] rows on pages[i] pages, table[i * table_ld + c],
+ * c < pages[i], and brings new_rows[i] rows, packed in order.  Its missing
+ * pages come off the free list, free_pages[*head ...] of num_pages entries.
+ * Written: starts [n + 1] (first packed row of each request), slots
+ * [num_slots] (page * page_size + row of every new row; -1 past the last one),
+ * lens_out, pages_out, head_out, and the new table entries.  Requests are
+ * served in order; one that cannot be (DRY, LONG, SLOTS) keeps its lengths and
+ * its rows get slot -1, and after the first DRY one no later request gets a
+ * page.  The *_out arrays must not be the inputs, which are only read. */
+int dflash_paged_reserve(const int32_t* lens, const int32_t* new_rows, const int32_t* pages, int n, int page_size,
+                         int32_t* table, int64_t table_ld, int max_pages, const int32_t* free_pages, int num_pages,
+                         const int32_t* head, int32_t* starts, int32_t* slots, int num_slots, int32_t* lens_out,
+                         int32_t* pages_out, int32_t* head_out, int32_t* status, void* stream);
+/* Request i keeps ceil(keep[i] / page_size) of its pages (0: it is finished);
+ * the others are put back, in order, at free_pages[*head_out ... *head). */
+int dflash_paged_release(const int32_t* keep, const int32_t* pages, int n, int page_size, const int32_t* table,
+                         int64_t table_ld, int max_pages, int32_t* free_pages, int num_pages, const int32_t* head,
+                         int32_t* pages_out, int32_t* head_out, int32_t* status, void* stream);
+
+size_t dflash_q4_page_bytes(int nkv, int page_size);
+/* k, v [rows, nkv, 128], f16 or bf16 (bf16 != 0), strides in elements between
+ * rows and heads (multiples of 8; 16-byte aligned bases; they may be slices of
+ * a fused projection's output).  slots [rows], distinct; a row whose slot is
+ * outside the pool is skipped. */
+int dflash_q4_append(const uint16_t* k, int64_t k_row, int64_t k_head, const uint16_t* v, int64_t v_row,
+                     int64_t v_head, int bf16, const int32_t* slots, int rows, int nkv, uint8_t* pool, int num_pages,
+                     int page_size, int32_t* status, void* stream);
+/* The cached values of slots [rows] as f16 or bf16 (both exact) k, v
+ * [rows, nkv, 128]; zeros for a slot outside the pool. */
+int dflash_q4_read(const uint8_t* pool, int num_pages, int page_size, const int32_t* slots, int rows, int nkv,
+                   int bf16, uint16_t* k, uint16_t* v, void* stream);
+
+/* q [rows, nq, 128], f16 or bf16, strides in elements (multiples of 8); out
+ * [rows, nq, 128] of the same type.  Request i owns rows starts[i] ..
+ * starts[i + 1] - 1, at most max_rows of them (starts NULL: max_rows each),
+ * and holds lens[i] cached rows, its own new ones included.  With causal,
+ * query row j of m sees keys below e = lens[i] - m + j + 1, else below
+ * e = lens[i]; with a window only keys < sink or >= e - window.  A row that
+ * sees no key is zeros; rows of no request are not written.  Table entries
+ * outside the pool hide their rows.
+ * workspace: dflash_q4_attention_workspace_size() bytes, 16-byte aligned,
+ * zeroed once before its first use; every call leaves it ready for the next
+ * one of any shape it is large enough for.  Calls that may overlap on the GPU
+ * need workspaces of their own. */
+size_t dflash_q4_attention_workspace_size(int max_rows, int nq, int nkv);
+int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages,
+                        int page_size, const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens,
+                        const int32_t* starts, int n, int rows, int max_rows, int nq, int nkv, int causal, int sink,
+                        int window, float scale, uint16_t* out, int32_t* status, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

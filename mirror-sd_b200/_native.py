@@ -21,6 +21,8 @@ c_int32 = ctypes.c_int32
 c_float = ctypes.c_float
 c_void_p = ctypes.c_void_p
 c_size_t = ctypes.c_size_t
+c_int = ctypes.c_int
+c_int64 = ctypes.c_int64
 
 
 class DFlashDims(ctypes.Structure):
@@ -124,6 +126,19 @@ EXPORTS = {
     "dflash_lm_head_argmax": (c_int32, [c_void_p, c_void_p, ctypes.c_int, ctypes.c_int,
                                         ctypes.c_int, ctypes.c_int, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dflash_paged_reserve": (c_int32, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p,
+                                       c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p]),
+    "dflash_paged_release": (c_int32, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dflash_q4_page_bytes": (c_size_t, [c_int, c_int]),
+    "dflash_q4_append": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int,
+                                   c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "dflash_q4_read": (c_int32, [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "dflash_q4_attention_workspace_size": (c_size_t, [c_int] * 3),
+    "dflash_q4_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_void_p, c_int64,
+                                      c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p,
+                                                                                  c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

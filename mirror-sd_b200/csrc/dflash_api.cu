@@ -11,14 +11,16 @@
 #include <vector>
 
 #include "../../include/dflash_b200.h"
+#include "api_error.cuh"
 #include "kernels.cuh"
 
 using namespace dfl;
 
 namespace {
-
 thread_local std::string g_err;
+}  // namespace
 
+namespace dfl {
 int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -28,18 +30,9 @@ int fail(int code, const char* fmt, ...) {
   g_err = buf;
   return code;
 }
+}  // namespace dfl
 
-#define CK(call)                                                                        \
-  do {                                                                                  \
-    cudaError_t e_ = (call);                                                            \
-    if (e_ != cudaSuccess) {                                                            \
-      if (e_ == cudaErrorInvalidValue)                                                  \
-        return fail(DFLASH_ERR_INVALID, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), \
-                    __FILE__, __LINE__);                                                \
-      return fail(e_ == cudaErrorMemoryAllocation ? DFLASH_ERR_OOM : DFLASH_ERR_CUDA,   \
-                  "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__);  \
-    }                                                                                   \
-  } while (0)
+namespace {
 
 // device allocations owned by a handle, released together
 struct Arena {

@@ -1,0 +1,111 @@
+// Layout of the paged 4-bit K/V cache, its number format, and the host
+// launchers of its kernels (paged.cu, q4_cache.cu, q4_attention.cu).
+//
+// A pool holds pages of `page_size` cached rows (16, 32, 64, 128 or 256):
+//   [page][kv head][page_size / 16 row blocks][kQ4Block bytes]
+// A row block holds 16 rows of one kv head, K then V:
+//   K values  [16 rows][64 B]           4 bits a channel
+//   K scales  [16 rows][8 groups]       1 byte a group of 16 channels
+//   V values  [8 row pairs][8 groups][16 B]
+//   V scales  [8 groups][16 rows]
+// so a block is one contiguous copy and its pieces are the register fragments
+// of a 16x16 matrix tile: K with the rows and V with the channels as the
+// tile's rows, read from shared memory 16 bytes a lane without conflicts.
+//   K, row r, channel d = 32c + 8w + 2n + h: word w of the 16 bytes at
+//     64 r + 16 c, bits 16h + 4n .. + 3
+//   V, row r = 2j + h, channel d = 16g + 4w + n: word w of the 16 bytes at
+//     16 (8 j + g), bits 16h + 4n .. + 3
+// (both: half h of a word holds one side of a register's f16 pair).
+//
+// Numbers: a group of 16 channels of a row is x = (u - 8) * s, u the 4-bit
+// code (1..15 as written here), s a scale with 5 exponent and 3 mantissa bits,
+// float16's top bits below the sign: its f16 form is the byte << 7.  u - 8 has
+// 3 significant bits and s has 4, so every x is exact in f16 and in bf16.
+//   s = the smallest such number >= max |x| / 7.5, within [2^-17, 9216]
+//   u - 8 = x / s rounded to nearest, halves away from zero, within [-7, 7]
+// NaN is stored as 0 and counts as 0 in the maximum; infinities and values
+// beyond 7 * 9216 saturate.  The pool therefore only ever reads back finite
+// numbers, so rows hidden by a mask cannot reach a result through 0 * inf.
+#pragma once
+#include "common.cuh"
+
+namespace dfl {
+
+constexpr int kQ4Rows = 16;            // rows of a block
+constexpr int kQ4KS = 1024;            // byte offsets inside a block
+constexpr int kQ4V = 1152;
+constexpr int kQ4VS = 2176;
+constexpr int kQ4Block = 2304;
+constexpr int kPagedMaxSeqs = 2048;    // requests of one call
+
+// status bits of the paged operators (device word, or-ed)
+enum PagedStatus : int {
+  kPagedDry = 1,        // a request found too few free pages
+  kPagedLong = 2,       // a request's rows do not fit its row of the block table
+  kPagedSlots = 4,      // the new rows do not fit the slot array
+  kPagedCorrupt = 8,    // more pages come back than the free list lent out
+  kPagedNonFinite = 16, // an appended row held a NaN or an infinity
+  kPagedTimeout = 32,   // a bounded wait of the attention kernel expired
+};
+
+__host__ __device__ __forceinline__ size_t q4_block_offset(int slot, int head, int nkv, int page_size) {
+  const int page = slot / page_size, r = slot - page * page_size;
+  return (((size_t)page * nkv + head) * (page_size / kQ4Rows) + r / kQ4Rows) * kQ4Block;
+}
+
+struct ReserveParams {
+  const int32_t *lens, *new_rows, *pages, *free_pages, *head;
+  int32_t* table;
+  int n, page_size, max_pages, num_pages, num_slots;
+  long long table_ld;
+  int32_t *starts, *slots, *lens_out, *pages_out, *head_out, *status;
+};
+cudaError_t paged_reserve_launch(const ReserveParams& p, int num_sms, cudaStream_t st);
+
+struct ReleaseParams {
+  const int32_t *keep, *pages, *table, *head;
+  int32_t* free_pages;
+  int n, page_size, max_pages, num_pages;
+  long long table_ld;
+  int32_t *pages_out, *head_out, *status;
+};
+cudaError_t paged_release_launch(const ReleaseParams& p, int num_sms, cudaStream_t st);
+
+struct Q4AppendParams {
+  const void *k, *v;                 // [T, NKV, 128], f16 or bf16
+  long long k_row, k_head, v_row, v_head;   // strides in elements
+  int bf16;
+  const int32_t* slots;              // [T]; outside [0, num_slots): the row is skipped
+  int T, nkv, page_size, num_slots;  // num_slots: pages * page_size
+  uint8_t* pool;
+  int32_t* status;
+};
+cudaError_t q4_append_launch(const Q4AppendParams& p, cudaStream_t st);
+
+struct Q4ReadParams {
+  const uint8_t* pool;
+  const int32_t* slots;
+  int T, nkv, page_size, num_slots, bf16;
+  void *k, *v;                       // [T, NKV, 128] contiguous
+};
+cudaError_t q4_read_launch(const Q4ReadParams& p, cudaStream_t st);
+
+struct Q4AttnParams {
+  const void* q;                     // [T, NQ, 128], f16 or bf16
+  long long q_row, q_head;           // strides in elements
+  int bf16;
+  const uint8_t* pool;
+  const int32_t *table, *lens, *starts;   // starts NULL: max_rows rows each
+  long long table_ld;
+  int n, T, max_rows, nq, nkv, page_size, max_pages, num_pages;
+  int causal, sink, window;
+  float scale_log2;                  // softmax scale * log2(e)
+  void* out;                         // [T, NQ, 128] contiguous, q's type
+  int* counters;                     // [num_sms], zero between calls
+  float* part;                       // partial results
+  int32_t* status;                   // or NULL
+};
+size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms);
+cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
+
+}  // namespace dfl

@@ -1,0 +1,318 @@
+"""Paged 4-bit K/V cache shared by many requests: block tables built on the
+GPU, rows appended as 4-bit numbers, attention read straight from them.
+
+The cache of one draft sequence (``DFlashKVCache``) is an f16 ring whose length
+the host tracks.  A target model's cache grows by what was accepted, a number
+that only the GPU knows after ``accept``, and every request's is as long as its
+text.  Here the lengths, the block table and the free pages stay on the device;
+one step of a batch is
+
+    step = cache.reserve(new_rows)                     # slots of the new rows
+    for layer in range(num_layers):
+        cache.append(layer, k, v, step)                # [rows, NKV, 128] each
+        o = cache.attend(layer, q, step, max_rows)     # [rows, NQ, 128]
+    cache.trim(rejected)                               # lengths only
+    cache.release()                                    # spare pages go back
+
+without a host synchronisation.  The same operators as plain functions on
+tensors are ``paged_reserve``, ``paged_release``, ``q4_append``, ``q4_read``
+and ``q4_attention``.  Number format and page layout: ``csrc/q4.cuh``.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence, Union
+
+import torch
+
+from . import _native as N
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIM = 128
+BLOCK_BYTES = 2304                   # 16 rows of one kv head, K and V with their scales
+STATUS_BITS = {1: "too few free pages", 2: "a request outgrew its row of the block table",
+               4: "more new rows than slots", 8: "more pages came back than were lent",
+               16: "a NaN or an infinity was appended", 32: "a device-side wait expired"}
+
+
+class PagedStep(NamedTuple):
+    """Result of ``paged_reserve``: where each request's packed rows start
+    [n + 1], the slot of every new row [num_slots], and the requests' lengths,
+    page counts and the free list's head afterwards."""
+    starts: torch.Tensor
+    slots: torch.Tensor
+    lens: torch.Tensor
+    pages: torch.Tensor
+    head: torch.Tensor
+
+
+def _i32(name, t, shape=None):
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    return t.data_ptr()
+
+
+def _table(table, n):
+    if table.dtype is not torch.int32 or not table.is_cuda or table.dim() != 2 or table.shape[0] != n \
+            or table.stride(1) != 1 and table.shape[1] > 1:
+        raise ValueError(f"table must be an int32 CUDA tensor [{n}, max_pages] with contiguous rows")
+    return table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1]
+
+
+def _pool(pool):
+    """(num_pages, NKV, page_size) of a pool."""
+    if pool.dtype is not torch.uint8 or not pool.is_cuda or pool.dim() != 4 or not pool.is_contiguous() \
+            or pool.shape[3] != BLOCK_BYTES:
+        raise ValueError("pool must be a contiguous uint8 CUDA tensor from q4_pool()")
+    return pool.shape[0], pool.shape[1], pool.shape[2] * 16
+
+
+def _rows(name, t, heads=None):
+    if t.dtype not in (torch.float16, torch.bfloat16) or not t.is_cuda or t.dim() != 3 or t.shape[2] != HEAD_DIM \
+            or heads is not None and t.shape[1] != heads:
+        raise ValueError(f"{name} must be an f16 or bf16 CUDA tensor [rows, {heads or 'heads'}, {HEAD_DIM}]")
+    if t.stride(2) != 1 or (t.stride(0) | t.stride(1)) % 8 or t.data_ptr() % 16:
+        return t.contiguous()
+    return t
+
+
+def _same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+class _On:
+    """The tensors' device made current, and its current stream."""
+
+    def __init__(self, t):
+        self.dev = t.device.index
+        self.was = torch.cuda.current_device()
+
+    def __enter__(self):
+        if self.was != self.dev:
+            torch.cuda.set_device(self.dev)
+        return torch.cuda.current_stream(self.dev).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.was != self.dev:
+            torch.cuda.set_device(self.was)
+
+
+def _opt(status):
+    return None if status is None else _i32("status", status, (1,))
+
+
+def paged_reserve(lens, new_rows, pages, table, free_pages, head, page_size: int, num_slots: int,
+                  status=None) -> PagedStep:
+    """Pages and cache slots for the rows that each request brings.
+
+    lens, new_rows, pages [n], table [n, max_pages], free_pages [num_pages] and
+    head [1] are int32 device tensors; request i holds lens[i] rows on pages[i]
+    pages.  New pages come off ``free_pages`` at ``head`` and are written into
+    ``table``; the other inputs are only read.  ``num_slots`` bounds the new
+    rows of all requests (known on the host); surplus slots are -1.  A request
+    that cannot be served keeps its length and sets a bit of ``status``
+    (STATUS_BITS)."""
+    n = lens.shape[0]
+    lib = N.load()
+    _same_device(lens, new_rows, pages, table, free_pages, head, status)
+    t, ld, max_pages = _table(table, n)
+    out = torch.empty(3 * n + 2 + max(num_slots, 0), dtype=torch.int32, device=lens.device)
+    starts, lens_out, pages_out, head_out, slots = out.split([n + 1, n, n, 1, max(num_slots, 0)])
+    a, b, c = _i32("lens", lens, (n,)), _i32("new_rows", new_rows, (n,)), _i32("pages", pages, (n,))
+    f, h = _i32("free_pages", free_pages), _i32("head", head, (1,))
+    with _On(lens) as st:
+        N.check(lib.dflash_paged_reserve(a, b, c, n, page_size, t, ld, max_pages, f, free_pages.numel(), h,
+                                         starts.data_ptr(), slots.data_ptr(), num_slots, lens_out.data_ptr(),
+                                         pages_out.data_ptr(), head_out.data_ptr(), _opt(status), st),
+                "dflash_paged_reserve")
+    return PagedStep(starts, slots, lens_out, pages_out, head_out)
+
+
+def paged_release(keep, pages, table, free_pages, head, page_size: int, status=None):
+    """Request i keeps the pages of its first keep[i] rows; the others go back
+    into ``free_pages`` below ``head``.  Returns (pages, head) afterwards."""
+    n = keep.shape[0]
+    lib = N.load()
+    _same_device(keep, pages, table, free_pages, head, status)
+    t, ld, max_pages = _table(table, n)
+    out = torch.empty(n + 1, dtype=torch.int32, device=keep.device)
+    pages_out, head_out = out.split([n, 1])
+    a, b = _i32("keep", keep, (n,)), _i32("pages", pages, (n,))
+    f, h = _i32("free_pages", free_pages), _i32("head", head, (1,))
+    with _On(keep) as st:
+        N.check(lib.dflash_paged_release(a, b, n, page_size, t, ld, max_pages, f, free_pages.numel(), h,
+                                         pages_out.data_ptr(), head_out.data_ptr(), _opt(status), st),
+                "dflash_paged_release")
+    return pages_out, head_out
+
+
+def q4_pool(num_pages: int, num_kv_heads: int, page_size: int = 64, device="cuda") -> torch.Tensor:
+    """An empty pool of one layer: uint8 [num_pages, NKV, page_size / 16, 2304]."""
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}")
+    if num_pages < 1 or num_kv_heads < 1:
+        raise ValueError("num_pages and num_kv_heads must be positive")
+    return torch.zeros(num_pages, num_kv_heads, page_size // 16, BLOCK_BYTES, dtype=torch.uint8, device=device)
+
+
+def q4_append(k, v, slots, pool, status=None) -> None:
+    """Quantise the rows k, v [rows, NKV, 128] (f16 or bf16, strided rows and
+    heads) into their slots [rows] of the pool; slots must be distinct, and a
+    row whose slot is outside the pool is skipped."""
+    num_pages, nkv, page_size = _pool(pool)
+    k, v = _rows("k", k, nkv), _rows("v", v, nkv)
+    if k.dtype != v.dtype or k.shape != v.shape:
+        raise ValueError("k and v must have the same type and shape")
+    _same_device(pool, k, v, slots, status)
+    with _On(pool) as st:
+        N.check(N.load().dflash_q4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                          v.stride(1), k.dtype is torch.bfloat16, _i32("slots", slots, (k.shape[0],)),
+                                          k.shape[0], nkv, pool.data_ptr(), num_pages, page_size, _opt(status), st),
+                "dflash_q4_append")
+
+
+def q4_read(pool, slots, dtype=torch.float16):
+    """What the cache stands for at ``slots``: (k, v) [rows, NKV, 128], exact
+    in f16 and bf16; zeros for a slot outside the pool."""
+    num_pages, nkv, page_size = _pool(pool)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+    if slots.dim() != 1:
+        raise ValueError("slots must be one-dimensional")
+    _same_device(pool, slots)
+    rows = slots.shape[0]
+    k, v = torch.empty((2, rows, nkv, HEAD_DIM), dtype=dtype, device=pool.device)
+    with _On(pool) as st:
+        N.check(N.load().dflash_q4_read(pool.data_ptr(), num_pages, page_size, _i32("slots", slots), rows, nkv,
+                                        dtype is torch.bfloat16, k.data_ptr(), v.data_ptr(), st), "dflash_q4_read")
+    return k, v
+
+
+def q4_attention_workspace(n: int, max_rows: int, num_heads: int, num_kv_heads: int, device="cuda") -> torch.Tensor:
+    """Workspace of ``q4_attention`` for up to ``max_rows`` query rows a
+    request; it may serve any number of calls that do not overlap."""
+    device = torch.device(device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    with torch.cuda.device(device):
+        size = N.load().dflash_q4_attention_workspace_size(max_rows, num_heads, num_kv_heads)
+    if size == 0:
+        raise ValueError(f"no such attention: {max_rows} rows, {num_heads} / {num_kv_heads} heads")
+    return torch.zeros(size, dtype=torch.uint8, device=device)
+
+
+def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: bool = False, sink: int = 0,
+                 window: int = 0, scale: Optional[float] = None, out=None, status=None, workspace=None):
+    """Grouped-query attention of each request's query rows over its cached
+    rows.  q [rows, NQ, 128] (f16 or bf16; strided rows and heads) holds the
+    requests' rows one after another: request i owns starts[i] ..
+    starts[i + 1] - 1 (at most ``max_rows``), or ``max_rows`` each without
+    ``starts``.  lens [n] counts the cached rows, the new ones included.
+
+    causal: query row j of m sees the keys below lens - m + j + 1 (else below
+    lens); window: of those only the first ``sink`` and the last ``window``.
+    A row that sees no key gives zeros.  scale defaults to 128 ** -0.5."""
+    num_pages, nkv, page_size = _pool(pool)
+    q = _rows("q", q)
+    rows, nq = q.shape[0], q.shape[1]
+    n = lens.shape[0]
+    _same_device(pool, q, table, lens, starts, out, status, workspace)
+    t, ld, max_pages = _table(table, n)
+    if out is None:
+        out = torch.empty((rows, nq, HEAD_DIM), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape and type")
+    if workspace is None:
+        workspace = q4_attention_workspace(n, max_rows, nq, nkv, q.device)
+    with _On(pool) as st:
+        N.check(N.load().dflash_q4_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), q.dtype is torch.bfloat16, pool.data_ptr(), num_pages, page_size,
+            t, ld, max_pages, _i32("lens", lens, (n,)), None if starts is None else _i32("starts", starts, (n + 1,)),
+            n, rows, max_rows, nq, nkv, causal, sink, window, HEAD_DIM ** -0.5 if scale is None else scale,
+            out.data_ptr(), _opt(status), workspace.data_ptr(), workspace.numel(), st), "dflash_q4_attention")
+    return out
+
+
+class PagedKVCacheQ4:
+    """Cache of ``max_seqs`` requests over ``num_layers`` layers.  Every
+    method enqueues on the current stream; none waits for the device except
+    ``check`` and ``free_page_count``."""
+
+    def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, max_seqs: int, max_len: int,
+                 page_size: int = 64, device="cuda"):
+        if num_layers < 1 or max_seqs < 1 or max_len < 1:
+            raise ValueError("num_layers, max_seqs and max_len must be positive")
+        self.page_size, self.max_seqs, self.nkv = page_size, max_seqs, num_kv_heads
+        self.pools = [q4_pool(num_pages, num_kv_heads, page_size, device) for _ in range(num_layers)]
+        self.device = self.pools[0].device
+        i32 = dict(dtype=torch.int32, device=self.device)
+        self.table = torch.full((max_seqs, -(-max_len // page_size)), -1, **i32)
+        self.lens = torch.zeros(max_seqs, **i32)
+        self.pages = torch.zeros(max_seqs, **i32)
+        self.free_pages = torch.arange(num_pages, **i32)
+        self.head = torch.zeros(1, **i32)
+        self.status = torch.zeros(1, **i32)
+        self._workspace = {}
+
+    def reserve(self, new_rows: Union[torch.Tensor, Sequence[int]], num_slots: Optional[int] = None) -> PagedStep:
+        """Make room for new_rows[i] rows of request i (0 where it sits out).
+        ``num_slots`` bounds their sum; it is needed when new_rows is a device
+        tensor."""
+        if not torch.is_tensor(new_rows):
+            num_slots = sum(new_rows) if num_slots is None else num_slots
+            new_rows = torch.tensor(list(new_rows), dtype=torch.int32).to(self.device, non_blocking=True)
+        elif num_slots is None:
+            raise ValueError("num_slots is needed with new_rows on the device")
+        step = paged_reserve(self.lens, new_rows, self.pages, self.table, self.free_pages, self.head, self.page_size,
+                             num_slots, self.status)
+        self.lens, self.pages, self.head = step.lens, step.pages, step.head
+        return step
+
+    def append(self, layer: int, k, v, step: PagedStep) -> None:
+        q4_append(k, v, step.slots, self.pools[layer], self.status)
+
+    def attend(self, layer: int, q, step: PagedStep, max_rows: int, causal: bool = True, sink: int = 0,
+               window: int = 0, scale: Optional[float] = None, out=None):
+        """Attention of the step's query rows over everything cached."""
+        key = (max_rows, q.shape[1], torch.cuda.current_stream(self.device).cuda_stream)
+        ws = self._workspace.get(key)      # one for each stream: calls on different streams may overlap
+        if ws is None:
+            ws = self._workspace[key] = q4_attention_workspace(self.max_seqs, max_rows, q.shape[1], self.nkv, self.device)
+        return q4_attention(q, self.pools[layer], self.table, self.lens, step.starts, max_rows, causal, sink, window,
+                            scale, out, self.status, ws)
+
+    def trim(self, counts: Union[int, torch.Tensor, Sequence[int]]) -> None:
+        """Drop the last counts[i] rows of request i (one number: of every
+        request).  Pages stay with the request until ``release``."""
+        if not torch.is_tensor(counts) and not isinstance(counts, int):
+            counts = torch.tensor(list(counts), dtype=torch.int32).to(self.device, non_blocking=True)
+        self.lens = (self.lens - counts).clamp_(min=0).to(torch.int32)
+
+    def release(self, seqs: Sequence[int] = ()) -> None:
+        """Give spare pages back; requests ``seqs`` are finished and emptied."""
+        seqs = [int(s) for s in seqs]
+        if any(not 0 <= s < self.max_seqs for s in seqs):
+            raise ValueError(f"sequences must lie in [0, {self.max_seqs})")
+        if seqs:
+            self.lens = self.lens.index_fill(0, torch.tensor(seqs).to(self.device), 0)
+        self.pages, self.head = paged_release(self.lens, self.pages, self.table, self.free_pages, self.head,
+                                              self.page_size, self.status)
+
+    def read(self, layer: int, seq: int, length: int, dtype=torch.float16):
+        """The first ``length`` rows of a request as (k, v) [length, NKV, 128]."""
+        pos = torch.arange(length, device=self.device)
+        slots = self.table[seq][pos // self.page_size] * self.page_size + (pos % self.page_size).to(torch.int32)
+        return q4_read(self.pools[layer], slots.to(torch.int32), dtype)
+
+    def free_page_count(self) -> int:
+        return self.free_pages.numel() - int(self.head)
+
+    def check(self) -> None:
+        """Raise what any call since the last check recorded on the device."""
+        bits = int(self.status)
+        if bits:
+            self.status.zero_()
+            raise RuntimeError("paged cache: " + "; ".join(m for b, m in STATUS_BITS.items() if bits & b))
