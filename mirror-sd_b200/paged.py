@@ -45,63 +45,69 @@ class PagedStep(NamedTuple):
     head: torch.Tensor
 
 
-def _i32(name, t, shape=None):
-    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+# The calls below are a few microseconds of GPU work in a decode step, so the
+# checks read each tensor's fields once and nothing else runs on the host.
+_I32 = torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream().cuda_stream without the Stream object
+
+
+def _device(t):
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("the paged cache's tensors must be on a CUDA device")
+    return dev
+
+
+def _i32(name, t, n, dev):
+    """Address of a contiguous int32 vector of n entries (any number if None) on device dev."""
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 1 or not t.is_contiguous() \
+            or n is not None and t.numel() != n:
+        raise ValueError(f"{name} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on cuda:{dev}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _table(table, n):
-    if table.dtype is not torch.int32 or not table.is_cuda or table.dim() != 2 or table.shape[0] != n \
-            or table.stride(1) != 1 and table.shape[1] > 1:
-        raise ValueError(f"table must be an int32 CUDA tensor [{n}, max_pages] with contiguous rows")
-    return table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1]
+def _table(table, n, dev):
+    """(address, row stride, max_pages)"""
+    if table.dtype is not _I32 or table.get_device() != dev or table.dim() != 2:
+        raise ValueError(f"table must be an int32 matrix [{n}, max_pages] on cuda:{dev}")
+    rows, width = table.shape
+    if rows != n or table.stride(1) != 1 and width > 1:
+        raise ValueError(f"table must be [{n}, max_pages] with contiguous rows, got {tuple(table.shape)}")
+    return table.data_ptr(), max(table.stride(0), width), width
 
 
 def _pool(pool):
     """(num_pages, NKV, page_size) of a pool."""
-    if pool.dtype is not torch.uint8 or not pool.is_cuda or pool.dim() != 4 or not pool.is_contiguous() \
-            or pool.shape[3] != BLOCK_BYTES:
-        raise ValueError("pool must be a contiguous uint8 CUDA tensor from q4_pool()")
-    return pool.shape[0], pool.shape[1], pool.shape[2] * 16
+    if pool.dtype is not torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] != BLOCK_BYTES:
+        raise ValueError("pool must be a contiguous uint8 tensor from q4_pool()")
+    num_pages, nkv, blocks, _ = pool.shape
+    return num_pages, nkv, blocks * 16
 
 
-def _rows(name, t, heads=None):
-    if t.dtype not in (torch.float16, torch.bfloat16) or not t.is_cuda or t.dim() != 3 or t.shape[2] != HEAD_DIM \
-            or heads is not None and t.shape[1] != heads:
-        raise ValueError(f"{name} must be an f16 or bf16 CUDA tensor [rows, {heads or 'heads'}, {HEAD_DIM}]")
-    if t.stride(2) != 1 or (t.stride(0) | t.stride(1)) % 8 or t.data_ptr() % 16:
-        return t.contiguous()
-    return t
+def _rows(name, t, heads, dev):
+    """t, or a copy where the kernels could not read it in whole 16 bytes; and its strides."""
+    if t.dtype is not torch.float16 and t.dtype is not torch.bfloat16 or t.get_device() != dev or t.dim() != 3 \
+            or t.shape[2] != HEAD_DIM or heads is not None and t.shape[1] != heads:
+        raise ValueError(f"{name} must be f16 or bf16 [rows, {heads or 'heads'}, {HEAD_DIM}] on cuda:{dev}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    a, b, c = t.stride()
+    if c != 1 or (a | b) % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+        a, b, c = t.stride()
+    return t, a, b
 
 
-def _same_device(first, *others):
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
-
-
-class _On:
-    """The tensors' device made current, and its current stream."""
-
-    def __init__(self, t):
-        self.dev = t.device.index
-        self.was = torch.cuda.current_device()
-
-    def __enter__(self):
-        if self.was != self.dev:
-            torch.cuda.set_device(self.dev)
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.was != self.dev:
-            torch.cuda.set_device(self.was)
-
-
-def _opt(status):
-    return None if status is None else _i32("status", status, (1,))
+def _call(name, dev, *args):
+    """A C entry on the tensors' device and its current stream."""
+    fn = getattr(N.load(), name)
+    if torch.cuda.current_device() == dev:
+        status = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _raw_stream(dev))
+    if status:
+        N.check(status, name)
 
 
 def paged_reserve(lens, new_rows, pages, table, free_pages, head, page_size: int, num_slots: int,
@@ -115,38 +121,31 @@ def paged_reserve(lens, new_rows, pages, table, free_pages, head, page_size: int
     rows of all requests (known on the host); surplus slots are -1.  A request
     that cannot be served keeps its length and sets a bit of ``status``
     (STATUS_BITS)."""
-    n = lens.shape[0]
-    lib = N.load()
-    _same_device(lens, new_rows, pages, table, free_pages, head, status)
-    t, ld, max_pages = _table(table, n)
-    out = torch.empty(3 * n + 2 + max(num_slots, 0), dtype=torch.int32, device=lens.device)
-    starts, lens_out, pages_out, head_out, slots = out.split([n + 1, n, n, 1, max(num_slots, 0)])
-    a, b, c = _i32("lens", lens, (n,)), _i32("new_rows", new_rows, (n,)), _i32("pages", pages, (n,))
-    f, h = _i32("free_pages", free_pages), _i32("head", head, (1,))
-    with _On(lens) as st:
-        N.check(lib.dflash_paged_reserve(a, b, c, n, page_size, t, ld, max_pages, f, free_pages.numel(), h,
-                                         starts.data_ptr(), slots.data_ptr(), num_slots, lens_out.data_ptr(),
-                                         pages_out.data_ptr(), head_out.data_ptr(), _opt(status), st),
-                "dflash_paged_reserve")
+    dev, n = _device(lens), lens.numel()
+    if num_slots < 0:
+        raise ValueError(f"num_slots {num_slots}")
+    t, ld, max_pages = _table(table, n, dev)
+    out = torch.empty(3 * n + 2 + num_slots, dtype=_I32, device=lens.device)
+    o = out.data_ptr()      # [starts | lens | pages | head | slots]
+    _call("dflash_paged_reserve", dev, _i32("lens", lens, n, dev), _i32("new_rows", new_rows, n, dev),
+          _i32("pages", pages, n, dev), n, page_size, t, ld, max_pages, _i32("free_pages", free_pages, None, dev),
+          free_pages.numel(), _i32("head", head, 1, dev), o, o + 4 * (3 * n + 2), num_slots, o + 4 * (n + 1),
+          o + 4 * (2 * n + 1), o + 4 * (3 * n + 1), None if status is None else _i32("status", status, 1, dev))
+    starts, lens_out, pages_out, head_out, slots = out.split_with_sizes([n + 1, n, n, 1, num_slots])
     return PagedStep(starts, slots, lens_out, pages_out, head_out)
 
 
 def paged_release(keep, pages, table, free_pages, head, page_size: int, status=None):
     """Request i keeps the pages of its first keep[i] rows; the others go back
     into ``free_pages`` below ``head``.  Returns (pages, head) afterwards."""
-    n = keep.shape[0]
-    lib = N.load()
-    _same_device(keep, pages, table, free_pages, head, status)
-    t, ld, max_pages = _table(table, n)
-    out = torch.empty(n + 1, dtype=torch.int32, device=keep.device)
-    pages_out, head_out = out.split([n, 1])
-    a, b = _i32("keep", keep, (n,)), _i32("pages", pages, (n,))
-    f, h = _i32("free_pages", free_pages), _i32("head", head, (1,))
-    with _On(keep) as st:
-        N.check(lib.dflash_paged_release(a, b, n, page_size, t, ld, max_pages, f, free_pages.numel(), h,
-                                         pages_out.data_ptr(), head_out.data_ptr(), _opt(status), st),
-                "dflash_paged_release")
-    return pages_out, head_out
+    dev, n = _device(keep), keep.numel()
+    t, ld, max_pages = _table(table, n, dev)
+    out = torch.empty(n + 1, dtype=_I32, device=keep.device)
+    o = out.data_ptr()
+    _call("dflash_paged_release", dev, _i32("keep", keep, n, dev), _i32("pages", pages, n, dev), n, page_size, t, ld,
+          max_pages, _i32("free_pages", free_pages, None, dev), free_pages.numel(), _i32("head", head, 1, dev), o,
+          o + 4 * n, None if status is None else _i32("status", status, 1, dev))
+    return out.split_with_sizes([n, 1])
 
 
 def q4_pool(num_pages: int, num_kv_heads: int, page_size: int = 64, device="cuda") -> torch.Tensor:
@@ -162,32 +161,30 @@ def q4_append(k, v, slots, pool, status=None) -> None:
     """Quantise the rows k, v [rows, NKV, 128] (f16 or bf16, strided rows and
     heads) into their slots [rows] of the pool; slots must be distinct, and a
     row whose slot is outside the pool is skipped."""
+    dev = _device(pool)
     num_pages, nkv, page_size = _pool(pool)
-    k, v = _rows("k", k, nkv), _rows("v", v, nkv)
-    if k.dtype != v.dtype or k.shape != v.shape:
-        raise ValueError("k and v must have the same type and shape")
-    _same_device(pool, k, v, slots, status)
-    with _On(pool) as st:
-        N.check(N.load().dflash_q4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                          v.stride(1), k.dtype is torch.bfloat16, _i32("slots", slots, (k.shape[0],)),
-                                          k.shape[0], nkv, pool.data_ptr(), num_pages, page_size, _opt(status), st),
-                "dflash_q4_append")
+    k, k_row, k_head = _rows("k", k, nkv, dev)
+    v, v_row, v_head = _rows("v", v, nkv, dev)
+    rows = k.shape[0]
+    if k.dtype is not v.dtype or v.shape[0] != rows:
+        raise ValueError("k and v must have the same type and number of rows")
+    _call("dflash_q4_append", dev, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, k.dtype is torch.bfloat16,
+          _i32("slots", slots, rows, dev), rows, nkv, pool.data_ptr(), num_pages, page_size,
+          None if status is None else _i32("status", status, 1, dev))
 
 
 def q4_read(pool, slots, dtype=torch.float16):
     """What the cache stands for at ``slots``: (k, v) [rows, NKV, 128], exact
     in f16 and bf16; zeros for a slot outside the pool."""
+    dev = _device(pool)
     num_pages, nkv, page_size = _pool(pool)
-    if dtype not in (torch.float16, torch.bfloat16):
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise ValueError("dtype must be torch.float16 or torch.bfloat16")
-    if slots.dim() != 1:
-        raise ValueError("slots must be one-dimensional")
-    _same_device(pool, slots)
-    rows = slots.shape[0]
-    k, v = torch.empty((2, rows, nkv, HEAD_DIM), dtype=dtype, device=pool.device)
-    with _On(pool) as st:
-        N.check(N.load().dflash_q4_read(pool.data_ptr(), num_pages, page_size, _i32("slots", slots), rows, nkv,
-                                        dtype is torch.bfloat16, k.data_ptr(), v.data_ptr(), st), "dflash_q4_read")
+    at, rows = _i32("slots", slots, None, dev), slots.numel()
+    k = torch.empty((rows, nkv, HEAD_DIM), dtype=dtype, device=pool.device)
+    v = torch.empty_like(k)
+    _call("dflash_q4_read", dev, pool.data_ptr(), num_pages, page_size, at, rows, nkv, dtype is torch.bfloat16,
+          k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -215,24 +212,25 @@ def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: b
     causal: query row j of m sees the keys below lens - m + j + 1 (else below
     lens); window: of those only the first ``sink`` and the last ``window``.
     A row that sees no key gives zeros.  scale defaults to 128 ** -0.5."""
+    dev = _device(pool)
     num_pages, nkv, page_size = _pool(pool)
-    q = _rows("q", q)
-    rows, nq = q.shape[0], q.shape[1]
-    n = lens.shape[0]
-    _same_device(pool, q, table, lens, starts, out, status, workspace)
-    t, ld, max_pages = _table(table, n)
+    q, q_row, q_head = _rows("q", q, None, dev)
+    rows, nq, _ = q.shape
+    n = lens.numel()
+    t, ld, max_pages = _table(table, n, dev)
     if out is None:
         out = torch.empty((rows, nq, HEAD_DIM), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of q's shape and type")
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape, type and device")
     if workspace is None:
         workspace = q4_attention_workspace(n, max_rows, nq, nkv, q.device)
-    with _On(pool) as st:
-        N.check(N.load().dflash_q4_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), q.dtype is torch.bfloat16, pool.data_ptr(), num_pages, page_size,
-            t, ld, max_pages, _i32("lens", lens, (n,)), None if starts is None else _i32("starts", starts, (n + 1,)),
-            n, rows, max_rows, nq, nkv, causal, sink, window, HEAD_DIM ** -0.5 if scale is None else scale,
-            out.data_ptr(), _opt(status), workspace.data_ptr(), workspace.numel(), st), "dflash_q4_attention")
+    elif workspace.get_device() != dev:
+        raise ValueError(f"workspace must be on cuda:{dev}")
+    _call("dflash_q4_attention", dev, q.data_ptr(), q_row, q_head, q.dtype is torch.bfloat16, pool.data_ptr(), num_pages,
+          page_size, t, ld, max_pages, _i32("lens", lens, n, dev),
+          None if starts is None else _i32("starts", starts, n + 1, dev), n, rows, max_rows, nq, nkv, causal, sink,
+          window, HEAD_DIM ** -0.5 if scale is None else scale, out.data_ptr(),
+          None if status is None else _i32("status", status, 1, dev), workspace.data_ptr(), workspace.nbytes)
     return out
 
 
