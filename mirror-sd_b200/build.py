@@ -18,8 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libdflash_b200.so")
 SOURCES = ["quant.cu", "w8_tc.cu", "attention.cu", "attention_tc.cu", "tc_gemm.cu", "lm_head.cu", "misc.cu", "anchor.cu",
-           "f32_path.cu", "paged.cu", "q4_cache.cu", "q4_attention.cu", "dflash_api.cu", "paged_api.cu"]
-HEADERS = ["common.cuh", "kernels.cuh", "q4.cuh", "api_error.cuh"]
+           "f32_path.cu", "paged.cu", "q4_cache.cu", "q4_attention.cu", "q4_attention_tc.cu", "dflash_api.cu", "paged_api.cu"]
+HEADERS = ["common.cuh", "kernels.cuh", "q4.cuh", "q4_attn.cuh", "api_error.cuh"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills"]
 

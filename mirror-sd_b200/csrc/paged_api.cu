@@ -43,7 +43,7 @@ int check_pool(int rows, int nkv, const void* pool, int num_pages, int page_size
   return DFLASH_OK;
 }
 
-constexpr size_t kCounterBytes = 4096;   // one counter per SM, then the partials
+constexpr size_t kCounterBytes = 4096;   // two counters per SM, then the partials
 
 }  // namespace
 
@@ -129,7 +129,10 @@ size_t dflash_q4_attention_workspace_size(int max_rows, int nq, int nkv) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return kCounterBytes + q4_attn_part_floats(max_rows, nq, nkv, sms) * sizeof(float);
+  // either kernel (fewer rows than max_rows may run in a later call)
+  const size_t few = q4_attn_part_floats(max_rows, nq, nkv, sms);
+  const size_t many = (long long)max_rows * (nq / nkv) <= kQ4FewRows ? 0 : q4_attn_tc_part_floats(max_rows, nq, nkv, sms);
+  return kCounterBytes + (few > many ? few : many) * sizeof(float);
 }
 
 int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages,
@@ -148,12 +151,15 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
     return fail(DFLASH_ERR_INVALID, "without starts every request has max_rows rows (%d x %d, got %d)", n, max_rows, rows);
   if (sink < 0 || window < 0) return fail(DFLASH_ERR_INVALID, "sink %d, window %d", sink, window);
   if (sink > 0 && window == 0) return fail(DFLASH_ERR_INVALID, "sink needs a window (window 0 sees every row)");
-  if (!std::isfinite(scale)) return fail(DFLASH_ERR_INVALID, "scale is not finite");
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(DFLASH_ERR_INVALID, "scale must be positive and finite");
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_row % 8 || q_head % 8)
     return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");
   const int G = nq / nkv;
+  if (G > 256 || nkv > 1024 || ((double)max_rows * G / 8 + 1) * nkv * nkv > 4e9)
+    return fail(DFLASH_ERR_INVALID, "%d query heads a kv head, %d kv heads, %d rows: too many", G, nkv, max_rows);
   // tiles of all items together are counted in 32 bits
   const double units = (double)n * ((double)max_pages * page_size / 64 + 2) * nkv * ((double)max_rows * G / 8 + 1);
+  if ((long long)rows * nq > INT32_MAX) return fail(DFLASH_ERR_INVALID, "rows x nq must stay below 2^31");
   if (units > 2e9) return fail(DFLASH_ERR_INVALID, "n x table x heads x rows is too large for one call");
   if (workspace_bytes < dflash_q4_attention_workspace_size(max_rows, nq, nkv))
     return fail(DFLASH_ERR_INVALID, "workspace too small (%zu < %zu)", workspace_bytes,
@@ -161,17 +167,24 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
   if (rows == 0) return DFLASH_OK;
   int sms = 0;
   if (int rc = num_sms(&sms)) return rc;
-  if ((size_t)sms * sizeof(int) > kCounterBytes) return fail(DFLASH_ERR_INVALID, "%d SMs", sms);
+  if ((size_t)sms * 2 * sizeof(int) > kCounterBytes) return fail(DFLASH_ERR_INVALID, "%d SMs", sms);
   Q4AttnParams p{};
   p.q = q; p.q_row = q_row; p.q_head = q_head; p.bf16 = bf16 != 0; p.pool = pool;
   p.table = table; p.lens = lens; p.starts = starts; p.table_ld = table_ld;
-  p.n = n; p.T = rows; p.max_rows = max_rows; p.nq = nq; p.nkv = nkv; p.page_size = page_size;
+  p.n = n; p.T = rows; p.max_rows = max_rows; p.nq = nq; p.nkv = nkv;
+  p.by_g = Divisor(G); p.by_nkv = Divisor(nkv);
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.max_pages = max_pages; p.num_pages = num_pages; p.causal = causal != 0; p.sink = sink; p.window = window;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.out = out; p.status = status;
   p.counters = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-  CK(q4_attn_launch(p, sms, static_cast<cudaStream_t>(stream)));
+  // Up to 16 query rows a kv head each warp multiplies on its own (mma.sync, no
+  // hand-over between warps); above, tcgen05 with the rows as columns.
+  if ((long long)max_rows * G <= kQ4FewRows)
+    CK(q4_attn_launch(p, sms, static_cast<cudaStream_t>(stream)));
+  else
+    CK(q4_attn_tc_launch(p, sms, static_cast<cudaStream_t>(stream)));
   return DFLASH_OK;
 }
 

@@ -8,14 +8,16 @@
 //   K scales  [16 rows][8 groups]       1 byte a group of 16 channels
 //   V values  [8 row pairs][8 groups][16 B]
 //   V scales  [8 groups][16 rows]
-// so a block is one contiguous copy and its pieces are the register fragments
-// of a 16x16 matrix tile: K with the rows and V with the channels as the
-// tile's rows, read from shared memory 16 bytes a lane without conflicts.
-//   K, row r, channel d = 32c + 8w + 2n + h: word w of the 16 bytes at
-//     64 r + 16 c, bits 16h + 4n .. + 3
-//   V, row r = 2j + h, channel d = 16g + 4w + n: word w of the 16 bytes at
-//     16 (8 j + g), bits 16h + 4n .. + 3
-// (both: half h of a word holds one side of a register's f16 pair).
+// so a block is one contiguous copy and its 16-byte pieces are the register
+// fragments of a 16x16 matrix tile, K with the rows and V with the channels as
+// the tile's rows:
+//   K, row r, channel d = 32c + 8w + 2n + h: word w of piece (r, c), bits 16h + 4n .. + 3
+//   V, row r = 2j + h, channel d = 16g + 4w + n: word w of piece (j, g), bits 16h + 4n .. + 3
+// (half h of a word holds one side of a register's f16 pair).  Pieces are
+// permuted inside their rows (q4_k_piece, q4_v_piece) so that 8 lanes read 8
+// different 16-byte columns of shared memory whether they hold different rows
+// of one piece column (a thread per cached row), or 2 rows and every piece
+// (the fragments of mma.sync), or the row halves of different blocks.
 //
 // Numbers: a group of 16 channels of a row is x = (u - 8) * s, u the 4-bit
 // code (1..15 as written here), s a scale with 5 exponent and 3 mantissa bits,
@@ -52,6 +54,10 @@ __host__ __device__ __forceinline__ size_t q4_block_offset(int slot, int head, i
   const int page = slot / page_size, r = slot - page * page_size;
   return (((size_t)page * nkv + head) * (page_size / kQ4Rows) + r / kQ4Rows) * kQ4Block;
 }
+
+// byte offsets of the pieces inside the block's K and V values
+__host__ __device__ __forceinline__ int q4_k_piece(int r, int c) { return 64 * r + 16 * (c ^ (r >> 1 & 3)); }
+__host__ __device__ __forceinline__ int q4_v_piece(int j, int g) { return 16 * (8 * j + (g ^ 2 * (j & 3) ^ j >> 2)); }
 
 struct ReserveParams {
   const int32_t *lens, *new_rows, *pages, *free_pages, *head;
@@ -90,6 +96,15 @@ struct Q4ReadParams {
 };
 cudaError_t q4_read_launch(const Q4ReadParams& p, cudaStream_t st);
 
+// x / d for x * d < 2^32
+struct Divisor {
+  uint32_t m;
+  int d;
+  Divisor() = default;
+  explicit Divisor(int by) : m((uint32_t)(((1ull << 32) + by - 1) / by)), d(by) {}
+  __device__ __forceinline__ int of(int x) const { return d == 1 ? x : (int)__umulhi((uint32_t)x, m); }
+};
+
 struct Q4AttnParams {
   const void* q;                     // [T, NQ, 128], f16 or bf16
   long long q_row, q_head;           // strides in elements
@@ -97,15 +112,21 @@ struct Q4AttnParams {
   const uint8_t* pool;
   const int32_t *table, *lens, *starts;   // starts NULL: max_rows rows each
   long long table_ld;
-  int n, T, max_rows, nq, nkv, page_size, max_pages, num_pages;
+  int n, T, max_rows, nq, nkv, page_shift, max_pages, num_pages;   // pages of 2^page_shift rows
+  Divisor by_g, by_nkv;              // G = NQ / NKV; NKV
   int causal, sink, window;
   float scale_log2;                  // softmax scale * log2(e)
   void* out;                         // [T, NQ, 128] contiguous, q's type
-  int* counters;                     // [num_sms], zero between calls
+  int* counters;                     // [2 * num_sms], zero between calls
   float* part;                       // partial results
   int32_t* status;                   // or NULL
 };
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms);
 cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
+// the same for blocks of query rows (q4_attention_tc.cu)
+size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms);
+cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
+// query rows of a kv head up to which the first kernel runs
+constexpr int kQ4FewRows = 16;
 
 }  // namespace dfl

@@ -31,7 +31,7 @@
 //
 // The running maximum is only raised when a score passes it by 2^8 (then O
 // and the sum are rescaled), as P below 256 loses nothing in f16.
-#include "q4.cuh"
+#include "q4_attn.cuh"
 
 namespace dfl {
 
@@ -42,118 +42,11 @@ constexpr int QA_STAGE = QA_TILE / kQ4Rows * kQ4Block;
 constexpr int QA_STAGES = 3;
 constexpr float QA_RAISE = 8.f;
 
-// ---- which cached rows a request's queries see ------------------------------
-// Query row j of `rows` of a request with L cached rows ends at key
-// e = causal ? L - rows + j + 1 : L and sees k < e with k < sink or
-// k >= e - window (window 0: all of them).  The request as a whole touches
-// tiles [0, a) (sink) and [b, c).
-struct TileSpan {
-  int a, b, c;   // count = a + c - b
-};
-__device__ __forceinline__ TileSpan tile_span(const Q4AttnParams& p, int L, int rows) {
-  TileSpan t{0, 0, (L + QA_TILE - 1) / QA_TILE};
-  if (p.window > 0) {
-    const int lo = max((p.causal ? L - rows + 1 : L) - p.window, 0);
-    t.a = (min(p.sink, L) + QA_TILE - 1) / QA_TILE;
-    t.b = max(min(lo, L) / QA_TILE, t.a);
-  }
-  return t;
-}
-
-struct Item {          // one (request, query group, kv head)
-  int seq, L, rows, row0;   // cached rows, query rows, first packed query row
-  TileSpan span;
-  int ntile;           // >= 1: a request without visible keys still writes zeros
-  int groups;          // query groups of the request
-};
-
-__device__ __forceinline__ int seq_rows(const Q4AttnParams& p, int i, int* row0) {
-  int a = i * p.max_rows, b = a + p.max_rows;
-  if (p.starts) {
-    a = __ldg(p.starts + i);
-    b = __ldg(p.starts + i + 1);
-  }
-  // device data the host has not seen: stay inside the query array
-  a = min(max(a, 0), p.T);
-  b = min(max(b, a), p.T);
-  *row0 = a;
-  return min(b - a, p.max_rows);
-}
-template <int QT>
-__device__ __forceinline__ Item load_item(const Q4AttnParams& p, int i) {
-  Item it;
-  it.seq = i;
-  it.rows = seq_rows(p, i, &it.row0);
-  it.L = min(max(__ldg(p.lens + i), 0), p.max_pages * p.page_size);
-  it.span = tile_span(p, it.L, it.rows);
-  it.ntile = max(it.span.a + it.span.c - it.span.b, 1);
-  it.groups = (it.rows * (p.nq / p.nkv) + QT - 1) / QT;
-  return it;
-}
-__device__ __forceinline__ int item_tile(const Item& it, int j) {
-  return j < it.span.a ? j : j - it.span.a + it.span.b;
-}
-
-// position of a warp in the flat order of tiles
-struct Cursor {
-  Item it;
-  int sub;    // query group * NKV + kv head
-  int j;      // tile of the item
-};
-
-template <int QT>
-__device__ __forceinline__ void cursor_at(const Q4AttnParams& p, const int* base, int u, Cursor& c) {
-  int lo = 0, hi = p.n - 1;
-  while (lo < hi) {   // last request whose first tile is <= u
-    const int mid = (lo + hi + 1) >> 1;
-    if (base[mid] <= u) lo = mid; else hi = mid - 1;
-  }
-  c.it = load_item<QT>(p, lo);
-  const int rel = u - base[lo];
-  c.sub = rel / c.it.ntile;
-  c.j = rel - c.sub * c.it.ntile;
-}
-template <int QT>
-__device__ __forceinline__ void cursor_next(const Q4AttnParams& p, Cursor& c) {
-  if (++c.j < c.it.ntile) return;
-  c.j = 0;
-  if (++c.sub < c.it.groups * p.nkv) return;
-  c.sub = 0;
-  int i = c.it.seq;
-  do {
-    if (++i >= p.n) return;   // past the end: the caller's run is over
-    c.it = load_item<QT>(p, i);
-  } while (c.it.groups == 0);
-}
-
-// ---- fragments --------------------------------------------------------------
-// u16 holding two scale bytes -> f16 pair (byte << 7)
-__device__ __forceinline__ uint32_t scale_pair(uint32_t two) { return __byte_perm(two, 0, 0x1404) >> 1; }
-__device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t hfma2_u(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// nibble n of both halves of w -> (x / 16) pair, s the scale pair, ns = -1.5 s
-template <int N>
-__device__ __forceinline__ uint32_t dequant(uint32_t w, uint32_t s, uint32_t ns) {
-  const uint32_t t = N == 0 ? w << 6 : N == 1 ? w << 2 : N == 2 ? w >> 2 : w >> 6;
-  return hfma2_u((t & 0x03C003C0u) | 0x3C003C00u, s, ns);
-}
+// ---- fragments
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ float col_max(float v) {   // over the 8 lanes that share lane % 4
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
@@ -188,7 +81,7 @@ template <int NT, class SlotAt>
 __device__ __forceinline__ void merge_partials(const Q4AttnParams& p, int count, SlotAt slots, float* dst,
                                                const Item* out_item, int sub, int t, int nt) {
   constexpr int QT = QaCfg<NT>::QT;
-  const int G = p.nq / p.nkv;
+  const int G = p.by_g.d;
   for (int e = t; e < QT * 32; e += nt) {
     const int q = e >> 5, d = (e & 31) * 4;
     float M = -INFINITY;
@@ -206,11 +99,11 @@ __device__ __forceinline__ void merge_partials(const Q4AttnParams& p, int count,
       o[3] = fmaf(w, v.w, o[3]);
     }
     if (out_item) {
-      const int r = sub / p.nkv * QT + q, j = r / G;
+      const int grp = p.by_nkv.of(sub), r = grp * QT + q, j = p.by_g.of(r);
       if (j < out_item->rows) {
         const float f = l == 0.f ? 0.f : 16.f / l;
         for (int x = 0; x < 4; ++x) o[x] *= f;
-        store_out4(p, out_item->row0 + j, sub % p.nkv * G + r % G, d, o);
+        store_out4(p, out_item->row0 + j, (sub - grp * p.nkv) * G + r - j * G, d, o);
       }
     } else {
       *reinterpret_cast<float4*>(dst + q * 128 + d) = make_float4(o[0], o[1], o[2], o[3]);
@@ -235,7 +128,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
   __shared__ int last_run[2];               // runs (of the CTA's two borders) this CTA must finish
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int G = p.nq / p.nkv;
+  const int G = p.by_g.d;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < QA_WARPS * QA_STAGES; ++i) mbar_init(&bars[i], 1);
@@ -249,7 +142,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
     const int i = i0 + threadIdx.x;
     int v = 0;
     if (i < p.n) {
-      const Item it = load_item<QT>(p, i);
+      const Item it = load_item<QA_TILE, QT>(p, i);
       v = it.ntile * it.groups * p.nkv;
     }
     int x = v;
@@ -275,22 +168,23 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
   const int ctas = min((int)gridDim.x, total);   // CTAs with work
   const int cta = blockIdx.x;
   if (cta >= ctas) return;
-  const int c0 = (int)((long long)cta * total / ctas), c1 = (int)((long long)(cta + 1) * total / ctas);
-  const int u0 = c0 + (int)((long long)warp * (c1 - c0) / QA_WARPS);
-  const int u1 = c0 + (int)((long long)(warp + 1) * (c1 - c0) / QA_WARPS);
+  const Runs runs(total, ctas);
+  const int c0 = runs.start(cta), c1 = runs.start(cta + 1);
+  const Runs mine(c1 - c0, QA_WARPS);
+  const int u0 = c0 + mine.start(warp), u1 = c0 + mine.start(warp + 1);
 
   if (u0 < u1) {
     uint8_t* ring = smem + warp * QA_STAGES * QA_STAGE;
     uint64_t* bar = bars + warp * QA_STAGES;
     Cursor cur, ahead;
-    cursor_at<QT>(p, base, u0, cur);
+    cursor_at<QA_TILE, QT>(p, base, u0, cur);
     ahead = cur;
     // lane b < 4 looks after row block b of a tile: its page, then its copy
     auto page_of = [&](const Cursor& k) {
       const int pos = item_tile(k.it, k.j) * QA_TILE + (lane & 3) * kQ4Rows;
       int pg = -1;
       if (lane < 4 && pos < k.it.L) {
-        pg = __ldg(p.table + (size_t)k.it.seq * p.table_ld + pos / p.page_size);
+        pg = __ldg(p.table + (size_t)k.it.seq * p.table_ld + (pos >> p.page_shift));
         if (pg < 0 || pg >= p.num_pages) pg = -1;   // hidden, like a masked block
       }
       return pg;
@@ -304,15 +198,15 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
       __syncwarp();
       if (next_page >= 0) {
         const int pos = item_tile(ahead.it, ahead.j) * QA_TILE + lane * kQ4Rows;
-        const int head = ahead.sub % p.nkv, bpp = p.page_size / kQ4Rows;
+        const int head = ahead.sub - p.by_nkv.of(ahead.sub) * p.nkv, bits = p.page_shift - 4;   // 16-row blocks a page: 2^bits
         bulk_load(ring + s * QA_STAGE + lane * kQ4Block,
-                  p.pool + (((size_t)next_page * p.nkv + head) * bpp + pos / kQ4Rows % bpp) * kQ4Block, kQ4Block,
+                  p.pool + ((((size_t)next_page * p.nkv + head) << bits) + (pos / kQ4Rows & ((1 << bits) - 1))) * kQ4Block, kQ4Block,
                   &bar[s]);
       }
       loaded = (loaded & ~(15u << (4 * s))) | mask << (4 * s);
       ++fill;
       if (fill < fill_end) {
-        cursor_next<QT>(p, ahead);
+        cursor_next<QA_TILE, QT>(p, ahead);
         next_page = page_of(ahead);
       }
     };
@@ -330,15 +224,15 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
       if (fresh) {
         fresh = false;
         seg_first = u;
-        const int r0 = cur.sub / p.nkv * QT, head0 = cur.sub % p.nkv * G;
+        const int grp = p.by_nkv.of(cur.sub), r0 = grp * QT, head0 = (cur.sub - grp * p.nkv) * G;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const int r = r0 + nt * 8 + g, j = r / G;
+          const int r = r0 + nt * 8 + g, j = p.by_g.of(r);
           uint4 w[4] = {};
           if (j < cur.it.rows) {
             const uint4* src = reinterpret_cast<const uint4*>(
                 static_cast<const uint16_t*>(p.q) + (size_t)(cur.it.row0 + j) * p.q_row +
-                (size_t)(head0 + r % G) * p.q_head + 32 * c);
+                (size_t)(head0 + r - j * G) * p.q_head + 32 * c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = __ldg(src + i);
           }
@@ -371,7 +265,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
           qscale[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int jj = (r0 + nt * 8 + 2 * c + x) / G;
+            const int jj = p.by_g.of(r0 + nt * 8 + 2 * c + x);
             key_end[nt][x] = jj < cur.it.rows ? (p.causal ? cur.it.L - cur.it.rows + jj + 1 : cur.it.L) : 0;
             m[nt][x] = -INFINITY;
             l[nt][x] = 0.f;
@@ -405,8 +299,8 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
             for (int x = 0; x < 4; ++x) sc[b][nt][x] = 0.f;
           if (!(have >> b & 1)) continue;
           const uint8_t* blk = tile + b * kQ4Block;
-          const uint4 wa = *reinterpret_cast<const uint4*>(blk + g * 64 + c * 16);
-          const uint4 wb = *reinterpret_cast<const uint4*>(blk + 512 + g * 64 + c * 16);
+          const uint4 wa = *reinterpret_cast<const uint4*>(blk + q4_k_piece(g, c));
+          const uint4 wb = *reinterpret_cast<const uint4*>(blk + 512 + q4_k_piece(g, c));
           const uint32_t s2a = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4KS + g * 8 + 2 * c));
           const uint32_t s2b = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4KS + 64 + g * 8 + 2 * c));
           const uint32_t ka[4] = {wa.x, wa.y, wa.z, wa.w}, kb[4] = {wb.x, wb.y, wb.z, wb.w};
@@ -477,8 +371,8 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
             pb[nt][1] = transpose8x8(pack_f16x2(p2, p3));
           }
           const uint8_t* blk = tile + b * kQ4Block;
-          const uint4 wa = *reinterpret_cast<const uint4*>(blk + kQ4V + c * 128 + g * 16);
-          const uint4 wb = *reinterpret_cast<const uint4*>(blk + kQ4V + 512 + c * 128 + g * 16);
+          const uint4 wa = *reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(c, g));
+          const uint4 wb = *reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(c + 4, g));
           uint32_t sa = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4VS + g * 16 + 2 * c));
           uint32_t sb = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4VS + g * 16 + 8 + 2 * c));
           if (row0 + 16 * b + 16 > cur.it.L) {
@@ -511,7 +405,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
       const bool item_end = cur.j + 1 == cur.it.ntile;
       if (item_end || u == u1) {
         const bool whole = item_end && seg_first == item0;
-        const int G0 = cur.sub % p.nkv * G, r0 = cur.sub / p.nkv * QT;
+        const int grp = p.by_nkv.of(cur.sub), r0 = grp * QT, G0 = (cur.sub - grp * p.nkv) * G;
         // the first slot of a warp: a segment that began before the run or fills it
         const int slot = 2 * warp + (seg_first == u0 ? 0 : 1);
         float* part = p.part + ((size_t)cta * 2 * QA_WARPS + slot) * C::SLOT;
@@ -520,7 +414,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float sum = col_sum(l[nt][x]);
-            const int q = nt * 8 + 2 * c + x, r = r0 + q, j = r / G;
+            const int q = nt * 8 + 2 * c + x, r = r0 + q, j = p.by_g.of(r);
             const float f = whole ? (sum == 0.f ? 0.f : 16.f / sum) : 1.f;
 #pragma unroll
             for (int t = 0; t < 8; t += 2) {
@@ -528,7 +422,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
               if (!whole)
                 *reinterpret_cast<float4*>(part + q * 128 + 16 * g + 2 * t) = make_float4(v[0], v[1], v[2], v[3]);
               else if (j < cur.it.rows)
-                store_out4(p, cur.it.row0 + j, G0 + r % G, 16 * g + 2 * t, v);
+                store_out4(p, cur.it.row0 + j, G0 + r - j * G, 16 * g + 2 * t, v);
             }
             if (!whole && g == 0) {
               part[QT * 128 + q] = m[nt][x];
@@ -542,7 +436,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
         }
         fresh = true;
       }
-      if (u < u1) cursor_next<QT>(p, cur);
+      if (u < u1) cursor_next<QA_TILE, QT>(p, cur);
     }
   }
   __syncthreads();   // partials of the CTA's warps are written (and visible to its threads)
@@ -563,24 +457,24 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
         last = k;
       }
       if (run++ % QA_WARPS != warp) continue;
-      const Item it = load_item<QT>(p, slot_info[first][0]);
+      const Item it = load_item<QA_TILE, QT>(p, slot_info[first][0]);
       const int sub = slot_info[first][1];
       int list[2 * QA_WARPS], count = 0;
       for (int x = first; x <= last; ++x)
         if (slot_item[x] >= 0) list[count++] = x;
-      const float* mine = p.part + (size_t)cta * 2 * QA_WARPS * C::SLOT;
+      const float* parts = p.part + (size_t)cta * 2 * QA_WARPS * C::SLOT;
       const bool inside = item0 >= c0 && item0 + it.ntile <= c1;
       const int border = item0 < c0 ? 0 : 1;
       float* dst = cta_part + ((size_t)cta * 2 + border) * C::SLOT;
-      merge_partials<NT>(p, count, [&](int x) { return mine + (size_t)list[x] * C::SLOT; }, dst,
+      merge_partials<NT>(p, count, [&](int x) { return parts + (size_t)list[x] * C::SLOT; }, dst,
                          inside ? &it : nullptr, sub, lane, 32);
       if (!inside) {
         __threadfence();
         __syncwarp();
         if (lane == 0) {
           // CTAs that hold part of the item: counted at the one holding its first tile
-          const int from = (int)((((long long)item0 + 1) * ctas - 1) / total);
-          const int to = (int)((((long long)item0 + it.ntile) * ctas - 1) / total);
+          const int from = runs.of(item0);
+          const int to = runs.of(item0 + it.ntile - 1);
           if (atomicAdd(&p.counters[from], 1) == to - from) {
             p.counters[from] = 0;   // for the next call
             __threadfence();
@@ -596,9 +490,9 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
     if (first < 0) continue;
     __threadfence();
     const int item0 = slot_item[first], sub = slot_info[first][1];
-    const Item it = load_item<QT>(p, slot_info[first][0]);
-    const int from = (int)((((long long)item0 + 1) * ctas - 1) / total);
-    const int to = (int)((((long long)item0 + it.ntile) * ctas - 1) / total);
+    const Item it = load_item<QA_TILE, QT>(p, slot_info[first][0]);
+    const int from = runs.of(item0);
+    const int to = runs.of(item0 + it.ntile - 1);
     // the first CTA holds the item's start, so its part is at its right border
     // unless the item also began before that CTA's range, which it did not
     merge_partials<NT>(p, to - from + 1,

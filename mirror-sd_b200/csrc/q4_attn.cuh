@@ -1,0 +1,132 @@
+// Device code shared by the two attention kernels over the 4-bit cache
+// (q4_attention.cu, q4_attention_tc.cu): which cached rows a request's queries
+// see, the flat order of the work, and codes to f16.
+#pragma once
+#include "q4.cuh"
+
+namespace dfl {
+
+// ---- which cached rows a request's queries see ------------------------------
+// Query row j of `rows` of a request with L cached rows ends at key
+// e = causal ? L - rows + j + 1 : L and sees k < e with k < sink or
+// k >= e - window (window 0: all of them).  The request as a whole touches
+// tiles [0, a) (sink) and [b, c).
+struct TileSpan {
+  int a, b, c;   // count = a + c - b
+};
+template <int TILE>
+__device__ __forceinline__ TileSpan tile_span(const Q4AttnParams& p, int L, int rows) {
+  TileSpan t{0, 0, (L + TILE - 1) / TILE};
+  if (p.window > 0) {
+    const int lo = max((p.causal ? L - rows + 1 : L) - p.window, 0);
+    t.a = (min(p.sink, L) + TILE - 1) / TILE;
+    t.b = max(min(lo, L) / TILE, t.a);
+  }
+  return t;
+}
+
+struct Item {          // one (request, query group, kv head)
+  int seq, L, rows, row0;   // cached rows, query rows, first packed query row
+  TileSpan span;
+  int ntile;           // >= 1: a request without visible keys still writes zeros
+  int groups;          // query groups of the request
+};
+
+__device__ __forceinline__ int seq_rows(const Q4AttnParams& p, int i, int* row0) {
+  int a = i * p.max_rows, b = a + p.max_rows;
+  if (p.starts) {
+    a = __ldg(p.starts + i);
+    b = __ldg(p.starts + i + 1);
+  }
+  // device data the host has not seen: stay inside the query array
+  a = min(max(a, 0), p.T);
+  b = min(max(b, a), p.T);
+  *row0 = a;
+  return min(b - a, p.max_rows);
+}
+template <int TILE, int QT>
+__device__ __forceinline__ Item load_item(const Q4AttnParams& p, int i) {
+  Item it;
+  it.seq = i;
+  it.rows = seq_rows(p, i, &it.row0);
+  it.L = min(max(__ldg(p.lens + i), 0), p.max_pages << p.page_shift);
+  it.span = tile_span<TILE>(p, it.L, it.rows);
+  it.ntile = max(it.span.a + it.span.c - it.span.b, 1);
+  it.groups = (it.rows * p.by_g.d + QT - 1) / QT;
+  return it;
+}
+__device__ __forceinline__ int item_tile(const Item& it, int j) {
+  return j < it.span.a ? j : j - it.span.a + it.span.b;
+}
+
+// The tiles of all items in one row, cut into `parts` runs whose lengths differ
+// by at most one.
+struct Runs {
+  int each, longer;   // run length, and how many runs have one more
+  __device__ __forceinline__ Runs(int total, int parts) : each(total / parts), longer(total - total / parts * parts) {}
+  __device__ __forceinline__ int start(int i) const { return i * each + min(i, longer); }
+  __device__ __forceinline__ int of(int u) const {   // the run that holds tile u
+    const int head = longer * (each + 1);
+    return u < head ? u / (each + 1) : longer + (u - head) / each;
+  }
+};
+
+// a place in the row of tiles
+struct Cursor {
+  Item it;
+  int sub;    // query group * NKV + kv head
+  int j;      // tile of the item
+};
+
+template <int TILE, int QT>
+__device__ __forceinline__ void cursor_at(const Q4AttnParams& p, const int* base, int u, Cursor& c) {
+  int lo = 0, hi = p.n - 1;
+  while (lo < hi) {   // last request whose first tile is <= u
+    const int mid = (lo + hi + 1) >> 1;
+    if (base[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  c.it = load_item<TILE, QT>(p, lo);
+  const int rel = u - base[lo];
+  c.sub = rel / c.it.ntile;
+  c.j = rel - c.sub * c.it.ntile;
+}
+template <int TILE, int QT>
+__device__ __forceinline__ void cursor_next(const Q4AttnParams& p, Cursor& c) {
+  if (++c.j < c.it.ntile) return;
+  c.j = 0;
+  if (++c.sub < c.it.groups * p.nkv) return;
+  c.sub = 0;
+  int i = c.it.seq;
+#pragma unroll 1
+  do {
+    if (++i >= p.n) return;   // past the end: the caller's run is over
+    c.it = load_item<TILE, QT>(p, i);
+  } while (c.it.groups == 0);
+}
+
+// ---- fragments --------------------------------------------------------------
+// u16 holding two scale bytes -> f16 pair (byte << 7)
+__device__ __forceinline__ uint32_t scale_pair(uint32_t two) { return __byte_perm(two, 0, 0x1404) >> 1; }
+__device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t hfma2_u(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// nibble n of both halves of w -> (x / 16) pair, s the scale pair, ns = -1.5 s
+template <int N>
+__device__ __forceinline__ uint32_t dequant(uint32_t w, uint32_t s, uint32_t ns) {
+  const uint32_t t = N == 0 ? w << 6 : N == 1 ? w << 2 : N == 2 ? w >> 2 : w >> 6;
+  return hfma2_u((t & 0x03C003C0u) | 0x3C003C00u, s, ns);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace dfl

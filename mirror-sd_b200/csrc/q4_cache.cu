@@ -86,13 +86,13 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const Q4AppendParams p) 
 #pragma unroll
       for (int n = 0; n < 4; ++n) w[j] |= u[8 * j + 2 * n] << (4 * n) | u[8 * j + 2 * n + 1] << (16 + 4 * n);
     }
-    *reinterpret_cast<uint2*>(blk + rr * 64 + g * 8) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8) = make_uint2(w[0], w[1]);
     blk[kQ4KS + rr * 8 + g] = (uint8_t)code;
   } else {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const uint32_t hw = u[4 * w] | u[4 * w + 1] << 4 | u[4 * w + 2] << 8 | u[4 * w + 3] << 12;
-      *reinterpret_cast<uint16_t*>(blk + kQ4V + ((rr >> 1) * 8 + g) * 16 + w * 4 + (rr & 1) * 2) = (uint16_t)hw;
+      *reinterpret_cast<uint16_t*>(blk + kQ4V + q4_v_piece(rr >> 1, g) + w * 4 + (rr & 1) * 2) = (uint16_t)hw;
     }
     blk[kQ4VS + g * 16 + rr] = (uint8_t)code;
   }
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
     const int rr = slot % kQ4Rows;
     uint32_t u[16], code;
     if (which == 0) {
-      const uint2 w = *reinterpret_cast<const uint2*>(blk + rr * 64 + g * 8);
+      const uint2 w = *reinterpret_cast<const uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8);
 #pragma unroll
       for (int i = 0; i < 16; ++i) u[i] = ((i < 8 ? w.x : w.y) >> (16 * (i & 1) + 4 * ((i & 7) >> 1))) & 15;
       code = blk[kQ4KS + rr * 8 + g];
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint32_t hw =
-            *reinterpret_cast<const uint16_t*>(blk + kQ4V + ((rr >> 1) * 8 + g) * 16 + w * 4 + (rr & 1) * 2);
+            *reinterpret_cast<const uint16_t*>(blk + kQ4V + q4_v_piece(rr >> 1, g) + w * 4 + (rr & 1) * 2);
 #pragma unroll
         for (int n = 0; n < 4; ++n) u[4 * w + n] = (hw >> (4 * n)) & 15;
       }

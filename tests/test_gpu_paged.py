@@ -211,8 +211,10 @@ class Case:
     def check(self, pkg, out=None, scale=None, **kw):
         mine = out is None
         if mine:
+            status = torch.zeros(1, dtype=i32).cuda()
             out = pkg.q4_attention(self.q, self.pool, self.pg.dev("table"), self.pg.dev("lens"), starts=self.starts,
-                                   max_rows=max(self.rows + [1]), scale=scale, **kw)
+                                   max_rows=max(self.rows + [1]), scale=scale, status=status, **kw)
+            assert status.tolist() == [0]
         ref, bound = U.attention(self.q, self.k, self.v, self.rows, scale or 128 ** -0.5, **kw)
         err = (out.double().cpu() - ref).abs()
         tol = U.attention_tolerance(ref, bound, self.q.dtype)
