@@ -29,18 +29,17 @@
 // makes the P^T fragment.  P is rounded to f16 (2^-12 relative, the operand
 // type), sums and statistics stay fp32.
 //
-// The running maximum is only raised when a score passes it by 2^8 (then O
-// and the sum are rescaled), as P below 256 loses nothing in f16.
+// A column's reference (what its scores are measured against) only moves when a
+// score passes it by 2^8, then O and the sum are rescaled: P below 256 loses
+// nothing in f16.
 #include "q4_attn.cuh"
 
 namespace dfl {
 
-constexpr int QA_WARPS = 8;
-constexpr int QA_THREADS = QA_WARPS * 32;
 constexpr int QA_TILE = 64;                      // cached rows of a tile
 constexpr int QA_STAGE = QA_TILE / kQ4Rows * kQ4Block;
-constexpr int QA_STAGES = 3;
 constexpr float QA_RAISE = 8.f;
+constexpr float QA_UNSET = 1e30f;                // -reference of a column that has seen no key
 
 // ---- fragments
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -62,8 +61,10 @@ __device__ __forceinline__ float col_sum(float v) {
 template <int NT>
 struct QaCfg {
   static constexpr int QT = 8 * NT;
+  // as many warps as the registers allow, the rest of shared memory for tiles
+  static constexpr int WARPS = NT == 1 ? 12 : 8, STAGES = NT == 1 ? 2 : 3, THREADS = 32 * WARPS;
   static constexpr int SLOT = QT * 130;   // floats of a partial: O [QT][128], m [QT], l [QT]
-  static constexpr int RING = QA_WARPS * QA_STAGES * QA_STAGE;
+  static constexpr int RING = WARPS * STAGES * QA_STAGE;
 };
 
 // write 4 consecutive output values of one query row
@@ -74,71 +75,128 @@ __device__ __forceinline__ void store_out4(const Q4AttnParams& p, int row, int h
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + off) = w;
 }
 
-// Merge `count` partials (slot k at slots(k)) of one item and write either the
-// item's output rows (out_item != nullptr) or another partial at dst.  `t` of
-// `nt` threads; every thread takes whole groups of 4 channels of a query row.
-template <int NT, class SlotAt>
-__device__ __forceinline__ void merge_partials(const Q4AttnParams& p, int count, SlotAt slots, float* dst,
-                                               const Item* out_item, int sub, int t, int nt) {
-  constexpr int QT = QaCfg<NT>::QT;
-  const int G = p.by_g.d;
-  for (int e = t; e < QT * 32; e += nt) {
-    const int q = e >> 5, d = (e & 31) * 4;
-    float M = -INFINITY;
-    for (int k = 0; k < count; ++k) M = fmaxf(M, __ldcg(slots(k) + QT * 128 + q));
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < count; ++k) {
-      const float* s = slots(k);
-      const float m = __ldcg(s + QT * 128 + q);
-      const float w = m == -INFINITY ? 0.f : exp2_fast(m - M);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(s + q * 128 + d));
-      l = fmaf(w, __ldcg(s + QT * 129 + q), l);
-      o[0] = fmaf(w, v.x, o[0]);
-      o[1] = fmaf(w, v.y, o[1]);
-      o[2] = fmaf(w, v.z, o[2]);
-      o[3] = fmaf(w, v.w, o[3]);
+// A warp merges the partials of one item that the slots of `mask` hold (slot k
+// at parts + k * SLOT), all queries at once: 8 (16) loads of a partial's O are
+// on their way together.  Writes the item's output rows (finish) or one partial
+// at dst.
+template <int NT>
+__device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask, const float* parts, float* dst,
+                                            const Item& it, int sub, bool finish, int lane) {
+  constexpr int QT = QaCfg<NT>::QT, SLOT = QaCfg<NT>::SLOT;
+  const int q = lane & (QT - 1);
+  float M = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (uint32_t m = mask; m; m &= m - 1) M = fmaxf(M, __ldcg(parts + (__ffs(m) - 1) * SLOT + QT * 128 + q));
+  float4 o[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (uint32_t m = mask; m; m &= m - 1) {
+    const float* s = parts + (__ffs(m) - 1) * SLOT;
+    const float mk = __ldcg(s + QT * 128 + q), lk = __ldcg(s + QT * 129 + q);
+    float4 v[QT];
+#pragma unroll
+    for (int i = 0; i < QT; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(s + i * 128 + 4 * lane));
+    const float w = mk == -INFINITY ? 0.f : exp2_fast(mk - M);
+    l = fmaf(w, lk, l);
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      o[i].x = fmaf(wi, v[i].x, o[i].x);
+      o[i].y = fmaf(wi, v[i].y, o[i].y);
+      o[i].z = fmaf(wi, v[i].z, o[i].z);
+      o[i].w = fmaf(wi, v[i].w, o[i].w);
     }
-    if (out_item) {
-      const int grp = p.by_nkv.of(sub), r = grp * QT + q, j = p.by_g.of(r);
-      if (j < out_item->rows) {
-        const float f = l == 0.f ? 0.f : 16.f / l;
-        for (int x = 0; x < 4; ++x) o[x] *= f;
-        store_out4(p, out_item->row0 + j, (sub - grp * p.nkv) * G + r - j * G, d, o);
-      }
+  }
+  if (!finish && lane < QT) {
+    dst[QT * 128 + q] = M;
+    dst[QT * 129 + q] = l;
+  }
+  const float fin = l == 0.f ? 0.f : 16.f / l;
+  const int grp = p.by_nkv.of(sub);
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    if (finish) {
+      const float f = __shfl_sync(0xffffffffu, fin, i);
+      const int r = grp * QT + i, j = p.by_g.of(r);
+      const float v[4] = {o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f};
+      if (j < it.rows) store_out4(p, it.row0 + j, (sub - grp * p.nkv) * p.by_g.d + r - j * p.by_g.d, 4 * lane, v);
     } else {
-      *reinterpret_cast<float4*>(dst + q * 128 + d) = make_float4(o[0], o[1], o[2], o[3]);
-      if (d == 0) {
-        dst[QT * 128 + q] = M;
-        dst[QT * 129 + q] = l;
-      }
+      *reinterpret_cast<float4*>(dst + i * 128 + 4 * lane) = o[i];
     }
   }
 }
 
+// A warp merges query q of an item from `count` CTAs' partials (slots(k)).
+template <int NT, class SlotAt>
+__device__ __forceinline__ void merge_query(const Q4AttnParams& p, int count, SlotAt slots, const Item& it, int sub, int q,
+                                            int lane) {
+  constexpr int QT = QaCfg<NT>::QT;
+  const int grp = p.by_nkv.of(sub), r = grp * QT + q, j = p.by_g.of(r);
+  if (j >= it.rows) return;
+  float M = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (int k = lane; k < count; k += 32) M = fmaxf(M, __ldcg(slots(k) + QT * 128 + q));
+  M = warp_max(M);
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int k0 = 0; k0 < count; k0 += 32) {
+    float w = 0.f;
+    if (k0 + lane < count) {
+      const float m = __ldcg(slots(k0 + lane) + QT * 128 + q);
+      w = m == -INFINITY ? 0.f : exp2_fast(m - M);
+      l = fmaf(w, __ldcg(slots(k0 + lane) + QT * 129 + q), l);
+    }
+    const int n = min(count - k0, 32);
+#pragma unroll 1
+    for (int k = 0; k < n; k += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)   // (past the end: the last one again, with weight 0)
+        v[i] = __ldcg(reinterpret_cast<const float4*>(slots(k0 + min(k + i, n - 1)) + q * 128 + 4 * lane));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, k + i);
+        if (k + i < n) {
+          o[0] = fmaf(wi, v[i].x, o[0]);
+          o[1] = fmaf(wi, v[i].y, o[1]);
+          o[2] = fmaf(wi, v[i].z, o[2]);
+          o[3] = fmaf(wi, v[i].w, o[3]);
+        }
+      }
+    }
+  }
+  l = warp_sum(l);
+  const float f = l == 0.f ? 0.f : 16.f / l;
+  const float v[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+  store_out4(p, it.row0 + j, (sub - grp * p.nkv) * p.by_g.d + r - j * p.by_g.d, 4 * lane, v);
+}
+
 template <int NT>
-__global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnParams p) {
+__global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4AttnParams p) {
   using C = QaCfg<NT>;
   constexpr int QT = C::QT;
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING);          // [warp][stage]
-  int* base = reinterpret_cast<int*>(bars + QA_WARPS * QA_STAGES);       // [n + 1] first tile of each request
-  __shared__ int wtot[QA_WARPS];
-  __shared__ int slot_item[2 * QA_WARPS];   // unit at which the partial's item starts, or -1
-  __shared__ int slot_info[2 * QA_WARPS][2];   // request, sub
+  int* base = reinterpret_cast<int*>(bars + C::WARPS * C::STAGES);       // [n + 1] first tile of each request
+  __shared__ int wtot[C::WARPS];
+  __shared__ int slot_item[2 * C::WARPS];   // unit at which the partial's item starts, or -1
+  __shared__ Item slot_info[2 * C::WARPS];
+  __shared__ int slot_sub[2 * C::WARPS];
   __shared__ int last_run[2];               // runs (of the CTA's two borders) this CTA must finish
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int G = p.by_g.d;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < QA_WARPS * QA_STAGES; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < C::WARPS * C::STAGES; ++i) mbar_init(&bars[i], 1);
     fence_mbar_init();
     last_run[0] = last_run[1] = -1;
   }
-  if (threadIdx.x < 2 * QA_WARPS) slot_item[threadIdx.x] = -1;
-  // tiles of every request, added up (kPagedMaxSeqs / QA_THREADS passes at most)
+  if (threadIdx.x < 2 * C::WARPS) slot_item[threadIdx.x] = -1;
+  // tiles of every request, added up (kPagedMaxSeqs / C::THREADS passes at most)
   int total = 0;
-  for (int i0 = 0; i0 < p.n; i0 += QA_THREADS) {
+  for (int i0 = 0; i0 < p.n; i0 += C::THREADS) {
     const int i = i0 + threadIdx.x;
     int v = 0;
     if (i < p.n) {
@@ -156,7 +214,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
     __syncthreads();
     int before = total;
 #pragma unroll
-    for (int w = 0; w < QA_WARPS; ++w) {
+    for (int w = 0; w < C::WARPS; ++w) {
       if (w < warp) before += wtot[w];
       total += wtot[w];
     }
@@ -170,12 +228,12 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
   if (cta >= ctas) return;
   const Runs runs(total, ctas);
   const int c0 = runs.start(cta), c1 = runs.start(cta + 1);
-  const Runs mine(c1 - c0, QA_WARPS);
+  const Runs mine(c1 - c0, C::WARPS);
   const int u0 = c0 + mine.start(warp), u1 = c0 + mine.start(warp + 1);
 
   if (u0 < u1) {
-    uint8_t* ring = smem + warp * QA_STAGES * QA_STAGE;
-    uint64_t* bar = bars + warp * QA_STAGES;
+    uint8_t* ring = smem + warp * C::STAGES * QA_STAGE;
+    uint64_t* bar = bars + warp * C::STAGES;
     Cursor cur, ahead;
     cursor_at<QA_TILE, QT>(p, base, u0, cur);
     ahead = cur;
@@ -210,15 +268,17 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
         next_page = page_of(ahead);
       }
     };
-    for (int s = 0; s < QA_STAGES && fill < fill_end; ++s) issue(s);
+#pragma unroll 1
+    for (int s = 0; s < C::STAGES && fill < fill_end; ++s) issue(s);
 
     uint32_t qf[NT][16];
-    float qscale[NT][2], m[NT][2], l[NT][2], o[8][NT][4];
+    float qscale[NT][2], negm[NT][2], l[NT][2], o[8][NT][4];
     int key_end[NT][2];
     int u = u0, stage = 0;
     uint32_t phase = 0;
     bool fresh = true, alive = true;
     int seg_first = u0;   // first unit of the running segment
+#pragma unroll 1
     while (u < u1) {
       const int item0 = u - cur.j;   // the item's first unit
       if (fresh) {
@@ -267,7 +327,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
           for (int x = 0; x < 2; ++x) {
             const int jj = p.by_g.of(r0 + nt * 8 + 2 * c + x);
             key_end[nt][x] = jj < cur.it.rows ? (p.causal ? cur.it.L - cur.it.rows + jj + 1 : cur.it.L) : 0;
-            m[nt][x] = -INFINITY;
+            negm[nt][x] = QA_UNSET;
             l[nt][x] = 0.f;
           }
         }
@@ -290,116 +350,138 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
       if (have && alive) {
         const uint8_t* tile = ring + stage * QA_STAGE;
         const int row0 = item_tile(cur.it, cur.j) * QA_TILE;
-        float sc[4][NT][4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) sc[b][nt][x] = 0.f;
-          if (!(have >> b & 1)) continue;
-          const uint8_t* blk = tile + b * kQ4Block;
-          const uint4 wa = *reinterpret_cast<const uint4*>(blk + q4_k_piece(g, c));
-          const uint4 wb = *reinterpret_cast<const uint4*>(blk + 512 + q4_k_piece(g, c));
-          const uint32_t s2a = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4KS + g * 8 + 2 * c));
-          const uint32_t s2b = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4KS + 64 + g * 8 + 2 * c));
-          const uint32_t ka[4] = {wa.x, wa.y, wa.z, wa.w}, kb[4] = {wb.x, wb.y, wb.z, wb.w};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {   // channels 32c + 8w .. + 7: group 2c + w / 2
-            const uint32_t sa = __byte_perm(s2a, 0, w < 2 ? 0x1010 : 0x3232);
-            const uint32_t sb = __byte_perm(s2b, 0, w < 2 ? 0x1010 : 0x3232);
-            const uint32_t na = hmul2_u(sa, 0xBE00BE00u), nb = hmul2_u(sb, 0xBE00BE00u);   // -1.5 s
-            const uint32_t a0 = dequant<0>(ka[w], sa, na), a2 = dequant<1>(ka[w], sa, na);
-            const uint32_t a1 = dequant<0>(kb[w], sb, nb), a3 = dequant<1>(kb[w], sb, nb);
-            const uint32_t e0 = dequant<2>(ka[w], sa, na), e2 = dequant<3>(ka[w], sa, na);
-            const uint32_t e1 = dequant<2>(kb[w], sb, nb), e3 = dequant<3>(kb[w], sb, nb);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_f16_16816(sc[b][nt], a0, a1, a2, a3, qf[nt][4 * w], qf[nt][4 * w + 1]);
-              mma_f16_16816(sc[b][nt], e0, e1, e2, e3, qf[nt][4 * w + 2], qf[nt][4 * w + 3]);
-            }
-          }
-        }
-        // base-2 scores; hidden keys get -inf
         const bool all_seen = have == 15u && row0 + QA_TILE <= (p.causal ? cur.it.L - cur.it.rows + 1 : cur.it.L) &&
                               (p.window == 0 || row0 + QA_TILE <= p.sink || row0 >= cur.it.L - p.window);
+        // Two row blocks at a time: one leaves the pipes idle between dependent
+        // steps, and the whole tile unrolled outgrows the instruction cache.
+#pragma unroll 1
+        for (int b0 = 0; b0 < 4; b0 += 2) {
+          if (!(have >> b0 & 3)) continue;
+          float sc[2][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float top[2] = {-INFINITY, -INFINITY};
+          for (int i = 0; i < 2; ++i) {
+            const uint8_t* blk = tile + (b0 + i) * kQ4Block;
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              float y = sc[b][nt][x] * qscale[nt][x & 1];
-              if (!all_seen) {
-                const int key = row0 + 16 * b + g + 8 * (x >> 1), end = key_end[nt][x & 1];
-                const bool seen = (have >> b & 1) && key < end &&
-                                  (p.window == 0 || key < p.sink || key >= end - p.window);
-                if (!seen) y = -INFINITY;
+              for (int x = 0; x < 4; ++x) sc[i][nt][x] = 0.f;
+            const uint4 wa = *reinterpret_cast<const uint4*>(blk + q4_k_piece(g, c));
+            const uint4 wb = *reinterpret_cast<const uint4*>(blk + 512 + q4_k_piece(g, c));
+            const uint32_t s2a = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4KS + g * 8 + 2 * c));
+            const uint32_t s2b = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4KS + 64 + g * 8 + 2 * c));
+            const uint32_t ka[4] = {wa.x, wa.y, wa.z, wa.w}, kb[4] = {wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {   // channels 32c + 8w .. + 7: group 2c + w / 2
+              const uint32_t sa = __byte_perm(s2a, 0, w < 2 ? 0x1010 : 0x3232);
+              const uint32_t sb = __byte_perm(s2b, 0, w < 2 ? 0x1010 : 0x3232);
+              const uint32_t na = hmul2_u(sa, 0xBE00BE00u), nb = hmul2_u(sb, 0xBE00BE00u);   // -1.5 s
+              const uint32_t a0 = dequant<0>(ka[w], sa, na), a2 = dequant<1>(ka[w], sa, na);
+              const uint32_t a1 = dequant<0>(kb[w], sb, nb), a3 = dequant<1>(kb[w], sb, nb);
+              const uint32_t e0 = dequant<2>(ka[w], sa, na), e2 = dequant<3>(ka[w], sa, na);
+              const uint32_t e1 = dequant<2>(kb[w], sb, nb), e3 = dequant<3>(kb[w], sb, nb);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_f16_16816(sc[i][nt], a0, a1, a2, a3, qf[nt][4 * w], qf[nt][4 * w + 1]);
+                mma_f16_16816(sc[i][nt], e0, e1, e2, e3, qf[nt][4 * w + 2], qf[nt][4 * w + 3]);
               }
-              sc[b][nt][x] = y;
-              top[x & 1] = fmaxf(top[x & 1], y);
             }
+          }
+          // Base-2 scores less the columns' references (negm = 1e30 until a column
+          // has seen a key); hidden keys get -inf.  Where one passes 2^8 the
+          // references move first.
+          float y[2][NT][4];
+          auto scores = [&]() {
+            float top = -INFINITY;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            top[x] = col_max(top[x]);
-            if (top[x] > m[nt][x] + QA_RAISE) {   // also the first visible key (m = -inf)
-              const float f = exp2_fast(m[nt][x] - top[x]);
-              m[nt][x] = top[x];
-              l[nt][x] *= f;
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int t = 0; t < 8; ++t) {
-                o[t][nt][x] *= f;
-                o[t][nt][2 + x] *= f;
+              for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) y[i][nt][x] = fmaf(sc[i][nt][x], qscale[nt][x & 1], negm[nt][x & 1]);
+                if (!all_seen) {
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) {
+                    const int key = row0 + 16 * (b0 + i) + g + 8 * (x >> 1), end = key_end[nt][x & 1];
+                    const bool seen = (have >> (b0 + i) & 1) & (key < end) &
+                                      ((p.window == 0) | (key < p.sink) | (key >= end - p.window));
+                    y[i][nt][x] = seen ? y[i][nt][x] : -INFINITY;
+                  }
+                }
+                top = fmaxf(fmaxf(fmaxf(y[i][nt][0], y[i][nt][1]), fmaxf(y[i][nt][2], y[i][nt][3])), top);
               }
-            }
-          }
-        }
+            return top;
+          };
+          if (__any_sync(0xffffffffu, scores() > QA_RAISE)) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (!(have >> b & 1)) continue;
-          uint32_t pb[NT][2];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            // a column without a visible key so far: every score is -inf, P = 0
-            const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-            const float p0 = exp2_fast(sc[b][nt][0] - m0), p1 = exp2_fast(sc[b][nt][1] - m1);
-            const float p2 = exp2_fast(sc[b][nt][2] - m0), p3 = exp2_fast(sc[b][nt][3] - m1);
-            l[nt][0] += p0 + p2;
-            l[nt][1] += p1 + p3;
-            pb[nt][0] = transpose8x8(pack_f16x2(p0, p1));
-            pb[nt][1] = transpose8x8(pack_f16x2(p2, p3));
-          }
-          const uint8_t* blk = tile + b * kQ4Block;
-          const uint4 wa = *reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(c, g));
-          const uint4 wb = *reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(c + 4, g));
-          uint32_t sa = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4VS + g * 16 + 2 * c));
-          uint32_t sb = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4VS + g * 16 + 8 + 2 * c));
-          if (row0 + 16 * b + 16 > cur.it.L) {
-            // rows past the end may never have been written: their scale could be any bits
-            const int left = cur.it.L - (row0 + 16 * b);
-            sa &= (2 * c < left ? 0xffffu : 0u) | (2 * c + 1 < left ? 0xffff0000u : 0u);
-            sb &= (2 * c + 8 < left ? 0xffffu : 0u) | (2 * c + 9 < left ? 0xffff0000u : 0u);
-          }
-          const uint32_t na = hmul2_u(sa, 0xBE00BE00u), nb = hmul2_u(sb, 0xBE00BE00u);
-          const uint32_t va[4] = {wa.x, wa.y, wa.z, wa.w}, vb[4] = {wb.x, wb.y, wb.z, wb.w};
+              for (int x = 0; x < 2; ++x) {
+                // the column's largest score, rounded up so that none lies above its reference
+                float top = -INFINITY;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {   // channels 16g + 4w .. + 3: tiles 2w and 2w + 1
-            const uint32_t a0 = dequant<0>(va[w], sa, na), a1 = dequant<1>(va[w], sa, na);
-            const uint32_t a2 = dequant<0>(vb[w], sb, nb), a3 = dequant<1>(vb[w], sb, nb);
-            const uint32_t e0 = dequant<2>(va[w], sa, na), e1 = dequant<3>(va[w], sa, na);
-            const uint32_t e2 = dequant<2>(vb[w], sb, nb), e3 = dequant<3>(vb[w], sb, nb);
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                  for (int h = 0; h < 4; h += 2)
+                    if (y[i][nt][h + x] != -INFINITY) top = fmaxf(top, __fmul_ru(sc[i][nt][h + x], qscale[nt][x]));
+                top = col_max(top);
+                const bool up = top > QA_RAISE - negm[nt][x];
+                const float f = up ? exp2_fast(-negm[nt][x] - top) : 1.f;
+                negm[nt][x] = up ? -top : negm[nt][x];
+                l[nt][x] *= f;
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                  o[t][nt][x] *= f;
+                  o[t][nt][2 + x] *= f;
+                }
+              }
+            scores();
+          }
+          uint32_t pb[2][NT][2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_f16_16816(o[2 * w][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-              mma_f16_16816(o[2 * w + 1][nt], e0, e1, e2, e3, pb[nt][0], pb[nt][1]);
+              const float p0 = exp2_fast(y[i][nt][0]), p1 = exp2_fast(y[i][nt][1]);
+              const float p2 = exp2_fast(y[i][nt][2]), p3 = exp2_fast(y[i][nt][3]);
+              l[nt][0] += p0 + p2;
+              l[nt][1] += p1 + p3;
+              pb[i][nt][0] = transpose8x8(pack_f16x2(p0, p1));
+              pb[i][nt][1] = transpose8x8(pack_f16x2(p2, p3));
+            }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint8_t* blk = tile + (b0 + i) * kQ4Block;
+            const uint4 wa = *reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(c, g));
+            const uint4 wb = *reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(c + 4, g));
+            uint32_t sa = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4VS + g * 16 + 2 * c));
+            uint32_t sb = scale_pair(*reinterpret_cast<const uint16_t*>(blk + kQ4VS + g * 16 + 8 + 2 * c));
+            if (!all_seen) {
+              // rows that were not copied, or lie past the end and may never have
+              // been written: any bits, so their scale becomes 0
+              const int left = (have >> (b0 + i) & 1) ? cur.it.L - (row0 + 16 * (b0 + i)) : 0;
+              sa &= (2 * c < left ? 0xffffu : 0u) | (2 * c + 1 < left ? 0xffff0000u : 0u);
+              sb &= (2 * c + 8 < left ? 0xffffu : 0u) | (2 * c + 9 < left ? 0xffff0000u : 0u);
+            }
+            const uint32_t na = hmul2_u(sa, 0xBE00BE00u), nb = hmul2_u(sb, 0xBE00BE00u);
+            const uint32_t va[4] = {wa.x, wa.y, wa.z, wa.w}, vb[4] = {wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {   // channels 16g + 4w .. + 3: tiles 2w and 2w + 1
+              const uint32_t a0 = dequant<0>(va[w], sa, na), a1 = dequant<1>(va[w], sa, na);
+              const uint32_t a2 = dequant<0>(vb[w], sb, nb), a3 = dequant<1>(vb[w], sb, nb);
+              const uint32_t e0 = dequant<2>(va[w], sa, na), e1 = dequant<3>(va[w], sa, na);
+              const uint32_t e2 = dequant<2>(vb[w], sb, nb), e3 = dequant<3>(vb[w], sb, nb);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_f16_16816(o[2 * w][nt], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+                mma_f16_16816(o[2 * w + 1][nt], e0, e1, e2, e3, pb[i][nt][0], pb[i][nt][1]);
+              }
             }
           }
         }
       }
       __syncwarp();   // every lane has read the stage
       if (fill < fill_end) issue(stage);
-      stage = stage + 1 == QA_STAGES ? 0 : stage + 1;
+      stage = stage + 1 == C::STAGES ? 0 : stage + 1;
       ++u;
 
       const bool item_end = cur.j + 1 == cur.it.ntile;
@@ -408,7 +490,7 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
         const int grp = p.by_nkv.of(cur.sub), r0 = grp * QT, G0 = (cur.sub - grp * p.nkv) * G;
         // the first slot of a warp: a segment that began before the run or fills it
         const int slot = 2 * warp + (seg_first == u0 ? 0 : 1);
-        float* part = p.part + ((size_t)cta * 2 * QA_WARPS + slot) * C::SLOT;
+        float* part = p.part + ((size_t)cta * 2 * C::WARPS + slot) * C::SLOT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -425,14 +507,14 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
                 store_out4(p, cur.it.row0 + j, G0 + r - j * G, 16 * g + 2 * t, v);
             }
             if (!whole && g == 0) {
-              part[QT * 128 + q] = m[nt][x];
+              part[QT * 128 + q] = negm[nt][x] == QA_UNSET ? -INFINITY : -negm[nt][x];
               part[QT * 129 + q] = sum;
             }
           }
         if (!whole && lane == 0) {
           slot_item[slot] = item0;
-          slot_info[slot][0] = cur.it.seq;
-          slot_info[slot][1] = cur.sub;
+          slot_info[slot] = cur.it;
+          slot_sub[slot] = cur.sub;
         }
         fresh = true;
       }
@@ -441,33 +523,24 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
   }
   __syncthreads();   // partials of the CTA's warps are written (and visible to its threads)
 
-  // Runs of slots that belong to one item, in order; run k goes to warp k % 8.
+  // Runs of slots that belong to one item, in order; the runs go to the warps in turn.
   // An item inside the CTA's range ends here; one that reaches past a border
   // leaves one partial of the CTA and the last CTA to arrive finishes it.
-  float* cta_part = p.part + (size_t)gridDim.x * 2 * QA_WARPS * C::SLOT;
+  float* cta_part = p.part + (size_t)gridDim.x * 2 * C::WARPS * C::SLOT;
   {
     int run = 0, k = 0;
-    while (k < 2 * QA_WARPS) {
+    while (k < 2 * C::WARPS) {
       if (slot_item[k] < 0) { ++k; continue; }
       const int item0 = slot_item[k], first = k;
-      int last = k;
-      for (++k; k < 2 * QA_WARPS; ++k) {
-        if (slot_item[k] < 0) continue;
-        if (slot_item[k] != item0) break;
-        last = k;
-      }
-      if (run++ % QA_WARPS != warp) continue;
-      const Item it = load_item<QA_TILE, QT>(p, slot_info[first][0]);
-      const int sub = slot_info[first][1];
-      int list[2 * QA_WARPS], count = 0;
-      for (int x = first; x <= last; ++x)
-        if (slot_item[x] >= 0) list[count++] = x;
-      const float* parts = p.part + (size_t)cta * 2 * QA_WARPS * C::SLOT;
+      uint32_t mask = 0;
+      for (; k < 2 * C::WARPS && (slot_item[k] < 0 || slot_item[k] == item0); ++k)
+        if (slot_item[k] == item0) mask |= 1u << k;
+      if (run++ % C::WARPS != warp) continue;
+      const Item it = slot_info[first];
       const bool inside = item0 >= c0 && item0 + it.ntile <= c1;
       const int border = item0 < c0 ? 0 : 1;
-      float* dst = cta_part + ((size_t)cta * 2 + border) * C::SLOT;
-      merge_partials<NT>(p, count, [&](int x) { return parts + (size_t)list[x] * C::SLOT; }, dst,
-                         inside ? &it : nullptr, sub, lane, 32);
+      merge_slots<NT>(p, mask, p.part + (size_t)cta * 2 * C::WARPS * C::SLOT, cta_part + ((size_t)cta * 2 + border) * C::SLOT,
+                      it, slot_sub[first], inside, lane);
       if (!inside) {
         __threadfence();
         __syncwarp();
@@ -489,15 +562,14 @@ __global__ void __launch_bounds__(QA_THREADS, 1) q4_attn_kernel(const Q4AttnPara
     const int first = last_run[border];
     if (first < 0) continue;
     __threadfence();
-    const int item0 = slot_item[first], sub = slot_info[first][1];
-    const Item it = load_item<QA_TILE, QT>(p, slot_info[first][0]);
-    const int from = runs.of(item0);
-    const int to = runs.of(item0 + it.ntile - 1);
-    // the first CTA holds the item's start, so its part is at its right border
-    // unless the item also began before that CTA's range, which it did not
-    merge_partials<NT>(p, to - from + 1,
-                       [&](int x) { return cta_part + ((size_t)(from + x) * 2 + (x == 0 ? 1 : 0)) * C::SLOT; },
-                       nullptr, &it, sub, threadIdx.x, QA_THREADS);
+    const int item0 = slot_item[first], sub = slot_sub[first];
+    const Item it = slot_info[first];
+    const int from = runs.of(item0), to = runs.of(item0 + it.ntile - 1);
+    // the first CTA holds the item's start, at its right border; the others have it at their left one
+#pragma unroll 1
+    for (int q = warp; q < QT; q += C::WARPS)
+      merge_query<NT>(p, to - from + 1,
+                      [&](int k) { return cta_part + ((size_t)(from + k) * 2 + (k == 0 ? 1 : 0)) * C::SLOT; }, it, sub, q, lane);
   }
 }
 
@@ -505,14 +577,14 @@ static int q4_attn_nt(int max_rows, int nq, int nkv) { return (long long)max_row
 
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms) {
   const int nt = q4_attn_nt(max_rows, nq, nkv);
-  return (size_t)num_sms * (2 * QA_WARPS + 2) * (nt == 1 ? QaCfg<1>::SLOT : QaCfg<2>::SLOT);
+  return (size_t)num_sms * (nt == 1 ? (2 * QaCfg<1>::WARPS + 2) * QaCfg<1>::SLOT : (2 * QaCfg<2>::WARPS + 2) * QaCfg<2>::SLOT);
 }
 
 template <int NT>
 static cudaError_t launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
-  const size_t smem = QaCfg<NT>::RING + QA_WARPS * QA_STAGES * 8 + ((size_t)p.n + 1) * 4;
+  const size_t smem = QaCfg<NT>::RING + QaCfg<NT>::WARPS * QaCfg<NT>::STAGES * 8 + ((size_t)p.n + 1) * 4;
   DFL_TRY(cudaFuncSetAttribute(q4_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  q4_attn_kernel<NT><<<num_sms, QA_THREADS, smem, st>>>(p);
+  q4_attn_kernel<NT><<<num_sms, QaCfg<NT>::THREADS, smem, st>>>(p);
   return cudaGetLastError();
 }
 
