@@ -12,6 +12,12 @@ namespace {
 bool page_size_ok(int page_size) { return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+int log2_of(int page_size) {
+  int b = 0;
+  while ((1 << b) < page_size) ++b;
+  return b;
+}
+
 int num_sms(int* sms) {
   int dev = 0;
   CK(cudaGetDevice(&dev));
@@ -34,7 +40,7 @@ int check_paging(int n, int page_size, long long table_ld, int max_pages, int nu
 }
 
 int check_pool(int rows, int nkv, const void* pool, int num_pages, int page_size) {
-  if (rows < 0 || nkv < 1) return fail(DFLASH_ERR_INVALID, "rows %d, nkv %d", rows, nkv);
+  if (rows < 0 || nkv < 1 || nkv > 65535) return fail(DFLASH_ERR_INVALID, "rows %d, nkv %d", rows, nkv);
   if (!page_size_ok(page_size))
     return fail(DFLASH_ERR_INVALID, "page_size must be 16, 32, 64, 128 or 256 (got %d)", page_size);
   if (num_pages < 1 || (long long)num_pages * page_size > INT32_MAX)
@@ -105,7 +111,7 @@ int dflash_q4_append(const uint16_t* k, int64_t k_row, int64_t k_head, const uin
   if (rows == 0) return DFLASH_OK;
   Q4AppendParams p{};
   p.k = k; p.v = v; p.k_row = k_row; p.k_head = k_head; p.v_row = v_row; p.v_head = v_head;
-  p.bf16 = bf16 != 0; p.slots = slots; p.T = rows; p.nkv = nkv; p.page_size = page_size;
+  p.bf16 = bf16 != 0; p.slots = slots; p.T = rows; p.nkv = nkv; p.page_shift = log2_of(page_size);
   p.num_slots = num_pages * page_size; p.pool = pool; p.status = status;
   CK(q4_append_launch(p, static_cast<cudaStream_t>(stream)));
   return DFLASH_OK;
@@ -118,7 +124,7 @@ int dflash_q4_read(const uint8_t* pool, int num_pages, int page_size, const int3
   if (!aligned16(k) || !aligned16(v)) return fail(DFLASH_ERR_INVALID, "k and v must be 16-byte aligned");
   if (rows == 0) return DFLASH_OK;
   Q4ReadParams p{};
-  p.pool = pool; p.slots = slots; p.T = rows; p.nkv = nkv; p.page_size = page_size;
+  p.pool = pool; p.slots = slots; p.T = rows; p.nkv = nkv; p.page_shift = log2_of(page_size);
   p.num_slots = num_pages * page_size; p.bf16 = bf16 != 0; p.k = k; p.v = v;
   CK(q4_read_launch(p, static_cast<cudaStream_t>(stream)));
   return DFLASH_OK;
@@ -173,7 +179,7 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
   p.table = table; p.lens = lens; p.starts = starts; p.table_ld = table_ld;
   p.n = n; p.T = rows; p.max_rows = max_rows; p.nq = nq; p.nkv = nkv;
   p.by_g = Divisor(G); p.by_nkv = Divisor(nkv);
-  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  p.page_shift = log2_of(page_size);
   p.max_pages = max_pages; p.num_pages = num_pages; p.causal = causal != 0; p.sink = sink; p.window = window;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.out = out; p.status = status;

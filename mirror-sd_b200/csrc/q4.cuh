@@ -50,11 +50,6 @@ enum PagedStatus : int {
   kPagedTimeout = 32,   // a bounded wait of the attention kernel expired
 };
 
-__host__ __device__ __forceinline__ size_t q4_block_offset(int slot, int head, int nkv, int page_size) {
-  const int page = slot / page_size, r = slot - page * page_size;
-  return (((size_t)page * nkv + head) * (page_size / kQ4Rows) + r / kQ4Rows) * kQ4Block;
-}
-
 // byte offsets of the pieces inside the block's K and V values
 __host__ __device__ __forceinline__ int q4_k_piece(int r, int c) { return 64 * r + 16 * (c ^ (r >> 1 & 3)); }
 __host__ __device__ __forceinline__ int q4_v_piece(int j, int g) { return 16 * (8 * j + (g ^ 2 * (j & 3) ^ j >> 2)); }
@@ -82,7 +77,7 @@ struct Q4AppendParams {
   long long k_row, k_head, v_row, v_head;   // strides in elements
   int bf16;
   const int32_t* slots;              // [T]; outside [0, num_slots): the row is skipped
-  int T, nkv, page_size, num_slots;  // num_slots: pages * page_size
+  int T, nkv, page_shift, num_slots;  // pages of 2^page_shift rows; num_slots: rows of all pages
   uint8_t* pool;
   int32_t* status;
 };
@@ -91,7 +86,7 @@ cudaError_t q4_append_launch(const Q4AppendParams& p, cudaStream_t st);
 struct Q4ReadParams {
   const uint8_t* pool;
   const int32_t* slots;
-  int T, nkv, page_size, num_slots, bf16;
+  int T, nkv, page_shift, num_slots, bf16;
   void *k, *v;                       // [T, NKV, 128] contiguous
 };
 cudaError_t q4_read_launch(const Q4ReadParams& p, cudaStream_t st);

@@ -1,29 +1,15 @@
 // Rows into and out of the paged 4-bit cache (layout and numbers: q4.cuh).
 //
 // Both directions stream: 2 bytes a channel on one side, 9/16 on the other, a
-// maximum and a rounding between, so HBM bounds them (and a launch's latency
-// for the few rows of a decode step).  One thread owns one group of 16
-// channels of one row and head, 32 contiguous bytes, so a group's maximum
-// needs no exchange between threads.
-#include "q4.cuh"
+// maximum and a rounding between, so HBM should bound them (and a launch's
+// latency for the few rows of a decode step); what bounds them first is the
+// number of instructions a channel, hence the packing below.  One thread owns
+// one group of 16 channels of one row and head, 32 contiguous bytes, so a
+// group's maximum needs no exchange between threads.  A block is 16 rows of a
+// head: threads 16 i .. + 7 hold row i's K groups, the next 8 its V groups.
+#include "q4_attn.cuh"
 
 namespace dfl {
-
-template <bool BF16>
-__device__ __forceinline__ void unpack8(const uint4& w, float* x) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (BF16) {
-      x[2 * i] = __uint_as_float(u[i] << 16);
-      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
-}
 
 // Scale byte of a group whose largest magnitude is a: the smallest scale
 // >= a / 7.5.  a has at most 11 significant bits and a scale 4, so a / 7.5 is
@@ -42,115 +28,182 @@ __device__ __forceinline__ uint32_t q4_scale_code(float a) {
   return up - ((127 - 15) << 3);
 }
 
+// largest magnitude of 16 values, NaN if one is NaN
+template <bool BF16>
+__device__ __forceinline__ float group_max(const uint32_t (&u)[8]) {
+  uint32_t m = u[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    if (BF16)
+      asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(u[i] & 0x7fff7fffu));
+    else
+      asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(u[i] & 0x7fff7fffu));
+  }
+  const float lo = BF16 ? __uint_as_float(m << 16) : __half2float(__ushort_as_half((unsigned short)m));
+  const float hi = BF16 ? __uint_as_float(m & 0xffff0000u) : __half2float(__ushort_as_half((unsigned short)(m >> 16)));
+  float a;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(lo), "f"(hi));
+  return a;
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(256) q4_append_kernel(const Q4AppendParams p) {
-  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int g = idx & 7, which = (idx >> 3) & 1;
-  const long long rh = idx >> 4;
-  const int row = (int)(rh / p.nkv), h = (int)(rh - (long long)row * p.nkv);
-  if (row >= p.T) return;
-  const int slot = __ldg(p.slots + row);
-  if (slot < 0 || slot >= p.num_slots) return;
-  const char* src = static_cast<const char*>(which ? p.v : p.k) +
-                    2 * ((which ? row * p.v_row + h * p.v_head : row * p.k_row + h * p.k_head) + 16 * g);
+  const int t = threadIdx.x, g = t & 7, which = (t >> 3) & 1;
+  const int row = blockIdx.x * 16 + (t >> 4), h = blockIdx.y;
+  int slot = row < p.T ? __ldg(p.slots + row) : -1;
+  if (slot >= p.num_slots) slot = -1;
+  const int other_slot = __shfl_xor_sync(0xffffffffu, slot, 16);   // of the row beside it
+  uint32_t u[8] = {};
+  if (slot >= 0) {
+    const char* src = static_cast<const char*>(which ? p.v : p.k) +
+                      2 * ((which ? row * p.v_row + h * p.v_head : row * p.k_row + h * p.k_head) + 16 * g);
+    const uint4 w0 = ldg_stream(src), w1 = ldg_stream(src + 16);
+    u[0] = w0.x; u[1] = w0.y; u[2] = w0.z; u[3] = w0.w;
+    u[4] = w1.x; u[5] = w1.y; u[6] = w1.z; u[7] = w1.w;
+  }
   float x[16];
-  unpack8<BF16>(ldg_stream(src), x);
-  unpack8<BF16>(ldg_stream(src + 16), x + 8);
-  float a = 0.f;
-  bool odd = false;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    a = fmaxf(a, fabsf(x[i]));                 // fmaxf drops a NaN
-    odd |= !(fabsf(x[i]) < INFINITY);
-  }
-  if (odd && p.status) atomicOr(p.status, kPagedNonFinite);
-  const uint32_t code = q4_scale_code(a);
-  const float inv = 1.f / __half2float(__ushort_as_half((unsigned short)(code << 7)));
-  // Half-way cases are exact quotients; every other one is at least 2^-12 away
-  // from a half, so adding 2^-14 beside the 0.5 rounds halves away from zero
-  // whatever the reciprocal's last bit, and nothing else differently.
-  uint32_t u[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float r = fminf(floorf(fmaf(fabsf(x[i]), inv, 0.5f + 1.f / 16384)), 7.f);   // a NaN gives 7: see below
-    const int q = x[i] != x[i] ? 0 : (int)r;
-    u[i] = x[i] < 0.f ? 8 - q : 8 + q;
-  }
-  uint8_t* blk = p.pool + q4_block_offset(slot, h, p.nkv, p.page_size);
-  const int rr = slot % kQ4Rows;
-  if (which == 0) {
-    uint32_t w[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      w[j] = 0;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) w[j] |= u[8 * j + 2 * n] << (4 * n) | u[8 * j + 2 * n + 1] << (16 + 4 * n);
+  for (int i = 0; i < 8; ++i) {
+    if (BF16) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
     }
-    *reinterpret_cast<uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8) = make_uint2(w[0], w[1]);
+  }
+  float a = group_max<BF16>(u);
+  if (!(a < INFINITY)) {   // NaN counts as 0 and is stored as 0
+    if (p.status) atomicOr(p.status, kPagedNonFinite);
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = x[i] != x[i] ? 0.f : x[i];
+      a = fmaxf(a, fabsf(x[i]));
+    }
+  }
+  const uint32_t code = q4_scale_code(a);
+  // x / s rounded to nearest, halves away from zero: half-way cases are exact
+  // quotients and every other one is at least 2^-12 from a half, so a factor
+  // 1 + 2^-16 (2^-13 at 7.5; the reciprocal is off by 2^-22) carries halves
+  // outwards and changes nothing else.
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__half2float(__ushort_as_half((unsigned short)(code << 7)))));
+  inv *= 1.f + 1.f / 65536;
+  if (a * inv >= 7.5f) {   // the maximum itself would round to 8
+    const float most = 7.25f / inv;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = fminf(fmaxf(x[i], -most), most);
+  }
+  // The sum with 1.5 * 2^23 + 8 rounds, and leaves u = q + 8 in the lowest bits;
+  // shifting and adding such numbers packs them (the rest stays above bit 16).
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = fmaf(x[i], inv, 12582920.f);
+  auto pack4 = [&](int a0, int a1, int a2, int a3) {
+    return __float_as_uint(x[a0]) + (__float_as_uint(x[a1]) << 4) + (__float_as_uint(x[a2]) << 8) +
+           (__float_as_uint(x[a3]) << 12);
+  };
+  const int bits = p.page_shift - 4;
+  uint8_t* blk = p.pool + ((((size_t)(slot >> p.page_shift) * p.nkv + h) << bits) +
+                           (slot / kQ4Rows & ((1 << bits) - 1))) * kQ4Block;
+  const int rr = slot & 15;
+  const uint32_t hw[4] = {pack4(0, 1, 2, 3), pack4(4, 5, 6, 7), pack4(8, 9, 10, 11), pack4(12, 13, 14, 15)};
+  const uint32_t h01 = __byte_perm(hw[0], hw[1], 0x5410), h23 = __byte_perm(hw[2], hw[3], 0x5410);
+  const uint32_t o01 = __shfl_xor_sync(0xffffffffu, h01, 16), o23 = __shfl_xor_sync(0xffffffffu, h23, 16);
+  if (slot < 0) return;
+  if (which == 0) {
+    // channel 2n of a word in its lower half, 2n + 1 in the upper
+    *reinterpret_cast<uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8) =
+        make_uint2(__byte_perm(pack4(0, 2, 4, 6), pack4(1, 3, 5, 7), 0x5410),
+                   __byte_perm(pack4(8, 10, 12, 14), pack4(9, 11, 13, 15), 0x5410));
     blk[kQ4KS + rr * 8 + g] = (uint8_t)code;
   } else {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t hw = u[4 * w] | u[4 * w + 1] << 4 | u[4 * w + 2] << 8 | u[4 * w + 3] << 12;
-      *reinterpret_cast<uint16_t*>(blk + kQ4V + q4_v_piece(rr >> 1, g) + w * 4 + (rr & 1) * 2) = (uint16_t)hw;
+    uint8_t* piece = blk + kQ4V + q4_v_piece(rr >> 1, g);
+    const bool first = !(rr & 1);
+    if (other_slot == (slot ^ 1) && first == !(t & 16)) {
+      // both rows of the piece are here: half of it each
+      if (first)
+        *reinterpret_cast<uint2*>(piece) = make_uint2(__byte_perm(h01, o01, 0x5410), __byte_perm(h01, o01, 0x7632));
+      else
+        *reinterpret_cast<uint2*>(piece + 8) = make_uint2(__byte_perm(o23, h23, 0x5410), __byte_perm(o23, h23, 0x7632));
+    } else {
+      uint16_t* d = reinterpret_cast<uint16_t*>(piece) + (rr & 1);
+      d[0] = (uint16_t)h01;
+      d[2] = (uint16_t)(h01 >> 16);
+      d[4] = (uint16_t)h23;
+      d[6] = (uint16_t)(h23 >> 16);
     }
     blk[kQ4VS + g * 16 + rr] = (uint8_t)code;
   }
 }
 
+template <bool BF16>
 __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
-  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int g = idx & 7, which = (idx >> 3) & 1;
-  const long long rh = idx >> 4;
-  const int row = (int)(rh / p.nkv), h = (int)(rh - (long long)row * p.nkv);
+  const int t = threadIdx.x, g = t & 7, which = (t >> 3) & 1;
+  const int row = blockIdx.x * 16 + (t >> 4), h = blockIdx.y;
   if (row >= p.T) return;
   const int slot = __ldg(p.slots + row);
   uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (slot >= 0 && slot < p.num_slots) {
-    const uint8_t* blk = p.pool + q4_block_offset(slot, h, p.nkv, p.page_size);
-    const int rr = slot % kQ4Rows;
-    uint32_t u[16], code;
+    const int bits = p.page_shift - 4;
+    const uint8_t* blk = p.pool + ((((size_t)(slot >> p.page_shift) * p.nkv + h) << bits) +
+                                   (slot / kQ4Rows & ((1 << bits) - 1))) * kQ4Block;
+    const int rr = slot & 15;
+    const uint32_t code = __ldg(blk + (which ? kQ4VS + g * 16 + rr : kQ4KS + rr * 8 + g));
+    const uint32_t s = code << 7 | code << 23, ns = hmul2_u(s, 0xBE00BE00u);   // the scale twice; -1.5 s
     if (which == 0) {
-      const uint2 w = *reinterpret_cast<const uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8);
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) u[i] = ((i < 8 ? w.x : w.y) >> (16 * (i & 1) + 4 * ((i & 7) >> 1))) & 15;
-      code = blk[kQ4KS + rr * 8 + g];
-    } else {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t hw =
-            *reinterpret_cast<const uint16_t*>(blk + kQ4V + q4_v_piece(rr >> 1, g) + w * 4 + (rr & 1) * 2);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) u[4 * w + n] = (hw >> (4 * n)) & 15;
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t ww = i ? w.y : w.x;
+        o[4 * i] = dequant<0>(ww, s, ns);
+        o[4 * i + 1] = dequant<1>(ww, s, ns);
+        o[4 * i + 2] = dequant<2>(ww, s, ns);
+        o[4 * i + 3] = dequant<3>(ww, s, ns);
       }
-      code = blk[kQ4VS + g * 16 + rr];
+    } else {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(rr >> 1, g)));
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t hw = (rr & 1) ? ww[i] >> 16 : ww[i] & 0xffffu;
+        const uint32_t both = hw | hw << 12;   // channels 4i and 4i + 1 (4i + 2 and 4i + 3) one half apart
+        o[2 * i] = dequant<0>(both, s, ns);
+        o[2 * i + 1] = dequant<2>(both, s, ns);
+      }
     }
-    const float s = __half2float(__ushort_as_half((unsigned short)(code << 7)));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float lo = ((int)u[2 * i] - 8) * s, hi = ((int)u[2 * i + 1] - 8) * s;
-      o[i] = p.bf16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+      o[i] = hmul2_u(o[i], 0x4C004C00u);   // times 16
+      if (BF16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
+        o[i] = pack_bf16x2(f.x, f.y);
+      }
     }
   }
-  uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(which ? p.v : p.k) + 2 * (rh * 128 + 16 * g));
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(which ? p.v : p.k) + 2 * (((size_t)row * p.nkv + h) * 128 + 16 * g));
   dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
   dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 cudaError_t q4_append_launch(const Q4AppendParams& p, cudaStream_t st) {
-  const long long blocks = ((long long)p.T * p.nkv * 16 + 255) / 256;
-  if (blocks < 1 || blocks > INT32_MAX) return cudaErrorInvalidValue;
+  if (p.T < 1 || p.nkv < 1 || p.nkv > 65535) return cudaErrorInvalidValue;
+  const dim3 grid((p.T + 15) / 16, p.nkv);
   if (p.bf16)
-    q4_append_kernel<true><<<(unsigned)blocks, 256, 0, st>>>(p);
+    q4_append_kernel<true><<<grid, 256, 0, st>>>(p);
   else
-    q4_append_kernel<false><<<(unsigned)blocks, 256, 0, st>>>(p);
+    q4_append_kernel<false><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
 cudaError_t q4_read_launch(const Q4ReadParams& p, cudaStream_t st) {
-  const long long blocks = ((long long)p.T * p.nkv * 16 + 255) / 256;
-  if (blocks < 1 || blocks > INT32_MAX) return cudaErrorInvalidValue;
-  q4_read_kernel<<<(unsigned)blocks, 256, 0, st>>>(p);
+  if (p.T < 1 || p.nkv < 1 || p.nkv > 65535) return cudaErrorInvalidValue;
+  const dim3 grid((p.T + 15) / 16, p.nkv);
+  if (p.bf16)
+    q4_read_kernel<true><<<grid, 256, 0, st>>>(p);
+  else
+    q4_read_kernel<false><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
