@@ -6,7 +6,7 @@
 // number of instructions a channel, hence the packing below.  One thread owns
 // one group of 16 channels of one row and head, 32 contiguous bytes, so a
 // group's maximum needs no exchange between threads.  A block is 16 rows of a
-// head: threads 16 i .. + 7 hold row i's K groups, the next 8 its V groups.
+// head, 4 warps for K and 4 for V (a warp with both would run both codes).
 #include "q4_attn.cuh"
 
 namespace dfl {
@@ -48,11 +48,11 @@ __device__ __forceinline__ float group_max(const uint32_t (&u)[8]) {
 
 template <bool BF16>
 __global__ void __launch_bounds__(256) q4_append_kernel(const Q4AppendParams p) {
-  const int t = threadIdx.x, g = t & 7, which = (t >> 3) & 1;
-  const int row = blockIdx.x * 16 + (t >> 4), h = blockIdx.y;
+  const int t = threadIdx.x, g = t & 7, which = t >> 7;
+  const int row = blockIdx.x * 16 + (t >> 3 & 15), h = blockIdx.y;
   int slot = row < p.T ? __ldg(p.slots + row) : -1;
   if (slot >= p.num_slots) slot = -1;
-  const int other_slot = __shfl_xor_sync(0xffffffffu, slot, 16);   // of the row beside it
+  const int other_slot = __shfl_xor_sync(0xffffffffu, slot, 8);   // of the row beside it
   uint32_t u[8] = {};
   if (slot >= 0) {
     const char* src = static_cast<const char*>(which ? p.v : p.k) +
@@ -108,20 +108,21 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const Q4AppendParams p) 
   uint8_t* blk = p.pool + ((((size_t)(slot >> p.page_shift) * p.nkv + h) << bits) +
                            (slot / kQ4Rows & ((1 << bits) - 1))) * kQ4Block;
   const int rr = slot & 15;
-  const uint32_t hw[4] = {pack4(0, 1, 2, 3), pack4(4, 5, 6, 7), pack4(8, 9, 10, 11), pack4(12, 13, 14, 15)};
-  const uint32_t h01 = __byte_perm(hw[0], hw[1], 0x5410), h23 = __byte_perm(hw[2], hw[3], 0x5410);
-  const uint32_t o01 = __shfl_xor_sync(0xffffffffu, h01, 16), o23 = __shfl_xor_sync(0xffffffffu, h23, 16);
-  if (slot < 0) return;
   if (which == 0) {
+    if (slot < 0) return;
     // channel 2n of a word in its lower half, 2n + 1 in the upper
     *reinterpret_cast<uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8) =
         make_uint2(__byte_perm(pack4(0, 2, 4, 6), pack4(1, 3, 5, 7), 0x5410),
                    __byte_perm(pack4(8, 10, 12, 14), pack4(9, 11, 13, 15), 0x5410));
     blk[kQ4KS + rr * 8 + g] = (uint8_t)code;
   } else {
+    const uint32_t h01 = __byte_perm(pack4(0, 1, 2, 3), pack4(4, 5, 6, 7), 0x5410);
+    const uint32_t h23 = __byte_perm(pack4(8, 9, 10, 11), pack4(12, 13, 14, 15), 0x5410);
+    const uint32_t o01 = __shfl_xor_sync(0xffffffffu, h01, 8), o23 = __shfl_xor_sync(0xffffffffu, h23, 8);
+    if (slot < 0) return;
     uint8_t* piece = blk + kQ4V + q4_v_piece(rr >> 1, g);
     const bool first = !(rr & 1);
-    if (other_slot == (slot ^ 1) && first == !(t & 16)) {
+    if (other_slot == (slot ^ 1) && first == !(t & 8)) {
       // both rows of the piece are here: half of it each
       if (first)
         *reinterpret_cast<uint2*>(piece) = make_uint2(__byte_perm(h01, o01, 0x5410), __byte_perm(h01, o01, 0x7632));
@@ -140,8 +141,8 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const Q4AppendParams p) 
 
 template <bool BF16>
 __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
-  const int t = threadIdx.x, g = t & 7, which = (t >> 3) & 1;
-  const int row = blockIdx.x * 16 + (t >> 4), h = blockIdx.y;
+  const int t = threadIdx.x, g = t & 7, which = t >> 7;
+  const int row = blockIdx.x * 16 + (t >> 3 & 15), h = blockIdx.y;
   if (row >= p.T) return;
   const int slot = __ldg(p.slots + row);
   uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
