@@ -26,7 +26,7 @@
 //       (always for a side's first tile of an item).
 //   4 warps  K codes to f16, into TMEM
 //   4 warps  V codes to f16, transposed, into shared memory
-//   1 warp   issues the MMAs: S(t+1), then PV(t)
+//   2 warps  issue the MMAs, one those of S, one those of PV
 //   1 warp   page look-up and bulk copies of the packed tiles
 //   1 warp   the next item's query rows
 // Every wait is bounded; after one expires the roles run to their end without
@@ -61,7 +61,7 @@ struct QbCfg {
 };
 // warps: softmax of even tiles 0-3, of odd tiles 4-7, then (all in whole
 // warpgroups, whose registers are dealt out anew after the common start)
-constexpr int QB_KDEC = 8, QB_VDEC = 12, QB_MMA = 16, QB_LOAD = 17, QB_QUERY = 18;   // 19 is idle
+constexpr int QB_KDEC = 8, QB_VDEC = 12, QB_MMA = 16, QB_LOAD = 17, QB_QUERY = 18, QB_MMA2 = 19;
 constexpr int QB_THREADS = 640;
 // 96 registers a thread at the start: 640 * 96 = 256 * 144 + 384 * 64
 constexpr int QB_SOFT_REGS = 144, QB_REST_REGS = 64;
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           }
           __syncwarp();
           float sum = 0.f;
-#pragma unroll 1
+#pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float4 v = *reinterpret_cast<const float4*>(stage + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * i);
             sum += (v.x + v.y) + (v.z + v.w);
@@ -913,74 +913,65 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       cur.j += nt - 1;
       if (u < c1) cursor_next<QB_TILE, N>(p, cur);
     }
-    } else if (warp == QB_MMA) {
-    // ---- MMA issue
-    if (T > 0) {
-      const uint32_t idesc_s = umma_idesc_f16(128, N, 0);
-      const uint32_t idesc_o = umma_idesc_f16(128, N, 0) | (1u << 16);   // B (P^T) with the columns contiguous
-      const uint64_t vd = umma_desc_sw128(smem_u32(smem + C::V_OFF)), qd = umma_desc_sw128(smem_u32(smem + C::Q_OFF));
-      const uint64_t pd = desc_sw128_mn(smem_u32(smem + C::P_OFF), 16384);
-      int s_seg = 0, s_k = 0, s_nt = 0;          // position of the next S
-      int p_seg = 0, p_k = 0, p_nt = 0;          // position of the next PV
-      auto issue_s = [&](int t) {
-        const int qb = s_seg % C::QB;
-        if (s_k == 0) {
-          qb_wait(&ms.q_ready[qb], (s_seg / C::QB) & 1, dead);
-          s_nt = ms.seg[s_seg % C::SEGS].nt;
+    } else if (warp == QB_MMA && T > 0) {
+      // ---- S(t) = K(t) Q^T, as soon as K is there and the softmax has read S(t - 2)
+      const uint32_t idesc = umma_idesc_f16(128, N, 0);
+      const uint64_t qd = umma_desc_sw128(smem_u32(smem + C::Q_OFF));
+      int seg = 0, k = 0, nt = 0;
+#pragma unroll 1
+      for (int t = 0; t < T; ++t) {
+        const int qb = seg % C::QB;
+        if (k == 0) {
+          qb_wait(&ms.q_ready[qb], (seg / C::QB) & 1, dead);
+          nt = ms.seg[seg % C::SEGS].nt;
         }
+        if (t >= 2) qb_wait(&ms.p_ready[t & 1], ((t >> 1) - 1) & 1, dead);
         qb_wait(&ms.kready[t & 1], (t >> 1) & 1, dead);
-        const bool last = ++s_k == s_nt;
-        __syncwarp();
+        const bool last = ++k == nt;
         if (elect_one()) {
           tc_fence_after();
           const uint32_t d = tmem + C::S_COL + (t & 1) * N, ka = tmem + C::K_COL + (t & 1) * 64;
           const uint64_t q = qd + qb * (C::Q_BYTES >> 4);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            umma_ts(d, ka + ks * 8, q + ((ks >> 2) * (N * 128) >> 4) + 2 * (ks & 3), idesc_s, ks > 0);
+            umma_ts(d, ka + ks * 8, q + ((ks >> 2) * (N * 128) >> 4) + 2 * (ks & 3), idesc, ks > 0);
           umma_commit(&ms.s_ready[t & 1]);
           umma_commit(&ms.kfree[t & 1]);
           if (last) umma_commit(&ms.q_free[qb]);
         }
         __syncwarp();
         if (last) {
-          s_k = 0;
-          ++s_seg;
+          k = 0;
+          ++seg;
         }
-      };
-      auto issue_pv = [&](int t) {
-        if (p_k == 0) {
-          p_nt = ms.seg[p_seg % C::SEGS].nt;
-          if (p_seg >= 1) qb_wait(&ms.o_free, (p_seg - 1) & 1, dead);
-        }
+      }
+    } else if (warp == QB_MMA2 && T > 0) {
+      // ---- O(side of t) += V^T(t) P^T(t)
+      const uint32_t idesc = umma_idesc_f16(128, N, 0) | (1u << 16);   // B (P^T) with the columns contiguous
+      const uint64_t vd = umma_desc_sw128(smem_u32(smem + C::V_OFF)), pd = desc_sw128_mn(smem_u32(smem + C::P_OFF), 16384);
+      int seg = 0, k = 0, nt = 0;
+#pragma unroll 1
+      for (int t = 0; t < T; ++t) {
         qb_wait(&ms.vready[t & 1], (t >> 1) & 1, dead);
         qb_wait(&ms.p_ready[t & 1], (t >> 1) & 1, dead);
-        __syncwarp();
+        if (k == 0) {
+          nt = ms.seg[seg % C::SEGS].nt;
+          if (seg > 0) qb_wait(&ms.o_free, (seg - 1) & 1, dead);
+        }
         if (elect_one()) {
           tc_fence_after();
           const uint64_t v = vd + (t & 1) * (C::V_BYTES >> 4), pp = pd + (t & 1) * (C::P_BYTES >> 4);
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            umma_f16(tmem + C::O_COL + (t & 1) * N, v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc_o, p_k > 1 || ks > 0);   // a side's first tile of the item starts O
+          for (int ks = 0; ks < 8; ++ks)   // (a side's first tile of the item starts its O)
+            umma_f16(tmem + C::O_COL + (t & 1) * N, v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc, k > 1 || ks > 0);
           umma_commit(&ms.pvdone[t & 1]);
         }
         __syncwarp();
-        if (++p_k == p_nt) {
-          p_k = 0;
-          ++p_seg;
+        if (++k == nt) {
+          k = 0;
+          ++seg;
         }
-      };
-      // S runs one tile ahead, except into the next item, whose queries may
-      // still be on their way
-      int next_s = 0;
-#pragma unroll 1
-      for (int t = 0; t < T; ++t) {
-#pragma unroll 1
-        // (S(t+1) takes the buffer of S(t-1), whose readers PV(t-1) has awaited)
-        while (next_s < T && (next_s <= t || (next_s == t + 1 && s_k != 0))) issue_s(next_s++);
-        issue_pv(t);
       }
-    }
     }
   }
   tc_fence_before();
