@@ -47,6 +47,7 @@ template <int N_>
 struct QbCfg {
   static constexpr int N = N_, CH = N / 16;
   static constexpr int QB = 2;                  // query buffers
+  static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S)
   static constexpr int NS = N <= 64 ? 4 : 2;    // packed stages
   static constexpr bool AHEAD = N <= 64;        // registers for the next 16 scores
   static constexpr int SEGS = 8;                // ring of item records
@@ -76,7 +77,7 @@ struct QbSeg {          // a run of tiles of one item
 
 template <class C>
 struct QbMisc {
-  uint64_t full[4], empty[4], kready[2], kfree[2], vready[2], pvdone[2], s_ready[2], p_ready[2];
+  uint64_t full[4], empty[4], kready[2], kfree[2], vready[2], pvdone[2], s_ready[4], s_free[4], p_ready[2];
   uint64_t q_ready[2], q_free[2], o_free;
   uint32_t tmem;
   int abort;
@@ -255,10 +256,11 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ms.kready[i], 4); mbar_init(&ms.kfree[i], 1);
       mbar_init(&ms.vready[i], 4); mbar_init(&ms.pvdone[i], 1);
-      mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.p_ready[i], 4);
+      mbar_init(&ms.p_ready[i], 4);
       mbar_init(&ms.q_ready[i], 1); mbar_init(&ms.q_free[i], 1);
     }
     mbar_init(&ms.o_free, 8);
+    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], 4); }
     ms.abort = 0;
     ms.border[0].seq = ms.border[1].seq = -1;
     fence_mbar_init();
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     const int x = warp >> 2, gt = threadIdx.x & 127;
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_t = tmem + C::S_COL + x * N + lanes, o_t = tmem + C::O_COL + x * N + lanes;
+    const uint32_t o_t = tmem + C::O_COL + x * N + lanes;
     const int window = p.window > 0 ? p.window : 1 << 30;   // wider than any cache
     float* negm = ms.negm[x];
     float* facs = ms.fac[x];
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
 #pragma unroll 1
     for (int seg = 0; u < c1; ++seg) {
       // S of the item's first tile is only issued once its record is there
-      if ((t0 & 1) == x) qb_wait(&ms.s_ready[x], (t0 >> 1) & 1, dead);
+      if ((t0 & 1) == x) qb_wait(&ms.s_ready[t0 % C::SB], (t0 / C::SB) & 1, dead);
       const QbSeg& sg = ms.seg[seg % C::SEGS];
       // after an expired wait there may be no record: run to the end, writing nothing
       const bool bad = named_bar_or<256>(3, *dead);
@@ -372,8 +374,12 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
 #pragma unroll 1
       for (int k = (t0 & 1) == x ? 0 : 1; k < nt; k += 2) {
         const int t = t0 + k;
-        if (k > 0) qb_wait(&ms.s_ready[x], (t >> 1) & 1, dead);
-        if (t >= 2) qb_wait(&ms.pvdone[x], ((t >> 1) - 1) & 1, dead);   // P of this side is read, its O complete
+        const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + lanes;
+        // P of this side is read, and its O holds the tiles before t
+        auto wait_pv = [&]() {
+          if (t >= 2) qb_wait(&ms.pvdone[x], ((t >> 1) - 1) & 1, dead);
+        };
+        if (k > 0) qb_wait(&ms.s_ready[t % C::SB], (t / C::SB) & 1, dead);
         tc_fence_after();
         const int row0 = item_tile(it, j0 + k) * QB_TILE;
         const int2 info = ms.tile[t & 15];
@@ -450,6 +456,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               l[8 * c + i] = fma2(y[i], make_float2(on, on), l[8 * c + i]);
               w[i] = pack_f16x2(y[i].x, y[i].y);
             }
+            if (c == 0) wait_pv();
             uint8_t* d = pr + (c >> 2) * 16384;
             *reinterpret_cast<uint4*>(d + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<uint4*>(d + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -491,7 +498,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               ms.cmax[x][gt] = float_key(-INFINITY);
             }
             named_bar_sync(1 + x, 128);
-            if (k >= 2) {   // O of this side holds its tiles before t
+            if (k >= 2) {
+              wait_pv();
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < C::CH; ++c) {
                 uint32_t o[16];
@@ -518,8 +527,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           raise = true;
           __syncwarp();
         }
-        fence_proxy_async_smem();
         tc_fence_before();
+        warp_arrive(&ms.s_free[t % C::SB], lane);
+        fence_proxy_async_smem();
         warp_arrive(&ms.p_ready[x], lane);
       }
       u += nt;
@@ -914,7 +924,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       if (u < c1) cursor_next<QB_TILE, N>(p, cur);
     }
     } else if (warp == QB_MMA && T > 0) {
-      // ---- S(t) = K(t) Q^T, as soon as K is there and the softmax has read S(t - 2)
+      // ---- S(t) = K(t) Q^T, as soon as K is there and the softmax has read the buffer's last S
       const uint32_t idesc = umma_idesc_f16(128, N, 0);
       const uint64_t qd = umma_desc_sw128(smem_u32(smem + C::Q_OFF));
       int seg = 0, k = 0, nt = 0;
@@ -925,17 +935,17 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           qb_wait(&ms.q_ready[qb], (seg / C::QB) & 1, dead);
           nt = ms.seg[seg % C::SEGS].nt;
         }
-        if (t >= 2) qb_wait(&ms.p_ready[t & 1], ((t >> 1) - 1) & 1, dead);
+        if (t >= C::SB) qb_wait(&ms.s_free[t % C::SB], (t / C::SB - 1) & 1, dead);
         qb_wait(&ms.kready[t & 1], (t >> 1) & 1, dead);
         const bool last = ++k == nt;
         if (elect_one()) {
           tc_fence_after();
-          const uint32_t d = tmem + C::S_COL + (t & 1) * N, ka = tmem + C::K_COL + (t & 1) * 64;
+          const uint32_t d = tmem + C::S_COL + (t % C::SB) * N, ka = tmem + C::K_COL + (t & 1) * 64;
           const uint64_t q = qd + qb * (C::Q_BYTES >> 4);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
             umma_ts(d, ka + ks * 8, q + ((ks >> 2) * (N * 128) >> 4) + 2 * (ks & 3), idesc, ks > 0);
-          umma_commit(&ms.s_ready[t & 1]);
+          umma_commit(&ms.s_ready[t % C::SB]);
           umma_commit(&ms.kfree[t & 1]);
           if (last) umma_commit(&ms.q_free[qb]);
         }
