@@ -67,14 +67,6 @@ struct QaCfg {
   static constexpr int RING = WARPS * STAGES * QA_STAGE;
 };
 
-// write 4 consecutive output values of one query row
-__device__ __forceinline__ void store_out4(const Q4AttnParams& p, int row, int head, int d, const float (&v)[4]) {
-  const size_t off = ((size_t)row * p.nq + head) * 128 + d;
-  const uint2 w = p.bf16 ? make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]))
-                         : make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + off) = w;
-}
-
 // A warp merges the partials of one item that the slots of `mask` hold (slot k
 // at parts + k * SLOT), all queries at once: 8 (16) loads of a partial's O are
 // on their way together.  Writes the item's output rows (finish) or one partial
@@ -125,51 +117,6 @@ __device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask
       *reinterpret_cast<float4*>(dst + i * 128 + 4 * lane) = o[i];
     }
   }
-}
-
-// A warp merges query q of an item from `count` CTAs' partials (slots(k)).
-template <int NT, class SlotAt>
-__device__ __forceinline__ void merge_query(const Q4AttnParams& p, int count, SlotAt slots, const Item& it, int sub, int q,
-                                            int lane) {
-  constexpr int QT = QaCfg<NT>::QT;
-  const int grp = p.by_nkv.of(sub), r = grp * QT + q, j = p.by_g.of(r);
-  if (j >= it.rows) return;
-  float M = -INFINITY, l = 0.f;
-#pragma unroll 1
-  for (int k = lane; k < count; k += 32) M = fmaxf(M, __ldcg(slots(k) + QT * 128 + q));
-  M = warp_max(M);
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int k0 = 0; k0 < count; k0 += 32) {
-    float w = 0.f;
-    if (k0 + lane < count) {
-      const float m = __ldcg(slots(k0 + lane) + QT * 128 + q);
-      w = m == -INFINITY ? 0.f : exp2_fast(m - M);
-      l = fmaf(w, __ldcg(slots(k0 + lane) + QT * 129 + q), l);
-    }
-    const int n = min(count - k0, 32);
-#pragma unroll 1
-    for (int k = 0; k < n; k += 8) {
-      float4 v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)   // (past the end: the last one again, with weight 0)
-        v[i] = __ldcg(reinterpret_cast<const float4*>(slots(k0 + min(k + i, n - 1)) + q * 128 + 4 * lane));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, k + i);
-        if (k + i < n) {
-          o[0] = fmaf(wi, v[i].x, o[0]);
-          o[1] = fmaf(wi, v[i].y, o[1]);
-          o[2] = fmaf(wi, v[i].z, o[2]);
-          o[3] = fmaf(wi, v[i].w, o[3]);
-        }
-      }
-    }
-  }
-  l = warp_sum(l);
-  const float f = l == 0.f ? 0.f : 16.f / l;
-  const float v[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
-  store_out4(p, it.row0 + j, (sub - grp * p.nkv) * p.by_g.d + r - j * p.by_g.d, 4 * lane, v);
 }
 
 template <int NT>
@@ -225,7 +172,10 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
 
   const int ctas = min((int)gridDim.x, total);   // CTAs with work
   const int cta = blockIdx.x;
-  if (cta >= ctas) return;
+  if (cta >= ctas) {
+    zero_rows(p, threadIdx.x, C::THREADS);
+    return;
+  }
   const Runs runs(total, ctas);
   const int c0 = runs.start(cta), c1 = runs.start(cta + 1);
   const Runs mine(c1 - c0, C::WARPS);
@@ -567,10 +517,16 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     const int from = runs.of(item0), to = runs.of(item0 + it.ntile - 1);
     // the first CTA holds the item's start, at its right border; the others have it at their left one
 #pragma unroll 1
-    for (int q = warp; q < QT; q += C::WARPS)
-      merge_query<NT>(p, to - from + 1,
-                      [&](int k) { return cta_part + ((size_t)(from + k) * 2 + (k == 0 ? 1 : 0)) * C::SLOT; }, it, sub, q, lane);
+    for (int q = warp; q < QT; q += C::WARPS) {
+      const int grp = p.by_nkv.of(sub), r = grp * QT + q, j = p.by_g.of(r);
+      if (j >= it.rows) continue;
+      float v[4];
+      merge_query(to - from + 1, [&](int k) { return cta_part + ((size_t)(from + k) * 2 + (k == 0 ? 1 : 0)) * C::SLOT; }, QT,
+                  q, lane, v);
+      store_out4(p, it.row0 + j, (sub - grp * p.nkv) * G + r - j * G, 4 * lane, v);
+    }
   }
+  zero_rows(p, threadIdx.x, C::THREADS);
 }
 
 static int q4_attn_nt(int max_rows, int nq, int nkv) { return (long long)max_rows * (nq / nkv) <= 8 ? 1 : 2; }

@@ -672,26 +672,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         for (int q = me + count * warp; q < N; q += count * 8) {
           const int r = grp * N + q, j = p.by_g.of(r);
           if (j >= it.rows) continue;
-          float M = -INFINITY;
-#pragma unroll 1
-          for (int i = 0; i < count; ++i) M = fmaxf(M, __ldcg(slot(i) + N * 128 + q));
-          float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int i = 0; i < count; ++i) {
-            const float m = __ldcg(slot(i) + N * 128 + q);
-            const float w = m == -INFINITY ? 0.f : exp2_fast(m - M);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (size_t)q * 128 + 4 * lane));
-            sum = fmaf(w, __ldcg(slot(i) + N * 129 + q), sum);
-            o[0] = fmaf(w, v.x, o[0]);
-            o[1] = fmaf(w, v.y, o[1]);
-            o[2] = fmaf(w, v.z, o[2]);
-            o[3] = fmaf(w, v.w, o[3]);
-          }
-          const float fin = sum == 0.f ? 0.f : 16.f / sum;
-          const size_t at = ((size_t)(it.row0 + j) * p.nq + (sub - grp * p.nkv) * G + r - j * G) * 128 + 4 * lane;
-          const uint2 w2 = p.bf16 ? make_uint2(pack_bf16x2(o[0] * fin, o[1] * fin), pack_bf16x2(o[2] * fin, o[3] * fin))
-                                  : make_uint2(pack_f16x2(o[0] * fin, o[1] * fin), pack_f16x2(o[2] * fin, o[3] * fin));
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = w2;
+          float v[4];
+          merge_query(count, slot, N, q, lane, v);
+          store_out4(p, it.row0 + j, (sub - grp * p.nkv) * G + r - j * G, 4 * lane, v);
         }
       }
       named_bar_sync(3, 256);
@@ -839,6 +822,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     // after an expired wait: what was requested and not yet waited for
     if (t < T)
       for (int i = max(t - NS, 0); i < t; ++i) mbar_wait(&ms.full[i % NS], (i / NS) & 1, nullptr, nullptr);
+    zero_rows(p, lane, 32);
+    } else if (warp == QB_LOAD) {
+      zero_rows(p, lane, 32);
     } else if (warp == QB_QUERY && T > 0) {
     // ---- query rows, as f16 with the factor that their scores take
     Cursor cur;
@@ -861,13 +847,14 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         int j = p.by_g.of(r), h = r - j * G;
         const uint16_t* q = static_cast<const uint16_t*>(p.q) + (size_t)cur.it.row0 * p.q_row + 8 * piece;
         uint8_t* dst = qs + (piece >> 3) * (N * 128);
-#pragma unroll 1
+#pragma unroll 4
         for (int i = lane >> 4; i < N; i += 2) {
           const bool real = j < cur.it.rows;
           cp_async16_zfill(smem_u32(dst + i * 128 + (((piece & 7) ^ (i & 7)) << 4)),
                            real ? q + (size_t)j * p.q_row + (size_t)(head0 + h) * p.q_head : p.q, real);
           h += 2;
-          while (h >= G) { h -= G; ++j; }
+          if (h >= G) { h -= G; ++j; }
+          if (h >= G) { h -= G; ++j; }   // (one head a kv head)
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -882,7 +869,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         // most); any other row is scaled by a power of two first.
         const int piece = lane & 15;
         uint8_t* src = qs + (piece >> 3) * (N * 128);
-#pragma unroll 1
+        const uint32_t half = lane < 16 ? 0xffffu : 0xffff0000u;   // the lanes of this lane's row
+#pragma unroll 4
         for (int i = lane >> 4; i < N; i += 2) {
           uint4* at = reinterpret_cast<uint4*>(src + i * 128 + (((piece & 7) ^ (i & 7)) << 4));
           const uint4 w = *at;
@@ -894,19 +882,21 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
             x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
             a = fmaxf(a, fmaxf(fabsf(x[2 * k]), fabsf(x[2 * k + 1])));
           }
+          const uint32_t big = __ballot_sync(0xffffffffu, a >= 0.125f), nonzero = __ballot_sync(0xffffffffu, a > 0.f);
+          const bool plain = (!(nonzero & half) || (big & half)) && a <= 32768.f;
+          if (!__all_sync(0xffffffffu, plain)) {
+#pragma unroll 1
+            for (int o = 1; o < 16; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            if (a != 0.f && !(a >= 0.125f && a <= 32768.f)) {
+              const int e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
+              const float down = __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
-          for (int o = 1; o < 16; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-          float f = base_f;
-          if (a != 0.f && !(a >= 0.125f && a <= 32768.f)) {
-            const int e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
-            const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-            f *= __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] *= down;
-            uniform = false;
+              for (int k = 0; k < 8; ++k) x[k] *= down;
+              if (piece == 0) qf[i] = base_f * __uint_as_float((uint32_t)e << 23);
+              uniform = false;
+            }
           }
           *at = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
-          if (piece == 0 && f != base_f) qf[i] = f;
         }
         uniform = __all_sync(0xffffffffu, uniform);
       }

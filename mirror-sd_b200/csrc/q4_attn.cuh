@@ -28,8 +28,8 @@ __device__ __forceinline__ TileSpan tile_span(const Q4AttnParams& p, int L, int 
 struct Item {          // one (request, query group, kv head)
   int seq, L, rows, row0;   // cached rows, query rows, first packed query row
   TileSpan span;
-  int ntile;           // >= 1: a request without visible keys still writes zeros
-  int groups;          // query groups of the request
+  int ntile;           // tiles that hold keys its queries see
+  int groups;          // query groups of the request; 0 where it has no rows or sees no key
 };
 
 __device__ __forceinline__ int seq_rows(const Q4AttnParams& p, int i, int* row0) {
@@ -51,9 +51,22 @@ __device__ __forceinline__ Item load_item(const Q4AttnParams& p, int i) {
   it.rows = seq_rows(p, i, &it.row0);
   it.L = min(max(__ldg(p.lens + i), 0), p.max_pages << p.page_shift);
   it.span = tile_span<TILE>(p, it.L, it.rows);
-  it.ntile = max(it.span.a + it.span.c - it.span.b, 1);
-  it.groups = (it.rows * p.by_g.d + QT - 1) / QT;
+  it.ntile = it.span.a + it.span.c - it.span.b;
+  it.groups = it.ntile > 0 ? (it.rows * p.by_g.d + QT - 1) / QT : 0;
   return it;
+}
+// The rows of requests without a cached row belong to no tile: zeros, from
+// thread t of `threads` of every CTA, which share the requests out.
+__device__ __forceinline__ void zero_rows(const Q4AttnParams& p, int t, int threads) {
+#pragma unroll 1
+  for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
+    if (__ldg(p.lens + i) > 0) continue;
+    int row0;
+    const int rows = seq_rows(p, i, &row0);
+    uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + (size_t)row0 * p.nq * 128);
+#pragma unroll 1
+    for (int e = t; e < rows * p.nq * 16; e += threads) out[e] = make_uint4(0, 0, 0, 0);
+  }
 }
 __device__ __forceinline__ int item_tile(const Item& it, int j) {
   return j < it.span.a ? j : j - it.span.a + it.span.b;
@@ -131,6 +144,56 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// A warp merges one query's partials of `count` CTAs: slots(k) holds O at
+// q * 128, m at qt * 128 + q and l at qt * 129 + q.  Returns channels 4 lane ..
+// of the output row.  8 loads of O are on their way together.
+template <class SlotAt>
+__device__ __forceinline__ void merge_query(int count, SlotAt slots, int qt, int q, int lane, float (&v)[4]) {
+  float M = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (int k = lane; k < count; k += 32) M = fmaxf(M, __ldcg(slots(k) + qt * 128 + q));
+  M = warp_max(M);
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int k0 = 0; k0 < count; k0 += 32) {
+    float w = 0.f;
+    if (k0 + lane < count) {
+      const float m = __ldcg(slots(k0 + lane) + qt * 128 + q);
+      w = m == -INFINITY ? 0.f : exp2_fast(m - M);
+      l = fmaf(w, __ldcg(slots(k0 + lane) + qt * 129 + q), l);
+    }
+    const int n = min(count - k0, 32);
+#pragma unroll 1
+    for (int k = 0; k < n; k += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)   // (past the end: the last one again, with weight 0)
+        x[i] = __ldcg(reinterpret_cast<const float4*>(slots(k0 + min(k + i, n - 1)) + q * 128 + 4 * lane));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, k + i);
+        if (k + i < n) {
+          o[0] = fmaf(wi, x[i].x, o[0]);
+          o[1] = fmaf(wi, x[i].y, o[1]);
+          o[2] = fmaf(wi, x[i].z, o[2]);
+          o[3] = fmaf(wi, x[i].w, o[3]);
+        }
+      }
+    }
+  }
+  l = warp_sum(l);
+  const float f = l == 0.f ? 0.f : 16.f / l;
+  for (int i = 0; i < 4; ++i) v[i] = o[i] * f;
+}
+
+// write 4 consecutive output values of one query row
+__device__ __forceinline__ void store_out4(const Q4AttnParams& p, int row, int head, int d, const float (&v)[4]) {
+  const size_t off = ((size_t)row * p.nq + head) * 128 + d;
+  const uint2 w = p.bf16 ? make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]))
+                         : make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + off) = w;
 }
 
 }  // namespace dfl
