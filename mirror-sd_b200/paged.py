@@ -211,7 +211,8 @@ def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: b
 
     causal: query row j of m sees the keys below lens - m + j + 1 (else below
     lens); window: of those only the first ``sink`` and the last ``window``.
-    A row that sees no key gives zeros.  scale defaults to 128 ** -0.5."""
+    A row that sees no key gives zeros; rows of q that no request owns leave
+    their rows of ``out`` unwritten.  scale (positive) defaults to 128 ** -0.5."""
     dev = _device(pool)
     num_pages, nkv, page_size = _pool(pool)
     q, q_row, q_head = _rows("q", q, None, dev)
@@ -237,7 +238,9 @@ def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: b
 class PagedKVCacheQ4:
     """Cache of ``max_seqs`` requests over ``num_layers`` layers.  Every
     method enqueues on the current stream; none waits for the device except
-    ``check`` and ``free_page_count``."""
+    ``check`` and ``free_page_count``.  Calls on different streams are the
+    caller's to order (an event between them); the state's memory then stays
+    until the last of the streams is done with it."""
 
     def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, max_seqs: int, max_len: int,
                  page_size: int = 64, device="cuda"):
@@ -253,12 +256,24 @@ class PagedKVCacheQ4:
         self.free_pages = torch.arange(num_pages, **i32)
         self.head = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
+        self._zeros = torch.zeros(max_seqs, **i32)
         self._workspace = {}
+        self._stream = _raw_stream(self.device.index)
+
+    def _enter(self):
+        """``lens``, ``pages`` and ``head`` are new tensors after each step: on another
+        stream than the last call's, tell the allocator that it reads the old ones."""
+        raw = _raw_stream(self.device.index)
+        if raw != self._stream:
+            self._stream = raw
+            for t in (self.lens, self.pages, self.head):
+                t.record_stream(torch.cuda.current_stream(self.device))
 
     def reserve(self, new_rows: Union[torch.Tensor, Sequence[int]], num_slots: Optional[int] = None) -> PagedStep:
         """Make room for new_rows[i] rows of request i (0 where it sits out).
         ``num_slots`` bounds their sum; it is needed when new_rows is a device
         tensor."""
+        self._enter()
         if not torch.is_tensor(new_rows):
             num_slots = sum(new_rows) if num_slots is None else num_slots
             new_rows = torch.tensor(list(new_rows), dtype=torch.int32).to(self.device, non_blocking=True)
@@ -275,6 +290,7 @@ class PagedKVCacheQ4:
     def attend(self, layer: int, q, step: PagedStep, max_rows: int, causal: bool = True, sink: int = 0,
                window: int = 0, scale: Optional[float] = None, out=None):
         """Attention of the step's query rows over everything cached."""
+        self._enter()
         key = (max_rows, q.shape[1], torch.cuda.current_stream(self.device).cuda_stream)
         ws = self._workspace.get(key)      # one for each stream: calls on different streams may overlap
         if ws is None:
@@ -285,22 +301,34 @@ class PagedKVCacheQ4:
     def trim(self, counts: Union[int, torch.Tensor, Sequence[int]]) -> None:
         """Drop the last counts[i] rows of request i (one number: of every
         request).  Pages stay with the request until ``release``."""
-        if not torch.is_tensor(counts) and not isinstance(counts, int):
-            counts = torch.tensor(list(counts), dtype=torch.int32).to(self.device, non_blocking=True)
-        self.lens = (self.lens - counts).clamp_(min=0).to(torch.int32)
+        self._enter()
+        if not torch.is_tensor(counts):
+            counts = counts if isinstance(counts, int) else torch.tensor(list(counts), dtype=torch.int32)
+            if counts < 0 if isinstance(counts, int) else bool((counts < 0).any()):
+                raise ValueError("trim counts must not be negative")
+        if torch.is_tensor(counts):
+            if counts.shape != self.lens.shape or counts.is_floating_point():
+                raise ValueError(f"counts must be {self.max_seqs} integers, got {counts.dtype} {tuple(counts.shape)}")
+            counts = counts.to(self.device, non_blocking=True)
+        # a negative count on the device, where nobody can raise, trims nothing
+        self.lens = torch.clamp(self.lens - counts, min=self._zeros, max=self.lens).to(torch.int32)
 
     def release(self, seqs: Sequence[int] = ()) -> None:
         """Give spare pages back; requests ``seqs`` are finished and emptied."""
         seqs = [int(s) for s in seqs]
         if any(not 0 <= s < self.max_seqs for s in seqs):
             raise ValueError(f"sequences must lie in [0, {self.max_seqs})")
+        self._enter()
         if seqs:
             self.lens = self.lens.index_fill(0, torch.tensor(seqs).to(self.device), 0)
         self.pages, self.head = paged_release(self.lens, self.pages, self.table, self.free_pages, self.head,
                                               self.page_size, self.status)
 
     def read(self, layer: int, seq: int, length: int, dtype=torch.float16):
-        """The first ``length`` rows of a request as (k, v) [length, NKV, 128]."""
+        """The first ``length`` rows of a request, which it must hold, as
+        (k, v) [length, NKV, 128]."""
+        if not 0 <= seq < self.max_seqs or not 0 <= length <= self.table.shape[1] * self.page_size:
+            raise ValueError(f"no rows 0..{length} of request {seq}")
         pos = torch.arange(length, device=self.device)
         slots = self.table[seq][pos // self.page_size] * self.page_size + (pos % self.page_size).to(torch.int32)
         return q4_read(self.pools[layer], slots.to(torch.int32), dtype)

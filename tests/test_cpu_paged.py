@@ -89,6 +89,8 @@ def test_q4_entry_points_refuse_bad_arguments(pkg, lib):
     _refused(pkg, attend(sink=4), "sink needs a window")
     _refused(pkg, attend(window=-4), "window")
     _refused(pkg, attend(scale=float("inf")), "finite")
+    _refused(pkg, attend(scale=0.0), "positive")
+    _refused(pkg, attend(scale=-0.1), "positive")
     _refused(pkg, attend(nbytes=100), "workspace too small")
     _refused(pkg, attend(width=9), "table_ld")
     assert attend(rows=0, starts=P) == 0
