@@ -780,45 +780,57 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   } else {
     set_registers<QB_REST_REGS, false>();
     if (warp == QB_LOAD && T > 0) {
-    // ---- packed tiles: lane b < 8 looks after row block b
+    // ---- packed tiles, four at a time: lane 8 i + b looks after row block b of
+    // tile i.  (One tile at a time, page number and addresses took this warp
+    // about 1,700 cycles a tile, as long as a tile takes the other roles.)
     Cursor cur;
     first_cursor(cur);
-    auto page_of = [&]() {
-      const int pos = item_tile(cur.it, cur.j) * QB_TILE + (lane & 7) * kQ4Rows;
-      int pg = -1;
-      if (lane < 8 && pos < cur.it.L) {
-        pg = __ldg(p.table + (size_t)cur.it.seq * p.table_ld + (pos >> p.page_shift));
-        if (pg < 0 || pg >= p.num_pages) pg = -1;   // hidden, like a masked block
-      }
-      return pg;
-    };
-    int t = 0, page = -1, row0 = 0;
+    const int bits = p.page_shift - 4;
+    int page, row0, left, head;   // of the lane's block: page, the tile's first row, rows below the request's end
+    auto look_up = [&](int t0) {   // tiles t0 .. t0 + 3 of the CTA
+      int seq = 0, sub = 0, L = 0;
+      row0 = 0;
 #pragma unroll 1
-    for (;; ++t) {
-      // (the next tile's page number travels while this tile's stage is awaited)
-      const int now = page, now_row0 = row0, now_L = cur.it.L, now_sub = cur.sub;
-      if (t > 0 && t < T) cursor_next<QB_TILE, N>(p, cur);
-      row0 = item_tile(cur.it, cur.j) * QB_TILE;
-      page = t < T ? page_of() : -1;
-      if (t == 0) continue;
-      const int u = t - 1, s = u % NS;   // tile u goes out
-      if (u >= NS) qb_wait(&ms.empty[s], ((u / NS) - 1) & 1, dead);
-      if (__any_sync(0xffffffffu, *dead)) break;
-      const uint32_t mask = __ballot_sync(0xffffffffu, now >= 0);
-      if (lane == 0) {
-        ms.tile[u & 15] = make_int2((int)mask, min(now_L - now_row0, QB_TILE));
-        mbar_arrive_expect_tx(&ms.full[s], __popc(mask) * kQ4Block);
+      for (int i = 0; i < 4 && t0 + i < T; ++i) {
+        if (lane >> 3 == i) {
+          row0 = item_tile(cur.it, cur.j) * QB_TILE;
+          seq = cur.it.seq;
+          sub = cur.sub;
+          L = cur.it.L;
+        }
+        if (t0 + i + 1 < T) cursor_next<QB_TILE, N>(p, cur);
       }
-      __syncwarp();
-      if (now >= 0) {
-        const int bits = p.page_shift - 4, head = now_sub - p.by_nkv.of(now_sub) * p.nkv;
-        bulk_load(smem + C::RING_OFF + s * QB_STAGE + lane * QB_BLK,
-                  p.pool + ((((size_t)now * p.nkv + head) << bits) + (now_row0 / kQ4Rows + lane & ((1 << bits) - 1))) * kQ4Block,
-                  kQ4Block, &ms.full[s]);
+      left = min(L - row0, QB_TILE);
+      head = sub - p.by_nkv.of(sub) * p.nkv;
+      const int pos = row0 + (lane & 7) * kQ4Rows;
+      page = -1;
+      if (pos < L) page = __ldg(p.table + (size_t)seq * p.table_ld + (pos >> p.page_shift));
+    };
+    look_up(0);
+    int t = 0;   // tiles requested
+#pragma unroll 1
+    while (t < T && !*dead) {
+      const bool there = page >= 0 && page < p.num_pages;   // (else hidden, like a masked block)
+      const uint8_t* src = p.pool + ((((size_t)(there ? page : 0) * p.nkv + head) << bits) +
+                                     (row0 / kQ4Rows + (lane & 7) & ((1 << bits) - 1))) * kQ4Block;
+      const uint32_t mask = __ballot_sync(0xffffffffu, there);
+      const int rows = left, end = min(t + 4, T);
+      look_up(t + 4);   // (the next four page numbers travel while these tiles wait for their stages)
+#pragma unroll 1
+      for (; t < end; ++t) {
+        const int s = t % NS, i = t & 3;
+        if (t >= NS) qb_wait(&ms.empty[s], ((t / NS) - 1) & 1, dead);
+        if (__any_sync(0xffffffffu, *dead)) break;
+        if (lane == 8 * i) {
+          const uint32_t blocks = mask >> 8 * i & 255;
+          ms.tile[t & 15] = make_int2((int)blocks, rows);
+          mbar_arrive_expect_tx(&ms.full[s], __popc(blocks) * kQ4Block);
+        }
+        __syncwarp();
+        if (lane >> 3 == i && there)
+          bulk_load(smem + C::RING_OFF + s * QB_STAGE + (lane & 7) * QB_BLK, src, kQ4Block, &ms.full[s]);
       }
-      if (t == T) { ++t; break; }
     }
-    --t;   // tiles requested
     // after an expired wait: what was requested and not yet waited for
     if (t < T)
       for (int i = max(t - NS, 0); i < t; ++i) mbar_wait(&ms.full[i % NS], (i / NS) & 1, nullptr, nullptr);
