@@ -5,11 +5,14 @@ There is no fallback: if it is missing or fails to load, every entry point
 raises.  ctypes releases the GIL around each call.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libdflash_b200.so")
+PAGED_PATH = os.path.join(HERE, "lib", "dflash_paged.so")
 
 DFLASH_OK = 0
 DFLASH_ERR_INVALID = 1
@@ -142,6 +145,7 @@ EXPORTS = {
 }
 
 _lib = None
+_paged = None
 _lock = threading.Lock()
 
 
@@ -159,6 +163,26 @@ def load():
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def load_paged():
+    """The Python binding of the paged operators (csrc/paged_binding.cpp), calling the library above."""
+    global _paged
+    if _paged is None:
+        lib = load()
+        with _lock:
+            if _paged is None:
+                if not os.path.exists(PAGED_PATH):
+                    raise RuntimeError(f"binding not built: {PAGED_PATH} (run mirror-sd_b200/build.py)")
+                import torch  # noqa: F401  (its libraries must be loaded first)
+                loader = importlib.machinery.ExtensionFileLoader("dflash_paged", PAGED_PATH)
+                mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("dflash_paged", loader))
+                loader.exec_module(mod)
+                mod.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in
+                           ("dflash_paged_reserve", "dflash_paged_release", "dflash_q4_append", "dflash_q4_read",
+                            "dflash_q4_attention", "dflash_last_error")))
+                _paged = mod
+    return _paged
 
 
 def last_error():

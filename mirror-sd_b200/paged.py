@@ -45,69 +45,9 @@ class PagedStep(NamedTuple):
     head: torch.Tensor
 
 
-# The calls below are a few microseconds of GPU work in a decode step, so the
-# checks read each tensor's fields once and nothing else runs on the host.
-_I32 = torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream().cuda_stream without the Stream object
 
-
-def _device(t):
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError("the paged cache's tensors must be on a CUDA device")
-    return dev
-
-
-def _i32(name, t, n, dev):
-    """Address of a contiguous int32 vector of n entries (any number if None) on device dev."""
-    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 1 or not t.is_contiguous() \
-            or n is not None and t.numel() != n:
-        raise ValueError(f"{name} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on cuda:{dev}, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _table(table, n, dev):
-    """(address, row stride, max_pages)"""
-    if table.dtype is not _I32 or table.get_device() != dev or table.dim() != 2:
-        raise ValueError(f"table must be an int32 matrix [{n}, max_pages] on cuda:{dev}")
-    rows, width = table.shape
-    if rows != n or table.stride(1) != 1 and width > 1:
-        raise ValueError(f"table must be [{n}, max_pages] with contiguous rows, got {tuple(table.shape)}")
-    return table.data_ptr(), max(table.stride(0), width), width
-
-
-def _pool(pool):
-    """(num_pages, NKV, page_size) of a pool."""
-    if pool.dtype is not torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] != BLOCK_BYTES:
-        raise ValueError("pool must be a contiguous uint8 tensor from q4_pool()")
-    num_pages, nkv, blocks, _ = pool.shape
-    return num_pages, nkv, blocks * 16
-
-
-def _rows(name, t, heads, dev):
-    """t, or a copy where the kernels could not read it in whole 16 bytes; and its strides."""
-    if t.dtype is not torch.float16 and t.dtype is not torch.bfloat16 or t.get_device() != dev or t.dim() != 3 \
-            or t.shape[2] != HEAD_DIM or heads is not None and t.shape[1] != heads:
-        raise ValueError(f"{name} must be f16 or bf16 [rows, {heads or 'heads'}, {HEAD_DIM}] on cuda:{dev}, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    a, b, c = t.stride()
-    if c != 1 or (a | b) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-        a, b, c = t.stride()
-    return t, a, b
-
-
-def _call(name, dev, *args):
-    """A C entry on the tensors' device and its current stream."""
-    fn = getattr(N.load(), name)
-    if torch.cuda.current_device() == dev:
-        status = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev))
-    if status:
-        N.check(status, name)
+# Arguments are checked, and outputs made, in csrc/paged_binding.cpp.
 
 
 def paged_reserve(lens, new_rows, pages, table, free_pages, head, page_size: int, num_slots: int,
@@ -121,31 +61,14 @@ def paged_reserve(lens, new_rows, pages, table, free_pages, head, page_size: int
     rows of all requests (known on the host); surplus slots are -1.  A request
     that cannot be served keeps its length and sets a bit of ``status``
     (STATUS_BITS)."""
-    dev, n = _device(lens), lens.numel()
-    if num_slots < 0:
-        raise ValueError(f"num_slots {num_slots}")
-    t, ld, max_pages = _table(table, n, dev)
-    out = torch.empty(3 * n + 2 + num_slots, dtype=_I32, device=lens.device)
-    o = out.data_ptr()      # [starts | lens | pages | head | slots]
-    _call("dflash_paged_reserve", dev, _i32("lens", lens, n, dev), _i32("new_rows", new_rows, n, dev),
-          _i32("pages", pages, n, dev), n, page_size, t, ld, max_pages, _i32("free_pages", free_pages, None, dev),
-          free_pages.numel(), _i32("head", head, 1, dev), o, o + 4 * (3 * n + 2), num_slots, o + 4 * (n + 1),
-          o + 4 * (2 * n + 1), o + 4 * (3 * n + 1), None if status is None else _i32("status", status, 1, dev))
-    starts, lens_out, pages_out, head_out, slots = out.split_with_sizes([n + 1, n, n, 1, num_slots])
-    return PagedStep(starts, slots, lens_out, pages_out, head_out)
+    return PagedStep._make(N.load_paged().reserve(lens, new_rows, pages, table, free_pages, head, page_size, num_slots,
+                                                  status))
 
 
 def paged_release(keep, pages, table, free_pages, head, page_size: int, status=None):
     """Request i keeps the pages of its first keep[i] rows; the others go back
     into ``free_pages`` below ``head``.  Returns (pages, head) afterwards."""
-    dev, n = _device(keep), keep.numel()
-    t, ld, max_pages = _table(table, n, dev)
-    out = torch.empty(n + 1, dtype=_I32, device=keep.device)
-    o = out.data_ptr()
-    _call("dflash_paged_release", dev, _i32("keep", keep, n, dev), _i32("pages", pages, n, dev), n, page_size, t, ld,
-          max_pages, _i32("free_pages", free_pages, None, dev), free_pages.numel(), _i32("head", head, 1, dev), o,
-          o + 4 * n, None if status is None else _i32("status", status, 1, dev))
-    return out.split_with_sizes([n, 1])
+    return N.load_paged().release(keep, pages, table, free_pages, head, page_size, status)
 
 
 def q4_pool(num_pages: int, num_kv_heads: int, page_size: int = 64, device="cuda") -> torch.Tensor:
@@ -161,31 +84,15 @@ def q4_append(k, v, slots, pool, status=None) -> None:
     """Quantise the rows k, v [rows, NKV, 128] (f16 or bf16, strided rows and
     heads) into their slots [rows] of the pool; slots must be distinct, and a
     row whose slot is outside the pool is skipped."""
-    dev = _device(pool)
-    num_pages, nkv, page_size = _pool(pool)
-    k, k_row, k_head = _rows("k", k, nkv, dev)
-    v, v_row, v_head = _rows("v", v, nkv, dev)
-    rows = k.shape[0]
-    if k.dtype is not v.dtype or v.shape[0] != rows:
-        raise ValueError("k and v must have the same type and number of rows")
-    _call("dflash_q4_append", dev, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, k.dtype is torch.bfloat16,
-          _i32("slots", slots, rows, dev), rows, nkv, pool.data_ptr(), num_pages, page_size,
-          None if status is None else _i32("status", status, 1, dev))
+    N.load_paged().append(k, v, slots, pool, status)
 
 
 def q4_read(pool, slots, dtype=torch.float16):
     """What the cache stands for at ``slots``: (k, v) [rows, NKV, 128], exact
     in f16 and bf16; zeros for a slot outside the pool."""
-    dev = _device(pool)
-    num_pages, nkv, page_size = _pool(pool)
     if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise ValueError("dtype must be torch.float16 or torch.bfloat16")
-    at, rows = _i32("slots", slots, None, dev), slots.numel()
-    k = torch.empty((rows, nkv, HEAD_DIM), dtype=dtype, device=pool.device)
-    v = torch.empty_like(k)
-    _call("dflash_q4_read", dev, pool.data_ptr(), num_pages, page_size, at, rows, nkv, dtype is torch.bfloat16,
-          k.data_ptr(), v.data_ptr())
-    return k, v
+    return N.load_paged().read(pool, slots, dtype is torch.bfloat16)
 
 
 def q4_attention_workspace(n: int, max_rows: int, num_heads: int, num_kv_heads: int, device="cuda") -> torch.Tensor:
@@ -213,26 +120,12 @@ def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: b
     lens); window: of those only the first ``sink`` and the last ``window``.
     A row that sees no key gives zeros; rows of q that no request owns leave
     their rows of ``out`` unwritten.  scale (positive) defaults to 128 ** -0.5."""
-    dev = _device(pool)
-    num_pages, nkv, page_size = _pool(pool)
-    q, q_row, q_head = _rows("q", q, None, dev)
-    rows, nq, _ = q.shape
-    n = lens.numel()
-    t, ld, max_pages = _table(table, n, dev)
-    if out is None:
-        out = torch.empty((rows, nq, HEAD_DIM), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of q's shape, type and device")
     if workspace is None:
-        workspace = q4_attention_workspace(n, max_rows, nq, nkv, q.device)
-    elif workspace.get_device() != dev:
-        raise ValueError(f"workspace must be on cuda:{dev}")
-    _call("dflash_q4_attention", dev, q.data_ptr(), q_row, q_head, q.dtype is torch.bfloat16, pool.data_ptr(), num_pages,
-          page_size, t, ld, max_pages, _i32("lens", lens, n, dev),
-          None if starts is None else _i32("starts", starts, n + 1, dev), n, rows, max_rows, nq, nkv, causal, sink,
-          window, HEAD_DIM ** -0.5 if scale is None else scale, out.data_ptr(),
-          None if status is None else _i32("status", status, 1, dev), workspace.data_ptr(), workspace.nbytes)
-    return out
+        if pool.dim() != 4 or q.dim() != 3:
+            raise ValueError("q must be [rows, heads, 128] and pool a tensor from q4_pool()")
+        workspace = q4_attention_workspace(lens.numel(), max_rows, q.shape[1], pool.shape[1], pool.device)
+    return N.load_paged().attention(q, pool, table, lens, starts, max_rows, causal, sink, window,
+                                    HEAD_DIM ** -0.5 if scale is None else scale, out, status, workspace)
 
 
 class PagedKVCacheQ4:
