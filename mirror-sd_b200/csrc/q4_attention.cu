@@ -68,27 +68,26 @@ struct QaCfg {
 };
 
 // A warp merges the partials of one item that the slots of `mask` hold (slot k
-// at parts + k * SLOT), all queries at once: 8 (16) loads of a partial's O are
-// on their way together.  Writes the item's output rows (finish) or one partial
-// at dst.
+// at at[k]), all queries at once: 8 (16) loads of a partial's O are on their way
+// together.  Writes the item's output rows (finish) or one partial at dst.
 template <int NT>
-__device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask, const float* parts, float* dst,
+__device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask, const float* const* at, float* dst,
                                             const Item& it, int sub, bool finish, int lane) {
-  constexpr int QT = QaCfg<NT>::QT, SLOT = QaCfg<NT>::SLOT;
+  constexpr int QT = QaCfg<NT>::QT;
   const int q = lane & (QT - 1);
   float M = -INFINITY, l = 0.f;
 #pragma unroll 1
-  for (uint32_t m = mask; m; m &= m - 1) M = fmaxf(M, __ldcg(parts + (__ffs(m) - 1) * SLOT + QT * 128 + q));
+  for (uint32_t m = mask; m; m &= m - 1) M = fmaxf(M, at[__ffs(m) - 1][QT * 128 + q]);
   float4 o[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
   for (uint32_t m = mask; m; m &= m - 1) {
-    const float* s = parts + (__ffs(m) - 1) * SLOT;
-    const float mk = __ldcg(s + QT * 128 + q), lk = __ldcg(s + QT * 129 + q);
+    const float* s = at[__ffs(m) - 1];
+    const float mk = s[QT * 128 + q], lk = s[QT * 129 + q];
     float4 v[QT];
 #pragma unroll
-    for (int i = 0; i < QT; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(s + i * 128 + 4 * lane));
+    for (int i = 0; i < QT; ++i) v[i] = *reinterpret_cast<const float4*>(s + i * 128 + 4 * lane);
     const float w = mk == -INFINITY ? 0.f : exp2_fast(mk - M);
     l = fmaf(w, lk, l);
 #pragma unroll
@@ -130,6 +129,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
   __shared__ int slot_item[2 * C::WARPS];   // unit at which the partial's item starts, or -1
   __shared__ Item slot_info[2 * C::WARPS];
   __shared__ int slot_sub[2 * C::WARPS];
+  __shared__ const float* slot_at[2 * C::WARPS];   // the partial: in the warp's ring if its run ended with it, else in p.part
   __shared__ int last_run[2];               // runs (of the CTA's two borders) this CTA must finish
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -190,21 +190,18 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     // lane b < 4 looks after row block b of a tile: its page, then its copy
     auto page_of = [&](const Cursor& k) {
       const int pos = item_tile(k.it, k.j) * QA_TILE + (lane & 3) * kQ4Rows;
-      int pg = -1;
-      if (lane < 4 && pos < k.it.L) {
-        pg = __ldg(p.table + (size_t)k.it.seq * p.table_ld + (pos >> p.page_shift));
-        if (pg < 0 || pg >= p.num_pages) pg = -1;   // hidden, like a masked block
-      }
-      return pg;
+      return lane < 4 && pos < k.it.L ? __ldg(p.table + (size_t)k.it.seq * p.table_ld + (pos >> p.page_shift)) : -1;
     };
     int next_page = page_of(ahead);
     uint32_t loaded = 0;   // 4 bits a stage: row blocks that were copied
     int fill = u0, fill_end = u1;   // tiles requested so far; fewer than the run after an expired wait
     auto issue = [&](int s) {
-      const uint32_t mask = __ballot_sync(0xffffffffu, next_page >= 0);
+      // (looked at only here, a tile after it was requested)
+      const bool there = next_page >= 0 && next_page < p.num_pages;   // else hidden, like a masked block
+      const uint32_t mask = __ballot_sync(0xffffffffu, there);
       if (lane == 0) mbar_arrive_expect_tx(&bar[s], __popc(mask) * kQ4Block);
       __syncwarp();
-      if (next_page >= 0) {
+      if (there) {
         const int pos = item_tile(ahead.it, ahead.j) * QA_TILE + lane * kQ4Rows;
         const int head = ahead.sub - p.by_nkv.of(ahead.sub) * p.nkv, bits = p.page_shift - 4;   // 16-row blocks a page: 2^bits
         bulk_load(ring + s * QA_STAGE + lane * kQ4Block,
@@ -440,7 +437,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
         const int grp = p.by_nkv.of(cur.sub), r0 = grp * QT, G0 = (cur.sub - grp * p.nkv) * G;
         // the first slot of a warp: a segment that began before the run or fills it
         const int slot = 2 * warp + (seg_first == u0 ? 0 : 1);
-        float* part = p.part + ((size_t)cta * 2 * C::WARPS + slot) * C::SLOT;
+        float* part = u == u1 ? reinterpret_cast<float*>(ring) : p.part + ((size_t)cta * C::WARPS + warp) * C::SLOT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -465,6 +462,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
           slot_item[slot] = item0;
           slot_info[slot] = cur.it;
           slot_sub[slot] = cur.sub;
+          slot_at[slot] = part;
         }
         fresh = true;
       }
@@ -473,24 +471,24 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
   }
   __syncthreads();   // partials of the CTA's warps are written (and visible to its threads)
 
-  // Runs of slots that belong to one item, in order; the runs go to the warps in turn.
-  // An item inside the CTA's range ends here; one that reaches past a border
-  // leaves one partial of the CTA and the last CTA to arrive finishes it.
-  float* cta_part = p.part + (size_t)gridDim.x * 2 * C::WARPS * C::SLOT;
+  // Slots that belong to one item lie side by side; the items go to the warps in
+  // turn.  An item inside the CTA's range ends here; one that reaches past a
+  // border leaves one partial of the CTA and the last CTA to arrive finishes it.
+  float* cta_part = p.part + (size_t)gridDim.x * C::WARPS * C::SLOT;
   {
-    int run = 0, k = 0;
-    while (k < 2 * C::WARPS) {
-      if (slot_item[k] < 0) { ++k; continue; }
-      const int item0 = slot_item[k], first = k;
-      uint32_t mask = 0;
-      for (; k < 2 * C::WARPS && (slot_item[k] < 0 || slot_item[k] == item0); ++k)
-        if (slot_item[k] == item0) mask |= 1u << k;
-      if (run++ % C::WARPS != warp) continue;
+    const int held = lane < 2 * C::WARPS ? slot_item[lane] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, held);
+    uint32_t heads = __ballot_sync(0xffffffffu, held >= 0 && lane == __ffs(same) - 1);
+#pragma unroll 1
+    for (int run = 0; heads; heads &= heads - 1, ++run) {
+      const int first = __ffs(heads) - 1;
+      const uint32_t mask = __shfl_sync(0xffffffffu, same, first);
+      if (run % C::WARPS != warp) continue;
+      const int item0 = slot_item[first];
       const Item it = slot_info[first];
       const bool inside = item0 >= c0 && item0 + it.ntile <= c1;
       const int border = item0 < c0 ? 0 : 1;
-      merge_slots<NT>(p, mask, p.part + (size_t)cta * 2 * C::WARPS * C::SLOT, cta_part + ((size_t)cta * 2 + border) * C::SLOT,
-                      it, slot_sub[first], inside, lane);
+      merge_slots<NT>(p, mask, slot_at, cta_part + ((size_t)cta * 2 + border) * C::SLOT, it, slot_sub[first], inside, lane);
       if (!inside) {
         __threadfence();
         __syncwarp();
@@ -533,7 +531,7 @@ static int q4_attn_nt(int max_rows, int nq, int nkv) { return (long long)max_row
 
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms) {
   const int nt = q4_attn_nt(max_rows, nq, nkv);
-  return (size_t)num_sms * (nt == 1 ? (2 * QaCfg<1>::WARPS + 2) * QaCfg<1>::SLOT : (2 * QaCfg<2>::WARPS + 2) * QaCfg<2>::SLOT);
+  return (size_t)num_sms * (nt == 1 ? (QaCfg<1>::WARPS + 2) * QaCfg<1>::SLOT : (QaCfg<2>::WARPS + 2) * QaCfg<2>::SLOT);
 }
 
 template <int NT>
