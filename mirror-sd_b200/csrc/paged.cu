@@ -67,6 +67,8 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
   __shared__ int taken;
   if (threadIdx.x == 0) taken = 0;
   __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
   const int head = min(max(__ldg(p.head), 0), p.num_pages);
   const int room = p.num_pages - head;
   long long carry_r = 0;
@@ -147,6 +149,8 @@ __global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(const Release
   const int n = p.n;
   int* first = sm;         // [n] pages given back before this request
   int* left = first + n;   // [n] pages kept
+  griddep_wait();
+  griddep_launch_dependents();
   const int head = min(max(__ldg(p.head), 0), p.num_pages);
   int carry = 0;
   for (int i0 = 0; i0 < n; i0 += PG_THREADS) {
@@ -184,16 +188,14 @@ cudaError_t paged_reserve_launch(const ReserveParams& p, int num_sms, cudaStream
   if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
   const int want = (p.num_slots + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
   const int grid = want < 1 ? 1 : want > num_sms ? num_sms : want;
-  paged_reserve_kernel<<<grid, PG_THREADS, (size_t)p.n * 16, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(paged_reserve_kernel, dim3(grid), dim3(PG_THREADS), (size_t)p.n * 16, st, p);
 }
 
 cudaError_t paged_release_launch(const ReleaseParams& p, int num_sms, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
   const long long want = ((long long)p.n * p.max_pages + 16 * PG_THREADS - 1) / (16 * PG_THREADS);
   const int grid = want < 1 ? 1 : want > num_sms ? num_sms : (int)want;
-  paged_release_kernel<<<grid, PG_THREADS, (size_t)p.n * 8, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(paged_release_kernel, dim3(grid), dim3(PG_THREADS), (size_t)p.n * 8, st, p);
 }
 
 }  // namespace dfl

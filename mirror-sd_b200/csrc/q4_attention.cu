@@ -141,6 +141,8 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     last_run[0] = last_run[1] = -1;
   }
   if (threadIdx.x < 2 * C::WARPS) slot_item[threadIdx.x] = -1;
+  griddep_wait();
+  griddep_launch_dependents();
   // tiles of every request, added up (kPagedMaxSeqs / C::THREADS passes at most)
   int total = 0;
   for (int i0 = 0; i0 < p.n; i0 += C::THREADS) {
@@ -538,8 +540,7 @@ template <int NT>
 static cudaError_t launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
   const size_t smem = QaCfg<NT>::RING + QaCfg<NT>::WARPS * QaCfg<NT>::STAGES * 8 + ((size_t)p.n + 1) * 4;
   DFL_TRY(cudaFuncSetAttribute(q4_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  q4_attn_kernel<NT><<<num_sms, QaCfg<NT>::THREADS, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(q4_attn_kernel<NT>, dim3(num_sms), dim3(QaCfg<NT>::THREADS), smem, st, p);
 }
 
 cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {

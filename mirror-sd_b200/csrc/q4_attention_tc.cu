@@ -265,6 +265,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     ms.border[0].seq = ms.border[1].seq = -1;
     fence_mbar_init();
   }
+  griddep_wait();
+  griddep_launch_dependents();
   if (warp == QB_MMA) {
     tmem_alloc(&ms.tmem, 512);
     tmem_relinquish();
@@ -1015,8 +1017,7 @@ static cudaError_t launch_tc(const Q4AttnParams& p, int num_sms, cudaStream_t st
   constexpr size_t smem = C::MISC_OFF + sizeof(QbMisc<C>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
   DFL_TRY(cudaFuncSetAttribute(q4_attn_tc_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  q4_attn_tc_kernel<N><<<num_sms, QB_THREADS, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(q4_attn_tc_kernel<N>, dim3(num_sms), dim3(QB_THREADS), smem, st, p);
 }
 
 cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {

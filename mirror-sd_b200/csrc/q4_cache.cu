@@ -50,6 +50,8 @@ template <bool BF16>
 __global__ void __launch_bounds__(256) q4_append_kernel(const Q4AppendParams p) {
   const int t = threadIdx.x, g = t & 7, which = t >> 7;
   const int row = blockIdx.x * 16 + (t >> 3 & 15), h = blockIdx.y;
+  griddep_wait();
+  griddep_launch_dependents();
   int slot = row < p.T ? __ldg(p.slots + row) : -1;
   if (slot >= p.num_slots) slot = -1;
   const int other_slot = __shfl_xor_sync(0xffffffffu, slot, 8);   // of the row beside it
@@ -143,6 +145,8 @@ template <bool BF16>
 __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
   const int t = threadIdx.x, g = t & 7, which = t >> 7;
   const int row = blockIdx.x * 16 + (t >> 3 & 15), h = blockIdx.y;
+  griddep_wait();
+  griddep_launch_dependents();
   if (row >= p.T) return;
   const int slot = __ldg(p.slots + row);
   uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -191,21 +195,13 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
 cudaError_t q4_append_launch(const Q4AppendParams& p, cudaStream_t st) {
   if (p.T < 1 || p.nkv < 1 || p.nkv > 65535) return cudaErrorInvalidValue;
   const dim3 grid((p.T + 15) / 16, p.nkv);
-  if (p.bf16)
-    q4_append_kernel<true><<<grid, 256, 0, st>>>(p);
-  else
-    q4_append_kernel<false><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(p.bf16 ? q4_append_kernel<true> : q4_append_kernel<false>, grid, dim3(256), 0, st, p);
 }
 
 cudaError_t q4_read_launch(const Q4ReadParams& p, cudaStream_t st) {
   if (p.T < 1 || p.nkv < 1 || p.nkv > 65535) return cudaErrorInvalidValue;
   const dim3 grid((p.T + 15) / 16, p.nkv);
-  if (p.bf16)
-    q4_read_kernel<true><<<grid, 256, 0, st>>>(p);
-  else
-    q4_read_kernel<false><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(p.bf16 ? q4_read_kernel<true> : q4_read_kernel<false>, grid, dim3(256), 0, st, p);
 }
 
 }  // namespace dfl
