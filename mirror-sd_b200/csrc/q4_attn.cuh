@@ -146,31 +146,44 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// A warp merges one query's partials of `count` CTAs: slots(k) holds O at
+// A warp merges one query's partials of `count` runs: slots(k) holds O at
 // q * 128, m at qt * 128 + q and l at qt * 129 + q.  Returns channels 4 lane ..
-// of the output row.  8 loads of O are on their way together.
+// of the output row.  8 loads of O are on their way together, the first ones
+// with those of m and l: few partials cost one round trip to L2.
 template <class SlotAt>
 __device__ __forceinline__ void merge_query(int count, SlotAt slots, int qt, int q, int lane, float (&v)[4]) {
-  float M = -INFINITY, l = 0.f;
+  float4 x[8];
+  auto load = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)   // (past the end: the last one again, with weight 0)
+      x[i] = __ldcg(reinterpret_cast<const float4*>(slots(min(k + i, count - 1)) + q * 128 + 4 * lane));
+  };
+  load(0);
+  float m = -INFINITY, s = 0.f;
+  if (lane < count) {
+    m = __ldcg(slots(lane) + qt * 128 + q);
+    s = __ldcg(slots(lane) + qt * 129 + q);
+  }
+  float M = m;
 #pragma unroll 1
-  for (int k = lane; k < count; k += 32) M = fmaxf(M, __ldcg(slots(k) + qt * 128 + q));
+  for (int k = lane + 32; k < count; k += 32) M = fmaxf(M, __ldcg(slots(k) + qt * 128 + q));
   M = warp_max(M);
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
 #pragma unroll 1
   for (int k0 = 0; k0 < count; k0 += 32) {
-    float w = 0.f;
-    if (k0 + lane < count) {
-      const float m = __ldcg(slots(k0 + lane) + qt * 128 + q);
-      w = m == -INFINITY ? 0.f : exp2_fast(m - M);
-      l = fmaf(w, __ldcg(slots(k0 + lane) + qt * 129 + q), l);
+    if (k0 > 0) {
+      m = -INFINITY;
+      if (k0 + lane < count) {
+        m = __ldcg(slots(k0 + lane) + qt * 128 + q);
+        s = __ldcg(slots(k0 + lane) + qt * 129 + q);
+      }
     }
+    const float w = m == -INFINITY ? 0.f : exp2_fast(m - M);
+    l = fmaf(w, s, l);
     const int n = min(count - k0, 32);
 #pragma unroll 1
     for (int k = 0; k < n; k += 8) {
-      float4 x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)   // (past the end: the last one again, with weight 0)
-        x[i] = __ldcg(reinterpret_cast<const float4*>(slots(k0 + min(k + i, n - 1)) + q * 128 + 4 * lane));
+      if (k0 + k > 0) load(k0 + k);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float wi = __shfl_sync(0xffffffffu, w, k + i);
