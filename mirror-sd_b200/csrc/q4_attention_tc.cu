@@ -40,6 +40,7 @@ namespace dfl {
 constexpr int QB_TILE = 128;
 constexpr int QB_BLK = kQ4Block + 32;      // a row block's stride in shared memory: 8 blocks on different banks
 constexpr int QB_STAGE = QB_TILE / kQ4Rows * QB_BLK;
+constexpr int QB_SLACK = 6;
 constexpr float QB_RAISE = 8.f;
 constexpr float QB_UNSET = 1e30f;          // -reference of a column that has seen no key
 
@@ -81,7 +82,8 @@ struct QbMisc {
   uint64_t q_ready[2], q_free[2], o_free;
   uint32_t tmem;
   int abort;
-  int where[3];                   // request of the CTA's first tile, and that request's first tile
+  int where[2];                   // request of the CTA's first tile, and that request's first tile
+  int run[2], share[2];           // whole CTAs to an item: this one's tiles; the item's first CTA and their number
   int wtot[QB_THREADS / 32];
   int2 tile[16];                  // row blocks copied, rows below the request's end
   QbSeg seg[C::SEGS];
@@ -263,6 +265,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], 4); }
     ms.abort = 0;
     ms.border[0].seq = ms.border[1].seq = -1;
+    ms.run[0] = ms.run[1] = 0;
     fence_mbar_init();
   }
   griddep_wait();
@@ -273,48 +276,92 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   }
   for (int i = threadIdx.x; i < 2 * N; i += QB_THREADS) ms.cmax[0][i] = float_key(-INFINITY);
 
-  // Tiles of all requests, and the request of this CTA's first one: two passes
-  // over the lengths (the total comes first).
-  int total = 0, ctas = 0, c0 = 0, c1 = 0;
+  // The CTA's run of tiles [c0, c1), from the lengths.
+  auto scan = [&](int v, int* sum) {   // what the threads before hold, and the sum of all
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) ms.wtot[warp] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < QB_THREADS / 32; ++w) {
+      if (w < warp) before += ms.wtot[w];
+      all += ms.wtot[w];
+    }
+    *sum = all;
+    return before + x - v;
+  };
+  const int grid = gridDim.x;
+  int total = 0, c0 = 0, c1 = 0, items = 0, ntile = 0, first = 0;   // (the last three of request threadIdx.x)
 #pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    int sum = 0;
+  for (int i0 = 0; i0 < p.n; i0 += QB_THREADS) {
+    const int i = i0 + threadIdx.x;
+    items = ntile = 0;
+    if (i < p.n) {
+      const Item it = load_item<QB_TILE, N>(p, i);
+      ntile = it.ntile;
+      items = it.groups * p.nkv;
+    }
+    int sum;
+    first = scan(items * ntile, &sum);
+    total += sum;
+  }
+  // With few items, whole CTAs to each: a run that crosses from one item into the
+  // next pays the start and the end of an item (6 to 8 us together) twice.  An
+  // item takes a CTA for every `quota` of its tiles, the least number with which
+  // the grid holds them all, if that is at most QB_SLACK tiles more than equal
+  // runs would have.  (8 items of 64 tiles 29.2 us in equal runs, 21.0 in whole
+  // CTAs; 16 of 257 tiles, 160 query rows, 64.3 and 55.7.)
+  int quota = 0;
+  if (p.n <= QB_THREADS && total > grid) {
+    int lo = (total + grid - 1) / grid, hi = lo + QB_SLACK + 1, sum;
+#pragma unroll 1
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      scan(items * ((ntile + mid - 1) / mid), &sum);
+      if (sum <= grid) { hi = mid; quota = mid; } else lo = mid + 1;
+    }
+  }
+  if (quota > 0) {
+    const int parts = (ntile + quota - 1) / quota;
+    int sum;
+    const int rel = (int)blockIdx.x - scan(items * parts, &sum);
+    if (rel >= 0 && rel < items * parts) {
+      const int sub = rel / parts, part = rel - sub * parts, item0 = first + sub * ntile;
+      const Runs runs(ntile, parts);
+      ms.where[0] = threadIdx.x;
+      ms.where[1] = first;
+      ms.run[0] = item0 + runs.start(part);
+      ms.run[1] = item0 + runs.start(part + 1);
+      ms.share[0] = blockIdx.x - part;
+      ms.share[1] = parts;
+    }
+  } else {
+    const int ctas = min(grid, total);
+    const Runs runs(total, ctas);
+    if ((int)blockIdx.x < ctas) {
+      c0 = runs.start(blockIdx.x);
+      c1 = runs.start(blockIdx.x + 1);
+    }
+    int before = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < p.n; i0 += QB_THREADS) {
       const int i = i0 + threadIdx.x;
-      int v = 0;
+      int v = 0, sum;
       if (i < p.n) {
         const Item it = load_item<QB_TILE, N>(p, i);
         v = it.ntile * it.groups * p.nkv;
       }
-      int x = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      __syncthreads();
-      if (lane == 31) ms.wtot[warp] = x;
-      __syncthreads();
-      int before = sum;
-#pragma unroll
-      for (int w = 0; w < QB_THREADS / 32; ++w) {
-        if (w < warp) before += ms.wtot[w];
-        sum += ms.wtot[w];
-      }
-      const int first = before + x - v;
-      if (pass == 1 && first <= c0 && c0 < first + v) {
+      const int at = before + scan(v, &sum);
+      before += sum;
+      if (at <= c0 && c0 < at + v) {
         ms.where[0] = i;
-        ms.where[1] = first;
-      }
-    }
-    if (pass == 0) {
-      total = sum;
-      ctas = min((int)gridDim.x, total);
-      if ((int)blockIdx.x < ctas) {
-        const Runs runs(total, ctas);
-        c0 = runs.start(blockIdx.x);
-        c1 = runs.start(blockIdx.x + 1);
+        ms.where[1] = at;
       }
     }
   }
@@ -322,7 +369,18 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ms.tmem;
+  if (quota > 0) {
+    c0 = ms.run[0];
+    c1 = ms.run[1];
+  }
   const int T = c1 - c0;
+  // the CTAs that hold an item (of ntile tiles, the first of them tile item0): the first one and their number
+  auto sharers = [&](int item0, int ntile) {
+    if (quota > 0) return make_int2(ms.share[0], ms.share[1]);
+    const Runs runs(total, min(grid, total));
+    const int from = runs.of(item0);
+    return make_int2(from, runs.of(item0 + ntile - 1) - from + 1);
+  };
 
   // ring cursors start at the same place in the producer and the query warp
   auto first_cursor = [&](Cursor& c) {
@@ -638,7 +696,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         named_bar_sync(3, 256);
         if (threadIdx.x == 0) {
           __threadfence();
-          atomicAdd(&p.counters[2 * Runs(total, ctas).of(sg.item0)], 1);
+          atomicAdd(&p.counters[2 * sharers(sg.item0, it.ntile).x], 1);
         }
       }
       t0 += nt;
@@ -649,10 +707,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     for (int border = 0; border < 2; ++border) {
       const auto bd = ms.border[border];
       if (bd.seq < 0) continue;
-      const int item0 = bd.item0;
-      const Runs runs(total, ctas);
-      const int from = runs.of(item0), to = runs.of(item0 + bd.nt - 1);
-      const int count = to - from + 1;
+      const int2 share = sharers(bd.item0, bd.nt);
+      const int from = share.x, count = share.y;
       if (threadIdx.x == 0) {
         int ok = 0;
         for (uint32_t i = 0; i < kSpinLimit && !ok && !*dead; ++i) {
