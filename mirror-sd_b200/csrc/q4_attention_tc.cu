@@ -47,9 +47,11 @@ constexpr float QB_UNSET = 1e30f;          // -reference of a column that has se
 template <int N_>
 struct QbCfg {
   static constexpr int N = N_, CH = N / 16;
-  static constexpr int QB = 2;                  // query buffers
+  // Query buffers and packed stages.  With 80 columns shared memory holds two and
+  // two or one and three (8 requests of 16,384 rows, 160 query rows: 178 and 174 us).
+  static constexpr int QB = N <= 64 ? 2 : 1;
   static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S)
-  static constexpr int NS = N <= 64 ? 4 : 2;    // packed stages
+  static constexpr int NS = N <= 64 ? 4 : 3;
   static constexpr bool AHEAD = N <= 64;        // registers for the next 16 scores
   static constexpr int SEGS = 8;                // ring of item records
   static constexpr int P_BYTES = (N + 63) / 64 * 16384;       // 64-column chunks of [128 rows][128 B]

@@ -141,35 +141,50 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const Q4AppendParams p) 
   }
 }
 
+// (Two heads a thread, their loads on the way together: what bounds this kernel
+// is the latency of slot, codes and scale, one after the other.)
 template <bool BF16>
 __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
   const int t = threadIdx.x, g = t & 7, which = t >> 7;
-  const int row = blockIdx.x * 16 + (t >> 3 & 15), h = blockIdx.y;
+  const int row = blockIdx.x * 16 + (t >> 3 & 15), h0 = 2 * blockIdx.y;
   griddep_wait();
   griddep_launch_dependents();
   if (row >= p.T) return;
   const int slot = __ldg(p.slots + row);
-  uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (slot >= 0 && slot < p.num_slots) {
-    const int bits = p.page_shift - 4;
-    const uint8_t* blk = p.pool + ((((size_t)(slot >> p.page_shift) * p.nkv + h) << bits) +
+  const bool there = slot >= 0 && slot < p.num_slots;
+  const int bits = p.page_shift - 4, rr = slot & 15;
+  uint4 w[2] = {};
+  uint32_t code[2] = {0, 0};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (!there || h0 + x >= p.nkv) continue;
+    const uint8_t* blk = p.pool + ((((size_t)(slot >> p.page_shift) * p.nkv + h0 + x) << bits) +
                                    (slot / kQ4Rows & ((1 << bits) - 1))) * kQ4Block;
-    const int rr = slot & 15;
-    const uint32_t code = __ldg(blk + (which ? kQ4VS + g * 16 + rr : kQ4KS + rr * 8 + g));
-    const uint32_t s = code << 7 | code << 23, ns = hmul2_u(s, 0xBE00BE00u);   // the scale twice; -1.5 s
+    code[x] = __ldg(blk + (which ? kQ4VS + g * 16 + rr : kQ4KS + rr * 8 + g));
     if (which == 0) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8));
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(blk + q4_k_piece(rr, g >> 1) + (g & 1) * 8));
+      w[x].x = v.x;
+      w[x].y = v.y;
+    } else {
+      w[x] = __ldg(reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(rr >> 1, g)));
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (h0 + x >= p.nkv) break;
+    uint32_t o[8];   // (a slot outside the pool: scale 0 and codes 0)
+    const uint32_t s = code[x] << 7 | code[x] << 23, ns = hmul2_u(s, 0xBE00BE00u);   // the scale twice; -1.5 s
+    if (which == 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t ww = i ? w.y : w.x;
+        const uint32_t ww = i ? w[x].y : w[x].x;
         o[4 * i] = dequant<0>(ww, s, ns);
         o[4 * i + 1] = dequant<1>(ww, s, ns);
         o[4 * i + 2] = dequant<2>(ww, s, ns);
         o[4 * i + 3] = dequant<3>(ww, s, ns);
       }
     } else {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(blk + kQ4V + q4_v_piece(rr >> 1, g)));
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      const uint32_t ww[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t hw = (rr & 1) ? ww[i] >> 16 : ww[i] & 0xffffu;
@@ -180,16 +195,16 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      o[i] = hmul2_u(o[i], 0x4C004C00u);   // times 16
+      o[i] = there ? hmul2_u(o[i], 0x4C004C00u) : 0u;   // times 16
       if (BF16) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
         o[i] = pack_bf16x2(f.x, f.y);
       }
     }
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(which ? p.v : p.k) + 2 * (((size_t)row * p.nkv + h0 + x) * 128 + 16 * g));
+    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
-  uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(which ? p.v : p.k) + 2 * (((size_t)row * p.nkv + h) * 128 + 16 * g));
-  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 cudaError_t q4_append_launch(const Q4AppendParams& p, cudaStream_t st) {
@@ -200,7 +215,7 @@ cudaError_t q4_append_launch(const Q4AppendParams& p, cudaStream_t st) {
 
 cudaError_t q4_read_launch(const Q4ReadParams& p, cudaStream_t st) {
   if (p.T < 1 || p.nkv < 1 || p.nkv > 65535) return cudaErrorInvalidValue;
-  const dim3 grid((p.T + 15) / 16, p.nkv);
+  const dim3 grid((p.T + 15) / 16, (p.nkv + 1) / 2);
   return launch_pdl(p.bf16 ? q4_read_kernel<true> : q4_read_kernel<false>, grid, dim3(256), 0, st, p);
 }
 
