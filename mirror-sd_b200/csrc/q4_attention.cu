@@ -21,8 +21,8 @@
 //   O^T[128, QT]    += V^T[128, 16] P^T    8 channel tiles
 // with the rows (then the channels) as the tile's 16 rows, so QT = 8 query
 // rows waste no half of the instruction as query-major tiles of 16 would.
-// Codes become f16 by bit placement: (w >> k) & 0x03C0 | 0x3C00 is 1 + u/16,
-// and one f16 FMA gives x / 16 = (1 + u/16) s - 1.5 s exactly (every term has
+// Codes become f16 by bit placement: (w >> k) & 0x00F0 | 0x3C00 is 1 + u/64,
+// and one f16 FMA gives x / 16 = (1 + u/64) 4s - 4.5s exactly (every term has
 // at most 7 significant bits).  The factors 16 go into the softmax scale and
 // the final division.  S^T leaves the products with a lane holding two query
 // columns of a row; packing those two and transposing 8x8 blocks (movmatrix)
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
             for (int w = 0; w < 4; ++w) {   // channels 32c + 8w .. + 7: group 2c + w / 2
               const uint32_t sa = __byte_perm(s2a, 0, w < 2 ? 0x1010 : 0x3232);
               const uint32_t sb = __byte_perm(s2b, 0, w < 2 ? 0x1010 : 0x3232);
-              const uint32_t na = hmul2_u(sa, 0xBE00BE00u), nb = hmul2_u(sb, 0xBE00BE00u);   // -1.5 s
+              const uint32_t na = scale_shift(sa), nb = scale_shift(sb);
               const uint32_t a0 = dequant<0>(ka[w], sa, na), a2 = dequant<1>(ka[w], sa, na);
               const uint32_t a1 = dequant<0>(kb[w], sb, nb), a3 = dequant<1>(kb[w], sb, nb);
               const uint32_t e0 = dequant<2>(ka[w], sa, na), e2 = dequant<3>(ka[w], sa, na);
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
               sa &= (2 * c < left ? 0xffffu : 0u) | (2 * c + 1 < left ? 0xffff0000u : 0u);
               sb &= (2 * c + 8 < left ? 0xffffu : 0u) | (2 * c + 9 < left ? 0xffff0000u : 0u);
             }
-            const uint32_t na = hmul2_u(sa, 0xBE00BE00u), nb = hmul2_u(sb, 0xBE00BE00u);
+            const uint32_t na = scale_shift(sa), nb = scale_shift(sb);
             const uint32_t va[4] = {wa.x, wa.y, wa.z, wa.w}, vb[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {   // channels 16g + 4w .. + 3: tiles 2w and 2w + 1

@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           uint32_t out[16];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t sp = __byte_perm(two, 0, i < 2 ? 0x1010 : 0x3232), ns = hmul2_u(sp, 0xBE00BE00u);
+            const uint32_t sp = __byte_perm(two, 0, i < 2 ? 0x1010 : 0x3232), ns = scale_shift(sp);
             out[4 * i] = dequant<0>(w[i], sp, ns);
             out[4 * i + 1] = dequant<1>(w[i], sp, ns);
             out[4 * i + 2] = dequant<2>(w[i], sp, ns);
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
           sp[jj] = scale_pair((jj < 2 ? sc.x : sc.y) >> (16 * (jj & 1)));
-          ns[jj] = hmul2_u(sp[jj], 0xBE00BE00u);
+          ns[jj] = scale_shift(sp[jj]);
         }
         uint8_t* vt = smem + C::V_OFF + (t & 1) * C::V_BYTES + chunk * 16384 + g * 2048;
 #pragma unroll 1

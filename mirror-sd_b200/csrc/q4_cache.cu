@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4ReadParams p) {
   for (int x = 0; x < 2; ++x) {
     if (h0 + x >= p.nkv) break;
     uint32_t o[8];   // (a slot outside the pool: scale 0 and codes 0)
-    const uint32_t s = code[x] << 7 | code[x] << 23, ns = hmul2_u(s, 0xBE00BE00u);   // the scale twice; -1.5 s
+    const uint32_t s = scale_pair(code[x] | code[x] << 8), ns = scale_shift(s);
     if (which == 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
