@@ -121,7 +121,11 @@ cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
 // the same for blocks of query rows (q4_attention_tc.cu)
 size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms);
 cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
-// query rows of a kv head up to which the first kernel runs
+// Query rows of a kv head (rows of a request times G) up to which the first
+// kernel runs; it takes them 16 at a time and decodes the cache for each group.
+// us, first kernel / second, on 1 request of 2,048 rows, 16 of 16,384, 256 of
+// 1,024 (8 kv heads): 16 query rows 14 / 14, 118 / 118, 125 / 155; 20 query rows
+// 15 / 14, 214 / 119, 224 / 158; 64 query rows 16 / 18, 412 / 151, 419 / 212.
 constexpr int kQ4FewRows = 16;
 
 }  // namespace dfl
