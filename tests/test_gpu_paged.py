@@ -448,3 +448,105 @@ def test_operators_refuse_bad_arguments(pkg):
     assert A(q[:0], pool, table, lens, starts=_dev([0, 0, 0])).shape == (0, 4, 128)
     pkg.q4_append(kv[:0], kv[:0], slots[:0], pool)
     assert pkg.q4_read(pool, slots[:0])[0].shape == (0, 2, 128)
+
+
+# ---------------------------------------------------------------- blocks of query rows (more than 16 a kv head)
+@pytest.mark.parametrize("lens,rows,nq,nkv", [
+    ([20000], [16], 4, 1),                                      # one item over the whole GPU
+    ([9000, 0, 3000, 130], [16, 8, 20, 3], 8, 2),               # few items, whole CTAs to each
+    ([40000] + [100] * 70, [5] * 71, 8, 2),                     # too uneven for that: equal runs
+    ([2000, 2100, 1900, 1, 2050], [40, 32, 33, 40, 0], 10, 2),  # groups of 80 columns, one not full
+])
+def test_block_attention_shares_out_the_work(pkg, lens, rows, nq, nkv):
+    c = Case(pkg, lens, rows, nq, nkv, 64, torch.float16, seed=len(lens))
+    c.check(pkg, causal=True)
+    a = c.check(pkg, sink=64, window=1000)
+    assert torch.equal(a, c.check(pkg, sink=64, window=1000))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("step", [0.02, 0.3])
+def test_block_attention_raises_the_maximum_late(pkg, causal, step):
+    """Keys that grow along the cache, by less and by more than a tile's reference allows; one query the other way."""
+    L = 1500
+    c = Case(pkg, [L], [12], 4, 1, 64, torch.float16)
+    k = torch.zeros(L, 1, 128)
+    k[:, 0, 0] = torch.linspace(0, step * L, L)
+    k = k.to(torch.float16)
+    v = (torch.randn(L, 1, 128, generator=torch.Generator().manual_seed(1)) * 0.5).to(torch.float16)
+    pkg.q4_append(k.cuda(), v.cuda(), c.pg.slots[0].cuda(), c.pool)
+    c.k[0], c.v[0] = U.q4_values(k), U.q4_values(v)
+    c.q[:] = 0
+    c.q[:, :, 0] = torch.tensor([10.0, 5.0, -10.0, 1.0]).cuda()
+    c.check(pkg, causal=causal)
+
+
+@pytest.mark.parametrize("dtype,qscale", [(torch.float16, 30.0), (torch.bfloat16, 30.0), (torch.bfloat16, 1e-6),
+                                          (torch.bfloat16, 1e6)])
+@pytest.mark.parametrize("nq,nkv", [(4, 1), (5, 1), (4, 4)])
+def test_block_attention_of_sharp_and_flat_softmax(pkg, dtype, qscale, nq, nkv):
+    c = Case(pkg, [300, 65, 900, 129], [8, 6, 17, 1], nq, nkv, 32, dtype, qscale=qscale)
+    if qscale == 1e6:
+        c.q[3] *= 1e-9                    # rows of very different sizes in one block
+    c.check(pkg, scale=128 ** -0.5 * (1e-5 if qscale == 1e6 else 1.0), causal=True)
+
+
+def test_operators_in_a_cuda_graph(pkg):
+    """A captured step gives the same bits at every replay, on changed rows."""
+    c = Case(pkg, [700, 33], [5, 5], 8, 2, 64, torch.float16)
+    ws = pkg.q4_attention_workspace(2, 5, 8, 2)
+    slots = torch.cat([s[-5:] for s in c.pg.slots]).to(i32).cuda()
+    k = torch.randn(10, 2, 128).half().cuda()
+    table, lens = c.pg.dev("table"), c.pg.dev("lens")
+
+    def step():
+        pkg.q4_append(k, k, slots, c.pool)
+        return pkg.q4_attention(c.q, c.pool, table, lens, starts=c.starts, max_rows=5, causal=True, workspace=ws)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2):
+        k.copy_(torch.randn(10, 2, 128, generator=torch.Generator().manual_seed(seed)).half())
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, step())
+
+
+def test_cache_object_used_on_two_streams(pkg):
+    """The same steps on one stream, and on two that take turns."""
+    g = torch.Generator().manual_seed(3)
+    rows = [torch.randn(40, 2, 128, generator=g).half().cuda() for _ in range(6)]
+    outs = []
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for two in (False, True):
+        cache, got = pkg.PagedKVCacheQ4(1, 64, 2, 2, 400, 16), []
+        for i, k in enumerate(rows):
+            st = streams[i % 2 if two else 0]
+            st.wait_stream(torch.cuda.current_stream())
+            st.wait_stream(streams[1 - i % 2 if two else 0])
+            with torch.cuda.stream(st):
+                step = cache.reserve([25, 15])
+                cache.append(0, k, k, step)
+                got.append(cache.attend(0, k.repeat(1, 2, 1), step, 25))
+                cache.trim([3, 2])
+                cache.release()
+        torch.cuda.synchronize()
+        cache.check()
+        outs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_cache_object_refuses(pkg):
+    cache = pkg.PagedKVCacheQ4(1, 8, 2, 2, 100, 16)
+    for bad in (lambda: cache.trim(-1), lambda: cache.trim([1, -1]), lambda: cache.trim(torch.ones(3, dtype=i32).cuda()),
+                lambda: cache.trim(torch.ones(2).cuda()), lambda: cache.release([2]), lambda: cache.read(0, 2, 1),
+                lambda: cache.read(0, 0, 1000), lambda: cache.reserve(torch.ones(2, dtype=i32).cuda())):
+        with pytest.raises(ValueError):
+            bad()
+    cache.reserve([20, 5])
+    cache.trim(torch.tensor([-4, 3], dtype=i32).cuda())       # a negative count on the device trims nothing
+    assert cache.lens.tolist() == [20, 2]
+    cache.trim(torch.tensor([30, 0]).cuda())
+    assert cache.lens.tolist() == [0, 2]
