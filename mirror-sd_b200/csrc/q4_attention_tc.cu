@@ -206,11 +206,6 @@ __device__ __forceinline__ bool named_bar_or(int id, bool v) {
       : "memory");
   return o != 0;
 }
-__device__ __forceinline__ float redux_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   uint64_t x, y, r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
@@ -542,20 +537,29 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
 #pragma unroll 1
         for (int round = 0; round < 2; ++round) {
           if (raise) {
-            // column maxima of the tile over the lanes, then over the warps
+            // Column maxima of the tile over the lanes, 16 columns at a time through
+            // this side's P (its last reader is done), then over the warps.
+            wait_pv();
+            float* stage = reinterpret_cast<float*>(smem + C::P_OFF + x * C::P_BYTES) + (warp & 3) * (16 * 36);
 #pragma unroll 1
             for (int c = 0; c < C::CH; ++c) {
               uint32_t s[16];
               tmem_ld16(s_t + 16 * c, s);
               tmem_ld_wait();
-              float mine = -INFINITY;
+              // rounded up: no score lies above its reference, however large both are
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                // rounded up: no score lies above its reference, however large both are
-                const float m = redux_max(__fmul_ru(__uint_as_float(s[i]), f));
-                mine = lane == i ? m : mine;
+              for (int i = 0; i < 16; ++i) stage[i * 36 + lane] = __fmul_ru(__uint_as_float(s[i]), f);
+              __syncwarp();
+              float top = -INFINITY, top2 = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(stage + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * i);
+                top = max3(top, v.x, v.y);
+                top2 = max3(top2, v.z, v.w);
               }
-              if (lane < 16) atomicMax(&ms.cmax[x][16 * c + lane], float_key(mine));
+              top = fmaxf(top, top2);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+              if (!(lane & 1)) atomicMax(&ms.cmax[x][16 * c + (lane >> 1)], float_key(top));
               __syncwarp();
             }
             named_bar_sync(1 + x, 128);
@@ -571,7 +575,6 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
             }
             named_bar_sync(1 + x, 128);
             if (k >= 2) {
-              wait_pv();
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < C::CH; ++c) {
