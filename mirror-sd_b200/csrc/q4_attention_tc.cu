@@ -50,6 +50,7 @@ namespace dfl {
 constexpr int QB_TILE = 128;
 constexpr int QB_BLK = kQ4Block + 32;      // a row block's stride in shared memory: 8 blocks on different banks
 constexpr int QB_STAGE = QB_TILE / kQ4Rows * QB_BLK;
+constexpr int QB_SEEN = 256;               // flag of a tile that every query of the item sees whole
 constexpr int QB_SLACK = 6;
 constexpr float QB_RAISE = 8.f;
 constexpr float QB_UNSET = 1e30f;          // -reference of a column that has seen no key
@@ -97,7 +98,7 @@ struct QbMisc {
   int where[2];                   // request of the CTA's first tile, and that request's first tile
   int run[2], share[2];           // whole CTAs to an item: this one's tiles; the item's first CTA and their number
   int wtot[QB_THREADS / 32];
-  int2 tile[16];                  // row blocks copied, rows below the request's end
+  int2 tile[16];                  // row blocks copied and QB_SEEN, rows below the request's end
   QbSeg seg[C::SEGS];
   alignas(16) float qf[C::SEGS][C::N];        // score factors
   alignas(16) float negm[2][C::N];            // minus the columns' references, of either side
@@ -423,7 +424,6 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       const float* qf = ms.qf[seg % C::SEGS];
       const bool uniform = sg.uniform;
       const float f = 16.f * p.scale_log2;
-      const int common_end = p.causal ? it.L - it.rows + 1 : it.L;   // keys below it are seen by all, window aside
       if (gt < N) {
         const int r = sg.q0 + gt, j = p.by_g.of(r);
         const bool real = j < it.rows;
@@ -448,12 +448,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         };
         if (k > 0) qb_wait(&ms.s_ready[t % C::SB], (t / C::SB) & 1, dead);
         tc_fence_after();
-        const int row0 = item_tile(it, j0 + k) * QB_TILE;
-        const int2 info = ms.tile[t & 15];
-        const bool all_seen = info.x == 255 && info.y >= QB_TILE && row0 + QB_TILE <= common_end &&
-                              (p.window == 0 || row0 + QB_TILE <= p.sink || row0 >= it.L - p.window);
-        const int key = (info.x >> (row >> 4) & 1) ? row0 + row : INT32_MAX;
-        if (!all_seen || !uniform) {
+        const int blocks = ms.tile[t & 15].x;
+        if (!(blocks & QB_SEEN) || !uniform) {
+          const int key = (blocks >> (row >> 4) & 1) ? item_tile(it, j0 + k) * QB_TILE + row : INT32_MAX;
           // Some key is hidden, or the columns have factors of their own: bring
           // the tile's scores to the common factor, hidden ones to -inf, where
           // they lie; the steps below then know one kind of tile.
@@ -810,7 +807,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         const int b = chunk * 4 + (oct >> 1), par = oct & 1;
         const uint8_t* blk = st + b * QB_BLK;
         uint2 sc = *reinterpret_cast<const uint2*>(blk + kQ4VS + g * 16 + par * 8);
-        if (info.x != 255 || info.y < QB_TILE) {
+        if ((info.x & 255) != 255 || info.y < QB_TILE) {
           // rows that were not copied, or lie past the end and may never have
           // been written: any bits, so their scale becomes 0
           const int left = (info.x >> b & 1) ? info.y - (16 * b + 8 * par) : 0;
@@ -860,8 +857,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     first_cursor(cur);
     const int bits = p.page_shift - 4;
     int page, row0, left, head;   // of the lane's block: page, the tile's first row, rows below the request's end
+    bool seen;                    // every query sees every key of the tile
     auto look_up = [&](int t0) {   // tiles t0 .. t0 + 3 of the CTA
-      int seq = 0, sub = 0, L = 0;
+      int seq = 0, sub = 0, L = 0, rows = 0;
       row0 = 0;
 #pragma unroll 1
       for (int i = 0; i < 4 && t0 + i < T; ++i) {
@@ -870,10 +868,13 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           seq = cur.it.seq;
           sub = cur.sub;
           L = cur.it.L;
+          rows = cur.it.rows;
         }
         if (t0 + i + 1 < T) cursor_next<QB_TILE, N>(p, cur);
       }
       left = min(L - row0, QB_TILE);
+      seen = row0 + QB_TILE <= (p.causal ? L - rows + 1 : L) &&
+             (p.window == 0 || row0 + QB_TILE <= p.sink || row0 >= L - p.window);
       head = sub - p.by_nkv.of(sub) * p.nkv;
       const int pos = row0 + (lane & 7) * kQ4Rows;
       page = -1;
@@ -887,7 +888,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       const uint8_t* src = p.pool + ((((size_t)(there ? page : 0) * p.nkv + head) << bits) +
                                      (row0 / kQ4Rows + (lane & 7) & ((1 << bits) - 1))) * kQ4Block;
       const uint32_t mask = __ballot_sync(0xffffffffu, there);
-      const int rows = left, end = min(t + 4, T);
+      const int rows = left, end = min(t + 4, T), all = seen ? QB_SEEN : 0;
       look_up(t + 4);   // (the next four page numbers travel while these tiles wait for their stages)
 #pragma unroll 1
       for (; t < end; ++t) {
@@ -896,7 +897,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         if (__any_sync(0xffffffffu, *dead)) break;
         if (lane == 8 * i) {
           const uint32_t blocks = mask >> 8 * i & 255;
-          ms.tile[t & 15] = make_int2((int)blocks, rows);
+          ms.tile[t & 15] = make_int2(blocks == 255 ? 255 | all : (int)blocks, rows);
           mbar_arrive_expect_tx(&ms.full[s], __popc(blocks) * kQ4Block);
         }
         __syncwarp();
