@@ -34,7 +34,7 @@
 // nothing in f16.
 //
 // 256 requests of up to 8,192 rows, 32 heads over 8 kv heads, are 1.34 GB, 205 us
-// of HBM; they take 301 us (4.5 TB/s).  What bounds it is instruction issue and
+// of HBM; they take 300 to 322 us (4.2 to 4.5 TB/s).  What bounds it is instruction issue and
 // latency: 1,300 instructions a tile and warp, 3 warps a scheduler (shared memory
 // holds two tiles for each of 12), 60 % of the issue slots taken.  Tiles of 32
 // rows, whose upkeep is paid twice as often, take 314 us for 256 requests of

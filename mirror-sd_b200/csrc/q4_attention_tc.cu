@@ -34,8 +34,8 @@
 // one kind of tile): the roles share the instruction cache.
 //
 // What it measures (8 kv heads): 256 requests x 16 rows x 32 heads over a sink of
-// 64 and a window of 1,040 rows 257 us, 16 requests of up to 32,768 rows with up to
-// 32 rows x 40 heads 228 us, one such request 57 us; HBM would allow 59, 31 and 6,
+// 64 and a window of 1,040 rows 252 us, 16 requests of up to 32,768 rows with up to
+// 32 rows x 40 heads 223 us, one such request 55 us; HBM would allow 59, 31 and 6,
 // the products alone 44, 37 and 13.  What bounds it: a tile takes each role 1,500
 // to 2,000 cycles (at 64 columns; 512 of them are MMAs), half the issue slots and
 // most of shared memory's bandwidth (V^T and P^T are written and read again), so
