@@ -410,8 +410,9 @@ int dflash_q4_read(const uint8_t* pool, int num_pages, int page_size, const int3
  * outside the pool hide their rows.  scale: positive and finite.
  * workspace: dflash_q4_attention_workspace_size() bytes, 16-byte aligned,
  * zeroed once before its first use; every call leaves it ready for the next
- * one of any shape it is large enough for.  Calls that may overlap on the GPU
- * need workspaces of their own. */
+ * one of any shape it is large enough for (unless DFLASH_PAGED_TIMEOUT was set:
+ * then zero it again).  Calls that may overlap on the GPU need workspaces of
+ * their own. */
 size_t dflash_q4_attention_workspace_size(int max_rows, int nq, int nkv);
 int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages,
                         int page_size, const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens,

@@ -95,17 +95,22 @@ def q4_read(pool, slots, dtype=torch.float16):
     return N.load_paged().read(pool, slots, dtype is torch.bfloat16)
 
 
-def q4_attention_workspace(n: int, max_rows: int, num_heads: int, num_kv_heads: int, device="cuda") -> torch.Tensor:
-    """Workspace of ``q4_attention`` for up to ``max_rows`` query rows a
-    request; it may serve any number of calls that do not overlap."""
-    device = torch.device(device)
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
+def _workspace_size(max_rows: int, num_heads: int, num_kv_heads: int, device) -> int:
     with torch.cuda.device(device):
         size = N.load().dflash_q4_attention_workspace_size(max_rows, num_heads, num_kv_heads)
     if size == 0:
         raise ValueError(f"no such attention: {max_rows} rows, {num_heads} / {num_kv_heads} heads")
-    return torch.zeros(size, dtype=torch.uint8, device=device)
+    return size
+
+
+def q4_attention_workspace(n: int, max_rows: int, num_heads: int, num_kv_heads: int, device="cuda") -> torch.Tensor:
+    """Workspace of ``q4_attention`` for up to ``max_rows`` query rows a
+    request and any number n of requests; it may serve any number of calls that
+    do not overlap."""
+    device = torch.device(device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return torch.zeros(_workspace_size(max_rows, num_heads, num_kv_heads, device), dtype=torch.uint8, device=device)
 
 
 def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: bool = False, sink: int = 0,
@@ -150,7 +155,7 @@ class PagedKVCacheQ4:
         self.head = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
         self._zeros = torch.zeros(max_seqs, **i32)
-        self._workspace = {}
+        self._workspace, self._sizes = {}, {}
         self._stream = _raw_stream(self.device.index)
 
     def _enter(self):
@@ -184,10 +189,13 @@ class PagedKVCacheQ4:
                window: int = 0, scale: Optional[float] = None, out=None):
         """Attention of the step's query rows over everything cached."""
         self._enter()
-        key = (max_rows, q.shape[1], torch.cuda.current_stream(self.device).cuda_stream)
-        ws = self._workspace.get(key)      # one for each stream: calls on different streams may overlap
-        if ws is None:
-            ws = self._workspace[key] = q4_attention_workspace(self.max_seqs, max_rows, q.shape[1], self.nkv, self.device)
+        key = (max_rows, q.shape[1])
+        size = self._sizes.get(key)
+        if size is None:
+            size = self._sizes[key] = _workspace_size(*key, self.nkv, self.device)
+        ws = self._workspace.get(self._stream)      # one for each stream: calls on different streams may overlap
+        if ws is None or ws.nbytes < size:
+            ws = self._workspace[self._stream] = torch.zeros(size, dtype=torch.uint8, device=self.device)
         return q4_attention(q, self.pools[layer], self.table, self.lens, step.starts, max_rows, causal, sink, window,
                             scale, out, self.status, ws)
 
@@ -234,4 +242,6 @@ class PagedKVCacheQ4:
         bits = int(self.status)
         if bits:
             self.status.zero_()
+            if bits & 32:
+                self._workspace.clear()     # its counters may be left half way
             raise RuntimeError("paged cache: " + "; ".join(m for b, m in STATUS_BITS.items() if bits & b))

@@ -550,3 +550,16 @@ def test_cache_object_refuses(pkg):
     assert cache.lens.tolist() == [20, 2]
     cache.trim(torch.tensor([30, 0]).cuda())
     assert cache.lens.tolist() == [0, 2]
+
+
+def test_cache_object_keeps_one_workspace(pkg):
+    """Steps of every size share the stream's workspace, grown where one needs more."""
+    cache = pkg.PagedKVCacheQ4(1, 64, 1, 1, 600, 16)
+    q = torch.randn(40, 4, 128, generator=torch.Generator().manual_seed(5)).half().cuda()
+    for m in (1, 40, 3, 17, 25, 2, 30):
+        step = cache.reserve([m])
+        cache.append(0, q[:m, :1], q[:m, :1], step)
+        out = cache.attend(0, q[:m], step, m)
+        assert torch.equal(out, pkg.q4_attention(q[:m], cache.pools[0], cache.table, cache.lens, step.starts, m, True))
+    cache.check()
+    assert len(cache._workspace) == 1
