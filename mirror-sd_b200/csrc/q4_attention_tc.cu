@@ -11,8 +11,10 @@
 //
 // Work: the tiles of 128 cached rows of all items, end to end, in equal runs
 // of one CTA per SM (q4_attn.cuh).  The CTAs that share an item write partial
-// results, wait for each other (they are all resident: one per SM) and each
-// merges its share of the item's query rows.
+// results, which a second small kernel merges.  No CTA waits for another:
+// nothing guarantees that they are all resident (a kernel of another stream, or
+// a partition of the GPU, may hold SMs).  (Merged by the last CTA to arrive: 64
+// query rows on 1 request of 2,048 rows 29 us, of 32,768 48; this way 21 and 36.)
 //
 // Roles, each running ahead as far as its buffers allow:
 //   2 x 4 warps  softmax of the even and the odd tiles; a thread owns a cached
@@ -34,8 +36,8 @@
 // one kind of tile): the roles share the instruction cache.
 //
 // What it measures (8 kv heads): 256 requests x 16 rows x 32 heads over a sink of
-// 64 and a window of 1,040 rows 252 us, 16 requests of up to 32,768 rows with up to
-// 32 rows x 40 heads 223 us, one such request 55 us; HBM would allow 59, 31 and 6,
+// 64 and a window of 1,040 rows 246 us, 16 requests of up to 32,768 rows with up to
+// 32 rows x 40 heads 215 us, one such request 56 us; HBM would allow 59, 31 and 6,
 // the products alone 44, 37 and 13.  What bounds it: a tile takes each role 1,500
 // to 2,000 cycles (at 64 columns; 512 of them are MMAs), half the issue slots and
 // most of shared memory's bandwidth (V^T and P^T are written and read again), so
@@ -96,7 +98,7 @@ struct QbMisc {
   uint32_t tmem;
   int abort;
   int where[2];                   // request of the CTA's first tile, and that request's first tile
-  int run[2], share[2];           // whole CTAs to an item: this one's tiles; the item's first CTA and their number
+  int run[2], share;              // whole CTAs to an item: this one's tiles, and their number
   int wtot[QB_THREADS / 32];
   int2 tile[16];                  // row blocks copied and QB_SEEN, rows below the request's end
   QbSeg seg[C::SEGS];
@@ -107,8 +109,7 @@ struct QbMisc {
   alignas(16) int cend[C::N];                 // where each column's keys end
   alignas(16) int coff[C::N];                 // output row of each column, or -1
   float lsum[8][C::N];
-  int done;                       // merge: whether the item's other CTAs have arrived
-  struct { int seq, sub, item0, nt; } border[2];   // items that reach past the CTA's first and last tile (seq -1: none)
+  int4 shared;                    // the item that starts here and reaches past the last tile (q4_tc_shared)
 };
 
 // One lane of a converged warp, chosen in a way that the compiler recognises:
@@ -249,6 +250,14 @@ __device__ __forceinline__ void scores16(const uint32_t (&s)[16], const float* n
   }
 }
 
+// What CTA b of the grid leaves behind its partials (two of n queries each): the
+// item that starts in its run and ends in a later CTA's, as the item's first
+// query row, its query rows, its group and kv head (sub), and the number of CTAs
+// that hold it (0: no such item).  Written at every launch.
+__host__ __device__ __forceinline__ int4* q4_tc_shared(float* part, int n, int grid) {
+  return reinterpret_cast<int4*>(part + (size_t)grid * 2 * n * 130);
+}
+
 template <int N>
 __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnParams p) {
   using C = QbCfg<N>;
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     mbar_init(&ms.o_free, 8);
     for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], 4); }
     ms.abort = 0;
-    ms.border[0].seq = ms.border[1].seq = -1;
+    ms.shared = make_int4(0, 0, 0, 0);
     ms.run[0] = ms.run[1] = 0;
     fence_mbar_init();
   }
@@ -346,8 +355,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       ms.where[1] = first;
       ms.run[0] = item0 + runs.start(part);
       ms.run[1] = item0 + runs.start(part + 1);
-      ms.share[0] = blockIdx.x - part;
-      ms.share[1] = parts;
+      ms.share = parts;
     }
   } else {
     const int ctas = min(grid, total);
@@ -382,12 +390,11 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     c1 = ms.run[1];
   }
   const int T = c1 - c0;
-  // the CTAs that hold an item (of ntile tiles, the first of them tile item0): the first one and their number
+  // number of CTAs that hold an item of ntile tiles, the first of them tile item0 and in this CTA
   auto sharers = [&](int item0, int ntile) {
-    if (quota > 0) return make_int2(ms.share[0], ms.share[1]);
+    if (quota > 0) return ms.share;
     const Runs runs(total, min(grid, total));
-    const int from = runs.of(item0);
-    return make_int2(from, runs.of(item0 + ntile - 1) - from + 1);
+    return runs.of(item0 + ntile - 1) - runs.of(item0) + 1;
   };
 
   // ring cursors start at the same place in the producer and the query warp
@@ -703,56 +710,13 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       tc_fence_before();
       warp_arrive(&ms.o_free, lane);
       if (!whole) {
-        if (threadIdx.x == 0) ms.border[border] = {it.seq, sg.sub, sg.item0, it.ntile};
-        __threadfence();
-        named_bar_sync(3, 256);
-        if (threadIdx.x == 0) {
-          __threadfence();
-          atomicAdd(&p.counters[2 * sharers(sg.item0, it.ntile).x], 1);
-        }
+        // (merged by the item's first CTA's entry; the others' partials follow its own)
+        if (threadIdx.x == 0 && border == 1) ms.shared = make_int4(it.row0, it.rows, sg.sub, sharers(sg.item0, it.ntile));
       }
       t0 += nt;
     }
 
-    // ---- items shared with other CTAs: each finishes its share of the query rows
-#pragma unroll 1
-    for (int border = 0; border < 2; ++border) {
-      const auto bd = ms.border[border];
-      if (bd.seq < 0) continue;
-      const int2 share = sharers(bd.item0, bd.nt);
-      const int from = share.x, count = share.y;
-      if (threadIdx.x == 0) {
-        int ok = 0;
-        for (uint32_t i = 0; i < kSpinLimit && !ok && !*dead; ++i) {
-          ok = ld_acquire_gpu(&p.counters[2 * from]) >= count;
-          if (!ok) __nanosleep(40);
-        }
-        ms.done = ok;
-        if (!ok) *dead = 1;
-      }
-      named_bar_sync(3, 256);
-      if (ms.done) {
-        __threadfence();
-        const Item it = load_item<QB_TILE, N>(p, bd.seq);
-        const int sub = bd.sub, me = (int)blockIdx.x - from;
-        // the first CTA holds the item's start at its right border, the others at their left
-        auto slot = [&](int i) { return p.part + ((size_t)(from + i) * 2 + (i == 0 ? 1 : 0)) * C::SLOT; };
-        const int grp = p.by_nkv.of(sub);
-#pragma unroll 1
-        for (int q = me + count * warp; q < N; q += count * 8) {
-          const int r = grp * N + q, j = p.by_g.of(r);
-          if (j >= it.rows) continue;
-          float v[4];
-          merge_query(count, slot, N, q, lane, v);
-          store_out4(p, it.row0 + j, (sub - grp * p.nkv) * G + r - j * G, 4 * lane, v);
-        }
-      }
-      named_bar_sync(3, 256);
-      if (threadIdx.x == 0 && atomicAdd(&p.counters[2 * from + 1], 1) == count - 1) {
-        p.counters[2 * from] = 0;       // the last one to leave: ready for the next call
-        p.counters[2 * from + 1] = 0;
-      }
-    }
+    if (threadIdx.x == 0) q4_tc_shared(p.part, N, grid)[blockIdx.x] = ms.shared;
   } else if (warp < QB_VDEC) {
     set_registers<QB_REST_REGS, false>();
     // ---- K codes to f16: thread = cached row
@@ -1069,6 +1033,27 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   }
 }
 
+// Merges the items that several CTAs of the kernel above hold: CTA (b, y) the
+// queries 16 y .. + 15 of the item that starts in CTA b, two a warp.  The item's
+// first partial is CTA b's second one, the others are the first ones of the CTAs
+// after it.
+__global__ void __launch_bounds__(256) q4_attn_tc_merge_kernel(const Q4AttnParams p, int n) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int4 item = __ldcg(q4_tc_shared(p.part, n, gridDim.x) + b);   // row0, rows, sub, count
+  auto slot = [&](int i) { return p.part + ((size_t)(b + i) * 2 + (i == 0 ? 1 : 0)) * n * 130; };
+  const int grp = p.by_nkv.of(item.z), G = p.by_g.d;
+#pragma unroll 1
+  for (int q = 16 * blockIdx.y + warp; q < 16 * blockIdx.y + 16; q += 8) {
+    const int r = grp * n + q, j = p.by_g.of(r);
+    if (item.w == 0 || j >= item.y) return;
+    float v[4];
+    merge_query(item.w, slot, n, q, lane, v);
+    store_out4(p, item.x + j, (item.z - grp * p.nkv) * G + r - j * G, 4 * lane, v);
+  }
+}
+
 // Columns of the instruction for R = max_rows * G query rows of a kv head: the
 // fewest groups of at most 80 (a thread keeps a sum for every column), evenly
 // filled, in steps of 16 and 32 at least (with fewer a tile costs no less: 32, 48,
@@ -1082,7 +1067,7 @@ static int q4_tc_columns(int max_rows, int nq, int nkv) {
 }
 
 size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms) {
-  return (size_t)num_sms * 2 * q4_tc_columns(max_rows, nq, nkv) * 130;
+  return (size_t)num_sms * (2 * q4_tc_columns(max_rows, nq, nkv) * 130 + sizeof(int4) / sizeof(float));
 }
 
 template <int N>
@@ -1091,7 +1076,8 @@ static cudaError_t launch_tc(const Q4AttnParams& p, int num_sms, cudaStream_t st
   constexpr size_t smem = C::MISC_OFF + sizeof(QbMisc<C>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
   DFL_TRY(cudaFuncSetAttribute(q4_attn_tc_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  return launch_pdl(q4_attn_tc_kernel<N>, dim3(num_sms), dim3(QB_THREADS), smem, st, p);
+  DFL_TRY(launch_pdl(q4_attn_tc_kernel<N>, dim3(num_sms), dim3(QB_THREADS), smem, st, p));
+  return launch_pdl(q4_attn_tc_merge_kernel, dim3(num_sms, C::CH), dim3(256), 0, st, p, N);
 }
 
 cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {

@@ -161,8 +161,8 @@ __device__ __forceinline__ void merge_query(int count, SlotAt slots, int qt, int
   float4 x[8];
   auto load = [&](int k) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)   // (past the end: the last one again, with weight 0)
-      x[i] = __ldcg(reinterpret_cast<const float4*>(slots(min(k + i, count - 1)) + q * 128 + 4 * lane));
+    for (int i = 0; i < 8; ++i)
+      if (k + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(slots(k + i) + q * 128 + 4 * lane));
   };
   load(0);
   float m = -INFINITY, s = 0.f;

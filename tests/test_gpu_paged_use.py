@@ -1,0 +1,37 @@
+"""The paged 4-bit cache in use beside other work: overlapping calls, CUDA
+graphs, refused requests, and the ends of the operators' ranges."""
+import numpy as np
+import pytest
+import torch
+
+import paged_util as U
+from test_gpu_paged import Case, _dev
+
+pytestmark = pytest.mark.gpu
+i32 = torch.int32
+
+
+# ---------------------------------------------------------------- overlapping calls
+
+def test_block_calls_overlap_on_streams_of_different_priority(pkg):
+    """Calls that share items over the whole GPU, on two streams that take SMs from each other: no CTA may depend on
+    another one's residency, and each call gives the bits that it gives alone."""
+    cases = [Case(pkg, [6000, 50], [16, 16], 8, 2, 64, torch.float16, seed=s) for s in (1, 2)]
+    spaces = [pkg.q4_attention_workspace(2, 16, 8, 2) for _ in cases]
+    tables = [(c.pg.dev("table"), c.pg.dev("lens")) for c in cases]
+    alone = [c.check(pkg, causal=True) for c in cases]
+    status = torch.zeros(2, dtype=i32).cuda()
+    outs = [[torch.empty_like(c.q) for _ in range(40)] for c in cases]
+    filler = torch.randn(1 << 22, device="cuda")
+    streams = [torch.cuda.Stream(priority=0), torch.cuda.Stream(priority=-1)]
+    torch.cuda.synchronize()
+    for k in range(40):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                if i == 0:
+                    filler.mul_(1.0)                    # leaves SMs to the two grids one by one
+                pkg.q4_attention(cases[i].q, cases[i].pool, *tables[i], starts=cases[i].starts, max_rows=16, causal=True,
+                                 out=outs[i][k], status=status[i:i + 1], workspace=spaces[i])
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, 0]
+    assert all(torch.equal(o, alone[i]) for i in range(2) for o in outs[i])
