@@ -157,6 +157,9 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
     return fail(DFLASH_ERR_INVALID, "without starts every request has max_rows rows (%d x %d, got %d)", n, max_rows, rows);
   if (sink < 0 || window < 0) return fail(DFLASH_ERR_INVALID, "sink %d, window %d", sink, window);
   if (sink > 0 && window == 0) return fail(DFLASH_ERR_INVALID, "sink needs a window (window 0 sees every row)");
+  // A window as wide as the table hides nothing; the kernels subtract the others
+  // from lengths less query rows, in 32 bits.
+  if (window >= max_pages * page_size) sink = window = 0;
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(DFLASH_ERR_INVALID, "scale must be positive and finite");
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_row % 8 || q_head % 8)
     return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");

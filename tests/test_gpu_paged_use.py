@@ -35,3 +35,13 @@ def test_block_calls_overlap_on_streams_of_different_priority(pkg):
     torch.cuda.synchronize()
     assert status.tolist() == [0, 0]
     assert all(torch.equal(o, alone[i]) for i in range(2) for o in outs[i])
+
+
+# ---------------------------------------------------------------- the ends of the ranges
+@pytest.mark.parametrize("rows,nq", [(12, 1), (400, 1)])
+@pytest.mark.parametrize("sink,window", [(0, 2 ** 31 - 1), (5, 2 ** 31 - 1), (0, 2 ** 31 - 400), (0, 304), (7, 305)])
+def test_windows_wider_than_the_cache_hide_nothing(pkg, rows, nq, sink, window):
+    """Also where there are more query rows than cached rows, so that lengths less rows are negative."""
+    for L in (8, 300):
+        c = Case(pkg, [L], [rows], nq, 1, 16, torch.float16, seed=L)
+        c.check(pkg, causal=True, sink=sink, window=window)
