@@ -150,6 +150,9 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
     return fail(DFLASH_ERR_INVALID, "NULL pointer");
   if (int rc = check_paging(n, page_size, table_ld, max_pages, num_pages)) return rc;
   if (int rc = check_pool(rows, nkv, pool, num_pages, page_size)) return rc;
+  // (the kernels add a tile, a window or the query rows to a position in 32 bits)
+  if ((long long)max_pages * page_size > 1ll << 30)
+    return fail(DFLASH_ERR_INVALID, "%d pages of %d rows a request: at most 2^30 rows", max_pages, page_size);
   if (nq < nkv || nq % nkv) return fail(DFLASH_ERR_INVALID, "nq %d must be a multiple of nkv %d", nq, nkv);
   if (max_rows < 1 || max_rows > DFLASH_Q4_MAX_ROWS)
     return fail(DFLASH_ERR_INVALID, "max_rows %d outside [1, %d]", max_rows, DFLASH_Q4_MAX_ROWS);

@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t o_t = tmem + C::O_COL + x * N + lanes;
-    const int window = p.window > 0 ? p.window : 1 << 30;   // wider than any cache
+    const int window = p.window > 0 ? p.window : 1 << 30;   // no cache is longer
     float* negm = ms.negm[x];
     float* facs = ms.fac[x];
     uint8_t* pr = smem + C::P_OFF + x * C::P_BYTES + row * 128;
