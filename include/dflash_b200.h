@@ -367,6 +367,7 @@ int dflash_lm_head_argmax(const uint16_t* hn, const uint16_t* E, int batch, int 
 #define DFLASH_PAGED_CORRUPT 8         /* more pages came back than were lent */
 #define DFLASH_PAGED_NONFINITE 16      /* a NaN or an infinity was appended */
 #define DFLASH_PAGED_TIMEOUT 32        /* a bounded device-side wait expired */
+#define DFLASH_PAGED_ROWS 64           /* more query rows than max_rows, or starts that do not fit q */
 
 /* Request i holds lens[i] rows on pages[i] pages, table[i * table_ld + c],
  * c < pages[i], and brings new_rows[i] rows, packed in order.  Its missing
@@ -402,7 +403,8 @@ int dflash_q4_read(const uint8_t* pool, int num_pages, int page_size, const int3
 
 /* q [rows, nq, 128], f16 or bf16, strides in elements (multiples of 8); out
  * [rows, nq, 128] of the same type.  Request i owns rows starts[i] ..
- * starts[i + 1] - 1, at most max_rows of them (starts NULL: max_rows each),
+ * starts[i + 1] - 1, at most max_rows of them (starts NULL: max_rows each;
+ * otherwise DFLASH_PAGED_ROWS is set and that request's rows are undefined),
  * and holds lens[i] cached rows, its own new ones included.  With causal,
  * query row j of m sees keys below e = lens[i] - m + j + 1, else below
  * e = lens[i]; with a window only keys < sink or >= e - window.  A row that

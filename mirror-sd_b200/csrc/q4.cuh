@@ -48,6 +48,7 @@ enum PagedStatus : int {
   kPagedCorrupt = 8,    // more pages come back than the free list lent out
   kPagedNonFinite = 16, // an appended row held a NaN or an infinity
   kPagedTimeout = 32,   // a bounded wait of the attention kernel expired
+  kPagedRows = 64,      // a request's query rows pass max_rows or lie outside the query array
 };
 
 // byte offsets of the pieces inside the block's K and V values

@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     if (i < p.n) {
       const Item it = load_item<QA_TILE, QT>(p, i);
       v = it.ntile * it.groups * p.nkv;
+      if (blockIdx.x == 0 && p.status && !rows_fit(p, i)) atomicOr(p.status, kPagedRows);
     }
     int x = v;
 #pragma unroll

@@ -323,6 +323,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       const Item it = load_item<QB_TILE, N>(p, i);
       ntile = it.ntile;
       items = it.groups * p.nkv;
+      if (blockIdx.x == 0 && p.status && !rows_fit(p, i)) atomicOr(p.status, kPagedRows);
     }
     int sum;
     first = scan(items * ntile, &sum);

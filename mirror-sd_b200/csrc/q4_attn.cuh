@@ -44,6 +44,13 @@ __device__ __forceinline__ int seq_rows(const Q4AttnParams& p, int i, int* row0)
   *row0 = a;
   return min(b - a, p.max_rows);
 }
+// Whether they are the rows that the caller meant; the host has not seen starts,
+// so what does not fit is cut off above and reported.
+__device__ __forceinline__ bool rows_fit(const Q4AttnParams& p, int i) {
+  if (!p.starts) return true;
+  const int a = __ldg(p.starts + i), b = __ldg(p.starts + i + 1);
+  return a >= 0 && a <= b && b <= p.T && b - a <= p.max_rows;
+}
 template <int TILE, int QT>
 __device__ __forceinline__ Item load_item(const Q4AttnParams& p, int i) {
   Item it;

@@ -31,7 +31,8 @@ HEAD_DIM = 128
 BLOCK_BYTES = 2304                   # 16 rows of one kv head, K and V with their scales
 STATUS_BITS = {1: "too few free pages", 2: "a request outgrew its row of the block table",
                4: "more new rows than slots", 8: "more pages came back than were lent",
-               16: "a NaN or an infinity was appended", 32: "a device-side wait expired"}
+               16: "a NaN or an infinity was appended", 32: "a device-side wait expired",
+               64: "a request brought more query rows than max_rows, or starts do not fit q"}
 
 
 class PagedStep(NamedTuple):
@@ -118,7 +119,8 @@ def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: b
     """Grouped-query attention of each request's query rows over its cached
     rows.  q [rows, NQ, 128] (f16 or bf16; strided rows and heads) holds the
     requests' rows one after another: request i owns starts[i] ..
-    starts[i + 1] - 1 (at most ``max_rows``), or ``max_rows`` each without
+    starts[i + 1] - 1 (at most ``max_rows``: a request with more sets a bit of
+    ``status``, and its rows are undefined), or ``max_rows`` each without
     ``starts``.  lens [n] counts the cached rows, the new ones included.
 
     causal: query row j of m sees the keys below lens - m + j + 1 (else below

@@ -45,3 +45,33 @@ def test_windows_wider_than_the_cache_hide_nothing(pkg, rows, nq, sink, window):
     for L in (8, 300):
         c = Case(pkg, [L], [rows], nq, 1, 16, torch.float16, seed=L)
         c.check(pkg, causal=True, sink=sink, window=window)
+
+
+@pytest.mark.parametrize("rows,most", [([2, 5, 1], 4), ([20, 33, 7], 32)])
+def test_more_query_rows_than_max_rows_are_reported(pkg, rows, most):
+    """Both kernels: the other requests' rows are right, and the status word names what happened."""
+    c = Case(pkg, [90, 200, 31], rows, 4, 2, 32, torch.float16)
+    args = (c.q, c.pool, c.pg.dev("table"), c.pg.dev("lens"))
+    ref = c.check(pkg, causal=True)
+    status = torch.zeros(1, dtype=i32).cuda()
+    out = pkg.q4_attention(*args, starts=c.starts, max_rows=most, causal=True, status=status)
+    assert status.tolist() == [64]
+    for a, b in ((0, rows[0]), (rows[0] + rows[1], sum(rows))):
+        err, tol = (out[a:b] - ref[a:b]).double().abs(), 2.0 ** -9 * ref[a:b].double().abs() + 2.0 ** -9
+        assert bool((err <= tol).all())
+    for starts in ([0, 3, 2, 3], [-1, 0, 1, 2], [0, 1, 2, sum(rows) + 1]):      # not ascending, or outside q
+        status.zero_()
+        pkg.q4_attention(*args, starts=_dev(starts), max_rows=sum(rows), causal=True, status=status)
+        assert status.tolist() == [64], starts
+
+
+def test_the_cache_object_reports_more_query_rows_than_max_rows(pkg):
+    cache = pkg.PagedKVCacheQ4(1, 8, 2, 2, 100, 16)
+    x = torch.zeros(8, 2, 128).half().cuda()
+    step = cache.reserve([3, 5])
+    cache.append(0, x, x, step)
+    cache.attend(0, x, step, 5)
+    cache.check()
+    cache.attend(0, x, step, 4)
+    with pytest.raises(RuntimeError, match="max_rows"):
+        cache.check()
