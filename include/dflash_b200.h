@@ -409,7 +409,9 @@ int dflash_q4_read(const uint8_t* pool, int num_pages, int page_size, const int3
  * query row j of m sees keys below e = lens[i] - m + j + 1, else below
  * e = lens[i]; with a window only keys < sink or >= e - window.  A row that
  * sees no key is zeros; rows of no request are not written.  Table entries
- * outside the pool hide their rows.  max_pages * page_size <= 2^30.  scale:
+ * outside the pool hide their rows.  max_pages * page_size <= 2^30, and the
+ * tiles of 64 or 128 cached rows (a full table of them for every group of query
+ * rows and kv head) are fewer than 2^31.  scale:
  * positive and finite.
  * workspace: dflash_q4_attention_workspace_size() bytes, 16-byte aligned,
  * zeroed once before its first use; every call leaves it ready for the next

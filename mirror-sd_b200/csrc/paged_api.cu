@@ -167,12 +167,18 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_row % 8 || q_head % 8)
     return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");
   const int G = nq / nkv;
-  if (G > 256 || nkv > 1024 || ((double)max_rows * G / 8 + 1) * nkv * nkv > 4e9)
+  // Up to 16 query rows a kv head each warp multiplies on its own (mma.sync, no
+  // hand-over between warps); above, tcgen05 with the rows as columns.
+  const bool few = (long long)max_rows * G <= kQ4FewRows;
+  const double columns = few ? q4_attn_columns(max_rows, nq, nkv) : q4_attn_tc_columns(max_rows, nq, nkv);
+  if (G > 256 || nkv > 1024 || ((double)max_rows * G / columns + 1) * nkv * nkv > 4e9)
     return fail(DFLASH_ERR_INVALID, "%d query heads a kv head, %d kv heads, %d rows: too many", G, nkv, max_rows);
-  // tiles of all items together are counted in 32 bits
-  const double units = (double)n * ((double)max_pages * page_size / 64 + 2) * nkv * ((double)max_rows * G / 8 + 1);
+  // Tiles of all items together are counted in 32 bits: a full table for each
+  // group of query rows, of which every request with rows has one in part.
+  const double units = std::ceil((double)max_pages * page_size / (few ? kQ4Tile : kQ4TcTile)) * nkv *
+                       ((double)rows * G / columns + (n < rows ? n : rows));
   if ((long long)rows * nq > INT32_MAX) return fail(DFLASH_ERR_INVALID, "rows x nq must stay below 2^31");
-  if (units > 2e9) return fail(DFLASH_ERR_INVALID, "n x table x heads x rows is too large for one call");
+  if (units >= INT32_MAX) return fail(DFLASH_ERR_INVALID, "n x table x heads x rows is too large for one call");
   if (workspace_bytes < dflash_q4_attention_workspace_size(max_rows, nq, nkv))
     return fail(DFLASH_ERR_INVALID, "workspace too small (%zu < %zu)", workspace_bytes,
                 dflash_q4_attention_workspace_size(max_rows, nq, nkv));
@@ -191,9 +197,7 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
   p.out = out; p.status = status;
   p.counters = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-  // Up to 16 query rows a kv head each warp multiplies on its own (mma.sync, no
-  // hand-over between warps); above, tcgen05 with the rows as columns.
-  if ((long long)max_rows * G <= kQ4FewRows)
+  if (few)
     CK(q4_attn_launch(p, sms, static_cast<cudaStream_t>(stream)));
   else
     CK(q4_attn_tc_launch(p, sms, static_cast<cudaStream_t>(stream)));

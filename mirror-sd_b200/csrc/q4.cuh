@@ -117,6 +117,11 @@ struct Q4AttnParams {
   float* part;                       // partial results
   int32_t* status;                   // or NULL
 };
+// Each kernel cuts a request's rows of a kv head into groups of `columns`, and
+// its cached rows into tiles.
+constexpr int kQ4Tile = 64, kQ4TcTile = 128;
+int q4_attn_columns(int max_rows, int nq, int nkv);
+int q4_attn_tc_columns(int max_rows, int nq, int nkv);
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms);
 cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
 // the same for blocks of query rows (q4_attention_tc.cu)

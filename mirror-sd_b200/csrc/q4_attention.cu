@@ -45,7 +45,7 @@
 
 namespace dfl {
 
-constexpr int QA_TILE = 64;                      // cached rows of a tile
+constexpr int QA_TILE = kQ4Tile;                     // cached rows of a tile
 constexpr int QA_STAGE = QA_TILE / kQ4Rows * kQ4Block;
 // Tiles of a CTA at least: a warp for each scheduler.  Fewer tiles spread an item
 // over more CTAs, whose partials the last one merges (2,049 rows: 13.3 us with 1,
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      if (lane >= o) x = tiles_sum(x, y);
     }
     __syncthreads();
     if (lane == 31) wtot[warp] = x;
@@ -178,11 +178,12 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     int before = total;
 #pragma unroll
     for (int w = 0; w < C::WARPS; ++w) {
-      if (w < warp) before += wtot[w];
-      total += wtot[w];
+      if (w < warp) before = tiles_sum(before, wtot[w]);
+      total = tiles_sum(total, wtot[w]);
     }
-    if (i < p.n) base[i] = before + x - v;
+    if (i < p.n) base[i] = tiles_sum(before, x - v);
   }
+  if (total == kTilesFull) total = 0;
   if (threadIdx.x == 0) base[p.n] = total;
   __syncthreads();
 
@@ -545,11 +546,10 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
 
 // 8 or 16 query columns.  Up to 8 rows, us with 8 columns / 16: 1 request of
 // 32,768 rows 22 / 27, 16 of 16,384 84 / 116, 256 of 1,024 85 / 123.
-static int q4_attn_nt(int max_rows, int nq, int nkv) { return (long long)max_rows * (nq / nkv) <= 8 ? 1 : 2; }
+int q4_attn_columns(int max_rows, int nq, int nkv) { return (long long)max_rows * (nq / nkv) <= 8 ? 8 : 16; }
 
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms) {
-  const int nt = q4_attn_nt(max_rows, nq, nkv);
-  return (size_t)num_sms * (nt == 1 ? (QaCfg<1>::WARPS + 2) * QaCfg<1>::SLOT : (QaCfg<2>::WARPS + 2) * QaCfg<2>::SLOT);
+  return (size_t)num_sms * (q4_attn_columns(max_rows, nq, nkv) == 8 ? (QaCfg<1>::WARPS + 2) * QaCfg<1>::SLOT : (QaCfg<2>::WARPS + 2) * QaCfg<2>::SLOT);
 }
 
 template <int NT>
@@ -561,7 +561,7 @@ static cudaError_t launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
 
 cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
-  return q4_attn_nt(p.max_rows, p.nq, p.nkv) == 1 ? launch<1>(p, num_sms, st) : launch<2>(p, num_sms, st);
+  return q4_attn_columns(p.max_rows, p.nq, p.nkv) == 8 ? launch<1>(p, num_sms, st) : launch<2>(p, num_sms, st);
 }
 
 }  // namespace dfl

@@ -49,7 +49,7 @@
 
 namespace dfl {
 
-constexpr int QB_TILE = 128;
+constexpr int QB_TILE = kQ4TcTile;
 constexpr int QB_BLK = kQ4Block + 32;      // a row block's stride in shared memory: 8 blocks on different banks
 constexpr int QB_STAGE = QB_TILE / kQ4Rows * QB_BLK;
 constexpr int QB_SEEN = 256;               // flag of a tile that every query of the item sees whole
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      if (lane >= o) x = tiles_sum(x, y);
     }
     __syncthreads();
     if (lane == 31) ms.wtot[warp] = x;
@@ -307,11 +307,11 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     int before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < QB_THREADS / 32; ++w) {
-      if (w < warp) before += ms.wtot[w];
-      all += ms.wtot[w];
+      if (w < warp) before = tiles_sum(before, ms.wtot[w]);
+      all = tiles_sum(all, ms.wtot[w]);
     }
     *sum = all;
-    return before + x - v;
+    return tiles_sum(before, x - v);
   };
   const int grid = gridDim.x;
   int total = 0, c0 = 0, c1 = 0, items = 0, ntile = 0, first = 0;   // (the last three of request threadIdx.x)
@@ -327,8 +327,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     }
     int sum;
     first = scan(items * ntile, &sum);
-    total += sum;
+    total = tiles_sum(total, sum);
   }
+  if (total == kTilesFull) total = 0;
   // With few items, whole CTAs to each: a run that crosses from one item into the
   // next pays the start and the end of an item (6 to 8 us together) twice.  An
   // item takes a CTA for every `quota` of its tiles, the least number with which
@@ -374,8 +375,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         const Item it = load_item<QB_TILE, N>(p, i);
         v = it.ntile * it.groups * p.nkv;
       }
-      const int at = before + scan(v, &sum);
-      before += sum;
+      const int at = tiles_sum(before, scan(v, &sum));
+      before = tiles_sum(before, sum);
       if (at <= c0 && c0 < at + v) {
         ms.where[0] = i;
         ms.where[1] = at;
@@ -1060,7 +1061,7 @@ __global__ void __launch_bounds__(256) q4_attn_tc_merge_kernel(const Q4AttnParam
 // filled, in steps of 16 and 32 at least (with fewer a tile costs no less: 32, 48,
 // 64 and 80 columns take 121, 132, 151 and 190 us for 16 requests of 16,384 rows).
 // 160 rows as two groups of 80 take 336 us there, three of 64 three times 151.
-static int q4_tc_columns(int max_rows, int nq, int nkv) {
+int q4_attn_tc_columns(int max_rows, int nq, int nkv) {
   const long long R = (long long)max_rows * (nq / nkv);
   const long long groups = (R + 79) / 80;
   const int n = (int)(((R + groups - 1) / groups + 15) / 16 * 16);
@@ -1068,7 +1069,7 @@ static int q4_tc_columns(int max_rows, int nq, int nkv) {
 }
 
 size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms) {
-  return (size_t)num_sms * (2 * q4_tc_columns(max_rows, nq, nkv) * 130 + sizeof(int4) / sizeof(float));
+  return (size_t)num_sms * (2 * q4_attn_tc_columns(max_rows, nq, nkv) * 130 + sizeof(int4) / sizeof(float));
 }
 
 template <int N>
@@ -1083,7 +1084,7 @@ static cudaError_t launch_tc(const Q4AttnParams& p, int num_sms, cudaStream_t st
 
 cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
-  switch (q4_tc_columns(p.max_rows, p.nq, p.nkv)) {
+  switch (q4_attn_tc_columns(p.max_rows, p.nq, p.nkv)) {
     case 32: return launch_tc<32>(p, num_sms, st);
     case 48: return launch_tc<48>(p, num_sms, st);
     case 64: return launch_tc<64>(p, num_sms, st);

@@ -79,6 +79,12 @@ __device__ __forceinline__ int item_tile(const Item& it, int j) {
   return j < it.span.a ? j : j - it.span.a + it.span.b;
 }
 
+// Sum of two tile counts that stays at kTilesFull once it is there.  The host
+// bounds the tiles by the rows of q, which holds for ascending starts only; a
+// call whose sum is full does nothing (its starts are reported, rows_fit).
+constexpr int kTilesFull = INT32_MAX;
+__device__ __forceinline__ int tiles_sum(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)kTilesFull); }
+
 // The tiles of all items in one row, cut into `parts` runs whose lengths differ
 // by at most one.
 struct Runs {

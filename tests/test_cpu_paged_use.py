@@ -3,6 +3,9 @@ on, importing and building, and refusals at the ends of the ranges."""
 import ctypes
 import os
 
+import numpy as np
+import torch
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mirror-sd_b200", "csrc")
 
 
@@ -37,3 +40,32 @@ def test_attention_refuses_tables_beyond_its_32_bit_sums(pkg):
     lib = pkg._native.load()
     _refused(pkg, _attend(lib, width=2 ** 24 + 1), "2^30")
     _refused(pkg, _attend(lib, width=2 ** 25 - 1, window=5), "2^30")
+
+
+def test_prompts_of_full_size_caches_are_taken(pkg):
+    """One request's prompt in a cache of many slots and long tables: the tiles that exist are bounded by the rows of q."""
+    lib = pkg._native.load()
+    for kw in (dict(n=256, width=512, rows=4096, max_rows=4096, nq=32, nkv=8),
+               dict(n=64, width=2048, rows=4096, max_rows=4096, nq=32, nkv=8),
+               dict(n=16, width=2048, rows=8192, max_rows=8192, nq=64, nkv=8),
+               dict(n=2048, width=512, rows=2048, max_rows=1, nq=32, nkv=8)):
+        status = _attend(lib, starts=P, q_row=kw["nq"] * 128, **kw) if not torch.cuda.is_available() else 0
+        assert status != pkg._native.DFLASH_ERR_INVALID, (kw, pkg._native.last_error())
+    _refused(pkg, _attend(lib, n=2048, width=2 ** 22, rows=65536, max_rows=65536, nq=32, nkv=8, starts=P, q_row=4096),
+             "too large")
+
+
+def test_tile_sums_stay_in_range():
+    """The device's sum of tile counts, restated: full is full, in any order of additions."""
+    full = 2 ** 31 - 1
+    add = lambda a, b: min((a + b) % 2 ** 32, full)
+    rng = np.random.default_rng(0)
+    for top in (10, 2 ** 20, 2 ** 30, full):
+        v = [int(x) for x in rng.integers(0, top, 64)]
+        tree = v
+        while len(tree) > 1:
+            tree = [add(a, b) for a, b in zip(tree[::2], tree[1::2])]
+        line = 0
+        for x in v:
+            line = add(line, x)
+        assert tree[0] == line == min(sum(v), full)

@@ -75,3 +75,41 @@ def test_the_cache_object_reports_more_query_rows_than_max_rows(pkg):
     cache.attend(0, x, step, 4)
     with pytest.raises(RuntimeError, match="max_rows"):
         cache.check()
+
+
+@pytest.mark.parametrize("rows,prefix", [(4096, 0), (1031, 700)])
+def test_prompt_in_a_cache_of_many_long_slots(pkg, rows, prefix):
+    """256 slots of up to 32,768 rows, 32 / 8 heads: one request's prompt, from empty or behind cached rows."""
+    nq, nkv, at = 32, 8, 37
+    cache = pkg.PagedKVCacheQ4(1, 90, nkv, 256, 32768, 64)
+    g = torch.Generator().manual_seed(rows)
+    k, v = ((torch.randn(prefix + rows, nkv, 128, generator=g) * s).half() for s in (1.0, 0.5))
+    q = torch.randn(rows, nq, 128, generator=g).half()
+    for a, b in ((0, prefix), (prefix, prefix + rows)):
+        if a < b:
+            step = cache.reserve([b - a if i == at else 0 for i in range(256)])
+            cache.append(0, k[a:b].cuda(), v[a:b].cuda(), step)
+    out = cache.attend(0, q.cuda(), step, rows).cpu()
+    cache.check()
+    ks, vs = U.q4_values(k), U.q4_values(v)
+    for j in [0, 1, 19, 20, 63, 64, 500, rows - 2, rows - 1]:      # groups of 20 rows
+        end = prefix + j + 1
+        ref, bound = U.attention(q[j:j + 1], [ks[:end]], [vs[:end]], [1], 128 ** -0.5)
+        assert bool(((out[j:j + 1].double() - ref).abs() <= U.attention_tolerance(ref, bound, torch.float16)).all()), j
+
+
+@pytest.mark.parametrize("rows,nkv,length", [(16, 256, 2 ** 21), (512, 64, 2 ** 21)])
+def test_starts_out_of_order_never_outgrow_the_tile_sums(pkg, rows, nkv, length):
+    """Every other request claims all of q: more than 2^32 tiles together.  Nothing runs, and the status says why."""
+    n = 2048
+    pool = pkg.q4_pool(1, nkv, 256)
+    q = torch.zeros(rows, nkv, 128, dtype=torch.float16).cuda()
+    table = torch.full((n, length // 256), -1, dtype=i32).cuda()
+    starts = torch.zeros(n + 1, dtype=i32).cuda()
+    starts[1::2] = rows
+    status = torch.zeros(1, dtype=i32).cuda()
+    group = 16 if rows == 16 else 80
+    tiles = length // (64 if rows == 16 else 128) * nkv * -(-rows // group)
+    assert tiles * (n // 2) > 2 ** 32
+    pkg.q4_attention(q, pool, table, torch.full((n,), length, dtype=i32).cuda(), starts=starts, max_rows=rows, status=status)
+    assert status.tolist() == [64]
