@@ -140,10 +140,19 @@ class PagedKVCacheQ4:
     method enqueues on the current stream; none waits for the device except
     ``check`` and ``free_page_count``.  Calls on different streams are the
     caller's to order (an event between them); the state's memory then stays
-    until the last of the streams is done with it."""
+    until the last of the streams is done with it.
+
+    ``lens``, ``pages`` and ``head`` are new tensors after every step, which a
+    CUDA graph could not follow: it would start each replay from the lengths
+    that it was captured with.  With ``capturable`` they are updated in place
+    (three small copies a ``reserve``, two a ``release``), so that every replay
+    of captured steps goes on where the last one ended; only then may
+    ``reserve``, ``attend``, ``trim`` and ``release`` be captured, with row
+    counts on the device (or one number).  Replays and calls in between are the
+    caller's to order like calls on different streams."""
 
     def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, max_seqs: int, max_len: int,
-                 page_size: int = 64, device="cuda"):
+                 page_size: int = 64, device="cuda", capturable: bool = False):
         if num_layers < 1 or max_seqs < 1 or max_len < 1:
             raise ValueError("num_layers, max_seqs and max_len must be positive")
         self.page_size, self.max_seqs, self.nkv = page_size, max_seqs, num_kv_heads
@@ -157,12 +166,35 @@ class PagedKVCacheQ4:
         self.head = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
         self._zeros = torch.zeros(max_seqs, **i32)
+        self.capturable = capturable
         self._workspace, self._sizes = {}, {}
         self._stream = _raw_stream(self.device.index)
+
+    def _capturing(self) -> bool:
+        if torch.cuda.current_device() == self.device.index:
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self.device):
+            return torch.cuda.is_current_stream_capturing()
+
+    def _keep(self, **state):
+        for name, t in state.items():
+            if self.capturable:
+                getattr(self, name).copy_(t)
+            else:
+                setattr(self, name, t)
+
+    def _upload(self, values, name: str):
+        """Host numbers on the device, without waiting for it."""
+        if self._capturing():
+            raise ValueError(f"{name} must be on the device in a CUDA graph, whose replays cannot read the host's")
+        values = values if torch.is_tensor(values) else torch.tensor(values, dtype=torch.int32)
+        return values.to(self.device, non_blocking=True)
 
     def _enter(self):
         """``lens``, ``pages`` and ``head`` are new tensors after each step: on another
         stream than the last call's, tell the allocator that it reads the old ones."""
+        if not self.capturable and self._capturing():
+            raise RuntimeError("a PagedKVCacheQ4 in a CUDA graph must be made with capturable=True")
         raw = _raw_stream(self.device.index)
         if raw != self._stream:
             self._stream = raw
@@ -176,12 +208,12 @@ class PagedKVCacheQ4:
         self._enter()
         if not torch.is_tensor(new_rows):
             num_slots = sum(new_rows) if num_slots is None else num_slots
-            new_rows = torch.tensor(list(new_rows), dtype=torch.int32).to(self.device, non_blocking=True)
+            new_rows = self._upload(list(new_rows), "new_rows")
         elif num_slots is None:
             raise ValueError("num_slots is needed with new_rows on the device")
         step = paged_reserve(self.lens, new_rows, self.pages, self.table, self.free_pages, self.head, self.page_size,
                              num_slots, self.status)
-        self.lens, self.pages, self.head = step.lens, step.pages, step.head
+        self._keep(lens=step.lens, pages=step.pages, head=step.head)
         return step
 
     def append(self, layer: int, k, v, step: PagedStep) -> None:
@@ -212,9 +244,10 @@ class PagedKVCacheQ4:
         if torch.is_tensor(counts):
             if counts.shape != self.lens.shape or counts.is_floating_point():
                 raise ValueError(f"counts must be {self.max_seqs} integers, got {counts.dtype} {tuple(counts.shape)}")
-            counts = counts.to(self.device, non_blocking=True)
+            if counts.device != self.device:
+                counts = self._upload(counts, "counts")
         # a negative count on the device, where nobody can raise, trims nothing
-        self.lens = torch.clamp(self.lens - counts, min=self._zeros, max=self.lens).to(torch.int32)
+        self._keep(lens=torch.clamp(self.lens - counts, min=self._zeros, max=self.lens).to(torch.int32))
 
     def release(self, seqs: Sequence[int] = ()) -> None:
         """Give spare pages back; requests ``seqs`` are finished and emptied."""
@@ -223,9 +256,12 @@ class PagedKVCacheQ4:
             raise ValueError(f"sequences must lie in [0, {self.max_seqs})")
         self._enter()
         if seqs:
-            self.lens = self.lens.index_fill(0, torch.tensor(seqs).to(self.device), 0)
-        self.pages, self.head = paged_release(self.lens, self.pages, self.table, self.free_pages, self.head,
-                                              self.page_size, self.status)
+            if self._capturing():
+                raise ValueError("finished requests cannot be named in a CUDA graph: every replay would empty them")
+            self._keep(lens=self.lens.index_fill(0, torch.tensor(seqs).to(self.device), 0))
+        pages, head = paged_release(self.lens, self.pages, self.table, self.free_pages, self.head, self.page_size,
+                                    self.status)
+        self._keep(pages=pages, head=head)
 
     def read(self, layer: int, seq: int, length: int, dtype=torch.float16):
         """The first ``length`` rows of a request, which it must hold, as

@@ -113,3 +113,70 @@ def test_starts_out_of_order_never_outgrow_the_tile_sums(pkg, rows, nkv, length)
     assert tiles * (n // 2) > 2 ** 32
     pkg.q4_attention(q, pool, table, torch.full((n,), length, dtype=i32).cuda(), starts=starts, max_rows=rows, status=status)
     assert status.tolist() == [64]
+
+
+# ---------------------------------------------------------------- CUDA graphs of the cache object
+def _rows(seed, rows, heads=2):
+    return torch.randn(rows, heads, 128, generator=torch.Generator().manual_seed(seed)).half().cuda()
+
+
+def _same_state(a, b):
+    return all(torch.equal(getattr(a, n), getattr(b, n)) for n in ("lens", "pages", "head", "table", "free_pages", "status"))
+
+
+@pytest.mark.parametrize("rows", [(2, 1, 0), (30, 7, 21)])
+def test_captured_steps_go_on_where_the_last_one_ended(pkg, rows):
+    """Replays of a captured step, with eager steps between them, against the same steps without a graph."""
+    total, most = sum(rows), max(rows)
+    k, q = _rows(1, total), _rows(2, total, 4)
+    new, drop = _dev(rows), _dev([1, 0, 0])
+    a, b = (pkg.PagedKVCacheQ4(1, 64, 2, 3, 400, 16, capturable=c) for c in (True, False))
+
+    def step(cache):
+        st = cache.reserve(new, num_slots=total)
+        cache.append(0, k, k, st)
+        out = cache.attend(0, q, st, most)
+        cache.trim(drop)
+        cache.release()
+        return st, out
+
+    for _ in range(2):
+        step(a), step(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st, out = step(a)
+    assert _same_state(a, b)                          # a capture runs nothing
+    for i in range(4):
+        k.copy_(_rows(10 + i, total))
+        graph.replay()
+        want_st, want = step(b)
+        assert torch.equal(out, want) and all(torch.equal(x, y) for x, y in zip(st, want_st))
+        assert _same_state(a, b), i
+        if i == 1:
+            st_a, _ = step(a)
+            st_b, _ = step(b)
+            assert torch.equal(st_a.slots, st_b.slots) and _same_state(a, b)
+            a.release([1])
+            b.release([1])
+    a.check()
+
+
+def test_the_cache_object_refuses_captures_that_it_cannot_follow(pkg):
+    cache = pkg.PagedKVCacheQ4(1, 8, 2, 2, 100, 16)
+    new, q = _dev([1, 1]), _rows(3, 2)
+    step = cache.reserve(new, num_slots=2)
+    lens = cache.lens.clone()
+    fixed = pkg.PagedKVCacheQ4(1, 8, 2, 2, 100, 16, capturable=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q.add_(0)
+        for call in (lambda: cache.reserve(new, num_slots=2), lambda: cache.attend(0, q, step, 1), lambda: cache.trim(1),
+                     lambda: cache.release()):
+            with pytest.raises(RuntimeError, match="capturable"):
+                call()
+        for call in (lambda: fixed.reserve([1, 1]), lambda: fixed.trim([1, 1]), lambda: fixed.release([0])):
+            with pytest.raises(ValueError, match="CUDA graph"):
+                call()
+    graph.replay()
+    assert torch.equal(cache.lens, lens) and fixed.lens.tolist() == [0, 0]
+    cache.check()
