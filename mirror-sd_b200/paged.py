@@ -190,9 +190,10 @@ class PagedKVCacheQ4:
         values = values if torch.is_tensor(values) else torch.tensor(values, dtype=torch.int32)
         return values.to(self.device, non_blocking=True)
 
-    def _enter(self):
+    def _enter(self) -> int:
         """``lens``, ``pages`` and ``head`` are new tensors after each step: on another
-        stream than the last call's, tell the allocator that it reads the old ones."""
+        stream than the last call's, tell the allocator that it reads the old ones.
+        Returns the current stream."""
         if not self.capturable and self._capturing():
             raise RuntimeError("a PagedKVCacheQ4 in a CUDA graph must be made with capturable=True")
         raw = _raw_stream(self.device.index)
@@ -200,6 +201,7 @@ class PagedKVCacheQ4:
             self._stream = raw
             for t in (self.lens, self.pages, self.head):
                 t.record_stream(torch.cuda.current_stream(self.device))
+        return raw
 
     def reserve(self, new_rows: Union[torch.Tensor, Sequence[int]], num_slots: Optional[int] = None) -> PagedStep:
         """Make room for new_rows[i] rows of request i (0 where it sits out).
@@ -220,18 +222,31 @@ class PagedKVCacheQ4:
         q4_append(k, v, step.slots, self.pools[layer], self.status)
 
     def attend(self, layer: int, q, step: PagedStep, max_rows: int, causal: bool = True, sink: int = 0,
-               window: int = 0, scale: Optional[float] = None, out=None):
-        """Attention of the step's query rows over everything cached."""
-        self._enter()
-        key = (max_rows, q.shape[1])
+               window: int = 0, scale: Optional[float] = None, out=None, workspace=None):
+        """Attention of the step's query rows over everything cached.  Without a
+        ``workspace`` (``q4_attention_workspace``) the object uses one of its own
+        for each stream; a call that is captured in a CUDA graph gets one of the
+        graph's, zeroed at every replay."""
+        stream = self._enter()
+        if workspace is None:
+            workspace = self._own_workspace(max_rows, q.shape[1], stream)
+        return q4_attention(q, self.pools[layer], self.table, self.lens, step.starts, max_rows, causal, sink, window,
+                            scale, out, self.status, workspace)
+
+    def _own_workspace(self, max_rows: int, num_heads: int, stream: int):
+        key = (max_rows, num_heads)
         size = self._sizes.get(key)
         if size is None:
             size = self._sizes[key] = _workspace_size(*key, self.nkv, self.device)
-        ws = self._workspace.get(self._stream)      # one for each stream: calls on different streams may overlap
+        zeros = lambda: torch.zeros(size, dtype=torch.uint8, device=self.device)
+        # A graph may be replayed on any stream, beside eager calls and other graphs, and long after a larger
+        # workspace has taken this one's place: it shares none with them.
+        if self._capturing():
+            return zeros()
+        ws = self._workspace.get(stream)            # calls on different streams may overlap
         if ws is None or ws.nbytes < size:
-            ws = self._workspace[self._stream] = torch.zeros(size, dtype=torch.uint8, device=self.device)
-        return q4_attention(q, self.pools[layer], self.table, self.lens, step.starts, max_rows, causal, sink, window,
-                            scale, out, self.status, ws)
+            ws = self._workspace[stream] = zeros()
+        return ws
 
     def trim(self, counts: Union[int, torch.Tensor, Sequence[int]]) -> None:
         """Drop the last counts[i] rows of request i (one number: of every

@@ -180,3 +180,84 @@ def test_the_cache_object_refuses_captures_that_it_cannot_follow(pkg):
     graph.replay()
     assert torch.equal(cache.lens, lens) and fixed.lens.tolist() == [0, 0]
     cache.check()
+
+
+def _two_caches(pkg, length, **kw):
+    caches = [pkg.PagedKVCacheQ4(1, 96, 1, 1, 6000, 64, **kw) for _ in range(2)]
+    k = _rows(5, length, 1)
+    for c in caches:
+        step = c.reserve([length])
+        c.append(0, k, k, step)
+    return caches, step
+
+
+@pytest.mark.parametrize("rows,heads", [(1, 8), (16, 4)])      # either kernel, the cached rows cut over many CTAs
+def test_a_graph_never_shares_the_objects_workspace(pkg, rows, heads):
+    """A captured attention writes into none of the object's workspaces, whichever is made, grown or dropped meanwhile."""
+    (cache, plain), _ = _two_caches(pkg, 5000, capturable=True)
+    q, big = _rows(6, rows, heads), _rows(7, 40, 8)
+    starts = pkg.PagedStep(_dev([0, rows]), None, None, None, None)
+    large = pkg.PagedStep(_dev([0, 40]), None, None, None, None)
+    want, want_big = plain.attend(0, q, starts, rows), plain.attend(0, big, large, 40)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        assert torch.equal(cache.attend(0, q, starts, rows), want)      # an eager call on the capturing stream first
+    side.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = cache.attend(0, q, starts, rows)
+        graphs.append((g, out))
+    with torch.cuda.stream(side):
+        eager = cache._workspace[side.cuda_stream]
+        eager.fill_(0x55)                                # (not used again: the larger call below takes its place)
+        for g, out in reversed(graphs):
+            g.replay()
+        assert bool((eager == 0x55).all())
+        for g, out in graphs:
+            assert torch.equal(out, want)
+        del eager, cache._workspace[side.cuda_stream]
+        assert torch.equal(cache.attend(0, big, large, 40), want_big)
+        held = cache._workspace[side.cuda_stream].clone()
+        spare = torch.full((1 << 24,), 0x66, dtype=torch.uint8, device="cuda")     # where a freed workspace might lie
+        for g, out in graphs:
+            out.zero_()
+            g.replay()
+            assert torch.equal(out, want)
+        assert torch.equal(held, cache._workspace[side.cuda_stream]) and bool((spare == 0x66).all())
+    side.synchronize()
+    cache.check()
+
+
+def test_attend_takes_a_workspace(pkg):
+    (cache, plain), _ = _two_caches(pkg, 3000)
+    q, step = _rows(6, 1, 8), pkg.PagedStep(_dev([0, 1]), None, None, None, None)
+    ws = pkg.q4_attention_workspace(1, 1, 8, 1)
+    assert torch.equal(cache.attend(0, q, step, 1, workspace=ws), plain.attend(0, q, step, 1))
+    assert not cache._workspace and len(plain._workspace) == 1
+    with pytest.raises(ValueError, match="workspace"):
+        cache.attend(0, q, step, 1, workspace=ws[:64])
+
+
+def test_threads_on_streams_of_their_own_use_workspaces_of_their_own(pkg):
+    """Two host threads attend at once; neither takes the other's stream."""
+    import threading
+    (cache, plain), _ = _two_caches(pkg, 5000)
+    q, step = _rows(6, 16, 4), pkg.PagedStep(_dev([0, 16]), None, None, None, None)
+    want = plain.attend(0, q, step, 16)
+    torch.cuda.synchronize()
+    outs = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(200):
+                outs[i].append(cache.attend(0, q, step, 16))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert len(cache._workspace) == 2 and all(torch.equal(o, want) for part in outs for o in part)
+    cache.check()
