@@ -145,7 +145,7 @@ class PagedKVCacheQ4:
     ``lens``, ``pages`` and ``head`` are new tensors after every step, which a
     CUDA graph could not follow: it would start each replay from the lengths
     that it was captured with.  With ``capturable`` they are updated in place
-    (three small copies a ``reserve``, two a ``release``), so that every replay
+    (four small copies a ``reserve``, two a ``release``), so that every replay
     of captured steps goes on where the last one ended; only then may
     ``reserve``, ``attend``, ``trim`` and ``release`` be captured, with row
     counts on the device (or one number).  Replays and calls in between are the
@@ -166,6 +166,7 @@ class PagedKVCacheQ4:
         self.head = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
         self._zeros = torch.zeros(max_seqs, **i32)
+        self._refused = torch.zeros(max_seqs, dtype=torch.bool, device=self.device)
         self.capturable = capturable
         self._workspace, self._sizes = {}, {}
         self._stream = _raw_stream(self.device.index)
@@ -191,7 +192,7 @@ class PagedKVCacheQ4:
         return values.to(self.device, non_blocking=True)
 
     def _enter(self) -> int:
-        """``lens``, ``pages`` and ``head`` are new tensors after each step: on another
+        """The state's tensors are new ones after each step: on another
         stream than the last call's, tell the allocator that it reads the old ones.
         Returns the current stream."""
         if not self.capturable and self._capturing():
@@ -199,14 +200,16 @@ class PagedKVCacheQ4:
         raw = _raw_stream(self.device.index)
         if raw != self._stream:
             self._stream = raw
-            for t in (self.lens, self.pages, self.head):
+            for t in (self.lens, self.pages, self.head, self._refused):
                 t.record_stream(torch.cuda.current_stream(self.device))
         return raw
 
     def reserve(self, new_rows: Union[torch.Tensor, Sequence[int]], num_slots: Optional[int] = None) -> PagedStep:
         """Make room for new_rows[i] rows of request i (0 where it sits out).
         ``num_slots`` bounds their sum; it is needed when new_rows is a device
-        tensor."""
+        tensor.  A request that cannot be served (``check`` says why) keeps its
+        length; its query rows of this step give nothing of use, and ``trim``
+        leaves it alone."""
         self._enter()
         if not torch.is_tensor(new_rows):
             num_slots = sum(new_rows) if num_slots is None else num_slots
@@ -215,7 +218,9 @@ class PagedKVCacheQ4:
             raise ValueError("num_slots is needed with new_rows on the device")
         step = paged_reserve(self.lens, new_rows, self.pages, self.table, self.free_pages, self.head, self.page_size,
                              num_slots, self.status)
-        self._keep(lens=step.lens, pages=step.pages, head=step.head)
+        asked = step.starts[1:] > step.starts[:-1]      # turned away: brought rows and has not grown since
+        self._keep(_refused=(step.lens == self.lens) & (asked | self._refused), lens=step.lens, pages=step.pages,
+                   head=step.head)
         return step
 
     def append(self, layer: int, k, v, step: PagedStep) -> None:
@@ -250,7 +255,9 @@ class PagedKVCacheQ4:
 
     def trim(self, counts: Union[int, torch.Tensor, Sequence[int]]) -> None:
         """Drop the last counts[i] rows of request i (one number: of every
-        request).  Pages stay with the request until ``release``."""
+        request).  Pages stay with the request until ``release``.  A request
+        that ``reserve`` turned away has no new rows to drop and keeps those it
+        holds, until it is served again or ``check`` has raised."""
         self._enter()
         if not torch.is_tensor(counts):
             counts = counts if isinstance(counts, int) else torch.tensor(list(counts), dtype=torch.int32)
@@ -262,6 +269,7 @@ class PagedKVCacheQ4:
             if counts.device != self.device:
                 counts = self._upload(counts, "counts")
         # a negative count on the device, where nobody can raise, trims nothing
+        counts = torch.where(self._refused, 0, counts)
         self._keep(lens=torch.clamp(self.lens - counts, min=self._zeros, max=self.lens).to(torch.int32))
 
     def release(self, seqs: Sequence[int] = ()) -> None:
@@ -295,6 +303,7 @@ class PagedKVCacheQ4:
         bits = int(self.status)
         if bits:
             self.status.zero_()
+            self._refused.zero_()
             if bits & 32:
                 self._workspace.clear()     # its counters may be left half way
             raise RuntimeError("paged cache: " + "; ".join(m for b, m in STATUS_BITS.items() if bits & b))

@@ -261,3 +261,52 @@ def test_threads_on_streams_of_their_own_use_workspaces_of_their_own(pkg):
     [t.join() for t in threads]
     assert len(cache._workspace) == 2 and all(torch.equal(o, want) for part in outs for o in part)
     cache.check()
+
+
+# ---------------------------------------------------------------- requests that reserve turns away
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("why", ["dry", "long", "slots"])
+def test_trim_keeps_the_rows_of_a_request_that_was_turned_away(pkg, why, capturable):
+    """The documented loop (reserve, append, trim, release, then check) on a request that could not be served."""
+    cache = pkg.PagedKVCacheQ4(1, 7 if why == "dry" else 40, 2, 3, 64 if why == "long" else 200, 16, capturable=capturable)
+    rows = _rows(1, 50)
+    first = cache.reserve([12, 30, 8])
+    cache.append(0, rows, rows, first)
+    held = cache.read(0, 1, 30)[0]
+    new = [4, 40, 4] if why == "slots" else [4, 36, 4] if why == "long" else [4, 60, 4]
+    step = cache.reserve(_dev(new), num_slots=40 if why == "slots" else 100)
+    served = {"dry": [16, 30, 12], "long": [16, 30, 12], "slots": [16, 30, 8]}[why]     # (what follows is over the slots too)
+    assert step.lens.tolist() == served
+    cache.append(0, _rows(2, step.slots.numel()), _rows(3, step.slots.numel()), step)
+    drop = [2, 15, 2]
+    cache.trim(_dev(drop) if why != "long" else drop)
+    cache.release()
+    after = [14, 30, 8 if why == "slots" else 10]
+    assert cache.lens.tolist() == after and cache.pages.tolist() == [-(-a // 16) for a in after]
+    assert torch.equal(cache.read(0, 1, 30)[0], held)
+    cache.reserve([1, 0, 1])                              # it sits out: still what it held
+    cache.trim(1)
+    assert cache.lens.tolist() == after
+    with pytest.raises(RuntimeError):
+        cache.check()
+    cache.trim([0, 3, 0])                                 # told: rows that it holds may be dropped
+    assert cache.lens.tolist() == [after[0], 27, after[2]]
+    cache.reserve([0, 5, 0])
+    cache.trim(2)                                         # served again
+    assert cache.lens.tolist() == [after[0] - 2, 30, after[2] - 2]
+    cache.check()
+
+
+def test_trim_in_a_graph_keeps_the_rows_of_a_request_that_was_turned_away(pkg):
+    cache = pkg.PagedKVCacheQ4(1, 4, 2, 2, 400, 16, capturable=True)
+    new = _dev([10, 3])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.reserve(new, num_slots=13)
+        cache.trim(2)
+        cache.release()
+    for want in [[8, 1], [16, 2], [24, 3], [32, 4], [40, 5], [40, 6], [40, 7]]:      # 50 rows would need a fourth page
+        graph.replay()
+        assert cache.lens.tolist() == want
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache.check()
