@@ -165,7 +165,6 @@ class PagedKVCacheQ4:
         self.free_pages = torch.arange(num_pages, **i32)
         self.head = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
-        self._zeros = torch.zeros(max_seqs, **i32)
         self._refused = torch.zeros(max_seqs, dtype=torch.bool, device=self.device)
         self.capturable = capturable
         self._workspace, self._sizes = {}, {}
@@ -268,9 +267,9 @@ class PagedKVCacheQ4:
                 raise ValueError(f"counts must be {self.max_seqs} integers, got {counts.dtype} {tuple(counts.shape)}")
             if counts.device != self.device:
                 counts = self._upload(counts, "counts")
-        # a negative count on the device, where nobody can raise, trims nothing
-        counts = torch.where(self._refused, 0, counts)
-        self._keep(lens=torch.clamp(self.lens - counts, min=self._zeros, max=self.lens).to(torch.int32))
+        # a negative count on the device, where nobody can raise, trims nothing (lens less a number >= 0 cannot wrap)
+        counts = torch.where(self._refused, 0, counts).clamp(min=0)
+        self._keep(lens=torch.clamp(self.lens - counts, min=0).to(torch.int32))
 
     def release(self, seqs: Sequence[int] = ()) -> None:
         """Give spare pages back; requests ``seqs`` are finished and emptied."""

@@ -310,3 +310,14 @@ def test_trim_in_a_graph_keeps_the_rows_of_a_request_that_was_turned_away(pkg):
         assert cache.lens.tolist() == want
     with pytest.raises(RuntimeError, match="free pages"):
         cache.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_trim_counts_at_the_ends_of_their_type(pkg, dtype):
+    cache = pkg.PagedKVCacheQ4(1, 8, 2, 3, 100, 16)
+    cache.reserve([20, 5, 7])
+    ends = torch.iinfo(dtype)
+    cache.trim(torch.tensor([ends.min, ends.min + 3, 2], dtype=dtype).cuda())      # negative: nothing
+    assert cache.lens.tolist() == [20, 5, 5]
+    cache.trim(torch.tensor([ends.max, 0, -1], dtype=dtype).cuda())
+    assert cache.lens.tolist() == [0, 5, 5]
