@@ -280,7 +280,7 @@ class PagedKVCacheQ4:
         if seqs:
             if self._capturing():
                 raise ValueError("finished requests cannot be named in a CUDA graph: every replay would empty them")
-            self._keep(lens=self.lens.index_fill(0, torch.tensor(seqs).to(self.device), 0))
+            self._keep(lens=self.lens.index_fill(0, torch.tensor(seqs).to(self.device, non_blocking=True), 0))
         pages, head = paged_release(self.lens, self.pages, self.table, self.free_pages, self.head, self.page_size,
                                     self.status)
         self._keep(pages=pages, head=head)

@@ -321,3 +321,29 @@ def test_trim_counts_at_the_ends_of_their_type(pkg, dtype):
     assert cache.lens.tolist() == [20, 5, 5]
     cache.trim(torch.tensor([ends.max, 0, -1], dtype=dtype).cuda())
     assert cache.lens.tolist() == [0, 5, 5]
+
+
+# ---------------------------------------------------------------- what waits for the device
+def test_only_check_and_free_page_count_wait_for_the_device(pkg):
+    cache = pkg.PagedKVCacheQ4(1, 16, 2, 3, 100, 16)
+    x, q, new = _rows(1, 6), _rows(2, 6, 4), _dev([1, 2, 3])
+    drop = _dev([0, 1, 1])
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for step in (cache.reserve([1, 2, 3]), cache.reserve(new, num_slots=6)):
+            cache.append(0, x, x, step)
+            cache.attend(0, q, step, 3)
+        cache.trim(drop)
+        cache.trim([1, 0, 0])
+        cache.trim(1)
+        cache.release()
+        cache.release([0, 2])
+        for wait in (cache.check, cache.free_page_count):
+            with pytest.raises(RuntimeError, match="synchroniz"):
+                wait()
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    assert cache.lens.tolist() == [0, 2, 0]
+    cache.check()
