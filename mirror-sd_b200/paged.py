@@ -46,7 +46,10 @@ class PagedStep(NamedTuple):
     head: torch.Tensor
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream().cuda_stream without the Stream object
+def _raw_stream(index: int) -> int:
+    """current_stream().cuda_stream without the Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)     # (a torch without CUDA lacks it, and still imports this package)
+
 
 # Arguments are checked, and outputs made, in csrc/paged_binding.cpp.
 

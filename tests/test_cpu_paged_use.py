@@ -2,6 +2,8 @@
 on, importing and building, and refusals at the ends of the ranges."""
 import ctypes
 import os
+import subprocess
+import sys
 
 import numpy as np
 import torch
@@ -69,3 +71,17 @@ def test_tile_sums_stay_in_range():
         for x in v:
             line = add(line, x)
         assert tree[0] == line == min(sum(v), full)
+
+
+# ---------------------------------------------------------------- importing and building
+ROOT = os.path.dirname(CSRC[:-len("/csrc")])
+
+
+def test_package_imports_on_a_torch_without_cuda():
+    code = ("import importlib, torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, n)\n"
+            "pkg = importlib.import_module('mirror-sd_b200')\n"
+            "assert pkg.PagedKVCacheQ4 and pkg.DFlashConfig\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
