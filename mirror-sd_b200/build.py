@@ -3,9 +3,11 @@ and ``lib/dflash_paged.so``, the Python binding of its paged-cache operators.
 
     python mirror-sd_b200/build.py [--force] [--verbose]
 
-Only nvcc, g++ and the headers of Python and torch are needed (no GPU); the
-library is what the Python host (`_native.py`) loads with ctypes and what the C
-ABI in include/dflash_b200.h describes.
+Only nvcc is needed for the library (no GPU), which is what the Python host
+(`_native.py`) loads with ctypes and what the C ABI in include/dflash_b200.h
+describes.  The binding needs g++ and the headers of Python and torch besides;
+without torch it is left out, and when it does not compile the library is there
+all the same (and the build says so and fails).
 """
 import argparse
 import hashlib
@@ -36,8 +38,18 @@ def _nvcc():
     return "nvcc"
 
 
+def _torch_dir():
+    spec = importlib.util.find_spec("torch")
+    return spec and os.path.dirname(spec.origin)
+
+
+def _torch_version():
+    with open(os.path.join(_torch_dir(), "version.py")) as fh:
+        return fh.read()
+
+
 def _binding_command(out):
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    torch = _torch_dir()
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-isystem", os.path.join(torch, "include"), "-isystem",
             os.path.join(torch, "include", "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"],
             "-I" + os.path.join(os.path.dirname(os.path.dirname(_nvcc())) or "/usr/local/cuda", "include"),
@@ -45,25 +57,49 @@ def _binding_command(out):
             "-ltorch_python", "-o", out]
 
 
-def _digest():
-    h = hashlib.sha256(" ".join(_binding_command("")).encode())
-    for f in SOURCES + HEADERS + [BINDING_SOURCE]:
+def _digest(sources, *how):
+    h = hashlib.sha256(" ".join(how).encode())
+    for f in sources:
         with open(os.path.join(CSRC, f), "rb") as fh:
             h.update(fh.read())
     with open(os.path.join(ROOT, "include", "dflash_b200.h"), "rb") as fh:
         h.update(fh.read())
-    h.update(" ".join(NVCC_FLAGS).encode())
     return h.hexdigest()
+
+
+def _stamped(path, digest):
+    if not os.path.exists(path) or not os.path.exists(path + ".sha256"):
+        return False
+    with open(path + ".sha256") as fh:
+        return fh.read().strip() == digest
+
+
+def _stamp(path, digest):
+    with open(path + ".sha256", "w") as fh:
+        fh.write(digest)
 
 
 def build(force=False, verbose=False, jobs=None):
     os.makedirs(LIB_DIR, exist_ok=True)
-    stamp = LIB + ".sha256"
-    dig = _digest()
-    if not force and os.path.exists(LIB) and os.path.exists(BINDING) and os.path.exists(stamp):
-        with open(stamp) as fh:
-            if fh.read().strip() == dig:
-                return LIB
+    lib_digest = _digest(SOURCES + HEADERS, *NVCC_FLAGS)
+    if force or not _stamped(LIB, lib_digest):
+        _build_library(verbose)
+        _stamp(LIB, lib_digest)
+    if _torch_dir() is None:
+        print(f"torch is not installed: {os.path.basename(BINDING)} (the paged operators' Python binding) is left out")
+        return LIB
+    # (an upgrade in place keeps torch's path, but not its headers)
+    binding_digest = _digest([BINDING_SOURCE], _torch_version(), sys.version, *_binding_command(""))
+    if force or not _stamped(BINDING, binding_digest):
+        r = subprocess.run(_binding_command(BINDING + ".tmp"), capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"{LIB} is built, its Python binding is not:\n--- {BINDING_SOURCE}\n{r.stdout}\n{r.stderr}")
+        os.replace(BINDING + ".tmp", BINDING)
+        _stamp(BINDING, binding_digest)
+    return LIB
+
+
+def _build_library(verbose):
     objs = []
     procs = []
     for src in SOURCES:
@@ -74,8 +110,6 @@ def build(force=False, verbose=False, jobs=None):
             print(" ".join(cmd))
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         objs.append(obj)
-    procs.append((BINDING_SOURCE, subprocess.Popen(_binding_command(BINDING + ".tmp"), stdout=subprocess.PIPE,
-                                                   stderr=subprocess.STDOUT)))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -93,12 +127,8 @@ def build(force=False, verbose=False, jobs=None):
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    os.replace(BINDING + ".tmp", BINDING)
     for o in objs:
         os.remove(o)
-    with open(stamp, "w") as fh:
-        fh.write(dig)
-    return LIB
 
 
 if __name__ == "__main__":

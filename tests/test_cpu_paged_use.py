@@ -1,11 +1,13 @@
 """Host side of the paged 4-bit cache without a GPU: what its kernels may rely
 on, importing and building, and refusals at the ends of the ranges."""
 import ctypes
+import importlib.util
 import os
 import subprocess
 import sys
 
 import numpy as np
+import pytest
 import torch
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mirror-sd_b200", "csrc")
@@ -85,3 +87,59 @@ def test_package_imports_on_a_torch_without_cuda():
             "assert pkg.PagedKVCacheQ4 and pkg.DFlashConfig\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+@pytest.fixture
+def builder(tmp_path, monkeypatch):
+    """build.py with an output folder of its own and a library that need not be compiled again."""
+    spec = importlib.util.spec_from_file_location("dflash_build", os.path.join(ROOT, "mirror-sd_b200", "build.py"))
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    for name, file in (("LIB_DIR", ""), ("LIB", "lib.so"), ("BINDING", "binding.so")):
+        monkeypatch.setattr(b, name, str(tmp_path / file))
+    b.compiled = []
+
+    def library(verbose):
+        b.compiled.append("library")
+        with open(b.LIB, "w") as f:
+            f.write("library")
+
+    monkeypatch.setattr(b, "_build_library", library, raising=False)
+    return b
+
+
+def _as_binding(b, monkeypatch, *how):
+    def command(out):
+        if out:
+            b.compiled.append("binding")
+        return ["cp", *how, os.path.join(CSRC, b.BINDING_SOURCE), out]
+    monkeypatch.setattr(b, "_binding_command", command)
+
+
+def test_library_builds_without_torch(builder, monkeypatch, capsys):
+    monkeypatch.setattr(builder.importlib.util, "find_spec", lambda name: None)
+    assert builder.build() == builder.LIB and os.path.exists(builder.LIB) and not os.path.exists(builder.BINDING)
+    assert "torch is not installed" in capsys.readouterr().out
+    builder.build()
+    assert builder.compiled == ["library"]
+
+
+def test_library_is_there_when_the_binding_does_not_compile(builder, monkeypatch):
+    _as_binding(builder, monkeypatch, "--no-such-flag")
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="binding"):
+            builder.build()
+    assert os.path.exists(builder.LIB) and not os.path.exists(builder.BINDING)
+    assert builder.compiled == ["library", "binding", "binding"]
+
+
+def test_binding_is_built_again_for_another_torch(builder, monkeypatch):
+    _as_binding(builder, monkeypatch)
+    builder.build()
+    builder.build()
+    assert builder.compiled == ["library", "binding"] and os.path.exists(builder.BINDING)
+    assert torch.__version__.split("+")[0] in builder._torch_version()
+    monkeypatch.setattr(builder, "_torch_version", lambda: "99.0")
+    builder.build()
+    builder.build()
+    assert builder.compiled == ["library", "binding", "binding"]
