@@ -133,7 +133,7 @@ Rows rows_of(PyObject* o, const char* name, int64_t heads, int dev) {
     refuse("%s must be f16 or bf16 [rows, %s, 128] on cuda:%d, got %s", name,
            heads >= 0 ? std::to_string(heads).c_str() : "heads", dev, describe(r.t).c_str());
   if (r.t.stride(2) != 1 || (r.t.stride(0) | r.t.stride(1)) % 8 || reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16)
-    r.t = r.t.contiguous();
+    r.t = r.t.clone(at::MemoryFormat::Contiguous);   // (contiguous() keeps a misaligned tensor, or a stride of one row)
   r.data = static_cast<const uint16_t*>(r.t.data_ptr());
   r.row = r.t.stride(0);
   r.head = r.t.stride(1);

@@ -347,3 +347,25 @@ def test_only_check_and_free_page_count_wait_for_the_device(pkg):
         torch.cuda.set_sync_debug_mode(mode)
     assert cache.lens.tolist() == [0, 2, 0]
     cache.check()
+
+
+# ---------------------------------------------------------------- arguments
+def test_rows_that_the_kernels_cannot_read_in_place_are_copied(pkg):
+    """Contiguous but not on 16 bytes; one row, or one head, of any stride."""
+    g = torch.Generator().manual_seed(4)
+    flat = torch.randn(4096, generator=g).half().cuda()
+    pool, slots = pkg.q4_pool(2, 2, 16), _dev([3, 17, 9])
+    shifted = flat[1:1 + 3 * 2 * 128].view(3, 2, 128)
+    assert shifted.is_contiguous() and shifted.data_ptr() % 16
+    row = flat.as_strided((1, 2, 128), (77, 128, 1))
+    for x in (shifted, row):
+        pkg.q4_append(x, x, slots[:x.shape[0]], pool)
+        assert torch.equal(pkg.q4_read(pool, slots[:x.shape[0]])[1].double().cpu(), U.q4_values(x.cpu()))
+    one, head = pkg.q4_pool(2, 1, 16), flat.as_strided((3, 1, 128), (256, 33, 1))
+    pkg.q4_append(head, head, slots, one)
+    assert torch.equal(pkg.q4_read(one, slots)[0].double().cpu(), U.q4_values(head.cpu()))
+    c = Case(pkg, [70], [3], 2, 1, 32, torch.float16)
+    want = c.check(pkg)
+    q = torch.cat([c.q.flatten()[:1], c.q.flatten()])[1:].view_as(c.q)
+    assert q.data_ptr() % 16
+    assert torch.equal(pkg.q4_attention(q, c.pool, c.pg.dev("table"), c.pg.dev("lens"), max_rows=3), want)
