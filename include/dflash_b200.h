@@ -402,17 +402,17 @@ int dflash_q4_read(const uint8_t* pool, int num_pages, int page_size, const int3
                    int bf16, uint16_t* k, uint16_t* v, void* stream);
 
 /* q [rows, nq, 128], f16 or bf16, strides in elements (multiples of 8); out
- * [rows, nq, 128] of the same type.  Request i owns rows starts[i] ..
- * starts[i + 1] - 1, at most max_rows of them (starts NULL: max_rows each;
- * otherwise DFLASH_PAGED_ROWS is set and that request's rows are undefined),
- * and holds lens[i] cached rows, its own new ones included.  With causal,
- * query row j of m sees keys below e = lens[i] - m + j + 1, else below
- * e = lens[i]; with a window only keys < sink or >= e - window.  A row that
- * sees no key is zeros; rows of no request are not written.  Table entries
- * outside the pool hide their rows.  max_pages * page_size <= 2^30, and the
- * tiles of 64 or 128 cached rows (a full table of them for every group of query
- * rows and kv head) are fewer than 2^31.  scale:
- * positive and finite.
+ * [rows, nq, 128] of the same type, not overlapping q.  Request i owns rows
+ * starts[i] .. starts[i + 1] - 1, at most max_rows of them (starts NULL:
+ * max_rows each; where starts do not fit, DFLASH_PAGED_ROWS is set and that
+ * request's rows are undefined), and holds lens[i] cached rows, its own new
+ * ones included.  With causal, query row j of m sees keys below
+ * e = lens[i] - m + j + 1, else below e = lens[i]; with a window only keys
+ * < sink or >= e - window.  A row that sees no key is zeros; rows of no request
+ * are not written.  Table entries outside the pool hide their rows.
+ * max_pages * page_size <= 2^30, and the tiles of 64 or 128 cached rows (a full
+ * table of them for every group of query rows and kv head) are fewer than 2^31.
+ * scale: positive and finite.
  * workspace: dflash_q4_attention_workspace_size() bytes, 16-byte aligned,
  * zeroed once before its first use; every call leaves it ready for the next
  * one of any shape it is large enough for (unless DFLASH_PAGED_TIMEOUT was set:

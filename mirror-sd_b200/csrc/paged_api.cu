@@ -49,6 +49,19 @@ int check_pool(int rows, int nkv, const void* pool, int num_pages, int page_size
   return DFLASH_OK;
 }
 
+// whether out [rows, nq, 128] touches a row of q (strides in elements)
+bool overlap(const uint16_t* out, const uint16_t* q, long long q_row, long long q_head, long long rows, int nq) {
+  const long long heads = (nq - 1) * q_head, all = (rows - 1) * q_row;
+  const long long span = (heads < 0 ? -heads : heads) + 128, stride = q_row < 0 ? -q_row : q_row;   // a row's elements
+  const long long lowest = (heads < 0 ? heads : 0) + (all < 0 ? all : 0);
+  // out in elements from q's lowest one on: [a, b)
+  const long long a = ((long long)(uintptr_t)out - (long long)(uintptr_t)q) / 2 - lowest, b = a + rows * nq * 128;
+  if (b <= 0) return false;
+  if (stride == 0) return a < span;
+  const long long first = a < span ? 0 : (a - span) / stride + 1;   // first row that ends behind a
+  return first < rows && first * stride < b;
+}
+
 constexpr size_t kCounterBytes = 4096;   // two counters per SM, then the partials
 
 }  // namespace
@@ -183,6 +196,8 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
     return fail(DFLASH_ERR_INVALID, "workspace too small (%zu < %zu)", workspace_bytes,
                 dflash_q4_attention_workspace_size(max_rows, nq, nkv));
   if (rows == 0) return DFLASH_OK;
+  // (the kernels read q through the non-coherent path, some rows after others are finished)
+  if (overlap(out, q, q_row, q_head, rows, nq)) return fail(DFLASH_ERR_INVALID, "out overlaps q");
   int sms = 0;
   if (int rc = num_sms(&sms)) return rc;
   if ((size_t)sms * 2 * sizeof(int) > kCounterBytes) return fail(DFLASH_ERR_INVALID, "%d SMs", sms);

@@ -129,7 +129,8 @@ def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: b
     causal: query row j of m sees the keys below lens - m + j + 1 (else below
     lens); window: of those only the first ``sink`` and the last ``window``.
     A row that sees no key gives zeros; rows of q that no request owns leave
-    their rows of ``out`` unwritten.  scale (positive) defaults to 128 ** -0.5."""
+    their rows of ``out`` unwritten.  ``out`` must not overlap q.  scale
+    (positive) defaults to 128 ** -0.5."""
     if workspace is None:
         if pool.dim() != 4 or q.dim() != 3:
             raise ValueError("q must be [rows, heads, 128] and pool a tensor from q4_pool()")

@@ -29,7 +29,8 @@ def test_paged_kernels_do_not_wait_for_other_ctas():
 P = ctypes.c_void_p(4096)      # never dereferenced: the checks fail first, or there is no device
 
 
-def _attend(lib, n=1, width=8, page=64, rows=1, max_rows=1, nq=2, nkv=2, window=0, starts=None, q=P, out=P, q_row=256):
+def _attend(lib, n=1, width=8, page=64, rows=1, max_rows=1, nq=2, nkv=2, window=0, starts=None, q=P,
+            out=ctypes.c_void_p(1 << 44), q_row=256):
     return lib.dflash_q4_attention(q, q_row, 128, 0, P, 16, page, P, width, width, P, starts, n, rows, max_rows, nq, nkv, 1,
                                    0, window, 0.1, out, None, P, 1 << 30, None)
 
@@ -143,3 +144,19 @@ def test_binding_is_built_again_for_another_torch(builder, monkeypatch):
     builder.build()
     builder.build()
     assert builder.compiled == ["library", "binding", "binding"]
+
+
+def test_attention_refuses_an_output_over_its_queries(pkg):
+    """Strided query rows: the output may lie beside them, in front or behind, or in the gap between two rows."""
+    lib = pkg._native.load()
+    at = lambda byte: ctypes.c_void_p((1 << 20) + byte)
+    call = lambda byte, rows, row, **kw: _attend(lib, rows=rows, max_rows=rows, q=at(0), out=at(byte), q_row=row, **kw)
+    size = lambda rows: rows * 2 * 256
+    for rows, row, byte in ((4, 256, 0), (4, 256, 16), (4, 256, -16), (4, 256, size(4) - 16), (4, 256, 16 - size(4)),
+                            (3, 1024, 2048), (3, 1024, 1024), (3, 1024, 4096 + 496), (3, 0, 0), (3, 0, 496), (2, 4096, 8192),
+                            (2, 4096, 8192 - 16), (3, -256, 0), (3, -256, -1024)):
+        _refused(pkg, call(byte, rows, row), "overlaps")
+    if not torch.cuda.is_available():           # (past the check there is no device)
+        for rows, row, byte in ((4, 256, size(4)), (4, 256, -size(4)), (3, 1024, 4096 + 512), (3, 0, 512), (2, 4096, 512),
+                                (2, 4096, 8192 - 1024), (1, 4096, 8192), (3, -256, 512), (3, -256, -1024 - size(3))):
+            assert call(byte, rows, row) != pkg._native.DFLASH_ERR_INVALID, (rows, row, byte, pkg._native.last_error())

@@ -369,3 +369,18 @@ def test_rows_that_the_kernels_cannot_read_in_place_are_copied(pkg):
     q = torch.cat([c.q.flatten()[:1], c.q.flatten()])[1:].view_as(c.q)
     assert q.data_ptr() % 16
     assert torch.equal(pkg.q4_attention(q, c.pool, c.pg.dev("table"), c.pg.dev("lens"), max_rows=3), want)
+
+
+def test_attention_writes_between_query_rows_but_not_over_them(pkg):
+    c = Case(pkg, [70], [2], 4, 2, 32, torch.float16)
+    want = c.check(pkg)
+    args = (c.pool, c.pg.dev("table"), c.pg.dev("lens"))
+    wide = torch.zeros(2, 16 * 128, dtype=torch.float16).cuda()
+    q = wide[:, :512].view(2, 4, 128)
+    q.copy_(c.q)
+    gap = wide.flatten()[512:512 + 1024].view(2, 4, 128)       # behind row 0, in front of row 1
+    assert pkg.q4_attention(q, *args, max_rows=2, out=gap) is gap and torch.equal(gap, want) and torch.equal(q, c.q)
+    with pytest.raises(ValueError, match="overlaps"):
+        pkg.q4_attention(c.q, *args, max_rows=2, out=c.q)
+    with pytest.raises(ValueError, match="overlaps"):
+        pkg.q4_attention(q, *args, max_rows=2, out=wide.flatten()[256:1280].view(2, 4, 128))
