@@ -3,7 +3,7 @@
 #include <cmath>
 
 #include "api_error.cuh"
-#include "q4.cuh"
+#include "q4_attn.cuh"
 
 using namespace dfl;
 
@@ -209,6 +209,7 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
   p.page_shift = log2_of(page_size);
   p.max_pages = max_pages; p.num_pages = num_pages; p.causal = causal != 0; p.sink = sink; p.window = window;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  p.factor = score_factor(16.f * p.scale_log2);
   p.out = out; p.status = status;
   p.counters = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);

@@ -112,6 +112,7 @@ struct Q4AttnParams {
   Divisor by_g, by_nkv;              // G = NQ / NKV; NKV
   int causal, sink, window;
   float scale_log2;                  // softmax scale * log2(e)
+  float factor;                      // score_factor of 16 times it (q4_attn.cuh)
   void* out;                         // [T, NQ, 128] contiguous, q's type
   int* counters;                     // [2 * num_sms], zero between calls
   float* part;                       // partial results

@@ -52,7 +52,6 @@ constexpr int QA_STAGE = QA_TILE / kQ4Rows * kQ4Block;
 // 11.7 with 2, 11.4 with 4, 12.3 with 8).
 constexpr int QA_LEAST = 4;
 constexpr float QA_RAISE = 8.f;
-constexpr float QA_UNSET = 1e30f;                // -reference of a column that has seen no key
 
 // ---- fragments
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -283,7 +282,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
             for (int i = 0; i < 16; ++i)
               qr[i] = pack_f16x2(__uint_as_float(qr[i] << 16) * down, __uint_as_float(qr[i] & 0xffff0000u) * down);
           }
-          f *= 16.f * p.scale_log2;
+          f = score_factor(f * 16.f * p.scale_log2);
           // the lane's score columns are queries 2c and 2c + 1 of this group of 8
           qscale[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c);
           qscale[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
@@ -291,7 +290,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
           for (int x = 0; x < 2; ++x) {
             const int jj = p.by_g.of(r0 + nt * 8 + 2 * c + x);
             key_end[nt][x] = jj < cur.it.rows ? (p.causal ? cur.it.L - cur.it.rows + jj + 1 : cur.it.L) : 0;
-            negm[nt][x] = QA_UNSET;
+            negm[nt][x] = kUnset;
             l[nt][x] = 0.f;
           }
         }
@@ -350,9 +349,9 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
               }
             }
           }
-          // Base-2 scores less the columns' references (negm = 1e30 until a column
-          // has seen a key); hidden keys get -inf.  Where one passes 2^8 the
-          // references move first.
+          // Scores less the columns' references (negm: minus the largest product that
+          // set it), base 2; hidden keys get -inf.  Where one passes 2^8 the references
+          // move first.
           float y[2][NT][4];
           auto scores = [&]() {
             float top = -INFINITY;
@@ -361,7 +360,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) y[i][nt][x] = fmaf(sc[i][nt][x], qscale[nt][x & 1], negm[nt][x & 1]);
+                for (int x = 0; x < 4; ++x) y[i][nt][x] = (sc[i][nt][x] + negm[nt][x & 1]) * qscale[nt][x & 1];
                 if (!all_seen) {
 #pragma unroll
                   for (int x = 0; x < 4; ++x) {
@@ -380,16 +379,17 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                // the column's largest score, rounded up so that none lies above its reference
+                // the column's largest product
                 float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                   for (int h = 0; h < 4; h += 2)
-                    if (y[i][nt][h + x] != -INFINITY) top = fmaxf(top, __fmul_ru(sc[i][nt][h + x], qscale[nt][x]));
+                    if (y[i][nt][h + x] != -INFINITY) top = fmaxf(top, sc[i][nt][h + x]);
                 top = col_max(top);
-                const bool up = top > QA_RAISE - negm[nt][x];
-                const float f = up ? exp2_fast(-negm[nt][x] - top) : 1.f;
+                const float rise = (top + negm[nt][x]) * qscale[nt][x];
+                const bool up = rise > QA_RAISE;
+                const float f = up ? exp2_fast(-rise) : 1.f;
                 negm[nt][x] = up ? -top : negm[nt][x];
                 l[nt][x] *= f;
 #pragma unroll
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
                 store_out4(p, cur.it.row0 + j, G0 + r - j * G, 16 * g + 2 * t, v);
             }
             if (!whole && g == 0) {
-              part[QT * 128 + q] = negm[nt][x] == QA_UNSET ? -INFINITY : -negm[nt][x];
+              part[QT * 128 + q] = partial_max(negm[nt][x], qscale[nt][x]);
               part[QT * 129 + q] = sum;
             }
           }

@@ -36,8 +36,8 @@
 // one kind of tile): the roles share the instruction cache.
 //
 // What it measures (8 kv heads): 256 requests x 16 rows x 32 heads over a sink of
-// 64 and a window of 1,040 rows 246 us, 16 requests of up to 32,768 rows with up to
-// 32 rows x 40 heads 215 us, one such request 56 us; HBM would allow 59, 31 and 6,
+// 64 and a window of 1,040 rows 250 us, 16 requests of up to 32,768 rows with up to
+// 32 rows x 40 heads 218 us, one such request 57 us; HBM would allow 59, 31 and 6,
 // the products alone 44, 37 and 13.  What bounds it: a tile takes each role 1,500
 // to 2,000 cycles (at 64 columns; 512 of them are MMAs), half the issue slots and
 // most of shared memory's bandwidth (V^T and P^T are written and read again), so
@@ -55,7 +55,6 @@ constexpr int QB_STAGE = QB_TILE / kQ4Rows * QB_BLK;
 constexpr int QB_SEEN = 256;               // flag of a tile that every query of the item sees whole
 constexpr int QB_SLACK = 6;
 constexpr float QB_RAISE = 8.f;
-constexpr float QB_UNSET = 1e30f;          // -reference of a column that has seen no key
 
 template <int N_>
 struct QbCfg {
@@ -217,6 +216,15 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(r));
   return o;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t x, y, r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  float2 o;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(r));
+  return o;
+}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   uint64_t x, y, z, r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
@@ -238,15 +246,13 @@ __device__ __forceinline__ int float_key(float f) {
   return i ^ (i >> 31 & 0x7fffffff);
 }
 __device__ __forceinline__ float key_float(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
-// scores of columns 16 c .. of this thread's cached row less the references
-// (negm; NULL: as they are)
-__device__ __forceinline__ void scores16(const uint32_t (&s)[16], const float* negm, float f, int c, float2 (&y)[8]) {
+// products of columns 16 c .. of this thread's cached row less the references
+__device__ __forceinline__ void scores16(const uint32_t (&s)[16], const float* negm, int c, float2 (&y)[8]) {
 #pragma unroll
   for (int i = 0; i < 16; i += 4) {
-    const float4 m = negm ? *reinterpret_cast<const float4*>(negm + 16 * c + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    y[i / 2] = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(f, f), make_float2(m.x, m.y));
-    y[i / 2 + 1] =
-        fma2(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(f, f), make_float2(m.z, m.w));
+    const float4 m = *reinterpret_cast<const float4*>(negm + 16 * c + i);
+    y[i / 2] = add2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(m.x, m.y));
+    y[i / 2 + 1] = add2(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(m.z, m.w));
   }
 }
 
@@ -432,11 +438,11 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       const int nt = bad ? c1 - u : sg.nt, j0 = bad ? 0 : sg.j0;
       const float* qf = ms.qf[seg % C::SEGS];
       const bool uniform = sg.uniform;
-      const float f = 16.f * p.scale_log2;
+      const float f = p.factor;
       if (gt < N) {
         const int r = sg.q0 + gt, j = p.by_g.of(r);
         const bool real = j < it.rows;
-        negm[gt] = real ? QB_UNSET : 0.f;
+        negm[gt] = real ? kUnset : 0.f;
         if (x == 0) {
           ms.cend[gt] = real ? (p.causal ? it.L - it.rows + j + 1 : it.L) : 0;
           ms.coff[gt] = real ? (it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;
@@ -511,19 +517,20 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
             uint32_t w[8];
             float2 y[8];
             const float on = c >= add ? 1.f : 0.f;
-            scores16(s, negm, f, c, y);
+            scores16(s, negm, c, y);
             float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
               top = max3(top, y[i].x, y[i].y);
               top2 = max3(top2, y[i + 1].x, y[i + 1].y);
             }
-            if (__any_sync(0xffffffffu, check && fmaxf(top, top2) > QB_RAISE)) {
+            if (__any_sync(0xffffffffu, check && fmaxf(top, top2) * f > QB_RAISE)) {
               tmem_ld_wait();
               return c;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
+              y[i] = mul2(y[i], make_float2(f, f));
               y[i].x = exp2_fast(y[i].x);
               y[i].y = exp2_fast(y[i].y);
               l[8 * c + i] = fma2(y[i], make_float2(on, on), l[8 * c + i]);
@@ -552,9 +559,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               uint32_t s[16];
               tmem_ld16(s_t + 16 * c, s);
               tmem_ld_wait();
-              // rounded up: no score lies above its reference, however large both are
 #pragma unroll
-              for (int i = 0; i < 16; ++i) stage[i * 36 + lane] = __fmul_ru(__uint_as_float(s[i]), f);
+              for (int i = 0; i < 16; ++i) stage[i * 36 + lane] = __uint_as_float(s[i]);
               __syncwarp();
               float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
@@ -571,9 +577,10 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
             named_bar_sync(1 + x, 128);
             if (gt < N) {
               const float nm = negm[gt], top = key_float(ms.cmax[x][gt]);
+              const float rise = (top + nm) * p.factor;
               float fac = 1.f;
-              if (top > QB_RAISE - nm) {   // an unset column's reference is -1e30: any visible key
-                fac = exp2_fast(-nm - top);
+              if (rise > QB_RAISE) {   // an unset column's: any visible key
+                fac = exp2_fast(-rise);
                 negm[gt] = -top;
               }
               facs[gt] = fac;
@@ -648,17 +655,15 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       float* part = p.part + ((size_t)blockIdx.x * 2 + border) * C::SLOT;
       if (x == 0 && gt < N) {
         // a side without a tile (one-tile run) or a column without a key has sum 0 and counts nothing
-        const float ma = ms.negm[0][gt] == QB_UNSET ? -INFINITY : -ms.negm[0][gt];
-        const float mb = ms.negm[1][gt] == QB_UNSET ? -INFINITY : -ms.negm[1][gt];
-        const float m = fmaxf(ma, mb);
-        const float wa = ma == -INFINITY ? 0.f : exp2_fast(ma - m), wb = mb == -INFINITY ? 0.f : exp2_fast(mb - m);
+        const float ma = -ms.negm[0][gt], mb = -ms.negm[1][gt], m = fmaxf(ma, mb);
+        const float wa = ma == -kUnset ? 0.f : exp2_fast((ma - m) * p.factor), wb = mb == -kUnset ? 0.f : exp2_fast((mb - m) * p.factor);
         const float sum = wa * ((ms.lsum[0][gt] + ms.lsum[1][gt]) + (ms.lsum[2][gt] + ms.lsum[3][gt])) +
                           wb * ((ms.lsum[4][gt] + ms.lsum[5][gt]) + (ms.lsum[6][gt] + ms.lsum[7][gt]));
         const float fin = whole ? (sum == 0.f ? 0.f : 16.f / sum) : 1.f;
         ms.fac[0][gt] = wa * fin;
         ms.fac[1][gt] = wb * fin;
         if (!whole) {
-          part[N * 128 + gt] = m;
+          part[N * 128 + gt] = partial_max(-m, p.factor);
           part[N * 129 + gt] = sum;
         }
       }
@@ -944,7 +949,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               const float down = __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
               for (int k = 0; k < 8; ++k) x[k] *= down;
-              if (piece == 0) qf[i] = base_f * __uint_as_float((uint32_t)e << 23);
+              if (piece == 0) qf[i] = fminf(base_f * __uint_as_float((uint32_t)e << 23), 3e38f);
               uniform = false;
             }
           }

@@ -159,6 +159,18 @@ __device__ __forceinline__ uint32_t dequant(uint32_t w, uint32_t s4, uint32_t sh
   asm("{\n .reg .b32 m, o;\n mov.b32 m, 0x00F000F0;\n mov.b32 o, 0x3C003C00;\n lop3.b32 %0, %1, m, o, 0xEA;\n}\n" : "=r"(h) : "r"(t));
   return hfma2_u(h, s4, shift);
 }
+// Scores are measured as (s - reference) * f, s as the products leave it and f
+// its factor to base 2: exactly 0 for the key that set the reference, however
+// large the score (s * f less a rounded reference is off by the rounding, which
+// from 2^27 on hides every key).  A column that has seen no key has -kUnset for
+// its reference; no s comes near (|s| < 2^36, or scores beyond fp32), and with f
+// in this range, which no s tells from its ends, the difference raises it.
+constexpr float kUnset = 3e38f;
+__host__ __device__ __forceinline__ float score_factor(float f) { return fminf(fmaxf(f, 0x1p-100f), 3e38f); }
+// the reference of a partial result in base-2 units, finite
+__device__ __forceinline__ float partial_max(float negm, float f) {
+  return negm == kUnset ? -INFINITY : fminf(fmaxf(-negm * f, -3e38f), 3e38f);
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -384,3 +384,26 @@ def test_attention_writes_between_query_rows_but_not_over_them(pkg):
         pkg.q4_attention(c.q, *args, max_rows=2, out=c.q)
     with pytest.raises(ValueError, match="overlaps"):
         pkg.q4_attention(q, *args, max_rows=2, out=wide.flatten()[256:1280].view(2, 4, 128))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("dtype,size,key", [(torch.bfloat16, -1e37, 1.0), (torch.bfloat16, -1e31, 1.0), (torch.bfloat16, 1e31, 1.0),
+                                            (torch.float16, 6e4, 6e4), (torch.float16, -6e4, 6e4), (torch.float16, 300.0, 3e3)])
+def test_scores_far_beyond_the_mantissa(pkg, dtype, size, key, rows):
+    """Every score of a row is huge: equal keys weigh the same, and of two keys the larger score wins."""
+    c = Case(pkg, [200, 200], [rows, rows], 2, 1, 64, dtype)
+    k = torch.full((200, 1, 128), key)
+    v = [torch.randn(200, 1, 128, generator=torch.Generator().manual_seed(s)).to(dtype) for s in (1, 2)]
+    pkg.q4_append(k.to(dtype).cuda(), v[0].cuda(), c.pg.slots[0].cuda(), c.pool)
+    k[150] *= 0.5 if size < 0 else 1.0
+    k[:150] *= 1.0 if size < 0 else 0.5
+    k[151:] *= 1.0 if size < 0 else 0.5
+    pkg.q4_append(k.to(dtype).cuda(), v[1].cuda(), c.pg.slots[1].cuda(), c.pool)
+    c.q.fill_(size)
+    status = torch.zeros(1, dtype=i32).cuda()
+    out = pkg.q4_attention(c.q, c.pool, c.pg.dev("table"), c.pg.dev("lens"), max_rows=rows, status=status, scale=0.01).double().cpu()
+    v = [U.q4_values(x)[:, 0] for x in v]
+    for got, want in ((out[:rows], v[0].mean(0)), (out[rows:], v[1][150])):
+        # the output's rounding, P exact (1 or 0), 200 fp32 additions of values below 5
+        assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 5 * 200 * 2.0 ** -24).all())
+    assert status.tolist() == [0]
