@@ -382,6 +382,19 @@ int dflash_paged_reserve(const int32_t* lens, const int32_t* new_rows, const int
                          int32_t* table, int64_t table_ld, int max_pages, const int32_t* free_pages, int num_pages,
                          const int32_t* head, int32_t* starts, int32_t* slots, int num_slots, int32_t* lens_out,
                          int32_t* pages_out, int32_t* head_out, int32_t* status, void* stream);
+/* The same, and refused [n] (or NULL) follows who was turned away: 1 for a
+ * request that brings rows and gets none, 0 for one that gets them; others keep
+ * their entry. */
+int dflash_paged_reserve_tracked(const int32_t* lens, const int32_t* new_rows, const int32_t* pages, int n,
+                                 int page_size, int32_t* table, int64_t table_ld, int max_pages,
+                                 const int32_t* free_pages, int num_pages, const int32_t* head, int32_t* starts,
+                                 int32_t* slots, int num_slots, int32_t* lens_out, int32_t* pages_out,
+                                 int32_t* head_out, int32_t* refused, int32_t* status, void* stream);
+/* lens_out[i] = max(lens[i] - counts[i], 0), with `count` for all where counts
+ * is NULL; negative counts and requests with refused[i] != 0 (refused may be
+ * NULL) lose nothing.  lens_out may be lens. */
+int dflash_paged_trim(const int32_t* lens, const int32_t* counts, int count, const int32_t* refused, int n,
+                      int32_t* lens_out, void* stream);
 /* Request i keeps ceil(keep[i] / page_size) of its pages (0: it is finished);
  * the others are put back, in order, at free_pages[*head_out ... *head). */
 int dflash_paged_release(const int32_t* keep, const int32_t* pages, int n, int page_size, const int32_t* table,

@@ -134,6 +134,10 @@ EXPORTS = {
                                        c_void_p, c_void_p]),
     "dflash_paged_release": (c_int32, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int,
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dflash_paged_reserve_tracked": (c_int32, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int,
+                                               c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                               c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dflash_paged_trim": (c_int32, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]),
     "dflash_q4_page_bytes": (c_size_t, [c_int, c_int]),
     "dflash_q4_append": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int,
                                    c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]),
@@ -179,8 +183,8 @@ def load_paged():
                 mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("dflash_paged", loader))
                 loader.exec_module(mod)
                 mod.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in
-                           ("dflash_paged_reserve", "dflash_paged_release", "dflash_q4_append", "dflash_q4_read",
-                            "dflash_q4_attention", "dflash_last_error")))
+                           ("dflash_paged_reserve_tracked", "dflash_paged_release", "dflash_paged_trim",
+                            "dflash_q4_append", "dflash_q4_read", "dflash_q4_attention", "dflash_last_error")))
                 _paged = mod
     return _paged
 

@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
         p.starts[i + 1] = (int)min(row_end, (long long)INT32_MAX);
         p.lens_out[i] = served ? li + ni : li;
         p.pages_out[i] = served ? max(hi, (int)want) : hi;
+        if (p.refused && ni > 0) p.refused[i] = !served;
       }
     }
     carry_r += tot_r;
@@ -187,6 +188,16 @@ __global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(const Release
   }
 }
 
+__global__ void __launch_bounds__(256) paged_trim_kernel(const int32_t* lens, const int32_t* counts, int count,
+                                                         const int32_t* refused, int n, int32_t* lens_out) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
+  if (i >= n) return;
+  const int drop = refused && refused[i] ? 0 : max(counts ? counts[i] : count, 0);
+  lens_out[i] = max(max(lens[i], 0) - drop, 0);
+}
+
 cudaError_t paged_reserve_launch(const ReserveParams& p, int num_sms, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
   const int want = (p.num_slots + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
@@ -199,6 +210,11 @@ cudaError_t paged_release_launch(const ReleaseParams& p, int num_sms, cudaStream
   const long long want = ((long long)p.n * p.max_pages + 16 * PG_THREADS - 1) / (16 * PG_THREADS);
   const int grid = want < 1 ? 1 : want > num_sms ? num_sms : (int)want;
   return launch_pdl(paged_release_kernel, dim3(grid), dim3(PG_THREADS), (size_t)p.n * 8, st, p);
+}
+
+cudaError_t paged_trim_launch(const int32_t* lens, const int32_t* counts, int count, const int32_t* refused, int n,
+                              int32_t* lens_out, cudaStream_t st) {
+  return launch_pdl(paged_trim_kernel, dim3((n + 255) / 256), dim3(256), 0, st, lens, counts, count, refused, n, lens_out);
 }
 
 }  // namespace dfl

@@ -72,6 +72,14 @@ int dflash_paged_reserve(const int32_t* lens, const int32_t* new_rows, const int
                          int32_t* table, int64_t table_ld, int max_pages, const int32_t* free_pages, int num_pages,
                          const int32_t* head, int32_t* starts, int32_t* slots, int num_slots, int32_t* lens_out,
                          int32_t* pages_out, int32_t* head_out, int32_t* status, void* stream) {
+  return dflash_paged_reserve_tracked(lens, new_rows, pages, n, page_size, table, table_ld, max_pages, free_pages, num_pages,
+                                      head, starts, slots, num_slots, lens_out, pages_out, head_out, nullptr, status, stream);
+}
+
+int dflash_paged_reserve_tracked(const int32_t* lens, const int32_t* new_rows, const int32_t* pages, int n, int page_size,
+                                 int32_t* table, int64_t table_ld, int max_pages, const int32_t* free_pages, int num_pages,
+                                 const int32_t* head, int32_t* starts, int32_t* slots, int num_slots, int32_t* lens_out,
+                                 int32_t* pages_out, int32_t* head_out, int32_t* refused, int32_t* status, void* stream) {
   if (!lens || !new_rows || !pages || !table || (num_pages > 0 && !free_pages) || !head || !starts || !lens_out || !pages_out ||
       !head_out || (num_slots > 0 && !slots))
     return fail(DFLASH_ERR_INVALID, "NULL pointer");
@@ -86,7 +94,7 @@ int dflash_paged_reserve(const int32_t* lens, const int32_t* new_rows, const int
   p.table = table; p.n = n; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
   p.num_slots = num_slots; p.table_ld = table_ld;
   p.starts = starts; p.slots = slots; p.lens_out = lens_out; p.pages_out = pages_out; p.head_out = head_out;
-  p.status = status;
+  p.refused = refused; p.status = status;
   CK(paged_reserve_launch(p, sms, static_cast<cudaStream_t>(stream)));
   return DFLASH_OK;
 }
@@ -106,6 +114,15 @@ int dflash_paged_release(const int32_t* keep, const int32_t* pages, int n, int p
   p.n = n; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages; p.table_ld = table_ld;
   p.pages_out = pages_out; p.head_out = head_out; p.status = status;
   CK(paged_release_launch(p, sms, static_cast<cudaStream_t>(stream)));
+  return DFLASH_OK;
+}
+
+int dflash_paged_trim(const int32_t* lens, const int32_t* counts, int count, const int32_t* refused, int n,
+                      int32_t* lens_out, void* stream) {
+  if (!lens || !lens_out) return fail(DFLASH_ERR_INVALID, "NULL pointer");
+  if (n < 1 || n > DFLASH_PAGED_MAX_SEQS)
+    return fail(DFLASH_ERR_INVALID, "n %d outside [1, %d]", n, DFLASH_PAGED_MAX_SEQS);
+  CK(paged_trim_launch(lens, counts, count, refused, n, lens_out, static_cast<cudaStream_t>(stream)));
   return DFLASH_OK;
 }
 

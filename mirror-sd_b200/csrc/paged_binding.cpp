@@ -7,6 +7,7 @@
 // library that it has loaded.
 #include <Python.h>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -32,8 +33,9 @@ struct PyError {};   // a Python exception is set
 
 // ---- the library's entries
 struct Lib {
-  decltype(&dflash_paged_reserve) reserve;
+  decltype(&dflash_paged_reserve_tracked) reserve;
   decltype(&dflash_paged_release) release;
+  decltype(&dflash_paged_trim) trim;
   decltype(&dflash_q4_append) append;
   decltype(&dflash_q4_read) read;
   decltype(&dflash_q4_attention) attention;
@@ -88,7 +90,8 @@ int32_t* i32(PyObject* o, const char* name, int64_t n, int dev, int64_t* count =
   if (count) *count = t.numel();
   return t.data_ptr<int32_t>();
 }
-int32_t* status_of(PyObject* o, int dev) { return o == Py_None ? nullptr : i32(o, "status", 1, dev); }
+int32_t* i32_or_none(PyObject* o, const char* name, int64_t n, int dev) { return o == Py_None ? nullptr : i32(o, name, n, dev); }
+int32_t* status_of(PyObject* o, int dev) { return i32_or_none(o, "status", 1, dev); }
 
 struct Table {
   int32_t* data;
@@ -200,7 +203,7 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return nullptr;
 }
 
-// (lens, new_rows, pages, table, free_pages, head, page_size, num_slots, status)
+// (lens, new_rows, pages, table, free_pages, head, page_size, num_slots, status, refused)
 PyObject* reserve(PyObject* const* a) {
   const at::Tensor& lens = tensor(a[0], "lens");
   const int dev = cuda_index(lens);
@@ -211,11 +214,12 @@ PyObject* reserve(PyObject* const* a) {
   const Table t = table_of(a[3], n, dev);
   int64_t num_pages;
   int32_t *l = i32(a[0], "lens", n, dev), *r = i32(a[1], "new_rows", n, dev), *p = i32(a[2], "pages", n, dev),
-          *f = i32(a[4], "free_pages", -1, dev, &num_pages), *h = i32(a[5], "head", 1, dev), *s = status_of(a[8], dev);
+          *f = i32(a[4], "free_pages", -1, dev, &num_pages), *h = i32(a[5], "head", 1, dev), *s = status_of(a[8], dev),
+          *refused = i32_or_none(a[9], "refused", n, dev);
   const at::Tensor out = empty({3 * n + 2 + num_slots}, at::kInt, dev);   // [starts | lens | pages | head | slots]
   int32_t* o = out.data_ptr<int32_t>();
   call("dflash_paged_reserve", lib.reserve, dev, l, r, p, (int)n, page_size, t.data, t.ld, t.width, f, (int)num_pages, h, o,
-       o + 3 * n + 2, (int)num_slots, o + n + 1, o + 2 * n + 1, o + 3 * n + 1, s);
+       o + 3 * n + 2, (int)num_slots, o + n + 1, o + 2 * n + 1, o + 3 * n + 1, refused, s);
   return tuple(slice(out, 0, n + 1), slice(out, 3 * n + 2, num_slots), slice(out, n + 1, n), slice(out, 2 * n + 1, n),
                slice(out, 3 * n + 1, 1));
 }
@@ -236,6 +240,22 @@ PyObject* release(PyObject* const* a) {
   call("dflash_paged_release", lib.release, dev, k, p, (int)n, page_size, t.data, t.ld, t.width, f, (int)num_pages, h, o,
        o + n, s);
   return tuple(slice(out, 0, n), slice(out, n, 1));
+}
+
+// (lens, counts: a tensor or a number, refused, out: or None) -> out
+PyObject* trim(PyObject* const* a) {
+  const at::Tensor& lens = tensor(a[0], "lens");
+  const int dev = cuda_index(lens);
+  const int64_t n = lens.numel();
+  if (n > DFLASH_PAGED_MAX_SEQS) refuse("%lld requests, at most %d", (long long)n, DFLASH_PAGED_MAX_SEQS);
+  const int32_t* l = i32(a[0], "lens", n, dev);
+  const int32_t* counts = PyLong_Check(a[1]) ? nullptr : i32(a[1], "counts", n, dev);
+  const int count = counts ? 0 : int32(a[1], "count");
+  const int32_t* refused = i32_or_none(a[2], "refused", n, dev);
+  const at::Tensor out = a[3] == Py_None ? empty({n}, at::kInt, dev) : tensor(a[3], "out");
+  int32_t* o = a[3] == Py_None ? out.data_ptr<int32_t>() : i32(a[3], "out", n, dev);
+  call("dflash_paged_trim", lib.trim, dev, l, counts, count, refused, (int)n, o);
+  return a[3] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[3]);
 }
 
 // (k, v, slots, pool, status)
@@ -289,24 +309,31 @@ PyObject* attention(PyObject* const* a) {
   return a[10] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[10]);
 }
 
+// (device) -> whether its current stream is being captured
+PyObject* capturing(PyObject* const* a) {
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)int32(a[0], "device"));
+  return PyBool_FromLong(c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None);
+}
+
 // addresses of the library's entries, in the order of Lib
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* at[6];
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "bind: 6 addresses expected");
+  void* at[7];
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "bind: 7 addresses expected");
     return nullptr;
   }
-  for (int i = 0; i < 6; ++i)
+  for (int i = 0; i < 7; ++i)
     if (!(at[i] = PyLong_AsVoidPtr(a[i]))) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: NULL");
       return nullptr;
     }
   lib.reserve = reinterpret_cast<decltype(lib.reserve)>(at[0]);
   lib.release = reinterpret_cast<decltype(lib.release)>(at[1]);
-  lib.append = reinterpret_cast<decltype(lib.append)>(at[2]);
-  lib.read = reinterpret_cast<decltype(lib.read)>(at[3]);
-  lib.attention = reinterpret_cast<decltype(lib.attention)>(at[4]);
-  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at[5]);
+  lib.trim = reinterpret_cast<decltype(lib.trim)>(at[2]);
+  lib.append = reinterpret_cast<decltype(lib.append)>(at[3]);
+  lib.read = reinterpret_cast<decltype(lib.read)>(at[4]);
+  lib.attention = reinterpret_cast<decltype(lib.attention)>(at[5]);
+  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at[6]);
   Py_RETURN_NONE;
 }
 
@@ -317,8 +344,10 @@ PyMethodDef method(const char* name) {
 
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
-    method<reserve, 9>("reserve"),
+    method<reserve, 10>("reserve"),
     method<release, 7>("release"),
+    method<trim, 4>("trim"),
+    method<capturing, 1>("capturing"),
     method<append, 5>("append"),
     method<read, 3>("read"),
     method<attention, 13>("attention"),

@@ -60,7 +60,7 @@ struct ReserveParams {
   int32_t* table;
   int n, page_size, max_pages, num_pages, num_slots;
   long long table_ld;
-  int32_t *starts, *slots, *lens_out, *pages_out, *head_out, *status;
+  int32_t *starts, *slots, *lens_out, *pages_out, *head_out, *refused, *status;
 };
 cudaError_t paged_reserve_launch(const ReserveParams& p, int num_sms, cudaStream_t st);
 
@@ -72,6 +72,8 @@ struct ReleaseParams {
   int32_t *pages_out, *head_out, *status;
 };
 cudaError_t paged_release_launch(const ReleaseParams& p, int num_sms, cudaStream_t st);
+cudaError_t paged_trim_launch(const int32_t* lens, const int32_t* counts, int count, const int32_t* refused, int n,
+                              int32_t* lens_out, cudaStream_t st);
 
 struct Q4AppendParams {
   const void *k, *v;                 // [T, NKV, 128], f16 or bf16

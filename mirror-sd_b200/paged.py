@@ -55,7 +55,7 @@ def _raw_stream(index: int) -> int:
 
 
 def paged_reserve(lens, new_rows, pages, table, free_pages, head, page_size: int, num_slots: int,
-                  status=None) -> PagedStep:
+                  status=None, refused=None) -> PagedStep:
     """Pages and cache slots for the rows that each request brings.
 
     lens, new_rows, pages [n], table [n, max_pages], free_pages [num_pages] and
@@ -64,9 +64,10 @@ def paged_reserve(lens, new_rows, pages, table, free_pages, head, page_size: int
     ``table``; the other inputs are only read.  ``num_slots`` bounds the new
     rows of all requests (known on the host); surplus slots are -1.  A request
     that cannot be served keeps its length and sets a bit of ``status``
-    (STATUS_BITS)."""
+    (STATUS_BITS) and its entry of ``refused`` [n], which a request that is
+    served clears."""
     return PagedStep._make(N.load_paged().reserve(lens, new_rows, pages, table, free_pages, head, page_size, num_slots,
-                                                  status))
+                                                  status, refused))
 
 
 def paged_release(keep, pages, table, free_pages, head, page_size: int, status=None):
@@ -149,7 +150,7 @@ class PagedKVCacheQ4:
     ``lens``, ``pages`` and ``head`` are new tensors after every step, which a
     CUDA graph could not follow: it would start each replay from the lengths
     that it was captured with.  With ``capturable`` they are updated in place
-    (four small copies a ``reserve``, two a ``release``), so that every replay
+    (three small copies a ``reserve``, two a ``release``), so that every replay
     of captured steps goes on where the last one ended; only then may
     ``reserve``, ``attend``, ``trim`` and ``release`` be captured, with row
     counts on the device (or one number).  Replays and calls in between are the
@@ -169,16 +170,13 @@ class PagedKVCacheQ4:
         self.free_pages = torch.arange(num_pages, **i32)
         self.head = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
-        self._refused = torch.zeros(max_seqs, dtype=torch.bool, device=self.device)
+        self._refused = torch.zeros(max_seqs, **i32)      # turned away when it last brought rows
         self.capturable = capturable
         self._workspace, self._sizes = {}, {}
         self._stream = _raw_stream(self.device.index)
 
     def _capturing(self) -> bool:
-        if torch.cuda.current_device() == self.device.index:
-            return torch.cuda.is_current_stream_capturing()
-        with torch.cuda.device(self.device):
-            return torch.cuda.is_current_stream_capturing()
+        return N.load_paged().capturing(self.device.index)
 
     def _keep(self, **state):
         for name, t in state.items():
@@ -203,7 +201,7 @@ class PagedKVCacheQ4:
         raw = _raw_stream(self.device.index)
         if raw != self._stream:
             self._stream = raw
-            for t in (self.lens, self.pages, self.head, self._refused):
+            for t in (self.lens, self.pages, self.head):
                 t.record_stream(torch.cuda.current_stream(self.device))
         return raw
 
@@ -220,10 +218,8 @@ class PagedKVCacheQ4:
         elif num_slots is None:
             raise ValueError("num_slots is needed with new_rows on the device")
         step = paged_reserve(self.lens, new_rows, self.pages, self.table, self.free_pages, self.head, self.page_size,
-                             num_slots, self.status)
-        asked = step.starts[1:] > step.starts[:-1]      # turned away: brought rows and has not grown since
-        self._keep(_refused=(step.lens == self.lens) & (asked | self._refused), lens=step.lens, pages=step.pages,
-                   head=step.head)
+                             num_slots, self.status, self._refused)
+        self._keep(lens=step.lens, pages=step.pages, head=step.head)
         return step
 
     def append(self, layer: int, k, v, step: PagedStep) -> None:
@@ -237,24 +233,20 @@ class PagedKVCacheQ4:
         graph's, zeroed at every replay."""
         stream = self._enter()
         if workspace is None:
-            workspace = self._own_workspace(max_rows, q.shape[1], stream)
+            key = (max_rows, q.shape[1])
+            size = self._sizes.get(key)
+            if size is None:
+                size = self._sizes[key] = _workspace_size(*key, self.nkv, self.device)
+            # A graph may be replayed on any stream, beside eager calls and other graphs, and long after a larger
+            # workspace has taken this one's place: it shares none with them.
+            own = None if self.capturable and self._capturing() else self._workspace
+            workspace = own.get(stream) if own is not None else None      # calls on different streams may overlap
+            if workspace is None or workspace.nbytes < size:
+                workspace = torch.zeros(size, dtype=torch.uint8, device=self.device)
+                if own is not None:
+                    own[stream] = workspace
         return q4_attention(q, self.pools[layer], self.table, self.lens, step.starts, max_rows, causal, sink, window,
                             scale, out, self.status, workspace)
-
-    def _own_workspace(self, max_rows: int, num_heads: int, stream: int):
-        key = (max_rows, num_heads)
-        size = self._sizes.get(key)
-        if size is None:
-            size = self._sizes[key] = _workspace_size(*key, self.nkv, self.device)
-        zeros = lambda: torch.zeros(size, dtype=torch.uint8, device=self.device)
-        # A graph may be replayed on any stream, beside eager calls and other graphs, and long after a larger
-        # workspace has taken this one's place: it shares none with them.
-        if self._capturing():
-            return zeros()
-        ws = self._workspace.get(stream)            # calls on different streams may overlap
-        if ws is None or ws.nbytes < size:
-            ws = self._workspace[stream] = zeros()
-        return ws
 
     def trim(self, counts: Union[int, torch.Tensor, Sequence[int]]) -> None:
         """Drop the last counts[i] rows of request i (one number: of every
@@ -271,9 +263,13 @@ class PagedKVCacheQ4:
                 raise ValueError(f"counts must be {self.max_seqs} integers, got {counts.dtype} {tuple(counts.shape)}")
             if counts.device != self.device:
                 counts = self._upload(counts, "counts")
-        # a negative count on the device, where nobody can raise, trims nothing (lens less a number >= 0 cannot wrap)
-        counts = torch.where(self._refused, 0, counts).clamp(min=0)
-        self._keep(lens=torch.clamp(self.lens - counts, min=0).to(torch.int32))
+            if counts.dtype is not torch.int32:
+                counts = counts.to(torch.int64).clamp(min=-1, max=2 ** 31 - 1).to(torch.int32)
+            counts = counts.contiguous()
+        else:
+            counts = min(counts, 2 ** 31 - 1)
+        # (a negative count on the device, where nobody can raise, trims nothing)
+        self.lens = N.load_paged().trim(self.lens, counts, self._refused, self.lens if self.capturable else None)
 
     def release(self, seqs: Sequence[int] = ()) -> None:
         """Give spare pages back; requests ``seqs`` are finished and emptied."""

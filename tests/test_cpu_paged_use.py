@@ -160,3 +160,13 @@ def test_attention_refuses_an_output_over_its_queries(pkg):
         for rows, row, byte in ((4, 256, size(4)), (4, 256, -size(4)), (3, 1024, 4096 + 512), (3, 0, 512), (2, 4096, 512),
                                 (2, 4096, 8192 - 1024), (1, 4096, 8192), (3, -256, 512), (3, -256, -1024 - size(3))):
             assert call(byte, rows, row) != pkg._native.DFLASH_ERR_INVALID, (rows, row, byte, pkg._native.last_error())
+
+
+def test_trim_and_tracked_reserve_refuse_bad_arguments(pkg):
+    lib = pkg._native.load()
+    _refused(pkg, lib.dflash_paged_trim(None, P, 0, P, 4, P, None), "NULL")
+    _refused(pkg, lib.dflash_paged_trim(P, None, 3, None, 4, None, None), "NULL")
+    _refused(pkg, lib.dflash_paged_trim(P, None, 3, None, 0, P, None), "n 0")
+    _refused(pkg, lib.dflash_paged_trim(P, None, 3, None, 2049, P, None), "n 2049")
+    _refused(pkg, lib.dflash_paged_reserve_tracked(P, P, P, 4, 48, P, 8, 8, P, 10, P, P, P, 4, ctypes.c_void_p(8192),
+                                                   ctypes.c_void_p(8192), ctypes.c_void_p(8192), P, None, None), "page_size")
