@@ -174,6 +174,7 @@ class PagedKVCacheQ4:
         self.capturable = capturable
         self._workspace, self._sizes = {}, {}
         self._stream = _raw_stream(self.device.index)
+        self._streams = {self._stream}
 
     def _capturing(self) -> bool:
         return N.load_paged().capturing(self.device.index)
@@ -192,18 +193,25 @@ class PagedKVCacheQ4:
         values = values if torch.is_tensor(values) else torch.tensor(values, dtype=torch.int32)
         return values.to(self.device, non_blocking=True)
 
-    def _enter(self) -> int:
-        """The state's tensors are new ones after each step: on another
-        stream than the last call's, tell the allocator that it reads the old ones.
-        Returns the current stream."""
-        if not self.capturable and self._capturing():
-            raise RuntimeError("a PagedKVCacheQ4 in a CUDA graph must be made with capturable=True")
+    def _on_stream(self) -> int:
+        """The current stream.  Where it is another one than the last call's, the
+        allocator learns that it uses the state: ``lens``, ``pages`` and ``head``,
+        which are new tensors after each step, and, once for a stream, all others."""
         raw = _raw_stream(self.device.index)
         if raw != self._stream:
             self._stream = raw
-            for t in (self.lens, self.pages, self.head):
+            state = [self.lens, self.pages, self.head]
+            if raw not in self._streams:
+                self._streams.add(raw)
+                state += [*self.pools, self.table, self.free_pages, self.status, self._refused]
+            for t in state:
                 t.record_stream(torch.cuda.current_stream(self.device))
         return raw
+
+    def _enter(self) -> int:
+        if not self.capturable and self._capturing():
+            raise RuntimeError("a PagedKVCacheQ4 in a CUDA graph must be made with capturable=True")
+        return self._on_stream()
 
     def reserve(self, new_rows: Union[torch.Tensor, Sequence[int]], num_slots: Optional[int] = None) -> PagedStep:
         """Make room for new_rows[i] rows of request i (0 where it sits out).
@@ -223,6 +231,7 @@ class PagedKVCacheQ4:
         return step
 
     def append(self, layer: int, k, v, step: PagedStep) -> None:
+        self._on_stream()
         q4_append(k, v, step.slots, self.pools[layer], self.status)
 
     def attend(self, layer: int, q, step: PagedStep, max_rows: int, causal: bool = True, sink: int = 0,
@@ -290,6 +299,7 @@ class PagedKVCacheQ4:
         (k, v) [length, NKV, 128]."""
         if not 0 <= seq < self.max_seqs or not 0 <= length <= self.table.shape[1] * self.page_size:
             raise ValueError(f"no rows 0..{length} of request {seq}")
+        self._on_stream()
         pos = torch.arange(length, device=self.device)
         slots = self.table[seq][pos // self.page_size] * self.page_size + (pos % self.page_size).to(torch.int32)
         return q4_read(self.pools[layer], slots.to(torch.int32), dtype)

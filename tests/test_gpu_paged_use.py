@@ -407,3 +407,26 @@ def test_scores_far_beyond_the_mantissa(pkg, dtype, size, key, rows):
         # the output's rounding, P exact (1 or 0), 200 fp32 additions of values below 5
         assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 5 * 200 * 2.0 ** -24).all())
     assert status.tolist() == [0]
+
+
+def test_the_caches_memory_stays_until_every_stream_is_done_with_it(pkg):
+    """A cache made on one stream, appended to on another and dropped while that one is busy."""
+    cache = pkg.PagedKVCacheQ4(1, 200, 2, 3, 400, 16)
+    x = _rows(1, 40)
+    step = cache.reserve([40, 0, 0])
+    pool = cache.pools[0]
+    size, at = pool.numel(), pool.data_ptr()
+    del pool
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)                  # about 0.1 s
+        cache.append(0, x, x, step)
+        busy = torch.cuda.Event()
+        busy.record()
+    del cache, step
+    taken = torch.empty(size, dtype=torch.uint8, device="cuda")
+    still = not busy.query()
+    assert not still or taken.data_ptr() != at
+    assert still, "the side stream was done too soon to tell"
+    side.synchronize()
