@@ -25,9 +25,9 @@ enum DevError : int {
   kDevBadShape = 2,
 };
 
-// 2^22 polls of try_wait (each poll suspends for a while when the phase is not
-// complete) is far longer than any legal wait in these kernels (a CTA waits at
-// most for its own main loop, well under a second) and still ends in seconds.
+// 2^22 polls of try_wait (a poll suspends for 4 us when the phase does not
+// complete, measured: 17 s) is far longer than any legal wait in these kernels (a
+// CTA waits at most for its own main loop, well under a second) and still ends.
 constexpr uint32_t kSpinLimit = 1u << 22;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

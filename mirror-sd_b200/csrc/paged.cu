@@ -2,14 +2,14 @@
 // requests' lengths (no host round trip between acceptance, which sets the
 // lengths on the device, and the next step's cache writes).
 //
-// Both operators are prefix sums over at most 2048 requests followed by an
+// Reserve and release are prefix sums over at most 2048 requests followed by an
 // even spread of small copies.  They move a few bytes per request and row, so
 // what bounds them is latency: one launch, in which every CTA repeats the
 // prefix sums for itself (the requests' counts are a few KB out of L2) instead
 // of waiting for another CTA, and then writes its own share.  Calls one after
 // another take 5.5 us (reserve, 1 or 256 requests), 4.2 us (release, 256) and
-// 6.7 us (release, 1,000 requests with 250 finished, 0.6 MB of table read); all
-// but the last are bound by the host's 4 to 6 us a call.
+// 5.7 to 6.7 us (release, 1,000 requests with 250 finished, 0.6 MB of table read);
+// all but the last are bound by the host's 4 to 7 us a call.
 #include "q4.cuh"
 
 namespace dfl {

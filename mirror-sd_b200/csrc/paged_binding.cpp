@@ -1,8 +1,9 @@
 // Python binding of the paged-cache operators (paged.py): argument checks,
 // output tensors and the C call in one step.  Their kernels run for 5 to 10 us
 // in a decode step; the same host work in Python with ctypes took 13 to 24 us a
-// call, here it takes 5 to 11 (reserve 17.3 -> 7.1, release 12.5 -> 5.1, append
-// and read together 23.7 -> 11.1, attention 15 -> 5.5).  Nothing here touches
+// call, here it takes 3 to 7 (reserve 17.3 -> 6.6, release 12.5 -> 4.2, append
+// and read together 23.7 -> 7.6, attention 15 -> 4.3, 6.4 for blocks of query
+// rows, which are two launches).  Nothing here touches
 // the device but the C ABI, whose entries paged.py hands over (bind) from the
 // library that it has loaded.
 #include <Python.h>

@@ -133,8 +133,8 @@ cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t s
 // Query rows of a kv head (rows of a request times G) up to which the first
 // kernel runs; it takes them 16 at a time and decodes the cache for each group.
 // us, first kernel / second, on 1 request of 2,048 rows, 16 of 16,384, 256 of
-// 1,024 (8 kv heads): 16 query rows 14 / 14, 118 / 118, 125 / 155; 20 query rows
-// 15 / 14, 214 / 119, 224 / 158; 64 query rows 16 / 18, 412 / 151, 419 / 212.
+// 1,024 (8 kv heads): 16 query rows 14 / 15, 116 / 114, 123 / 149; 20 query rows
+// 15 / 15, 210 / 114, 220 / 150; 64 query rows 16 / 20, 404 / 134, 412 / 206.
 constexpr int kQ4FewRows = 16;
 
 }  // namespace dfl

@@ -30,16 +30,17 @@
 // type), sums and statistics stay fp32.
 //
 // A column's reference (what its scores are measured against) only moves when a
-// score passes it by 2^8, then O and the sum are rescaled: P below 256 loses
-// nothing in f16.
+// score passes it by 2^8, then O and the sum are rescaled: P below 256 stays
+// in f16's range, and a weight below 2^-14 of the reference's loses 2^-25 of that
+// at most.
 //
 // 256 requests of up to 8,192 rows, 32 heads over 8 kv heads, are 1.34 GB, 205 us
-// of HBM; they take 300 to 322 us (4.2 to 4.5 TB/s).  What bounds it is instruction issue and
+// of HBM; they take 306 to 326 us (4.1 to 4.4 TB/s).  What bounds it is instruction issue and
 // latency: 1,300 instructions a tile and warp, 3 warps a scheduler (shared memory
 // holds two tiles for each of 12), 60 % of the issue slots taken.  Tiles of 32
-// rows, whose upkeep is paid twice as often, take 314 us for 256 requests of
+// rows, whose upkeep is paid twice as often, took 314 us for 256 requests of
 // 4,096 against 269, 16 warps of such tiles 285, 10 warps 326.  One token on
-// 2,049 rows takes 11.6 us, a chain of latencies: lengths, page numbers, tiles,
+// 2,049 rows takes 11.4 us, a chain of latencies: lengths, page numbers, tiles,
 // one tile's work, and two merges.
 #include "q4_attn.cuh"
 
@@ -544,8 +545,8 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
   zero_rows(p, threadIdx.x, C::THREADS);
 }
 
-// 8 or 16 query columns.  Up to 8 rows, us with 8 columns / 16: 1 request of
-// 32,768 rows 22 / 27, 16 of 16,384 84 / 116, 256 of 1,024 85 / 123.
+// 8 or 16 query columns.  8 query rows, us with 8 columns / 16: 1 request of
+// 32,768 rows 22 / 26, 16 of 16,384 81 / 114, 256 of 1,024 83 / 121.
 int q4_attn_columns(int max_rows, int nq, int nkv) { return (long long)max_rows * (nq / nkv) <= 8 ? 8 : 16; }
 
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms) {

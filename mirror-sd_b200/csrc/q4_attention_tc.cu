@@ -60,7 +60,7 @@ template <int N_>
 struct QbCfg {
   static constexpr int N = N_, CH = N / 16;
   // Query buffers and packed stages.  With 80 columns shared memory holds two and
-  // two or one and three (8 requests of 16,384 rows, 160 query rows: 178 and 174 us).
+  // two or one and three (8 requests of 16,384 rows, 160 query rows: 167 and 166 us).
   static constexpr int QB = N <= 64 ? 2 : 1;
   static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S)
   static constexpr int NS = N <= 64 ? 4 : 3;
@@ -340,8 +340,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   // next pays the start and the end of an item (6 to 8 us together) twice.  An
   // item takes a CTA for every `quota` of its tiles, the least number with which
   // the grid holds them all, if that is at most QB_SLACK tiles more than equal
-  // runs would have.  (8 items of 64 tiles 29.2 us in equal runs, 21.0 in whole
-  // CTAs; 16 of 257 tiles, 160 query rows, 64.3 and 55.7.)
+  // runs would have.  (8 items of 64 tiles 26.8 us in equal runs, 23.9 in whole
+  // CTAs; 16 of 257 tiles, 160 query rows, 59.9 and 56.6.)
   int quota = 0;
   if (p.n <= QB_THREADS && total > grid) {
     int lo = (total + grid - 1) / grid, hi = lo + QB_SLACK + 1, sum;
@@ -1064,8 +1064,8 @@ __global__ void __launch_bounds__(256) q4_attn_tc_merge_kernel(const Q4AttnParam
 // Columns of the instruction for R = max_rows * G query rows of a kv head: the
 // fewest groups of at most 80 (a thread keeps a sum for every column), evenly
 // filled, in steps of 16 and 32 at least (with fewer a tile costs no less: 32, 48,
-// 64 and 80 columns take 121, 132, 151 and 190 us for 16 requests of 16,384 rows).
-// 160 rows as two groups of 80 take 336 us there, three of 64 three times 151.
+// 64 and 80 columns take 115, 120, 134 and 164 us for 16 requests of 16,384 rows).
+// 160 rows as two groups of 80 take 303 us there, three of 64 three times 134.
 int q4_attn_tc_columns(int max_rows, int nq, int nkv) {
   const long long R = (long long)max_rows * (nq / nkv);
   const long long groups = (R + 79) / 80;
