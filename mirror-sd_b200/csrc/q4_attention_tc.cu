@@ -1074,7 +1074,9 @@ int q4_attn_tc_columns(int max_rows, int nq, int nkv) {
 }
 
 size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms) {
-  return (size_t)num_sms * (2 * q4_attn_tc_columns(max_rows, nq, nkv) * 130 + sizeof(int4) / sizeof(float));
+  // (for every number of rows up to max_rows: past 80 columns they start again at 48)
+  const int columns = (long long)max_rows * (nq / nkv) >= 80 ? 80 : q4_attn_tc_columns(max_rows, nq, nkv);
+  return (size_t)num_sms * (2 * columns * 130 + sizeof(int4) / sizeof(float));
 }
 
 template <int N>

@@ -170,3 +170,10 @@ def test_trim_and_tracked_reserve_refuse_bad_arguments(pkg):
     _refused(pkg, lib.dflash_paged_trim(P, None, 3, None, 2049, P, None), "n 2049")
     _refused(pkg, lib.dflash_paged_reserve_tracked(P, P, P, 4, 48, P, 8, 8, P, 10, P, P, P, 4, ctypes.c_void_p(8192),
                                                    ctypes.c_void_p(8192), ctypes.c_void_p(8192), P, None, None), "page_size")
+
+
+def test_a_workspace_serves_every_smaller_number_of_rows(pkg):
+    size = pkg._native.load().dflash_q4_attention_workspace_size
+    for nq, nkv in ((1, 1), (4, 1), (5, 1), (32, 8), (40, 8), (16, 1), (64, 2)):
+        sizes = [size(rows, nq, nkv) for rows in range(1, 300)]
+        assert all(sizes) and sizes == sorted(sizes), (nq, nkv)
