@@ -438,6 +438,51 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
                         int window, float scale, uint16_t* out, int32_t* status, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* ---- operators around a target's decode step --------------------------------
+ * No counterpart in the reference, whose targets are external models and whose
+ * loop is greedy (mirror_sd/generate.py:591-789). */
+#define DFLASH_F16 0
+#define DFLASH_BF16 1
+#define DFLASH_F32 2
+
+/* Rotary positions: out = x [rows, heads, dim] with its first rotary_dim
+ * channels turned, pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with
+ * interleaved, by position * turns[i] whole turns (turns [rotary_dim / 2] on the
+ * device: the frequencies over 2 pi), times factor; backwards with inverse.  The
+ * other channels are copied.  Positions: positions [rows], int32 (int64 with
+ * positions64), or, where it is NULL, of packed rows of n requests as in
+ * dflash_paged_reserve: row r of request i is at lens[i] - starts[i + 1] + r
+ * (lens with the new rows); rows of no request are not written.  Strides in
+ * elements between rows and heads; dim and rotary_dim even, dim <= 1024; out is x
+ * itself (same strides) or lies apart from it. */
+int dflash_rope(const void* x, int64_t x_row, int64_t x_head, int type, int rows, int heads, int dim, int rotary_dim,
+                int interleaved, int inverse, const double* turns, float factor, const void* positions, int positions64,
+                const int32_t* starts, const int32_t* lens, int n, void* out, int64_t out_row, int64_t out_head,
+                void* stream);
+
+/* Verification of drafted tokens by sampling.  logits [n, block, vocab] of the
+ * target at the block's positions (entries of a row contiguous; strides in
+ * elements), drafts [n, block - 1], uniforms [n, block] in [0, 1),
+ * temperatures [n] (or NULL: temperature for all); below 1e-5 a request is
+ * greedy, its probability on the first largest logit.  probs [n, block - 1,
+ * vocab]: the distributions that the drafts were sampled from, or NULL where
+ * they were not sampled.  num_drafts [n]: how many of its drafts each request
+ * uses (clamped to [0, block - 1]), or NULL: all.
+ *   accepted [n]: drafts j = 0, 1, ... while uniforms[j] * q(d_j) < p_j(d_j),
+ *     p_j = softmax(logits_j / temperature), q the draft's probability (1 without
+ *     probs).  A draft outside the vocabulary is refused.
+ *   tokens [n]: the one behind them, from max(p - q, 0) at the refused draft's
+ *     place (p without the draft itself where there are no probs; p where nothing
+ *     is left), from p behind the last draft: the first token whose running sum, in
+ *     vocabulary order, passes uniforms[block - 1] times the whole sum.
+ * NaN logits count as -inf (probability 0), others as clamped to +-1e30; a row
+ * with nothing above -inf refuses its draft, and its token is -1.  Rows behind
+ * the first refused draft are not read. */
+int dflash_verify_drafts(const void* logits, int64_t seq_stride, int64_t row_stride, int type, int n, int block, int vocab,
+                         const int32_t* drafts, const float* uniforms, const float* temperatures, float temperature,
+                         const float* probs, int64_t probs_seq_stride, int64_t probs_row_stride, const int32_t* num_drafts,
+                         int32_t* accepted, int32_t* tokens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

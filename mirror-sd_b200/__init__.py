@@ -14,6 +14,8 @@ from .generate import SpecDecodeStats, spec_generate
 from .loader import load_dflash_model, load_dflash_weights, save_q8_checkpoint
 from .paged import (PagedKVCacheQ4, PagedStep, paged_release, paged_reserve, q4_append, q4_attention,
                     q4_attention_workspace, q4_pool, q4_read)
+from .rope import Rope, apply_rope, rope_frequencies
+from .sampling import sample_tokens, verify_drafts
 from .serving import DraftServer
 
 __all__ = ["DFlashCache", "DFlashConfig", "DFlashDraftModel", "DFlashKVCache", "DFlashWeightsF32", "DFlashWeightsQ8",
@@ -23,4 +25,5 @@ __all__ = ["DFlashCache", "DFlashConfig", "DFlashDraftModel", "DFlashKVCache", "
            "synth_weights_f32", "synth_weights_q8", "weights_from_q8_numpy", "SpecDecodeStats", "spec_generate",
            "load_dflash_model", "load_dflash_weights", "save_q8_checkpoint", "DraftServer",
            "PagedKVCacheQ4", "PagedStep", "paged_release", "paged_reserve", "q4_append", "q4_attention",
-           "q4_attention_workspace", "q4_pool", "q4_read"]
+           "q4_attention_workspace", "q4_pool", "q4_read",
+           "Rope", "apply_rope", "rope_frequencies", "sample_tokens", "verify_drafts"]

@@ -146,7 +146,16 @@ EXPORTS = {
     "dflash_q4_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_void_p, c_int64,
                                       c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p,
                                                                                   c_void_p, c_size_t, c_void_p]),
+    "dflash_rope": (c_int32, [c_void_p, c_int64, c_int64] + [c_int] * 7 + [c_void_p, c_float, c_void_p, c_int, c_void_p,
+                                                                           c_void_p, c_int, c_void_p, c_int64, c_int64,
+                                                                           c_void_p]),
+    "dflash_verify_drafts": (c_int32, [c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                       c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
+
+# the entries that the binding calls, in the order of its Lib
+PAGED_ENTRIES = ("dflash_paged_reserve_tracked", "dflash_paged_release", "dflash_paged_trim", "dflash_q4_append",
+                 "dflash_q4_read", "dflash_q4_attention", "dflash_rope", "dflash_verify_drafts", "dflash_last_error")
 
 _lib = None
 _paged = None
@@ -182,9 +191,7 @@ def load_paged():
                 loader = importlib.machinery.ExtensionFileLoader("dflash_paged", PAGED_PATH)
                 mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("dflash_paged", loader))
                 loader.exec_module(mod)
-                mod.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in
-                           ("dflash_paged_reserve_tracked", "dflash_paged_release", "dflash_paged_trim",
-                            "dflash_q4_append", "dflash_q4_read", "dflash_q4_attention", "dflash_last_error")))
+                mod.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in PAGED_ENTRIES))
                 _paged = mod
     return _paged
 

@@ -1,4 +1,5 @@
-// Python binding of the paged-cache operators (paged.py): argument checks,
+// Python binding of the paged-cache operators (paged.py) and of those around a
+// decode step (rope.py, sampling.py): argument checks,
 // output tensors and the C call in one step.  Their kernels run for 5 to 10 us
 // in a decode step; the same host work in Python with ctypes took 13 to 24 us a
 // call, here it takes 3 to 7 (reserve 17.3 -> 6.6, release 12.5 -> 4.2, append
@@ -15,6 +16,7 @@
 #include <torch/torch.h>
 
 #include <cstdarg>
+#include <cstring>
 
 #include "../../include/dflash_b200.h"
 
@@ -40,6 +42,8 @@ struct Lib {
   decltype(&dflash_q4_append) append;
   decltype(&dflash_q4_read) read;
   decltype(&dflash_q4_attention) attention;
+  decltype(&dflash_rope) rope;
+  decltype(&dflash_verify_drafts) verify;
   decltype(&dflash_last_error) last_error;
 } lib;
 
@@ -316,25 +320,123 @@ PyObject* capturing(PyObject* const* a) {
   return PyBool_FromLong(c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None);
 }
 
+// ---- decode operators
+int elem_type(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kHalf: return DFLASH_F16;
+    case at::kBFloat16: return DFLASH_BF16;
+    case at::kFloat: return DFLASH_F32;
+    default: refuse("%s must be f16, bf16 or f32, got %s", name, describe(t).c_str());
+  }
+}
+int device_of(const at::Tensor& t, const char* name) {
+  if (!t.is_cuda()) refuse("%s must be on a CUDA device, got %s", name, describe(t).c_str());
+  return t.get_device();
+}
+const at::Tensor& on_device(PyObject* o, const char* name, at::ScalarType type, at::IntArrayRef size, int dev) {
+  const at::Tensor& t = tensor(o, name);
+  if (t.scalar_type() != type || !t.is_cuda() || t.get_device() != dev || !t.sizes().equals(size))
+    refuse("%s must be %s %s on cuda:%d, got %s", name, c10::toString(type), (std::ostringstream() << size).str().c_str(), dev,
+           describe(t).c_str());
+  return t;
+}
+template <class T>
+T* dense(PyObject* o, const char* name, at::ScalarType type, at::IntArrayRef size, int dev) {
+  const at::Tensor& t = on_device(o, name, type, size, dev);
+  if (!t.is_contiguous()) refuse("%s must be contiguous", name);
+  return static_cast<T*>(t.data_ptr());
+}
+
+// (x, turns, factor, rotary_dim, interleaved, inverse, positions, starts, lens, out) -> out
+PyObject* rope(PyObject* const* a) {
+  const at::Tensor& x = tensor(a[0], "x");
+  const int dev = device_of(x, "x"), type = elem_type(x, "x");
+  if (x.dim() != 3) refuse("x must be [rows, heads, dim], got %s", describe(x).c_str());
+  const int64_t rows = x.size(0), heads = x.size(1), dim = x.size(2), rot = int32(a[3], "rotary_dim");
+  if (rows > INT32_MAX || heads > INT32_MAX || dim > INT32_MAX) refuse("x is too large: %s", describe(x).c_str());
+  const double factor = PyFloat_AsDouble(a[2]);
+  if (factor == -1.0 && PyErr_Occurred()) throw PyError();
+  const double* turns = dense<double>(a[1], "turns", at::kDouble, {rot / 2}, dev);
+  const void* positions = nullptr;
+  bool wide = false;
+  const int32_t *starts = nullptr, *lens = nullptr;
+  int64_t n = 0;
+  if (a[6] != Py_None) {
+    const at::Tensor& t = tensor(a[6], "positions");
+    wide = t.scalar_type() == at::kLong;
+    positions = wide ? dense<void>(a[6], "positions", at::kLong, {rows}, dev) : dense<void>(a[6], "positions", at::kInt, {rows}, dev);
+    if (!positions) positions = turns;   // (no rows)
+  } else {
+    lens = i32(a[8], "lens", -1, dev, &n);
+    if (n > DFLASH_PAGED_MAX_SEQS) refuse("%lld requests, at most %d", (long long)n, DFLASH_PAGED_MAX_SEQS);
+    starts = i32(a[7], "starts", n + 1, dev);
+  }
+  // channels that do not lie side by side are copied first
+  const at::Tensor src = x.stride(2) == 1 ? x : x.clone(at::MemoryFormat::Contiguous);
+  at::Tensor out;
+  if (a[9] == Py_None) {
+    out = empty(x.sizes(), x.scalar_type(), dev);
+  } else {
+    out = on_device(a[9], "out", x.scalar_type(), x.sizes(), dev);
+    if (out.stride(2) != 1) refuse("out's channels must lie side by side");
+  }
+  // (the stride of a single row or head may be anything)
+  auto stride = [](const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+  call("dflash_rope", lib.rope, dev, src.data_ptr(), stride(src, 0), stride(src, 1), type, (int)rows, (int)heads, (int)dim,
+       (int)rot, (int)boolean(a[4]), (int)boolean(a[5]), turns, (float)factor, positions, (int)wide, starts, lens, (int)n,
+       out.data_ptr(), stride(out, 0), stride(out, 1));
+  return a[9] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[9]);
+}
+
+// (logits, drafts, uniforms, temperature: a number or a tensor, probs, counts) -> (accepted, tokens)
+PyObject* verify(PyObject* const* a) {
+  at::Tensor logits = tensor(a[0], "logits");
+  const int dev = device_of(logits, "logits"), type = elem_type(logits, "logits");
+  if (logits.dim() != 3 || logits.size(0) > INT32_MAX || logits.size(1) > INT32_MAX || logits.size(2) > INT32_MAX)
+    refuse("logits must be [requests, block, vocabulary], got %s", describe(logits).c_str());
+  const int64_t n = logits.size(0), block = logits.size(1), vocab = logits.size(2);
+  if (block < 1 || vocab < 1) refuse("logits must have rows and entries, got %s", describe(logits).c_str());
+  if (logits.stride(2) != 1 && vocab > 1) logits = logits.clone(at::MemoryFormat::Contiguous);
+  const int32_t* drafts = dense<int32_t>(a[1], "drafts", at::kInt, {n, block - 1}, dev);
+  const float* u = dense<float>(a[2], "uniforms", at::kFloat, {n, block}, dev);
+  const float* temps = nullptr;
+  double temp = 0.0;
+  if (THPVariable_Check(a[3])) {
+    temps = dense<float>(a[3], "temperature", at::kFloat, {n}, dev);
+  } else {
+    temp = PyFloat_AsDouble(a[3]);
+    if (temp == -1.0 && PyErr_Occurred()) throw PyError();
+  }
+  at::Tensor probs;
+  if (a[4] != Py_None) {
+    probs = on_device(a[4], "draft_probs", at::kFloat, {n, block - 1, vocab}, dev);
+    if (probs.stride(2) != 1 && vocab > 1) probs = probs.clone(at::MemoryFormat::Contiguous);
+  }
+  const int32_t* counts = a[5] == Py_None ? nullptr : dense<int32_t>(a[5], "num_drafts", at::kInt, {n}, dev);
+  const at::Tensor out = empty({2 * n}, at::kInt, dev);
+  int32_t* o = out.data_ptr<int32_t>();
+  const bool sampled = probs.defined() && block > 1;
+  call("dflash_verify_drafts", lib.verify, dev, logits.data_ptr(), logits.stride(0), logits.stride(1), type, (int)n, (int)block,
+       (int)vocab, drafts, u, temps, (float)temp, sampled ? probs.data_ptr<float>() : nullptr, sampled ? probs.stride(0) : 0,
+       sampled ? probs.stride(1) : 0, counts, o, o + n);
+  return tuple(slice(out, 0, n), slice(out, n, n));
+}
+
 // addresses of the library's entries, in the order of Lib
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* at[7];
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "bind: 7 addresses expected");
+  constexpr int COUNT = sizeof(Lib) / sizeof(void*);
+  void* at[COUNT];
+  if (n != COUNT) {
+    PyErr_Format(PyExc_TypeError, "bind: %d addresses expected", COUNT);
     return nullptr;
   }
-  for (int i = 0; i < 7; ++i)
+  for (int i = 0; i < COUNT; ++i)
     if (!(at[i] = PyLong_AsVoidPtr(a[i]))) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: NULL");
       return nullptr;
     }
-  lib.reserve = reinterpret_cast<decltype(lib.reserve)>(at[0]);
-  lib.release = reinterpret_cast<decltype(lib.release)>(at[1]);
-  lib.trim = reinterpret_cast<decltype(lib.trim)>(at[2]);
-  lib.append = reinterpret_cast<decltype(lib.append)>(at[3]);
-  lib.read = reinterpret_cast<decltype(lib.read)>(at[4]);
-  lib.attention = reinterpret_cast<decltype(lib.attention)>(at[5]);
-  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at[6]);
+  static_assert(std::is_trivially_copyable<Lib>::value, "Lib holds addresses only");
+  memcpy(&lib, at, sizeof lib);
   Py_RETURN_NONE;
 }
 
@@ -352,6 +454,8 @@ PyMethodDef methods[] = {
     method<append, 5>("append"),
     method<read, 3>("read"),
     method<attention, 13>("attention"),
+    method<rope, 10>("rope"),
+    method<verify, 6>("verify"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dflash_paged", "Paged 4-bit cache operators (see paged.py).", -1, methods,
