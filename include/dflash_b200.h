@@ -368,6 +368,8 @@ int dflash_lm_head_argmax(const uint16_t* hn, const uint16_t* E, int batch, int 
 #define DFLASH_PAGED_NONFINITE 16      /* a NaN or an infinity was appended */
 #define DFLASH_PAGED_TIMEOUT 32        /* a bounded device-side wait expired */
 #define DFLASH_PAGED_ROWS 64           /* more query rows than max_rows, or starts that do not fit q */
+#define DFLASH_PAGED_FORK 128          /* a fork names no request, or one that holds rows already */
+#define DFLASH_PAGED_SURPLUS 256       /* new rows would go into a page of others behind the request's rows */
 
 /* Request i holds lens[i] rows on pages[i] pages, table[i * table_ld + c],
  * c < pages[i], and brings new_rows[i] rows, packed in order.  Its missing
@@ -400,6 +402,46 @@ int dflash_paged_trim(const int32_t* lens, const int32_t* counts, int count, con
 int dflash_paged_release(const int32_t* keep, const int32_t* pages, int n, int page_size, const int32_t* table,
                          int64_t table_ld, int max_pages, int32_t* free_pages, int num_pages, const int32_t* head,
                          int32_t* pages_out, int32_t* head_out, int32_t* status, void* stream);
+
+/* ---- pages that several requests hold
+ * holders [2 * num_pages], zeroed once: entry p counts the requests beyond the
+ * first that hold page p; the second half is the calls' own and zero between
+ * them.  A cache whose pages are ever forked reserves and releases with the calls
+ * below.  The *_out arrays must not be the inputs. */
+/* Request dst[j] takes over the first rows[j] rows (rows NULL, or more than there
+ * are: all) of request src[j] by holding its pages too; no cached row moves.  dst[j]
+ * must hold no rows and no pages, and be named once; other forks are skipped and
+ * set DFLASH_PAGED_FORK.  src, dst, rows [m], m <= DFLASH_PAGED_MAX_SEQS.  refused
+ * (or NULL): cleared for forked requests. */
+int dflash_paged_fork(const int32_t* src, const int32_t* dst, const int32_t* rows, int m, const int32_t* lens,
+                      const int32_t* pages, int n, int page_size, int32_t* table, int64_t table_ld, int max_pages,
+                      int32_t* holders, int num_pages, int32_t* lens_out, int32_t* pages_out, int32_t* refused,
+                      int32_t* status, void* stream);
+/* dflash_paged_reserve_tracked, and a request whose new rows go into a page that
+ * others hold gets a page of its own first: copies [n][3] = its old page, the
+ * new one, and the rows to copy (-1, -1, 0 for other requests); the copies are the
+ * caller's to make (dflash_q4_copy_pages) before rows are appended.  Of the
+ * requests that write into one page the first ones take copies, as many as the
+ * page has other holders; all of them count as needing a page where pages run out.
+ * Pages that a request holds behind its rows (after a trim) must not be held by
+ * others where new rows would go into them: such a request is turned away
+ * (DFLASH_PAGED_SURPLUS); dflash_paged_release_forked gives them up. */
+int dflash_paged_reserve_forked(const int32_t* lens, const int32_t* new_rows, const int32_t* pages, int n, int page_size,
+                                int32_t* table, int64_t table_ld, int max_pages, const int32_t* free_pages, int num_pages,
+                                const int32_t* head, int32_t* holders, int32_t* starts, int32_t* slots, int num_slots,
+                                int32_t* lens_out, int32_t* pages_out, int32_t* head_out, int32_t* copies, int32_t* refused,
+                                int32_t* status, void* stream);
+/* dflash_paged_release where a page goes back when its last holder gives it up,
+ * in the order of (request, column) in which the last ones do. */
+int dflash_paged_release_forked(const int32_t* keep, const int32_t* pages, int n, int page_size, const int32_t* table,
+                                int64_t table_ld, int max_pages, int32_t* free_pages, int num_pages, const int32_t* head,
+                                int32_t* holders, int32_t* pages_out, int32_t* head_out, int32_t* status, void* stream);
+/* copies [n][3] on the device: page to copy, where to, and how many of its rows (in
+ * whole blocks of 16 rows), in each of the `layers` pools (a host array of device
+ * pointers).  Entries with a page outside the pools, with equal pages or without
+ * rows are skipped; no page may be copied to twice, or be copied to and from. */
+int dflash_q4_copy_pages(uint8_t* const* pools, int layers, int num_pages, int nkv, int page_size, const int32_t* copies, int n,
+                         void* stream);
 
 size_t dflash_q4_page_bytes(int nkv, int page_size);
 /* k, v [rows, nkv, 128], f16 or bf16 (bf16 != 0), strides in elements between

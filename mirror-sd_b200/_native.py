@@ -137,6 +137,13 @@ EXPORTS = {
     "dflash_paged_reserve_tracked": (c_int32, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int,
                                                c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                                c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dflash_paged_fork": (c_int32, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64,
+                                    c_int, c_void_p, c_int] + [c_void_p] * 5),
+    "dflash_paged_reserve_forked": (c_int32, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p,
+                                              c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int] + [c_void_p] * 7),
+    "dflash_paged_release_forked": (c_int32, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int]
+                                    + [c_void_p] * 6),
+    "dflash_q4_copy_pages": (c_int32, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p]),
     "dflash_paged_trim": (c_int32, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]),
     "dflash_q4_page_bytes": (c_size_t, [c_int, c_int]),
     "dflash_q4_append": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int,
@@ -155,7 +162,8 @@ EXPORTS = {
 
 # the entries that the binding calls, in the order of its Lib
 PAGED_ENTRIES = ("dflash_paged_reserve_tracked", "dflash_paged_release", "dflash_paged_trim", "dflash_q4_append",
-                 "dflash_q4_read", "dflash_q4_attention", "dflash_rope", "dflash_verify_drafts", "dflash_last_error")
+                 "dflash_q4_read", "dflash_q4_attention", "dflash_paged_fork", "dflash_paged_reserve_forked",
+                 "dflash_paged_release_forked", "dflash_q4_copy_pages", "dflash_rope", "dflash_verify_drafts", "dflash_last_error")
 
 _lib = None
 _paged = None

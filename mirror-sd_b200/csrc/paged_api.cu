@@ -117,6 +117,93 @@ int dflash_paged_release(const int32_t* keep, const int32_t* pages, int n, int p
   return DFLASH_OK;
 }
 
+int dflash_paged_fork(const int32_t* src, const int32_t* dst, const int32_t* rows, int m, const int32_t* lens,
+                      const int32_t* pages, int n, int page_size, int32_t* table, int64_t table_ld, int max_pages,
+                      int32_t* holders, int num_pages, int32_t* lens_out, int32_t* pages_out, int32_t* refused,
+                      int32_t* status, void* stream) {
+  if ((m > 0 && (!src || !dst)) || !lens || !pages || !table || !holders || !lens_out || !pages_out)
+    return fail(DFLASH_ERR_INVALID, "NULL pointer");
+  if (m < 0 || m > DFLASH_PAGED_MAX_SEQS) return fail(DFLASH_ERR_INVALID, "%d forks outside [0, %d]", m, DFLASH_PAGED_MAX_SEQS);
+  if (lens_out == lens || pages_out == pages) return fail(DFLASH_ERR_INVALID, "lens_out and pages_out must not be the inputs");
+  if (int rc = check_paging(n, page_size, table_ld, max_pages, num_pages)) return rc;
+  if (m == 0) {
+    CK(cudaMemcpyAsync(lens_out, lens, (size_t)n * 4, cudaMemcpyDeviceToDevice, static_cast<cudaStream_t>(stream)));
+    CK(cudaMemcpyAsync(pages_out, pages, (size_t)n * 4, cudaMemcpyDeviceToDevice, static_cast<cudaStream_t>(stream)));
+    return DFLASH_OK;
+  }
+  int sms = 0;
+  if (int rc = num_sms(&sms)) return rc;
+  ForkParams p{};
+  p.src = src; p.dst = dst; p.rows = rows; p.lens = lens; p.pages = pages; p.table = table; p.holders = holders;
+  p.m = m; p.n = n; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages; p.table_ld = table_ld;
+  p.lens_out = lens_out; p.pages_out = pages_out; p.refused = refused; p.status = status;
+  CK(paged_fork_launch(p, sms, static_cast<cudaStream_t>(stream)));
+  return DFLASH_OK;
+}
+
+int dflash_paged_reserve_forked(const int32_t* lens, const int32_t* new_rows, const int32_t* pages, int n, int page_size,
+                                int32_t* table, int64_t table_ld, int max_pages, const int32_t* free_pages, int num_pages,
+                                const int32_t* head, int32_t* holders, int32_t* starts, int32_t* slots, int num_slots,
+                                int32_t* lens_out, int32_t* pages_out, int32_t* head_out, int32_t* copies, int32_t* refused,
+                                int32_t* status, void* stream) {
+  if (!lens || !new_rows || !pages || !table || (num_pages > 0 && !free_pages) || !head || !holders || !starts || !lens_out ||
+      !pages_out || !head_out || !copies || (num_slots > 0 && !slots))
+    return fail(DFLASH_ERR_INVALID, "NULL pointer");
+  if (num_slots < 0) return fail(DFLASH_ERR_INVALID, "num_slots %d", num_slots);
+  if (lens_out == lens || pages_out == pages || head_out == head)
+    return fail(DFLASH_ERR_INVALID, "lens_out, pages_out and head_out must not be the inputs");
+  if (int rc = check_paging(n, page_size, table_ld, max_pages, num_pages)) return rc;
+  ReserveParams p{};
+  p.lens = lens; p.new_rows = new_rows; p.pages = pages; p.free_pages = free_pages; p.head = head;
+  p.table = table; p.n = n; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.num_slots = num_slots; p.table_ld = table_ld;
+  p.starts = starts; p.slots = slots; p.lens_out = lens_out; p.pages_out = pages_out; p.head_out = head_out;
+  p.refused = refused; p.status = status;
+  CK(paged_reserve_forked_launch(p, holders, copies, static_cast<cudaStream_t>(stream)));
+  return DFLASH_OK;
+}
+
+int dflash_paged_release_forked(const int32_t* keep, const int32_t* pages, int n, int page_size, const int32_t* table,
+                                int64_t table_ld, int max_pages, int32_t* free_pages, int num_pages, const int32_t* head,
+                                int32_t* holders, int32_t* pages_out, int32_t* head_out, int32_t* status, void* stream) {
+  if (!keep || !pages || !table || (num_pages > 0 && !free_pages) || !head || !holders || !pages_out || !head_out)
+    return fail(DFLASH_ERR_INVALID, "NULL pointer");
+  if (pages_out == pages || head_out == head)
+    return fail(DFLASH_ERR_INVALID, "pages_out and head_out must not be the inputs");
+  if (int rc = check_paging(n, page_size, table_ld, max_pages, num_pages)) return rc;
+  ReleaseParams p{};
+  p.keep = keep; p.pages = pages; p.table = table; p.head = head; p.free_pages = free_pages;
+  p.n = n; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages; p.table_ld = table_ld;
+  p.pages_out = pages_out; p.head_out = head_out; p.status = status;
+  CK(paged_release_forked_launch(p, holders, static_cast<cudaStream_t>(stream)));
+  return DFLASH_OK;
+}
+
+int dflash_q4_copy_pages(uint8_t* const* pools, int layers, int num_pages, int nkv, int page_size, const int32_t* copies, int n,
+                         void* stream) {
+  if (layers < 0 || n < 0) return fail(DFLASH_ERR_INVALID, "layers %d, n %d", layers, n);
+  if ((layers > 0 && !pools) || (n > 0 && !copies)) return fail(DFLASH_ERR_INVALID, "NULL pointer");
+  for (int i = 0; i < layers; ++i) {
+    if (!pools[i]) return fail(DFLASH_ERR_INVALID, "NULL pointer");
+    if (int rc = check_pool(0, nkv, pools[i], num_pages, page_size)) return rc;
+  }
+  if (layers == 0 || n == 0) return DFLASH_OK;
+  int sms = 0;
+  if (int rc = num_sms(&sms)) return rc;
+  CopyParams p{};
+  p.nkv = nkv; p.page_shift = log2_of(page_size); p.num_pages = num_pages;
+  for (int l = 0; l < layers; l += kCopyPools) {
+    p.layers = layers - l < kCopyPools ? layers - l : kCopyPools;
+    for (int i = 0; i < p.layers; ++i) p.pools[i] = pools[l + i];
+    for (int i = 0; i < n; i += DFLASH_PAGED_MAX_SEQS) {
+      p.copies = copies + 3 * (size_t)i;
+      p.n = n - i < DFLASH_PAGED_MAX_SEQS ? n - i : DFLASH_PAGED_MAX_SEQS;
+      CK(q4_copy_launch(p, sms, static_cast<cudaStream_t>(stream)));
+    }
+  }
+  return DFLASH_OK;
+}
+
 int dflash_paged_trim(const int32_t* lens, const int32_t* counts, int count, const int32_t* refused, int n,
                       int32_t* lens_out, void* stream) {
   if (!lens || !lens_out) return fail(DFLASH_ERR_INVALID, "NULL pointer");

@@ -42,6 +42,10 @@ struct Lib {
   decltype(&dflash_q4_append) append;
   decltype(&dflash_q4_read) read;
   decltype(&dflash_q4_attention) attention;
+  decltype(&dflash_paged_fork) fork;
+  decltype(&dflash_paged_reserve_forked) reserve_forked;
+  decltype(&dflash_paged_release_forked) release_forked;
+  decltype(&dflash_q4_copy_pages) copy_pages;
   decltype(&dflash_rope) rope;
   decltype(&dflash_verify_drafts) verify;
   decltype(&dflash_last_error) last_error;
@@ -320,6 +324,106 @@ PyObject* capturing(PyObject* const* a) {
   return PyBool_FromLong(c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None);
 }
 
+// ---- pages that several requests hold
+int32_t* holders_of(PyObject* o, int64_t num_pages, int dev) {
+  const at::Tensor& t = tensor(o, "holders");
+  if (t.scalar_type() != at::kInt || !t.is_cuda() || t.get_device() != dev || t.dim() != 2 || t.size(0) != 2 ||
+      (num_pages >= 0 && t.size(1) != num_pages) || t.size(1) > INT32_MAX || !t.is_contiguous())
+    refuse("holders must be a contiguous int32 tensor from page_holders(%lld) on cuda:%d, got %s", (long long)num_pages, dev,
+           describe(t).c_str());
+  return t.data_ptr<int32_t>();
+}
+
+// (src, dst, rows, lens, pages, table, holders, page_size, status, refused) -> (lens, pages)
+PyObject* fork(PyObject* const* a) {
+  const at::Tensor& lens = tensor(a[3], "lens");
+  const int dev = cuda_index(lens);
+  const int64_t n = lens.numel();
+  if (n > DFLASH_PAGED_MAX_SEQS) refuse("%lld requests, at most %d", (long long)n, DFLASH_PAGED_MAX_SEQS);
+  int64_t m;
+  const int32_t* src = i32(a[0], "src", -1, dev, &m);
+  const int32_t *dst = i32(a[1], "dst", m, dev), *rows = i32_or_none(a[2], "rows", m, dev), *l = i32(a[3], "lens", n, dev),
+                *p = i32(a[4], "pages", n, dev);
+  const Table t = table_of(a[5], n, dev);
+  int32_t* h = holders_of(a[6], -1, dev);
+  const int page_size = int32(a[7], "page_size");
+  int32_t *s = status_of(a[8], dev), *refused = i32_or_none(a[9], "refused", n, dev);
+  if (m > DFLASH_PAGED_MAX_SEQS) refuse("%lld forks, at most %d", (long long)m, DFLASH_PAGED_MAX_SEQS);
+  const at::Tensor out = empty({2 * n}, at::kInt, dev);
+  int32_t* o = out.data_ptr<int32_t>();
+  call("dflash_paged_fork", lib.fork, dev, src, dst, rows, (int)m, l, p, (int)n, page_size, t.data, t.ld, t.width, h,
+       (int)tensor(a[6], "holders").size(1), o, o + n, refused, s);
+  return tuple(slice(out, 0, n), slice(out, n, n));
+}
+
+// (lens, new_rows, pages, table, free_pages, head, holders, page_size, num_slots, status, refused)
+//   -> (starts, slots, lens, pages, head, copies)
+PyObject* reserve_forked(PyObject* const* a) {
+  const at::Tensor& lens = tensor(a[0], "lens");
+  const int dev = cuda_index(lens);
+  const int64_t n = lens.numel(), num_slots = int32(a[8], "num_slots");
+  const int page_size = int32(a[7], "page_size");
+  if (num_slots < 0) refuse("num_slots %lld", (long long)num_slots);
+  if (n > DFLASH_PAGED_MAX_SEQS) refuse("%lld requests, at most %d", (long long)n, DFLASH_PAGED_MAX_SEQS);
+  const Table t = table_of(a[3], n, dev);
+  int64_t num_pages;
+  int32_t *l = i32(a[0], "lens", n, dev), *r = i32(a[1], "new_rows", n, dev), *p = i32(a[2], "pages", n, dev),
+          *f = i32(a[4], "free_pages", -1, dev, &num_pages), *h = i32(a[5], "head", 1, dev),
+          *shared = holders_of(a[6], num_pages, dev), *s = status_of(a[9], dev), *refused = i32_or_none(a[10], "refused", n, dev);
+  const at::Tensor out = empty({6 * n + 2 + num_slots}, at::kInt, dev);   // [starts | lens | pages | head | copies | slots]
+  int32_t* o = out.data_ptr<int32_t>();
+  call("dflash_paged_reserve_forked", lib.reserve_forked, dev, l, r, p, (int)n, page_size, t.data, t.ld, t.width, f,
+       (int)num_pages, h, shared, o, o + 6 * n + 2, (int)num_slots, o + n + 1, o + 2 * n + 1, o + 3 * n + 1, o + 3 * n + 2, refused,
+       s);
+  PyObject* copies = THPVariable_Wrap(out.narrow(0, 3 * n + 2, 3 * n).view({n, 3}));
+  if (!copies) throw PyError();
+  return tuple(slice(out, 0, n + 1), slice(out, 6 * n + 2, num_slots), slice(out, n + 1, n), slice(out, 2 * n + 1, n),
+               slice(out, 3 * n + 1, 1), copies);
+}
+
+// (keep, pages, table, free_pages, head, holders, page_size, status)
+PyObject* release_forked(PyObject* const* a) {
+  const at::Tensor& keep = tensor(a[0], "keep");
+  const int dev = cuda_index(keep);
+  const int64_t n = keep.numel();
+  const int page_size = int32(a[6], "page_size");
+  if (n > DFLASH_PAGED_MAX_SEQS) refuse("%lld requests, at most %d", (long long)n, DFLASH_PAGED_MAX_SEQS);
+  const Table t = table_of(a[2], n, dev);
+  int64_t num_pages;
+  int32_t *k = i32(a[0], "keep", n, dev), *p = i32(a[1], "pages", n, dev),
+          *f = i32(a[3], "free_pages", -1, dev, &num_pages), *h = i32(a[4], "head", 1, dev),
+          *shared = holders_of(a[5], num_pages, dev), *s = status_of(a[7], dev);
+  const at::Tensor out = empty({n + 1}, at::kInt, dev);
+  int32_t* o = out.data_ptr<int32_t>();
+  call("dflash_paged_release_forked", lib.release_forked, dev, k, p, (int)n, page_size, t.data, t.ld, t.width, f, (int)num_pages,
+       h, shared, o, o + n, s);
+  return tuple(slice(out, 0, n), slice(out, n, 1));
+}
+
+// (pools: a list of tensors, copies)
+PyObject* copy_pages(PyObject* const* a) {
+  if (!PyList_Check(a[0]) && !PyTuple_Check(a[0])) refuse("pools must be a list of tensors from q4_pool()");
+  const Py_ssize_t layers = PySequence_Fast_GET_SIZE(a[0]);
+  if (layers > INT32_MAX) refuse("too many pools");
+  std::vector<uint8_t*> data;
+  Pool first{};
+  for (Py_ssize_t i = 0; i < layers; ++i) {
+    const Pool p = pool_of(PySequence_Fast_GET_ITEM(a[0], i));
+    if (i == 0) first = p;
+    if (p.pages != first.pages || p.nkv != first.nkv || p.page_size != first.page_size || p.dev != first.dev)
+      refuse("pools must have the same shape and device");
+    data.push_back(p.data);
+  }
+  if (layers == 0) Py_RETURN_NONE;
+  const at::Tensor& t = tensor(a[1], "copies");
+  if (t.scalar_type() != at::kInt || !t.is_cuda() || t.get_device() != first.dev || t.dim() != 2 || t.size(1) != 3 ||
+      t.size(0) > INT32_MAX || !t.is_contiguous())
+    refuse("copies must be a contiguous int32 [n, 3] on cuda:%d, got %s", first.dev, describe(t).c_str());
+  call("dflash_q4_copy_pages", lib.copy_pages, first.dev, data.data(), (int)layers, first.pages, first.nkv, first.page_size,
+       t.data_ptr<int32_t>(), (int)t.size(0));
+  Py_RETURN_NONE;
+}
+
 // ---- decode operators
 int elem_type(const at::Tensor& t, const char* name) {
   switch (t.scalar_type()) {
@@ -454,6 +558,10 @@ PyMethodDef methods[] = {
     method<append, 5>("append"),
     method<read, 3>("read"),
     method<attention, 13>("attention"),
+    method<fork, 10>("fork"),
+    method<reserve_forked, 11>("reserve_forked"),
+    method<release_forked, 8>("release_forked"),
+    method<copy_pages, 2>("copy_pages"),
     method<rope, 10>("rope"),
     method<verify, 6>("verify"),
     {nullptr, nullptr, 0, nullptr}};

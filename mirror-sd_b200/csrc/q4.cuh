@@ -49,6 +49,8 @@ enum PagedStatus : int {
   kPagedNonFinite = 16, // an appended row held a NaN or an infinity
   kPagedTimeout = 32,   // a bounded wait of the attention kernel expired
   kPagedRows = 64,      // a request's query rows pass max_rows or lie outside the query array
+  kPagedFork = 128,     // a fork names no request, or one that holds rows already
+  kPagedSurplus = 256,  // new rows would go into a page of others behind the request's rows
 };
 
 // byte offsets of the pieces inside the block's K and V values
@@ -74,6 +76,30 @@ struct ReleaseParams {
 cudaError_t paged_release_launch(const ReleaseParams& p, int num_sms, cudaStream_t st);
 cudaError_t paged_trim_launch(const int32_t* lens, const int32_t* counts, int count, const int32_t* refused, int n,
                               int32_t* lens_out, cudaStream_t st);
+
+// ---- pages that several requests hold (paged_share.cu)
+// holders[p], p < num_pages: the requests beyond the first that hold page p;
+// holders[num_pages + p] is the kernels' own and 0 between calls.
+struct ForkParams {
+  const int32_t *src, *dst, *rows;   // [m]; rows NULL: all
+  const int32_t *lens, *pages;       // [n]
+  int32_t *table, *holders;
+  int m, n, page_size, max_pages, num_pages;
+  long long table_ld;
+  int32_t *lens_out, *pages_out, *refused, *status;
+};
+cudaError_t paged_fork_launch(const ForkParams& p, int num_sms, cudaStream_t st);
+// copies [n][3]: page to copy, its new page, rows; -1, -1, 0 where there is none
+cudaError_t paged_reserve_forked_launch(const ReserveParams& p, int32_t* holders, int32_t* copies, cudaStream_t st);
+cudaError_t paged_release_forked_launch(const ReleaseParams& p, int32_t* holders, cudaStream_t st);
+
+constexpr int kCopyPools = 64;
+struct CopyParams {
+  uint8_t* pools[kCopyPools];
+  const int32_t* copies;             // [n][3]
+  int n, layers, nkv, page_shift, num_pages;
+};
+cudaError_t q4_copy_launch(const CopyParams& p, int num_sms, cudaStream_t st);
 
 struct Q4AppendParams {
   const void *k, *v;                 // [T, NKV, 128], f16 or bf16

@@ -14,9 +14,11 @@ one step of a batch is
     cache.trim(rejected)                               # lengths only
     cache.release()                                    # spare pages go back
 
-without a host synchronisation.  The same operators as plain functions on
+without a host synchronisation.  ``cache.fork`` starts a request from another
+one's rows, whose pages both then hold.  The same operators as plain functions on
 tensors are ``paged_reserve``, ``paged_release``, ``q4_append``, ``q4_read``
-and ``q4_attention``.  Number format and page layout: ``csrc/q4.cuh``.
+and ``q4_attention``, and, where requests hold pages together, ``paged_fork``,
+``paged_reserve_forked``, ``q4_copy_pages`` and ``paged_release_forked``.  Number format and page layout: ``csrc/q4.cuh``.
 """
 from __future__ import annotations
 
@@ -32,7 +34,9 @@ BLOCK_BYTES = 2304                   # 16 rows of one kv head, K and V with thei
 STATUS_BITS = {1: "too few free pages", 2: "a request outgrew its row of the block table",
                4: "more new rows than slots", 8: "more pages came back than were lent",
                16: "a NaN or an infinity was appended", 32: "a device-side wait expired",
-               64: "a request brought more query rows than max_rows, or starts do not fit q"}
+               64: "a request brought more query rows than max_rows, or starts do not fit q",
+               128: "a fork named no request, or one that held rows already",
+               256: "new rows would have gone into a page of other requests behind the request's rows"}
 
 
 class PagedStep(NamedTuple):
@@ -74,6 +78,51 @@ def paged_release(keep, pages, table, free_pages, head, page_size: int, status=N
     """Request i keeps the pages of its first keep[i] rows; the others go back
     into ``free_pages`` below ``head``.  Returns (pages, head) afterwards."""
     return N.load_paged().release(keep, pages, table, free_pages, head, page_size, status)
+
+
+def page_holders(num_pages: int, device="cuda") -> torch.Tensor:
+    """Counts of a cache whose pages several requests may hold: int32
+    [2, num_pages], row 0 the requests beyond the first that hold each page, row 1
+    the operators' own (zero between calls)."""
+    if num_pages < 1:
+        raise ValueError("num_pages must be positive")
+    return torch.zeros(2, num_pages, dtype=torch.int32, device=device)
+
+
+def paged_fork(src, dst, lens, pages, table, holders, page_size: int, rows=None, status=None, refused=None):
+    """Request dst[j] takes over the first rows[j] rows (all without ``rows``)
+    of request src[j]: it holds the same pages, and no cached row moves.  src, dst
+    and rows are int32 device vectors.  dst[j] must hold nothing and be named once;
+    a fork that cannot be made is skipped and sets a bit of ``status``.  The table
+    and ``holders`` change in place; returns (lens, pages) afterwards.  From then
+    on the cache reserves and releases with the operators below."""
+    return N.load_paged().fork(src, dst, rows, lens, pages, table, holders, page_size, status, refused)
+
+
+def paged_reserve_forked(lens, new_rows, pages, table, free_pages, head, holders, page_size: int, num_slots: int,
+                         status=None, refused=None):
+    """``paged_reserve`` where requests may hold pages together: one whose new
+    rows go into such a page gets a page of its own first.  Returns (PagedStep,
+    copies [n, 3]): old page, new page and rows to copy of each request (-1, -1, 0
+    where it keeps its page), for ``q4_copy_pages`` before rows are appended.  Pages
+    that a trim left behind a request's rows must not be held by others where its
+    new rows go (such a request is turned away): ``paged_release_forked`` first."""
+    *step, copies = N.load_paged().reserve_forked(lens, new_rows, pages, table, free_pages, head, holders, page_size, num_slots,
+                                                  status, refused)
+    return PagedStep._make(step), copies
+
+
+def paged_release_forked(keep, pages, table, free_pages, head, holders, page_size: int, status=None):
+    """``paged_release`` where a page goes back once its last holder gives it up."""
+    return N.load_paged().release_forked(keep, pages, table, free_pages, head, holders, page_size, status)
+
+
+def q4_copy_pages(pools: Sequence[torch.Tensor], copies) -> None:
+    """Copy pages in every pool of the list: copies [n, 3] int32 on the device
+    holds page, page to copy to, and how many of its rows (in whole blocks of 16).
+    Entries with -1 are skipped; no page may be copied to twice, or both to and
+    from."""
+    N.load_paged().copy_pages(list(pools), copies)
 
 
 def q4_pool(num_pages: int, num_kv_heads: int, page_size: int = 64, device="cuda") -> torch.Tensor:
@@ -154,10 +203,15 @@ class PagedKVCacheQ4:
     of captured steps goes on where the last one ended; only then may
     ``reserve``, ``attend``, ``trim`` and ``release`` be captured, with row
     counts on the device (or one number).  Replays and calls in between are the
-    caller's to order like calls on different streams."""
+    caller's to order like calls on different streams.
+
+    With ``forkable``, ``fork`` lets requests hold pages together: several
+    continuations of one prompt, or many prompts that begin alike.  ``reserve``
+    then copies a page, in all layers, before a request writes into one that others
+    hold, and ``release`` counts holders."""
 
     def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, max_seqs: int, max_len: int,
-                 page_size: int = 64, device="cuda", capturable: bool = False):
+                 page_size: int = 64, device="cuda", capturable: bool = False, forkable: bool = False):
         if num_layers < 1 or max_seqs < 1 or max_len < 1:
             raise ValueError("num_layers, max_seqs and max_len must be positive")
         self.page_size, self.max_seqs, self.nkv = page_size, max_seqs, num_kv_heads
@@ -172,6 +226,8 @@ class PagedKVCacheQ4:
         self.status = torch.zeros(1, **i32)
         self._refused = torch.zeros(max_seqs, **i32)      # turned away when it last brought rows
         self.capturable = capturable
+        self.holders = page_holders(num_pages, self.device) if forkable else None
+        self._trimmed = False
         self._workspace, self._sizes = {}, {}
         self._stream = _raw_stream(self.device.index)
         self._streams = {self._stream}
@@ -204,6 +260,7 @@ class PagedKVCacheQ4:
             if raw not in self._streams:
                 self._streams.add(raw)
                 state += [*self.pools, self.table, self.free_pages, self.status, self._refused]
+                state += [self.holders] if self.holders is not None else []
             for t in state:
                 t.record_stream(torch.cuda.current_stream(self.device))
         return raw
@@ -225,10 +282,46 @@ class PagedKVCacheQ4:
             new_rows = self._upload(list(new_rows), "new_rows")
         elif num_slots is None:
             raise ValueError("num_slots is needed with new_rows on the device")
-        step = paged_reserve(self.lens, new_rows, self.pages, self.table, self.free_pages, self.head, self.page_size,
-                             num_slots, self.status, self._refused)
+        if self.holders is None:
+            step = paged_reserve(self.lens, new_rows, self.pages, self.table, self.free_pages, self.head, self.page_size,
+                                 num_slots, self.status, self._refused)
+        else:
+            if self._trimmed or self.capturable:      # (a graph's replays may follow any trim)
+                self._give_back()                     # pages behind the rows may be held with others
+            step, copies = paged_reserve_forked(self.lens, new_rows, self.pages, self.table, self.free_pages, self.head,
+                                                self.holders, self.page_size, num_slots, self.status, self._refused)
+            q4_copy_pages(self.pools, copies)
         self._keep(lens=step.lens, pages=step.pages, head=step.head)
         return step
+
+    def fork(self, src: Union[int, torch.Tensor, Sequence[int]], dst: Union[torch.Tensor, Sequence[int]],
+             rows: Union[None, int, torch.Tensor, Sequence[int]] = None) -> None:
+        """Request dst[j], which must hold nothing, goes on from the first rows[j]
+        rows (default: all) of request src[j] (one number: of that request).  Their
+        pages are held together and copied where one is written into; ``check``
+        reports what could not be forked.  Device tensors are int32 vectors."""
+        if self.holders is None:
+            raise RuntimeError("a PagedKVCacheQ4 whose requests fork must be made with forkable=True")
+        self._enter()
+        if not torch.is_tensor(dst):
+            dst = [int(d) for d in dst]
+            if any(not 0 <= d < self.max_seqs for d in dst) or len(set(dst)) != len(dst):
+                raise ValueError(f"requests to fork into must be distinct and lie in [0, {self.max_seqs})")
+        count = len(dst)
+        named = {"src": src, "dst": dst, "rows": rows}
+        for name, v in named.items():
+            if v is None or torch.is_tensor(v):
+                continue
+            v = [int(v)] * count if isinstance(v, int) else [int(x) for x in v]
+            if len(v) != count or (name == "rows" and any(x < 0 for x in v)) or \
+                    (name == "src" and any(not 0 <= x < self.max_seqs for x in v)):
+                raise ValueError(f"{name} must be {count} numbers, requests in [0, {self.max_seqs}) and rows not negative")
+            named[name] = self._upload(v, name)
+        if self._trimmed or self.capturable:      # (a request trimmed to nothing holds pages until then)
+            self._give_back()
+        lens, pages = paged_fork(named["src"], named["dst"], self.lens, self.pages, self.table, self.holders, self.page_size,
+                                 named["rows"], self.status, self._refused)
+        self._keep(lens=lens, pages=pages)
 
     def append(self, layer: int, k, v, step: PagedStep) -> None:
         self._on_stream()
@@ -277,6 +370,7 @@ class PagedKVCacheQ4:
             counts = counts.contiguous()
         else:
             counts = min(counts, 2 ** 31 - 1)
+        self._trimmed = True
         # (a negative count on the device, where nobody can raise, trims nothing)
         self.lens = N.load_paged().trim(self.lens, counts, self._refused, self.lens if self.capturable else None)
 
@@ -290,9 +384,17 @@ class PagedKVCacheQ4:
             if self._capturing():
                 raise ValueError("finished requests cannot be named in a CUDA graph: every replay would empty them")
             self._keep(lens=self.lens.index_fill(0, torch.tensor(seqs).to(self.device, non_blocking=True), 0))
-        pages, head = paged_release(self.lens, self.pages, self.table, self.free_pages, self.head, self.page_size,
-                                    self.status)
+        self._give_back()
+
+    def _give_back(self) -> None:
+        if self.holders is None:
+            pages, head = paged_release(self.lens, self.pages, self.table, self.free_pages, self.head, self.page_size,
+                                        self.status)
+        else:
+            pages, head = paged_release_forked(self.lens, self.pages, self.table, self.free_pages, self.head, self.holders,
+                                               self.page_size, self.status)
         self._keep(pages=pages, head=head)
+        self._trimmed = False
 
     def read(self, layer: int, seq: int, length: int, dtype=torch.float16):
         """The first ``length`` rows of a request, which it must hold, as
