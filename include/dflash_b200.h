@@ -480,6 +480,34 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
                         int window, float scale, uint16_t* out, int32_t* status, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* Attention of requests whose first rows are the same: those are read once for
+ * all query rows of a group.  Groups are runs of requests, groups [num_groups + 1]
+ * their boundaries (ascending, within [0, n]; requests outside are on their own).
+ *
+ * The plan, once a step for all layers, compares the members' block tables: their
+ * prefix is the pages that the rows of all members with query rows begin with
+ * alike, as far as every query row sees them whole (starts, max_rows and causal as
+ * in dflash_q4_attention; lens [n]).  Written: group_starts [num_groups + 1],
+ * prefix [num_groups] (rows), row_of [num_groups], skip [n] (pages), own_lens [n].
+ *
+ * The attention gives what dflash_q4_attention gives without a window, up to the
+ * rounding of one more join in fp32: the group's query rows over its prefix, then
+ * each request's over its own rows, joined.  max_group: requests of a group at
+ * most (more set DFLASH_PAGED_ROWS, and their rows are undefined); max_rows *
+ * max_group <= DFLASH_Q4_MAX_ROWS.  workspace: dflash_q4_prefix_workspace_size()
+ * bytes, as for dflash_q4_attention. */
+int dflash_paged_prefix_plan(const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens, const int32_t* starts,
+                             int n, int max_rows, int page_size, const int32_t* groups, int num_groups, int causal,
+                             int32_t* group_starts, int32_t* prefix, int32_t* row_of, int32_t* skip, int32_t* own_lens,
+                             void* stream);
+size_t dflash_q4_prefix_workspace_size(int rows, int max_rows, int max_group, int nq, int nkv);
+int dflash_q4_prefix_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages,
+                               int page_size, const int32_t* table, int64_t table_ld, int max_pages, const int32_t* starts,
+                               int n, int rows, int max_rows, const int32_t* group_starts, const int32_t* prefix,
+                               const int32_t* row_of, int num_groups, int max_group, const int32_t* skip,
+                               const int32_t* own_lens, int nq, int nkv, int causal, float scale, uint16_t* out,
+                               int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- operators around a target's decode step --------------------------------
  * No counterpart in the reference, whose targets are external models and whose
  * loop is greedy (mirror_sd/generate.py:591-789). */

@@ -153,6 +153,13 @@ EXPORTS = {
     "dflash_q4_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_void_p, c_int64,
                                       c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p,
                                                                                   c_void_p, c_size_t, c_void_p]),
+    "dflash_paged_prefix_plan": (c_int32, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
+                                           c_int] + [c_void_p] * 6),
+    "dflash_q4_prefix_workspace_size": (c_size_t, [c_int] * 5),
+    "dflash_q4_prefix_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_int,
+                                             c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                             c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
+                                             c_size_t, c_void_p]),
     "dflash_rope": (c_int32, [c_void_p, c_int64, c_int64] + [c_int] * 7 + [c_void_p, c_float, c_void_p, c_int, c_void_p,
                                                                            c_void_p, c_int, c_void_p, c_int64, c_int64,
                                                                            c_void_p]),
@@ -163,7 +170,8 @@ EXPORTS = {
 # the entries that the binding calls, in the order of its Lib
 PAGED_ENTRIES = ("dflash_paged_reserve_tracked", "dflash_paged_release", "dflash_paged_trim", "dflash_q4_append",
                  "dflash_q4_read", "dflash_q4_attention", "dflash_paged_fork", "dflash_paged_reserve_forked",
-                 "dflash_paged_release_forked", "dflash_q4_copy_pages", "dflash_rope", "dflash_verify_drafts", "dflash_last_error")
+                 "dflash_paged_release_forked", "dflash_q4_copy_pages", "dflash_paged_prefix_plan",
+                 "dflash_q4_prefix_attention", "dflash_rope", "dflash_verify_drafts", "dflash_last_error")
 
 _lib = None
 _paged = None

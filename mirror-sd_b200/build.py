@@ -25,7 +25,7 @@ LIB = os.path.join(LIB_DIR, "libdflash_b200.so")
 BINDING = os.path.join(LIB_DIR, "dflash_paged.so")
 BINDING_SOURCE = "paged_binding.cpp"
 SOURCES = ["quant.cu", "w8_tc.cu", "attention.cu", "attention_tc.cu", "tc_gemm.cu", "lm_head.cu", "misc.cu", "anchor.cu",
-           "f32_path.cu", "paged.cu", "paged_share.cu", "q4_cache.cu", "q4_attention.cu", "q4_attention_tc.cu", "rope.cu", "verify.cu",
+           "f32_path.cu", "paged.cu", "paged_share.cu", "prefix_plan.cu", "q4_cache.cu", "q4_attention.cu", "q4_attention_tc.cu", "rope.cu", "verify.cu",
            "dflash_api.cu", "paged_api.cu", "decode_api.cu"]
 HEADERS = ["common.cuh", "kernels.cuh", "q4.cuh", "q4_attn.cuh", "paged_scan.cuh", "decode.cuh", "api_error.cuh"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

@@ -64,6 +64,71 @@ bool overlap(const uint16_t* out, const uint16_t* q, long long q_row, long long 
 
 constexpr size_t kCounterBytes = 4096;   // two counters per SM, then the partials
 
+// Checks of an attention call and its parameters; n, rows and max_rows of the
+// pass.  *few: which kernel (up to 16 query rows a kv head each warp multiplies on
+// its own (mma.sync, no hand-over between warps); above, tcgen05 with the rows as
+// columns).
+int attention_params(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages, int page_size,
+                     const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens, const int32_t* starts, int n,
+                     int rows, int max_rows, int nq, int nkv, int causal, int sink, int window, float scale, uint16_t* out,
+                     int32_t* status, Q4AttnParams* params, bool* few) {
+  if (int rc = check_paging(n, page_size, table_ld, max_pages, num_pages)) return rc;
+  if (int rc = check_pool(rows, nkv, pool, num_pages, page_size)) return rc;
+  // (the kernels add a tile, a window or the query rows to a position in 32 bits)
+  if ((long long)max_pages * page_size > 1ll << 30)
+    return fail(DFLASH_ERR_INVALID, "%d pages of %d rows a request: at most 2^30 rows", max_pages, page_size);
+  if (nq < nkv || nq % nkv) return fail(DFLASH_ERR_INVALID, "nq %d must be a multiple of nkv %d", nq, nkv);
+  if (max_rows < 1 || max_rows > DFLASH_Q4_MAX_ROWS)
+    return fail(DFLASH_ERR_INVALID, "max_rows %d outside [1, %d]", max_rows, DFLASH_Q4_MAX_ROWS);
+  if (!starts && (long long)n * max_rows != rows)
+    return fail(DFLASH_ERR_INVALID, "without starts every request has max_rows rows (%d x %d, got %d)", n, max_rows, rows);
+  if (sink < 0 || window < 0) return fail(DFLASH_ERR_INVALID, "sink %d, window %d", sink, window);
+  if (sink > 0 && window == 0) return fail(DFLASH_ERR_INVALID, "sink needs a window (window 0 sees every row)");
+  // A window as wide as the table hides nothing; the kernels subtract the others
+  // from lengths less query rows, in 32 bits.
+  if (window >= max_pages * page_size) sink = window = 0;
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(DFLASH_ERR_INVALID, "scale must be positive and finite");
+  if (!aligned16(q) || !aligned16(out) || q_row % 8 || q_head % 8)
+    return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");
+  const int G = nq / nkv;
+  *few = (long long)max_rows * G <= kQ4FewRows;
+  const double columns = *few ? q4_attn_columns(max_rows, nq, nkv) : q4_attn_tc_columns(max_rows, nq, nkv);
+  if (G > 256 || nkv > 1024 || ((double)max_rows * G / columns + 1) * nkv * nkv > 4e9)
+    return fail(DFLASH_ERR_INVALID, "%d query heads a kv head, %d kv heads, %d rows: too many", G, nkv, max_rows);
+  // Tiles of all items together are counted in 32 bits: a full table for each
+  // group of query rows, of which every request with rows has one in part.
+  const double units = std::ceil((double)max_pages * page_size / (*few ? kQ4Tile : kQ4TcTile)) * nkv *
+                       ((double)rows * G / columns + (n < rows ? n : rows));
+  if ((long long)rows * nq > INT32_MAX) return fail(DFLASH_ERR_INVALID, "rows x nq must stay below 2^31");
+  if (units >= INT32_MAX) return fail(DFLASH_ERR_INVALID, "n x table x heads x rows is too large for one call");
+  Q4AttnParams& p = *params;
+  p = Q4AttnParams{};
+  p.q = q; p.q_row = q_row; p.q_head = q_head; p.bf16 = bf16 != 0; p.pool = pool;
+  p.table = table; p.lens = lens; p.starts = starts; p.table_ld = table_ld;
+  p.n = n; p.T = rows; p.max_rows = max_rows; p.nq = nq; p.nkv = nkv;
+  p.by_g = Divisor(G); p.by_nkv = Divisor(nkv);
+  p.page_shift = log2_of(page_size);
+  p.max_pages = max_pages; p.num_pages = num_pages; p.causal = causal != 0; p.sink = sink; p.window = window;
+  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  p.factor = score_factor(16.f * p.scale_log2);
+  p.out = out; p.status = status;
+  return DFLASH_OK;
+}
+
+// The rest of the call, where there are rows: its workspace and the launch.
+int attention_launch(Q4AttnParams& p, bool few, int pass, void* workspace, void* stream) {
+  int sms = 0;
+  if (int rc = num_sms(&sms)) return rc;
+  if ((size_t)sms * 2 * sizeof(int) > kCounterBytes) return fail(DFLASH_ERR_INVALID, "%d SMs", sms);
+  p.counters = static_cast<int*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+  if (few)
+    CK(q4_attn_launch(p, pass, sms, static_cast<cudaStream_t>(stream)));
+  else
+    CK(q4_attn_tc_launch(p, pass, sms, static_cast<cudaStream_t>(stream)));
+  return DFLASH_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -265,63 +330,86 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
                         size_t workspace_bytes, void* stream) {
   if (!pool || !table || !lens || !workspace || (rows > 0 && (!q || !out)))
     return fail(DFLASH_ERR_INVALID, "NULL pointer");
-  if (int rc = check_paging(n, page_size, table_ld, max_pages, num_pages)) return rc;
-  if (int rc = check_pool(rows, nkv, pool, num_pages, page_size)) return rc;
-  // (the kernels add a tile, a window or the query rows to a position in 32 bits)
-  if ((long long)max_pages * page_size > 1ll << 30)
-    return fail(DFLASH_ERR_INVALID, "%d pages of %d rows a request: at most 2^30 rows", max_pages, page_size);
-  if (nq < nkv || nq % nkv) return fail(DFLASH_ERR_INVALID, "nq %d must be a multiple of nkv %d", nq, nkv);
-  if (max_rows < 1 || max_rows > DFLASH_Q4_MAX_ROWS)
-    return fail(DFLASH_ERR_INVALID, "max_rows %d outside [1, %d]", max_rows, DFLASH_Q4_MAX_ROWS);
-  if (!starts && (long long)n * max_rows != rows)
-    return fail(DFLASH_ERR_INVALID, "without starts every request has max_rows rows (%d x %d, got %d)", n, max_rows, rows);
-  if (sink < 0 || window < 0) return fail(DFLASH_ERR_INVALID, "sink %d, window %d", sink, window);
-  if (sink > 0 && window == 0) return fail(DFLASH_ERR_INVALID, "sink needs a window (window 0 sees every row)");
-  // A window as wide as the table hides nothing; the kernels subtract the others
-  // from lengths less query rows, in 32 bits.
-  if (window >= max_pages * page_size) sink = window = 0;
-  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(DFLASH_ERR_INVALID, "scale must be positive and finite");
-  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_row % 8 || q_head % 8)
+  Q4AttnParams p;
+  bool few;
+  if (int rc = attention_params(q, q_row, q_head, bf16, pool, num_pages, page_size, table, table_ld, max_pages, lens, starts, n,
+                                rows, max_rows, nq, nkv, causal, sink, window, scale, out, status, &p, &few))
+    return rc;
+  if (!aligned16(workspace))
     return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");
-  const int G = nq / nkv;
-  // Up to 16 query rows a kv head each warp multiplies on its own (mma.sync, no
-  // hand-over between warps); above, tcgen05 with the rows as columns.
-  const bool few = (long long)max_rows * G <= kQ4FewRows;
-  const double columns = few ? q4_attn_columns(max_rows, nq, nkv) : q4_attn_tc_columns(max_rows, nq, nkv);
-  if (G > 256 || nkv > 1024 || ((double)max_rows * G / columns + 1) * nkv * nkv > 4e9)
-    return fail(DFLASH_ERR_INVALID, "%d query heads a kv head, %d kv heads, %d rows: too many", G, nkv, max_rows);
-  // Tiles of all items together are counted in 32 bits: a full table for each
-  // group of query rows, of which every request with rows has one in part.
-  const double units = std::ceil((double)max_pages * page_size / (few ? kQ4Tile : kQ4TcTile)) * nkv *
-                       ((double)rows * G / columns + (n < rows ? n : rows));
-  if ((long long)rows * nq > INT32_MAX) return fail(DFLASH_ERR_INVALID, "rows x nq must stay below 2^31");
-  if (units >= INT32_MAX) return fail(DFLASH_ERR_INVALID, "n x table x heads x rows is too large for one call");
   if (workspace_bytes < dflash_q4_attention_workspace_size(max_rows, nq, nkv))
     return fail(DFLASH_ERR_INVALID, "workspace too small (%zu < %zu)", workspace_bytes,
                 dflash_q4_attention_workspace_size(max_rows, nq, nkv));
   if (rows == 0) return DFLASH_OK;
   // (the kernels read q through the non-coherent path, some rows after others are finished)
   if (overlap(out, q, q_row, q_head, rows, nq)) return fail(DFLASH_ERR_INVALID, "out overlaps q");
-  int sms = 0;
-  if (int rc = num_sms(&sms)) return rc;
-  if ((size_t)sms * 2 * sizeof(int) > kCounterBytes) return fail(DFLASH_ERR_INVALID, "%d SMs", sms);
-  Q4AttnParams p{};
-  p.q = q; p.q_row = q_row; p.q_head = q_head; p.bf16 = bf16 != 0; p.pool = pool;
-  p.table = table; p.lens = lens; p.starts = starts; p.table_ld = table_ld;
-  p.n = n; p.T = rows; p.max_rows = max_rows; p.nq = nq; p.nkv = nkv;
-  p.by_g = Divisor(G); p.by_nkv = Divisor(nkv);
-  p.page_shift = log2_of(page_size);
-  p.max_pages = max_pages; p.num_pages = num_pages; p.causal = causal != 0; p.sink = sink; p.window = window;
-  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  p.factor = score_factor(16.f * p.scale_log2);
-  p.out = out; p.status = status;
-  p.counters = static_cast<int*>(workspace);
-  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-  if (few)
-    CK(q4_attn_launch(p, sms, static_cast<cudaStream_t>(stream)));
-  else
-    CK(q4_attn_tc_launch(p, sms, static_cast<cudaStream_t>(stream)));
+  return attention_launch(p, few, kAttnAll, workspace, stream);
+}
+
+int dflash_paged_prefix_plan(const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens, const int32_t* starts,
+                             int n, int max_rows, int page_size, const int32_t* groups, int num_groups, int causal,
+                             int32_t* group_starts, int32_t* prefix, int32_t* row_of, int32_t* skip, int32_t* own_lens,
+                             void* stream) {
+  if (!table || !lens || !groups || !group_starts || !prefix || !row_of || !skip || !own_lens)
+    return fail(DFLASH_ERR_INVALID, "NULL pointer");
+  if (int rc = check_paging(n, page_size, table_ld, max_pages, 0)) return rc;
+  if (max_rows < 1 || max_rows > DFLASH_Q4_MAX_ROWS)
+    return fail(DFLASH_ERR_INVALID, "max_rows %d outside [1, %d]", max_rows, DFLASH_Q4_MAX_ROWS);
+  if (num_groups < 1 || num_groups > DFLASH_PAGED_MAX_SEQS)
+    return fail(DFLASH_ERR_INVALID, "%d groups outside [1, %d]", num_groups, DFLASH_PAGED_MAX_SEQS);
+  if (own_lens == lens) return fail(DFLASH_ERR_INVALID, "own_lens must not be lens");
+  PrefixPlanParams p{};
+  p.table = table; p.lens = lens; p.starts = starts; p.groups = groups; p.table_ld = table_ld;
+  p.n = n; p.g = num_groups; p.max_rows = max_rows; p.page_size = page_size; p.max_pages = max_pages; p.causal = causal != 0;
+  p.group_starts = group_starts; p.prefix = prefix; p.row_of = row_of; p.skip = skip; p.own_lens = own_lens;
+  CK(prefix_plan_launch(p, static_cast<cudaStream_t>(stream)));
   return DFLASH_OK;
+}
+
+size_t dflash_q4_prefix_workspace_size(int rows, int max_rows, int max_group, int nq, int nkv) {
+  if (rows < 0 || max_rows < 1 || max_group < 1 || (long long)max_rows * max_group > DFLASH_Q4_MAX_ROWS) return 0;
+  const size_t own = dflash_q4_attention_workspace_size(max_rows, nq, nkv);
+  const size_t group = dflash_q4_attention_workspace_size(max_rows * max_group, nq, nkv);
+  if (own == 0 || group == 0 || (long long)rows * nq > INT32_MAX) return 0;
+  return ((own > group ? own : group) + 15) / 16 * 16 + (size_t)rows * nq * 130 * sizeof(float);
+}
+
+int dflash_q4_prefix_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages,
+                               int page_size, const int32_t* table, int64_t table_ld, int max_pages, const int32_t* starts,
+                               int n, int rows, int max_rows, const int32_t* group_starts, const int32_t* prefix,
+                               const int32_t* row_of, int num_groups, int max_group, const int32_t* skip,
+                               const int32_t* own_lens, int nq, int nkv, int causal, float scale, uint16_t* out,
+                               int32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!pool || !table || !group_starts || !prefix || !row_of || !skip || !own_lens || !workspace || (rows > 0 && (!q || !out)))
+    return fail(DFLASH_ERR_INVALID, "NULL pointer");
+  if (num_groups < 1 || num_groups > DFLASH_PAGED_MAX_SEQS)
+    return fail(DFLASH_ERR_INVALID, "%d groups outside [1, %d]", num_groups, DFLASH_PAGED_MAX_SEQS);
+  if (max_group < 1 || (long long)max_rows * max_group > DFLASH_Q4_MAX_ROWS)
+    return fail(DFLASH_ERR_INVALID, "groups of %d requests of %d rows: at most %d rows", max_group, max_rows, DFLASH_Q4_MAX_ROWS);
+  Q4AttnParams group, own;
+  bool few_group, few_own;
+  if (int rc = attention_params(q, q_row, q_head, bf16, pool, num_pages, page_size, table, table_ld, max_pages, own_lens, starts,
+                                n, rows, max_rows, nq, nkv, causal, 0, 0, scale, out, status, &own, &few_own))
+    return rc;
+  if (int rc = attention_params(q, q_row, q_head, bf16, pool, num_pages, page_size, table, table_ld, max_pages, prefix,
+                                group_starts, num_groups, rows, max_rows * max_group, nq, nkv, 0, 0, 0, scale, out, status,
+                                &group, &few_group))
+    return rc;
+  if (!aligned16(workspace))
+    return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");
+  const size_t need = dflash_q4_prefix_workspace_size(rows, max_rows, max_group, nq, nkv);
+  if (workspace_bytes < need) return fail(DFLASH_ERR_INVALID, "workspace too small (%zu < %zu)", workspace_bytes, need);
+  if (rows == 0) return DFLASH_OK;
+  if (overlap(out, q, q_row, q_head, rows, nq)) return fail(DFLASH_ERR_INVALID, "out overlaps q");
+  // (the sums lie at the end, where they depend on this call's rows alone)
+  const size_t sums = need - (size_t)rows * nq * 130 * sizeof(float);
+  group.pre_o = own.pre_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + sums);
+  group.pre_ml = own.pre_ml = reinterpret_cast<float2*>(group.pre_o + (size_t)rows * nq * 128);
+  group.row_of = row_of;
+  group.table_rows = n;
+  own.skip = skip;
+  if (int rc = attention_launch(group, few_group, kAttnPrefix, workspace, stream)) return rc;
+  return attention_launch(own, few_own, kAttnOwn, workspace, stream);
 }
 
 }  // extern "C"

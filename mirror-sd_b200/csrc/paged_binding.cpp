@@ -46,6 +46,8 @@ struct Lib {
   decltype(&dflash_paged_reserve_forked) reserve_forked;
   decltype(&dflash_paged_release_forked) release_forked;
   decltype(&dflash_q4_copy_pages) copy_pages;
+  decltype(&dflash_paged_prefix_plan) prefix_plan;
+  decltype(&dflash_q4_prefix_attention) prefix_attention;
   decltype(&dflash_rope) rope;
   decltype(&dflash_verify_drafts) verify;
   decltype(&dflash_last_error) last_error;
@@ -289,6 +291,20 @@ PyObject* read(PyObject* const* a) {
   return tuple(THPVariable_Wrap(k), THPVariable_Wrap(v));
 }
 
+at::Tensor output_like(PyObject* o, const at::Tensor& q, int dev) {   // a new tensor for None
+  if (o == Py_None) return empty(q.sizes(), q.scalar_type(), dev);
+  const at::Tensor& out = tensor(o, "out");
+  if (!out.sizes().equals(q.sizes()) || out.scalar_type() != q.scalar_type() || !out.is_cuda() || out.get_device() != dev ||
+      !out.is_contiguous())
+    refuse("out must be contiguous, of q's shape, type and device");
+  return out;
+}
+const at::Tensor& workspace_of(PyObject* o, int dev) {
+  const at::Tensor& ws = tensor(o, "workspace");
+  if (!ws.is_cuda() || ws.get_device() != dev || !ws.is_contiguous()) refuse("workspace must be on cuda:%d", dev);
+  return ws;
+}
+
 // (q, pool, table, lens, starts, max_rows, causal, sink, window, scale, out, status, workspace)
 PyObject* attention(PyObject* const* a) {
   const Pool p = pool_of(a[1]);
@@ -300,22 +316,56 @@ PyObject* attention(PyObject* const* a) {
   const int32_t* starts = a[4] == Py_None ? nullptr : i32(a[4], "starts", n + 1, p.dev);
   const double scale = PyFloat_AsDouble(a[9]);
   if (scale == -1.0 && PyErr_Occurred()) throw PyError();
-  at::Tensor out;
-  if (a[10] == Py_None) {
-    out = empty(q.t.sizes(), q.t.scalar_type(), p.dev);
-  } else {
-    out = tensor(a[10], "out");
-    if (!out.sizes().equals(q.t.sizes()) || out.scalar_type() != q.t.scalar_type() || !out.is_cuda() ||
-        out.get_device() != p.dev || !out.is_contiguous())
-      refuse("out must be contiguous, of q's shape, type and device");
-  }
-  const at::Tensor& ws = tensor(a[12], "workspace");
-  if (!ws.is_cuda() || ws.get_device() != p.dev || !ws.is_contiguous()) refuse("workspace must be on cuda:%d", p.dev);
+  const at::Tensor out = output_like(a[10], q.t, p.dev);
+  const at::Tensor& ws = workspace_of(a[12], p.dev);
   call("dflash_q4_attention", lib.attention, p.dev, q.data, q.row, q.head, q.bf16, p.data, p.pages, p.page_size, t.data, t.ld,
        t.width, lens, starts, (int)n, q.rows, int32(a[5], "max_rows"), q.heads, p.nkv, (int)boolean(a[6]),
        int32(a[7], "sink"), int32(a[8], "window"), (float)scale, static_cast<uint16_t*>(out.data_ptr()),
        status_of(a[11], p.dev), ws.data_ptr(), (size_t)ws.nbytes());
   return a[10] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[10]);
+}
+
+// (table, lens, starts, max_rows, page_size, groups, causal) -> (group_starts, prefix, row_of, skip, own_lens)
+PyObject* prefix_plan(PyObject* const* a) {
+  const at::Tensor& lens = tensor(a[1], "lens");
+  const int dev = cuda_index(lens);
+  const int64_t n = lens.numel();
+  if (n > DFLASH_PAGED_MAX_SEQS) refuse("%lld requests, at most %d", (long long)n, DFLASH_PAGED_MAX_SEQS);
+  const Table t = table_of(a[0], n, dev);
+  const int32_t *l = i32(a[1], "lens", n, dev), *starts = a[2] == Py_None ? nullptr : i32(a[2], "starts", n + 1, dev);
+  int64_t bounds;
+  const int32_t* groups = i32(a[5], "groups", -1, dev, &bounds);
+  const int64_t g = bounds - 1;
+  if (g < 1 || g > DFLASH_PAGED_MAX_SEQS) refuse("%lld groups outside [1, %d]", (long long)g, DFLASH_PAGED_MAX_SEQS);
+  const at::Tensor out = empty({3 * g + 1 + 2 * n}, at::kInt, dev);   // [group_starts | prefix | row_of | skip | own_lens]
+  int32_t* o = out.data_ptr<int32_t>();
+  call("dflash_paged_prefix_plan", lib.prefix_plan, dev, t.data, t.ld, t.width, l, starts, (int)n, int32(a[3], "max_rows"),
+       int32(a[4], "page_size"), groups, (int)g, (int)boolean(a[6]), o, o + g + 1, o + 2 * g + 1, o + 3 * g + 1, o + 3 * g + 1 + n);
+  return tuple(slice(out, 0, g + 1), slice(out, g + 1, g), slice(out, 2 * g + 1, g), slice(out, 3 * g + 1, n),
+               slice(out, 3 * g + 1 + n, n));
+}
+
+// (q, pool, table, starts, max_rows, group_starts, prefix, row_of, max_group, skip, own_lens, causal, scale, out, status, workspace)
+PyObject* prefix_attention(PyObject* const* a) {
+  const Pool p = pool_of(a[1]);
+  const Rows q = rows_of(a[0], "q", -1, p.dev);
+  int64_t n, g;
+  const int32_t* own_lens = i32(a[10], "own_lens", -1, p.dev, &n);
+  if (n > DFLASH_PAGED_MAX_SEQS) refuse("%lld requests, at most %d", (long long)n, DFLASH_PAGED_MAX_SEQS);
+  const Table t = table_of(a[2], n, p.dev);
+  const int32_t* starts = a[3] == Py_None ? nullptr : i32(a[3], "starts", n + 1, p.dev);
+  const int32_t* prefix = i32(a[6], "prefix", -1, p.dev, &g);
+  const int32_t *group_starts = i32(a[5], "group_starts", g + 1, p.dev), *row_of = i32(a[7], "row_of", g, p.dev),
+                *skip = i32(a[9], "skip", n, p.dev);
+  const double scale = PyFloat_AsDouble(a[12]);
+  if (scale == -1.0 && PyErr_Occurred()) throw PyError();
+  const at::Tensor out = output_like(a[13], q.t, p.dev);
+  const at::Tensor& ws = workspace_of(a[15], p.dev);
+  call("dflash_q4_prefix_attention", lib.prefix_attention, p.dev, q.data, q.row, q.head, q.bf16, p.data, p.pages, p.page_size,
+       t.data, t.ld, t.width, starts, (int)n, q.rows, int32(a[4], "max_rows"), group_starts, prefix, row_of, (int)g,
+       int32(a[8], "max_group"), skip, own_lens, q.heads, p.nkv, (int)boolean(a[11]), (float)scale,
+       static_cast<uint16_t*>(out.data_ptr()), status_of(a[14], p.dev), ws.data_ptr(), (size_t)ws.nbytes());
+  return a[13] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[13]);
 }
 
 // (device) -> whether its current stream is being captured
@@ -562,6 +612,8 @@ PyMethodDef methods[] = {
     method<reserve_forked, 11>("reserve_forked"),
     method<release_forked, 8>("release_forked"),
     method<copy_pages, 2>("copy_pages"),
+    method<prefix_plan, 7>("prefix_plan"),
+    method<prefix_attention, 16>("prefix_attention"),
     method<rope, 10>("rope"),
     method<verify, 6>("verify"),
     {nullptr, nullptr, 0, nullptr}};

@@ -1,0 +1,88 @@
+// Which cached rows the requests of a group share, from the block tables: the
+// pages on which the rows of all its members with query rows begin alike, cut to
+// those that every query row sees whole.  Once a step, for all layers.
+//
+// One CTA a group; a warp compares a member's table row with the first member's,
+// 32 columns at a time, up to the first difference that any warp has found.  Few
+// numbers, so what it takes is latency.
+#include "q4.cuh"
+
+namespace dfl {
+
+constexpr int PP_THREADS = 512;
+
+__global__ void __launch_bounds__(PP_THREADS) prefix_plan_kernel(const PrefixPlanParams p) {
+  __shared__ int from, upto, first, members, limit;   // the group's requests; of those with query rows: first, number; pages
+  const int k = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    from = 0;
+    first = INT32_MAX;
+    members = 0;
+    limit = p.max_pages;
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  __syncthreads();
+  // groups[] as boundaries that never fall (device data that the host has not seen)
+  for (int i = threadIdx.x; i <= k; i += PP_THREADS) atomicMax(&from, min(max(__ldg(p.groups + i), 0), p.n));
+  __syncthreads();
+  if (threadIdx.x == 0) upto = max(from, min(max(__ldg(p.groups + k + 1), 0), p.n));
+  __syncthreads();
+  const int a = from, b = upto;
+  auto start = [&](int i) { return p.starts ? __ldg(p.starts + i) : i * p.max_rows; };
+  auto rows = [&](int i) { return start(i + 1) - start(i); };
+  auto length = [&](int i) { return (int)min((long long)max(__ldg(p.lens + i), 0), (long long)p.max_pages * p.page_size); };
+  for (int i = a + threadIdx.x; i < b; i += PP_THREADS) {
+    const int m = rows(i);
+    if (m <= 0) continue;
+    const int seen = max(length(i) - (p.causal ? m - 1 : 0), 0);   // keys that all its query rows see
+    atomicMin(&first, i);
+    atomicAdd(&members, 1);
+    atomicMin(&limit, seen / p.page_size);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && members < 2) limit = 0;
+  __syncthreads();
+  const int ref = first == INT32_MAX ? a : first;
+  const int32_t* one = p.table + (size_t)ref * p.table_ld;
+  for (int i = a + warp; i < b; i += PP_THREADS / 32) {
+    if (i == ref || rows(i) <= 0) continue;
+    const int32_t* other = p.table + (size_t)i * p.table_ld;
+    int most = *reinterpret_cast<volatile int*>(&limit);
+#pragma unroll 4
+    for (int c0 = 0; c0 < most; c0 += 32) {
+      const int c = c0 + lane;
+      const uint32_t differ = __ballot_sync(0xffffffffu, c < most && __ldg(one + c) != __ldg(other + c));
+      if (differ) {
+        most = c0 + __ffs(differ) - 1;
+        if (lane == 0) atomicMin(&limit, most);
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  const int pages = limit;
+  auto plan = [&](int i, int skip) {
+    p.skip[i] = skip;
+    p.own_lens[i] = max(length(i) - skip * p.page_size, 0);
+  };
+  for (int i = a + threadIdx.x; i < b; i += PP_THREADS) plan(i, rows(i) > 0 ? pages : 0);
+  if (threadIdx.x == 0) {
+    p.prefix[k] = pages * p.page_size;
+    p.row_of[k] = min(ref, p.n - 1);
+    p.group_starts[k] = start(a);
+    if (k == p.g - 1) p.group_starts[p.g] = start(b);
+  }
+  // requests of no group
+  if (k == 0)
+    for (int i = threadIdx.x; i < a; i += PP_THREADS) plan(i, 0);
+  if (k == p.g - 1)
+    for (int i = b + threadIdx.x; i < p.n; i += PP_THREADS) plan(i, 0);
+}
+
+cudaError_t prefix_plan_launch(const PrefixPlanParams& p, cudaStream_t st) {
+  if (p.n < 1 || p.n > kPagedMaxSeqs || p.g < 1 || p.g > kPagedMaxSeqs) return cudaErrorInvalidValue;
+  return launch_pdl(prefix_plan_kernel, dim3(p.g), dim3(PP_THREADS), 0, st, p);
+}
+
+}  // namespace dfl

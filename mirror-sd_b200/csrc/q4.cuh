@@ -101,6 +101,16 @@ struct CopyParams {
 };
 cudaError_t q4_copy_launch(const CopyParams& p, int num_sms, cudaStream_t st);
 
+// Which rows the members of each group share, once a step (prefix_plan.cu).
+struct PrefixPlanParams {
+  const int32_t *table, *lens, *starts, *groups;   // starts NULL: max_rows rows each; groups [g + 1]
+  long long table_ld;
+  int n, g, max_rows, page_size, max_pages, causal;
+  int32_t *group_starts, *prefix, *row_of;         // [g + 1], [g] rows, [g]
+  int32_t *skip, *own_lens;                        // [n] columns, [n]
+};
+cudaError_t prefix_plan_launch(const PrefixPlanParams& p, cudaStream_t st);
+
 struct Q4AppendParams {
   const void *k, *v;                 // [T, NKV, 128], f16 or bf16
   long long k_row, k_head, v_row, v_head;   // strides in elements
@@ -145,17 +155,27 @@ struct Q4AttnParams {
   int* counters;                     // [2 * num_sms], zero between calls
   float* part;                       // partial results
   int32_t* status;                   // or NULL
+  // passes over rows that several requests share (AttnPass)
+  const int32_t* row_of;             // kAttnPrefix: the table row of each group, of table_rows
+  int table_rows;
+  const int32_t* skip;               // kAttnOwn: columns of each request's table row that its group's pass covers
+  float* pre_o;                      // what that pass leaves: [T, NQ, 128] sums, and their (m, l) [T, NQ]
+  float2* pre_ml;
 };
+// An ordinary call; the query rows of groups of requests over the rows that each
+// group shares, which leaves sums and statistics; the requests' own rows, joined
+// with those.
+enum AttnPass : int { kAttnAll = 0, kAttnPrefix = 1, kAttnOwn = 2 };
 // Each kernel cuts a request's rows of a kv head into groups of `columns`, and
 // its cached rows into tiles.
 constexpr int kQ4Tile = 64, kQ4TcTile = 128;
 int q4_attn_columns(int max_rows, int nq, int nkv);
 int q4_attn_tc_columns(int max_rows, int nq, int nkv);
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms);
-cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
+cudaError_t q4_attn_launch(const Q4AttnParams& p, int pass, int num_sms, cudaStream_t st);
 // the same for blocks of query rows (q4_attention_tc.cu)
 size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms);
-cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st);
+cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int pass, int num_sms, cudaStream_t st);
 // Query rows of a kv head (rows of a request times G) up to which the first
 // kernel runs; it takes them 16 at a time and decodes the cache for each group.
 // us, first kernel / second, on 1 request of 2,048 rows, 16 of 16,384, 256 of

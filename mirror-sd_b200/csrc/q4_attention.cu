@@ -83,9 +83,9 @@ struct QaCfg {
 // A warp merges the partials of one item that the slots of `mask` hold (slot k
 // at at[k]), all queries at once: 8 (16) loads of a partial's O are on their way
 // together.  Writes the item's output rows (finish) or one partial at dst.
-template <int NT>
+template <int NT, int PASS>
 __device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask, const float* const* at, float* dst,
-                                            const Item& it, int sub, bool finish, int lane) {
+                                            const Item& it, int sub, bool whole, int lane) {
   constexpr int QT = QaCfg<NT>::QT;
   const int q = lane & (QT - 1);
   float M = -INFINITY, l = 0.f;
@@ -112,26 +112,33 @@ __device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask
       o[i].w = fmaf(wi, v[i].w, o[i].w);
     }
   }
-  if (!finish && lane < QT) {
+  if (!whole && lane < QT) {
     dst[QT * 128 + q] = M;
     dst[QT * 129 + q] = l;
   }
-  const float fin = l == 0.f ? 0.f : 16.f / l;
-  const int grp = p.by_nkv.of(sub);
+  const int grp = p.by_nkv.of(sub), head0 = (sub - grp * p.nkv) * p.by_g.d;
+  Finish fin{0.f, 0.f};
+  if (whole) {
+    const int r = grp * QT + q, j = p.by_g.of(r);
+    if (j < it.rows)
+      fin = finish<PASS>(p, has_prefix<PASS>(p, it.seq), (size_t)(it.row0 + j) * p.nq + head0 + r - j * p.by_g.d, M, l);
+  }
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    if (finish) {
-      const float f = __shfl_sync(0xffffffffu, fin, i);
+    if (whole) {
+      const Finish f{__shfl_sync(0xffffffffu, fin.own, i), PASS == kAttnOwn ? __shfl_sync(0xffffffffu, fin.pre, i) : 0.f};
+      const float mi = PASS == kAttnPrefix ? __shfl_sync(0xffffffffu, M, i) : 0.f;
+      const float li = PASS == kAttnPrefix ? __shfl_sync(0xffffffffu, l, i) : 0.f;
       const int r = grp * QT + i, j = p.by_g.of(r);
-      const float v[4] = {o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f};
-      if (j < it.rows) store_out4(p, it.row0 + j, (sub - grp * p.nkv) * p.by_g.d + r - j * p.by_g.d, 4 * lane, v);
+      const float v[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
+      if (j < it.rows) finish4<PASS>(p, it.row0 + j, head0 + r - j * p.by_g.d, 4 * lane, v, f, mi, li);
     } else {
       *reinterpret_cast<float4*>(dst + i * 128 + 4 * lane) = o[i];
     }
   }
 }
 
-template <int NT>
+template <int NT, int PASS>
 __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4AttnParams p) {
   using C = QaCfg<NT>;
   constexpr int QT = C::QT;
@@ -190,7 +197,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
   const int ctas = min((int)gridDim.x, (total + QA_LEAST - 1) / QA_LEAST);   // CTAs with work
   const int cta = blockIdx.x;
   if (cta >= ctas) {
-    zero_rows(p, threadIdx.x, C::THREADS);
+    zero_rows<PASS>(p, threadIdx.x, C::THREADS);
     return;
   }
   const Runs runs(total, ctas);
@@ -207,7 +214,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     // lane b < 4 looks after row block b of a tile: its page, then its copy
     auto page_of = [&](const Cursor& k) {
       const int pos = item_tile(k.it, k.j) * QA_TILE + (lane & 3) * kQ4Rows;
-      return lane < 4 && pos < k.it.L ? __ldg(p.table + (size_t)k.it.seq * p.table_ld + (pos >> p.page_shift)) : -1;
+      return lane < 4 && pos < k.it.L ? table_entry<PASS>(p, k.it.seq, pos >> p.page_shift) : -1;
     };
     int next_page = page_of(ahead);
     uint32_t loaded = 0;   // 4 bits a stage: row blocks that were copied
@@ -462,14 +469,17 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
           for (int x = 0; x < 2; ++x) {
             const float sum = col_sum(l[nt][x]);
             const int q = nt * 8 + 2 * c + x, r = r0 + q, j = p.by_g.of(r);
-            const float f = whole ? (sum == 0.f ? 0.f : 16.f / sum) : 1.f;
+            const float m = PASS == kAttnAll ? 0.f : partial_max(negm[nt][x], qscale[nt][x]);
+            Finish f{1.f, 0.f};
+            if (whole && j < cur.it.rows)
+              f = finish<PASS>(p, has_prefix<PASS>(p, cur.it.seq), (size_t)(cur.it.row0 + j) * p.nq + G0 + r - j * G, m, sum);
 #pragma unroll
             for (int t = 0; t < 8; t += 2) {
-              const float v[4] = {o[t][nt][x] * f, o[t][nt][2 + x] * f, o[t + 1][nt][x] * f, o[t + 1][nt][2 + x] * f};
+              const float v[4] = {o[t][nt][x], o[t][nt][2 + x], o[t + 1][nt][x], o[t + 1][nt][2 + x]};
               if (!whole)
                 *reinterpret_cast<float4*>(part + q * 128 + 16 * g + 2 * t) = make_float4(v[0], v[1], v[2], v[3]);
               else if (j < cur.it.rows)
-                store_out4(p, cur.it.row0 + j, G0 + r - j * G, 16 * g + 2 * t, v);
+                finish4<PASS>(p, cur.it.row0 + j, G0 + r - j * G, 16 * g + 2 * t, v, f, m, sum);
             }
             if (!whole && g == 0) {
               part[QT * 128 + q] = partial_max(negm[nt][x], qscale[nt][x]);
@@ -506,7 +516,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
       const Item it = slot_info[first];
       const bool inside = item0 >= c0 && item0 + it.ntile <= c1;
       const int border = item0 < c0 ? 0 : 1;
-      merge_slots<NT>(p, mask, slot_at, cta_part + ((size_t)cta * 2 + border) * C::SLOT, it, slot_sub[first], inside, lane);
+      merge_slots<NT, PASS>(p, mask, slot_at, cta_part + ((size_t)cta * 2 + border) * C::SLOT, it, slot_sub[first], inside, lane);
       if (!inside) {
         __threadfence();
         __syncwarp();
@@ -536,13 +546,15 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     for (int q = warp; q < QT; q += C::WARPS) {
       const int grp = p.by_nkv.of(sub), r = grp * QT + q, j = p.by_g.of(r);
       if (j >= it.rows) continue;
-      float v[4];
+      float v[4], m, l;
       merge_query(to - from + 1, [&](int k) { return cta_part + ((size_t)(from + k) * 2 + (k == 0 ? 1 : 0)) * C::SLOT; }, QT,
-                  q, lane, v);
-      store_out4(p, it.row0 + j, (sub - grp * p.nkv) * G + r - j * G, 4 * lane, v);
+                  q, lane, v, &m, &l);
+      const int head = (sub - grp * p.nkv) * G + r - j * G;
+      const Finish f = finish<PASS>(p, has_prefix<PASS>(p, it.seq), (size_t)(it.row0 + j) * p.nq + head, m, l);
+      finish4<PASS>(p, it.row0 + j, head, 4 * lane, v, f, m, l);
     }
   }
-  zero_rows(p, threadIdx.x, C::THREADS);
+  zero_rows<PASS>(p, threadIdx.x, C::THREADS);
 }
 
 // 8 or 16 query columns.  8 query rows, us with 8 columns / 16: 1 request of
@@ -553,16 +565,23 @@ size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms) {
   return (size_t)num_sms * (q4_attn_columns(max_rows, nq, nkv) == 8 ? (QaCfg<1>::WARPS + 2) * QaCfg<1>::SLOT : (QaCfg<2>::WARPS + 2) * QaCfg<2>::SLOT);
 }
 
-template <int NT>
+template <int NT, int PASS>
 static cudaError_t launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
   const size_t smem = QaCfg<NT>::RING + QaCfg<NT>::WARPS * QaCfg<NT>::STAGES * 8 + ((size_t)p.n + 1) * 4;
-  DFL_TRY(cudaFuncSetAttribute(q4_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  return launch_pdl(q4_attn_kernel<NT>, dim3(num_sms), dim3(QaCfg<NT>::THREADS), smem, st, p);
+  DFL_TRY(cudaFuncSetAttribute(q4_attn_kernel<NT, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  return launch_pdl(q4_attn_kernel<NT, PASS>, dim3(num_sms), dim3(QaCfg<NT>::THREADS), smem, st, p);
 }
 
-cudaError_t q4_attn_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
+template <int PASS>
+static cudaError_t launch_pass(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
+  return q4_attn_columns(p.max_rows, p.nq, p.nkv) == 8 ? launch<1, PASS>(p, num_sms, st) : launch<2, PASS>(p, num_sms, st);
+}
+
+cudaError_t q4_attn_launch(const Q4AttnParams& p, int pass, int num_sms, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
-  return q4_attn_columns(p.max_rows, p.nq, p.nkv) == 8 ? launch<1>(p, num_sms, st) : launch<2>(p, num_sms, st);
+  return pass == kAttnAll      ? launch_pass<kAttnAll>(p, num_sms, st)
+         : pass == kAttnPrefix ? launch_pass<kAttnPrefix>(p, num_sms, st)
+                               : launch_pass<kAttnOwn>(p, num_sms, st);
 }
 
 }  // namespace dfl

@@ -53,6 +53,7 @@ constexpr int QB_TILE = kQ4TcTile;
 constexpr int QB_BLK = kQ4Block + 32;      // a row block's stride in shared memory: 8 blocks on different banks
 constexpr int QB_STAGE = QB_TILE / kQ4Rows * QB_BLK;
 constexpr int QB_SEEN = 256;               // flag of a tile that every query of the item sees whole
+constexpr int QB_PREFIX = 1 << 16;         // beside an item's number of CTAs: there are sums over its group's rows
 constexpr int QB_SLACK = 6;
 constexpr float QB_RAISE = 8.f;
 
@@ -104,6 +105,7 @@ struct QbMisc {
   alignas(16) float qf[C::SEGS][C::N];        // score factors
   alignas(16) float negm[2][C::N];            // minus the columns' references, of either side
   alignas(16) float fac[2][C::N];             // rescale factors; at the end what O is multiplied by
+  alignas(16) float pre[C::N];                // and what the sums over the group's rows are (kAttnOwn)
   int cmax[2][C::N];                 // column maxima as ordered integers
   alignas(16) int cend[C::N];                 // where each column's keys end
   alignas(16) int coff[C::N];                 // output row of each column, or -1
@@ -264,7 +266,7 @@ __host__ __device__ __forceinline__ int4* q4_tc_shared(float* part, int n, int g
   return reinterpret_cast<int4*>(part + (size_t)grid * 2 * n * 130);
 }
 
-template <int N>
+template <int N, int PASS>
 __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnParams p) {
   using C = QbCfg<N>;
   constexpr int NS = C::NS;
@@ -659,11 +661,17 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         const float wa = ma == -kUnset ? 0.f : exp2_fast((ma - m) * p.factor), wb = mb == -kUnset ? 0.f : exp2_fast((mb - m) * p.factor);
         const float sum = wa * ((ms.lsum[0][gt] + ms.lsum[1][gt]) + (ms.lsum[2][gt] + ms.lsum[3][gt])) +
                           wb * ((ms.lsum[4][gt] + ms.lsum[5][gt]) + (ms.lsum[6][gt] + ms.lsum[7][gt]));
-        const float fin = whole ? (sum == 0.f ? 0.f : 16.f / sum) : 1.f;
-        ms.fac[0][gt] = wa * fin;
-        ms.fac[1][gt] = wb * fin;
+        Finish fin{1.f, 0.f};
+        const float top = PASS == kAttnAll && whole ? 0.f : partial_max(-m, p.factor);
+        if (whole && ms.coff[gt] >= 0) {
+          fin = finish<PASS>(p, has_prefix<PASS>(p, it.seq), ms.coff[gt], top, sum);
+          if (PASS == kAttnPrefix) p.pre_ml[ms.coff[gt]] = make_float2(top, sum);
+        }
+        ms.fac[0][gt] = wa * fin.own;
+        ms.fac[1][gt] = wb * fin.own;
+        if (PASS == kAttnOwn) ms.pre[gt] = fin.pre;
         if (!whole) {
-          part[N * 128 + gt] = partial_max(-m, p.factor);
+          part[N * 128 + gt] = top;
           part[N * 129 + gt] = sum;
         }
       }
@@ -696,7 +704,21 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           float* dst = part + 16 * c * 128 + row;
 #pragma unroll
           for (int i = 0; i < 16; ++i) dst[i * 128] = __uint_as_float(oa[i]);
+        } else if (PASS == kAttnPrefix) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int to = ms.coff[16 * c + i];
+            if (to >= 0) p.pre_o[(size_t)to * 128 + row] = __uint_as_float(oa[i]);
+          }
         } else {
+          if (PASS == kAttnOwn) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float f = ms.pre[16 * c + i];
+              if (f != 0.f)
+                oa[i] = __float_as_uint(fmaf(__ldcg(p.pre_o + (size_t)ms.coff[16 * c + i] * 128 + row), f, __uint_as_float(oa[i])));
+            }
+          }
           if (p.bf16) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) oa[i] = pack_bf16x2(__uint_as_float(oa[i]), 0.f);
@@ -718,7 +740,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       warp_arrive(&ms.o_free, lane);
       if (!whole) {
         // (merged by the item's first CTA's entry; the others' partials follow its own)
-        if (threadIdx.x == 0 && border == 1) ms.shared = make_int4(it.row0, it.rows, sg.sub, sharers(sg.item0, it.ntile));
+        if (threadIdx.x == 0 && border == 1)
+          ms.shared = make_int4(it.row0, it.rows, sg.sub,
+                                sharers(sg.item0, it.ntile) + (has_prefix<PASS>(p, it.seq) ? QB_PREFIX : 0));
       }
       t0 += nt;
     }
@@ -849,7 +873,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       head = sub - p.by_nkv.of(sub) * p.nkv;
       const int pos = row0 + (lane & 7) * kQ4Rows;
       page = -1;
-      if (pos < L) page = __ldg(p.table + (size_t)seq * p.table_ld + (pos >> p.page_shift));
+      if (pos < L) page = table_entry<PASS>(p, seq, pos >> p.page_shift);
     };
     look_up(0);
     int t = 0;   // tiles requested
@@ -879,9 +903,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     // after an expired wait: what was requested and not yet waited for
     if (t < T)
       for (int i = max(t - NS, 0); i < t; ++i) mbar_wait(&ms.full[i % NS], (i / NS) & 1, nullptr, nullptr);
-    zero_rows(p, lane, 32);
+    zero_rows<PASS>(p, lane, 32);
     } else if (warp == QB_LOAD) {
-      zero_rows(p, lane, 32);
+      zero_rows<PASS>(p, lane, 32);
     } else if (warp == QB_QUERY && T > 0) {
     // ---- query rows, as f16 with the factor that their scores take
     Cursor cur;
@@ -1044,6 +1068,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
 // queries 16 y .. + 15 of the item that starts in CTA b, two a warp.  The item's
 // first partial is CTA b's second one, the others are the first ones of the CTAs
 // after it.
+template <int PASS>
 __global__ void __launch_bounds__(256) q4_attn_tc_merge_kernel(const Q4AttnParams p, int n) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x;
   griddep_wait();
@@ -1055,9 +1080,11 @@ __global__ void __launch_bounds__(256) q4_attn_tc_merge_kernel(const Q4AttnParam
   for (int q = 16 * blockIdx.y + warp; q < 16 * blockIdx.y + 16; q += 8) {
     const int r = grp * n + q, j = p.by_g.of(r);
     if (item.w == 0 || j >= item.y) return;
-    float v[4];
-    merge_query(item.w, slot, n, q, lane, v);
-    store_out4(p, item.x + j, (item.z - grp * p.nkv) * G + r - j * G, 4 * lane, v);
+    float v[4], m, l;
+    merge_query(PASS == kAttnOwn ? item.w & (QB_PREFIX - 1) : item.w, slot, n, q, lane, v, &m, &l);
+    const int head = (item.z - grp * p.nkv) * G + r - j * G;
+    const Finish f = finish<PASS>(p, PASS == kAttnOwn && item.w >= QB_PREFIX, (size_t)(item.x + j) * p.nq + head, m, l);
+    finish4<PASS>(p, item.x + j, head, 4 * lane, v, f, m, l);
   }
 }
 
@@ -1079,25 +1106,32 @@ size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms) {
   return (size_t)num_sms * (2 * columns * 130 + sizeof(int4) / sizeof(float));
 }
 
-template <int N>
+template <int N, int PASS>
 static cudaError_t launch_tc(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
   using C = QbCfg<N>;
   constexpr size_t smem = C::MISC_OFF + sizeof(QbMisc<C>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
-  DFL_TRY(cudaFuncSetAttribute(q4_attn_tc_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  DFL_TRY(launch_pdl(q4_attn_tc_kernel<N>, dim3(num_sms), dim3(QB_THREADS), smem, st, p));
-  return launch_pdl(q4_attn_tc_merge_kernel, dim3(num_sms, C::CH), dim3(256), 0, st, p, N);
+  DFL_TRY(cudaFuncSetAttribute(q4_attn_tc_kernel<N, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  DFL_TRY(launch_pdl(q4_attn_tc_kernel<N, PASS>, dim3(num_sms), dim3(QB_THREADS), smem, st, p));
+  return launch_pdl(q4_attn_tc_merge_kernel<PASS>, dim3(num_sms, C::CH), dim3(256), 0, st, p, N);
 }
 
-cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
-  if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
+template <int PASS>
+static cudaError_t launch_pass(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
   switch (q4_attn_tc_columns(p.max_rows, p.nq, p.nkv)) {
-    case 32: return launch_tc<32>(p, num_sms, st);
-    case 48: return launch_tc<48>(p, num_sms, st);
-    case 64: return launch_tc<64>(p, num_sms, st);
-    case 80: return launch_tc<80>(p, num_sms, st);
+    case 32: return launch_tc<32, PASS>(p, num_sms, st);
+    case 48: return launch_tc<48, PASS>(p, num_sms, st);
+    case 64: return launch_tc<64, PASS>(p, num_sms, st);
+    case 80: return launch_tc<80, PASS>(p, num_sms, st);
   }
   return cudaErrorInvalidValue;
+}
+
+cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int pass, int num_sms, cudaStream_t st) {
+  if (p.n < 1 || p.n > kPagedMaxSeqs) return cudaErrorInvalidValue;
+  return pass == kAttnAll      ? launch_pass<kAttnAll>(p, num_sms, st)
+         : pass == kAttnPrefix ? launch_pass<kAttnPrefix>(p, num_sms, st)
+                               : launch_pass<kAttnOwn>(p, num_sms, st);
 }
 
 }  // namespace dfl

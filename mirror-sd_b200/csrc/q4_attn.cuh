@@ -51,6 +51,22 @@ __device__ __forceinline__ bool rows_fit(const Q4AttnParams& p, int i) {
   const int a = __ldg(p.starts + i), b = __ldg(p.starts + i + 1);
   return a >= 0 && a <= b && b <= p.T && b - a <= p.max_rows;
 }
+// the block table's entry for a column of request i
+template <int PASS>
+__device__ __forceinline__ int table_entry(const Q4AttnParams& p, int i, int column) {
+  // (device data the host has not seen: stay inside the table)
+  if (PASS == kAttnPrefix) i = min(max(__ldg(p.row_of + i), 0), p.table_rows - 1);
+  if (PASS == kAttnOwn) {
+    column += __ldg(p.skip + i);
+    if (column < 0 || column >= p.max_pages) return -1;
+  }
+  return __ldg(p.table + (size_t)i * p.table_ld + column);
+}
+// whether an earlier pass has left request i's sums over its group's rows
+template <int PASS>
+__device__ __forceinline__ bool has_prefix(const Q4AttnParams& p, int i) {
+  return PASS == kAttnOwn && __ldg(p.skip + i) > 0;
+}
 template <int TILE, int QT>
 __device__ __forceinline__ Item load_item(const Q4AttnParams& p, int i) {
   Item it;
@@ -62,14 +78,29 @@ __device__ __forceinline__ Item load_item(const Q4AttnParams& p, int i) {
   it.groups = it.ntile > 0 ? (it.rows * p.by_g.d + QT - 1) / QT : 0;
   return it;
 }
-// The rows of requests without a cached row belong to no tile: zeros, from
-// thread t of `threads` of every CTA, which share the requests out.
+// The rows of requests without a cached row belong to no tile: zeros (or what the
+// pass over their group's rows left), from thread t of `threads` of every CTA,
+// which share the requests out.
+template <int PASS>
 __device__ __forceinline__ void zero_rows(const Q4AttnParams& p, int t, int threads) {
+  if (PASS == kAttnPrefix) return;
 #pragma unroll 1
   for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
     if (__ldg(p.lens + i) > 0) continue;
     int row0;
     const int rows = seq_rows(p, i, &row0);
+    if (PASS == kAttnOwn && has_prefix<PASS>(p, i)) {
+#pragma unroll 1
+      for (long long e = t; e < (long long)rows * p.nq * 32; e += threads) {   // 4 channels each
+        const size_t at = (size_t)row0 * p.nq + (e >> 5);
+        const float l = __ldcg(p.pre_ml + at).y, f = l == 0.f ? 0.f : 16.f / l;
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(p.pre_o + at * 128) + (e & 31));
+        const uint2 w = p.bf16 ? make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f))
+                               : make_uint2(pack_f16x2(o.x * f, o.y * f), pack_f16x2(o.z * f, o.w * f));
+        reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * 128)[e & 31] = w;
+      }
+      continue;
+    }
     uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + (size_t)row0 * p.nq * 128);
 #pragma unroll 1
     for (int e = t; e < rows * p.nq * 16; e += threads) out[e] = make_uint4(0, 0, 0, 0);
@@ -177,12 +208,32 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// What an item's sums O (16 times too small), statistics m and l are multiplied
+// by for the output row at `at` (row * NQ + head), and what goes with the sums
+// that the pass over its group's rows left there (prefix: whether it did).
+struct Finish {
+  float own, pre;
+};
+template <int PASS>
+__device__ __forceinline__ Finish finish(const Q4AttnParams& p, bool prefix, size_t at, float m, float l) {
+  if (PASS == kAttnPrefix) return {1.f, 0.f};
+  if (PASS == kAttnOwn && prefix) {
+    const float2 a = __ldcg(p.pre_ml + at);
+    const float M = fmaxf(m, a.x);
+    const float wo = m == -INFINITY ? 0.f : exp2_fast(m - M), wp = a.x == -INFINITY ? 0.f : exp2_fast(a.x - M);
+    const float sum = fmaf(wo, l, wp * a.y), f = sum == 0.f ? 0.f : 16.f / sum;
+    return {wo * f, wp * f};
+  }
+  return {l == 0.f ? 0.f : 16.f / l, 0.f};
+}
+
 // A warp merges one query's partials of `count` runs: slots(k) holds O at
 // q * 128, m at qt * 128 + q and l at qt * 129 + q.  Returns channels 4 lane ..
-// of the output row.  8 loads of O are on their way together, the first ones
+// of the sums and the statistics.  8 loads of O are on their way together, the first ones
 // with those of m and l: few partials cost one round trip to L2.
 template <class SlotAt>
-__device__ __forceinline__ void merge_query(int count, SlotAt slots, int qt, int q, int lane, float (&v)[4]) {
+__device__ __forceinline__ void merge_query(int count, SlotAt slots, int qt, int q, int lane, float (&v)[4], float* M_out,
+                                            float* l_out) {
   float4 x[8];
   auto load = [&](int k) {
 #pragma unroll
@@ -227,9 +278,9 @@ __device__ __forceinline__ void merge_query(int count, SlotAt slots, int qt, int
       }
     }
   }
-  l = warp_sum(l);
-  const float f = l == 0.f ? 0.f : 16.f / l;
-  for (int i = 0; i < 4; ++i) v[i] = o[i] * f;
+  *l_out = warp_sum(l);
+  *M_out = M;
+  for (int i = 0; i < 4; ++i) v[i] = o[i];
 }
 
 // write 4 consecutive output values of one query row
@@ -238,6 +289,27 @@ __device__ __forceinline__ void store_out4(const Q4AttnParams& p, int row, int h
   const uint2 w = p.bf16 ? make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]))
                          : make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + off) = w;
+}
+// Write 4 consecutive sums o of one query row, finished with f, or (kAttnPrefix) as
+// they are with the statistics beside them (from the thread with d = 0).
+template <int PASS>
+__device__ __forceinline__ void finish4(const Q4AttnParams& p, int row, int head, int d, const float (&o)[4], Finish f, float m,
+                                        float l) {
+  const size_t at = (size_t)row * p.nq + head;
+  if (PASS == kAttnPrefix) {
+    *reinterpret_cast<float4*>(p.pre_o + at * 128 + d) = make_float4(o[0], o[1], o[2], o[3]);
+    if (d == 0) p.pre_ml[at] = make_float2(m, l);
+    return;
+  }
+  float v[4] = {o[0] * f.own, o[1] * f.own, o[2] * f.own, o[3] * f.own};
+  if (PASS == kAttnOwn && f.pre != 0.f) {
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.pre_o + at * 128 + d));
+    v[0] = fmaf(a.x, f.pre, v[0]);
+    v[1] = fmaf(a.y, f.pre, v[1]);
+    v[2] = fmaf(a.z, f.pre, v[2]);
+    v[3] = fmaf(a.w, f.pre, v[3]);
+  }
+  store_out4(p, row, head, d, v);
 }
 
 }  // namespace dfl

@@ -189,6 +189,83 @@ def q4_attention(q, pool, table, lens, starts=None, max_rows: int = 1, causal: b
                                     HEAD_DIM ** -0.5 if scale is None else scale, out, status, workspace)
 
 
+class PrefixPlan(NamedTuple):
+    """What ``paged_prefix_plan`` found, for all layers of a step: per group its
+    first packed row, the rows that its members share and whose table row names
+    them; per request the pages of those rows and its own rows behind them; and
+    what the plan was made for."""
+    group_starts: torch.Tensor
+    prefix: torch.Tensor
+    row_of: torch.Tensor
+    skip: torch.Tensor
+    own_lens: torch.Tensor
+    starts: Optional[torch.Tensor]
+    max_rows: int
+    max_group: int
+    page_size: int
+    causal: bool
+
+
+def paged_prefix_plan(table, lens, groups, page_size: int, starts=None, max_rows: int = 1, causal: bool = False,
+                      max_group: Optional[int] = None) -> PrefixPlan:
+    """Which cached rows the requests of each group share, found by comparing
+    their rows of the block table on the device: whole pages that all members with
+    query rows begin with and whose rows all their query rows see.  groups: the
+    sizes of consecutive runs of requests, or an int32 device tensor of their
+    boundaries [g + 1] with ``max_group``, the requests of a group at most.  A group
+    that shares nothing costs little; requests of no group are on their own.  lens,
+    starts, max_rows and causal as for ``q4_attention``."""
+    if not torch.is_tensor(groups):
+        sizes = [int(s) for s in groups]
+        if not sizes or any(s < 1 for s in sizes) or sum(sizes) > lens.numel():
+            raise ValueError(f"groups must be positive sizes of {lens.numel()} requests at most, got {sizes}")
+        bounds = [0]
+        for s in sizes:
+            bounds.append(bounds[-1] + s)
+        max_group = max(sizes) if max_group is None else max_group
+        if lens.is_cuda and N.load_paged().capturing(lens.device.index):
+            raise ValueError("groups must be on the device in a CUDA graph, whose replays cannot read the host's")
+        groups = torch.tensor(bounds, dtype=torch.int32).to(lens.device, non_blocking=True)
+    elif max_group is None:
+        raise ValueError("max_group is needed with groups on the device")
+    return PrefixPlan(*N.load_paged().prefix_plan(table, lens, starts, max_rows, page_size, groups, causal), starts, max_rows,
+                      max_group, page_size, bool(causal))
+
+
+def _prefix_workspace_size(rows, max_rows, max_group, num_heads, num_kv_heads, device) -> int:
+    with torch.cuda.device(device):
+        size = N.load().dflash_q4_prefix_workspace_size(rows, max_rows, max_group, num_heads, num_kv_heads)
+    if size == 0:
+        raise ValueError(f"no such attention: {rows} rows, groups of {max_group} x {max_rows}, {num_heads} / {num_kv_heads} heads")
+    return size
+
+
+def q4_prefix_workspace(rows: int, max_rows: int, max_group: int, num_heads: int, num_kv_heads: int, device="cuda") -> torch.Tensor:
+    """Workspace of ``q4_prefix_attention`` for up to ``rows`` query rows in all,
+    ``max_rows`` a request and ``max_group`` requests a group; it may serve any
+    number of calls that do not overlap."""
+    device = torch.device(device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return torch.zeros(_prefix_workspace_size(rows, max_rows, max_group, num_heads, num_kv_heads, device), dtype=torch.uint8,
+                       device=device)
+
+
+def q4_prefix_attention(q, pool, table, plan: PrefixPlan, scale: Optional[float] = None, out=None, status=None, workspace=None):
+    """``q4_attention`` (without a window) of the requests that ``plan`` was made
+    for: the rows that a group shares are read once for all its query rows, each
+    request's own rows for its own, and both are joined in fp32."""
+    if pool.dim() != 4 or q.dim() != 3:
+        raise ValueError("q must be [rows, heads, 128] and pool a tensor from q4_pool()")
+    if pool.shape[2] * 16 != plan.page_size:
+        raise ValueError(f"the plan is for pages of {plan.page_size} rows, the pool's have {pool.shape[2] * 16}")
+    if workspace is None:
+        workspace = q4_prefix_workspace(q.shape[0], plan.max_rows, plan.max_group, q.shape[1], pool.shape[1], pool.device)
+    return N.load_paged().prefix_attention(q, pool, table, plan.starts, plan.max_rows, plan.group_starts, plan.prefix, plan.row_of,
+                                           plan.max_group, plan.skip, plan.own_lens, plan.causal,
+                                           HEAD_DIM ** -0.5 if scale is None else scale, out, status, workspace)
+
+
 class PagedKVCacheQ4:
     """Cache of ``max_seqs`` requests over ``num_layers`` layers.  Every
     method enqueues on the current stream; none waits for the device except
@@ -327,18 +404,32 @@ class PagedKVCacheQ4:
         self._on_stream()
         q4_append(k, v, step.slots, self.pools[layer], self.status)
 
+    def prefix_plan(self, step: PagedStep, groups: Union[torch.Tensor, Sequence[int]], max_rows: int, causal: bool = True,
+                    max_group: Optional[int] = None) -> PrefixPlan:
+        """For ``attend``, once a step: the rows that consecutive requests share
+        (``paged_prefix_plan``; groups are their numbers, as forks of one prompt lie
+        side by side)."""
+        self._enter()
+        return paged_prefix_plan(self.table, self.lens, groups, self.page_size, step.starts, max_rows, causal, max_group)
+
     def attend(self, layer: int, q, step: PagedStep, max_rows: int, causal: bool = True, sink: int = 0,
-               window: int = 0, scale: Optional[float] = None, out=None, workspace=None):
-        """Attention of the step's query rows over everything cached.  Without a
-        ``workspace`` (``q4_attention_workspace``) the object uses one of its own
-        for each stream; a call that is captured in a CUDA graph gets one of the
-        graph's, zeroed at every replay."""
+               window: int = 0, scale: Optional[float] = None, out=None, workspace=None, plan: Optional[PrefixPlan] = None):
+        """Attention of the step's query rows over everything cached; with a
+        ``plan`` of the step, what its groups share is read once for all of them.
+        Without a ``workspace`` (``q4_attention_workspace``, ``q4_prefix_workspace``)
+        the object uses one of its own for each stream; a call that is captured in
+        a CUDA graph gets one of the graph's, zeroed at every replay."""
         stream = self._enter()
+        if plan is not None and (sink or window or max_rows != plan.max_rows or bool(causal) != plan.causal):
+            raise ValueError("a plan goes with the max_rows and causal that it was made for, and without a window")
         if workspace is None:
-            key = (max_rows, q.shape[1])
+            # (prefix attention keeps sums of every row: sizes by the next power of two)
+            key = (max_rows, q.shape[1]) if plan is None else (1 << max(q.shape[0] - 1, 0).bit_length(), max_rows, plan.max_group,
+                                                               q.shape[1])
             size = self._sizes.get(key)
             if size is None:
-                size = self._sizes[key] = _workspace_size(*key, self.nkv, self.device)
+                of = _workspace_size if plan is None else _prefix_workspace_size
+                size = self._sizes[key] = of(*key, self.nkv, self.device)
             # A graph may be replayed on any stream, beside eager calls and other graphs, and long after a larger
             # workspace has taken this one's place: it shares none with them.
             own = None if self.capturable and self._capturing() else self._workspace
@@ -347,6 +438,8 @@ class PagedKVCacheQ4:
                 workspace = torch.zeros(size, dtype=torch.uint8, device=self.device)
                 if own is not None:
                     own[stream] = workspace
+        if plan is not None:
+            return q4_prefix_attention(q, self.pools[layer], self.table, plan, scale, out, self.status, workspace)
         return q4_attention(q, self.pools[layer], self.table, self.lens, step.starts, max_rows, causal, sink, window,
                             scale, out, self.status, workspace)
 

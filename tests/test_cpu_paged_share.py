@@ -115,3 +115,54 @@ def test_restatement_keeps_rows_apart():
             s.lens = [0 if rng.random() < 0.2 else a for a in s.lens]
         s.release([0] * 7)
         assert s.head == 0 and sorted(s.free) == list(range(60))
+
+
+def test_prefix_attention_refuses_bad_arguments(pkg, lib):
+    def plan(table=P, ld=8, lens=P, n=4, max_rows=1, page=16, groups=P, g=2, own=Q):
+        return lib.dflash_paged_prefix_plan(table, ld, 8, lens, None, n, max_rows, page, groups, g, 1, P, P, P, P, own, None)
+
+    for kw in (dict(table=None), dict(lens=None), dict(groups=None), dict(own=None)):
+        _refused(pkg, plan(**kw), "NULL")
+    _refused(pkg, plan(ld=7), "table_ld")
+    _refused(pkg, plan(n=0), "n 0")
+    _refused(pkg, plan(max_rows=0), "max_rows")
+    _refused(pkg, plan(max_rows=65537), "max_rows")
+    _refused(pkg, plan(g=0), "groups")
+    _refused(pkg, plan(g=2049), "groups")
+    _refused(pkg, plan(own=P), "own_lens")
+
+    size = lib.dflash_q4_prefix_workspace_size
+    assert size(100, 1, 8, 32, 8) >= 100 * 32 * 130 * 4 + lib.dflash_q4_attention_workspace_size(8, 32, 8)
+    for bad in ((-1, 1, 8, 32, 8), (4, 0, 8, 32, 8), (4, 1, 0, 32, 8), (4, 1, 8, 7, 2), (4, 64, 1025, 8, 8), (2 ** 30, 1, 1, 8, 8)):
+        assert size(*bad) == 0
+
+    def attend(q=P, row=1024, ws=P, nbytes=1 << 40, starts=P, n=4, rows=4, max_rows=1, g=1, max_group=4, nq=8, nkv=2, scale=0.1,
+               prefix=P, out=ctypes.c_void_p(1 << 30), page=16):
+        return lib.dflash_q4_prefix_attention(q, row, 128, 0, P, 16, page, P, 8, 8, starts, n, rows, max_rows, P, prefix, P, g,
+                                              max_group, P, P, nq, nkv, 1, scale, out, None, ws, nbytes, None)
+
+    for kw in (dict(q=None), dict(ws=None), dict(prefix=None), dict(out=None)):
+        _refused(pkg, attend(**kw), "NULL")
+    _refused(pkg, attend(g=0), "groups")
+    _refused(pkg, attend(max_group=0), "groups of 0")
+    _refused(pkg, attend(max_group=2048, max_rows=64), "groups of 2048")
+    _refused(pkg, attend(rows=3, starts=None), "without starts")
+    _refused(pkg, attend(nq=7), "multiple")
+    _refused(pkg, attend(scale=0.0), "positive")
+    _refused(pkg, attend(row=1028), "strides")
+    _refused(pkg, attend(page=20), "page_size")
+    _refused(pkg, attend(ws=ctypes.c_void_p(4104)), "workspace")
+    _refused(pkg, attend(nbytes=1000), "workspace too small")
+    _refused(pkg, attend(out=P), "overlaps")
+    assert attend(rows=0) == 0
+
+
+def test_prefix_plan_refuses_bad_groups(pkg):
+    table, lens = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    for groups in ([], [0, 4], [3, 2], [-1]):
+        with pytest.raises(ValueError, match="groups"):
+            pkg.paged_prefix_plan(table, lens, groups, 16)
+    with pytest.raises(ValueError, match="max_group"):
+        pkg.paged_prefix_plan(table, lens, lens, 16)
+    with pytest.raises(ValueError):
+        pkg.paged_prefix_plan(table, lens, [4], 16)          # tensors on the CPU
