@@ -71,7 +71,7 @@ constexpr size_t kCounterBytes = 4096;   // two counters per SM, then the partia
 int attention_params(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages, int page_size,
                      const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens, const int32_t* starts, int n,
                      int rows, int max_rows, int nq, int nkv, int causal, int sink, int window, float scale, uint16_t* out,
-                     int32_t* status, Q4AttnParams* params, bool* few) {
+                     int32_t* status, int item_units, Q4AttnParams* params, bool* few) {
   if (int rc = check_paging(n, page_size, table_ld, max_pages, num_pages)) return rc;
   if (int rc = check_pool(rows, nkv, pool, num_pages, page_size)) return rc;
   // (the kernels add a tile, a window or the query rows to a position in 32 bits)
@@ -97,7 +97,8 @@ int attention_params(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16,
     return fail(DFLASH_ERR_INVALID, "%d query heads a kv head, %d kv heads, %d rows: too many", G, nkv, max_rows);
   // Tiles of all items together are counted in 32 bits: a full table for each
   // group of query rows, of which every request with rows has one in part.
-  const double units = std::ceil((double)max_pages * page_size / (*few ? kQ4Tile : kQ4TcTile)) * nkv *
+  // (and what the passes over shared and own rows add to an item)
+  const double units = (std::ceil((double)max_pages * page_size / (*few ? kQ4Tile : kQ4TcTile)) + item_units) * nkv *
                        ((double)rows * G / columns + (n < rows ? n : rows));
   if ((long long)rows * nq > INT32_MAX) return fail(DFLASH_ERR_INVALID, "rows x nq must stay below 2^31");
   if (units >= INT32_MAX) return fail(DFLASH_ERR_INVALID, "n x table x heads x rows is too large for one call");
@@ -333,7 +334,7 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
   Q4AttnParams p;
   bool few;
   if (int rc = attention_params(q, q_row, q_head, bf16, pool, num_pages, page_size, table, table_ld, max_pages, lens, starts, n,
-                                rows, max_rows, nq, nkv, causal, sink, window, scale, out, status, &p, &few))
+                                rows, max_rows, nq, nkv, causal, sink, window, scale, out, status, 0, &p, &few))
     return rc;
   if (!aligned16(workspace))
     return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");
@@ -389,11 +390,11 @@ int dflash_q4_prefix_attention(const uint16_t* q, int64_t q_row, int64_t q_head,
   Q4AttnParams group, own;
   bool few_group, few_own;
   if (int rc = attention_params(q, q_row, q_head, bf16, pool, num_pages, page_size, table, table_ld, max_pages, own_lens, starts,
-                                n, rows, max_rows, nq, nkv, causal, 0, 0, scale, out, status, &own, &few_own))
+                                n, rows, max_rows, nq, nkv, causal, 0, 0, scale, out, status, kQ4ItemUnits, &own, &few_own))
     return rc;
   if (int rc = attention_params(q, q_row, q_head, bf16, pool, num_pages, page_size, table, table_ld, max_pages, prefix,
                                 group_starts, num_groups, rows, max_rows * max_group, nq, nkv, 0, 0, 0, scale, out, status,
-                                &group, &few_group))
+                                kQ4ItemUnits, &group, &few_group))
     return rc;
   if (!aligned16(workspace))
     return fail(DFLASH_ERR_INVALID, "q, out and workspace must be 16-byte aligned, q's strides whole 16 bytes");

@@ -169,6 +169,7 @@ enum AttnPass : int { kAttnAll = 0, kAttnPrefix = 1, kAttnOwn = 2 };
 // Each kernel cuts a request's rows of a kv head into groups of `columns`, and
 // its cached rows into tiles.
 constexpr int kQ4Tile = 64, kQ4TcTile = 128;
+constexpr int kQ4ItemUnits = 8;        // at least what either kernel adds to an item where it weighs items
 int q4_attn_columns(int max_rows, int nq, int nkv);
 int q4_attn_tc_columns(int max_rows, int nq, int nkv);
 size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms);

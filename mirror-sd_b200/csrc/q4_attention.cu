@@ -52,6 +52,7 @@ constexpr int QA_STAGE = QA_TILE / kQ4Rows * kQ4Block;
 // over more CTAs, whose partials the last one merges (2,049 rows: 13.3 us with 1,
 // 11.7 with 2, 11.4 with 4, 12.3 with 8).
 constexpr int QA_LEAST = 4;
+constexpr int QA_ITEM = 3;                           // what an item's start and end cost beside its tiles, in tiles
 constexpr float QA_RAISE = 8.f;
 
 // ---- fragments
@@ -116,22 +117,23 @@ __device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask
     dst[QT * 128 + q] = M;
     dst[QT * 129 + q] = l;
   }
+  constexpr int END = PASS == kAttnPrefix ? kAttnPrefix : kAttnAll;   // (own rows went on from the group's)
   const int grp = p.by_nkv.of(sub), head0 = (sub - grp * p.nkv) * p.by_g.d;
   Finish fin{0.f, 0.f};
   if (whole) {
     const int r = grp * QT + q, j = p.by_g.of(r);
     if (j < it.rows)
-      fin = finish<PASS>(p, has_prefix<PASS>(p, it.seq), (size_t)(it.row0 + j) * p.nq + head0 + r - j * p.by_g.d, M, l);
+      fin = finish<END>(p, false, 0, M, l);
   }
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     if (whole) {
-      const Finish f{__shfl_sync(0xffffffffu, fin.own, i), PASS == kAttnOwn ? __shfl_sync(0xffffffffu, fin.pre, i) : 0.f};
+      const Finish f{__shfl_sync(0xffffffffu, fin.own, i), 0.f};
       const float mi = PASS == kAttnPrefix ? __shfl_sync(0xffffffffu, M, i) : 0.f;
       const float li = PASS == kAttnPrefix ? __shfl_sync(0xffffffffu, l, i) : 0.f;
       const int r = grp * QT + i, j = p.by_g.of(r);
       const float v[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
-      if (j < it.rows) finish4<PASS>(p, it.row0 + j, head0 + r - j * p.by_g.d, 4 * lane, v, f, mi, li);
+      if (j < it.rows) finish4<END>(p, it.row0 + j, head0 + r - j * p.by_g.d, 4 * lane, v, f, mi, li);
     } else {
       *reinterpret_cast<float4*>(dst + i * 128 + 4 * lane) = o[i];
     }
@@ -142,9 +144,15 @@ template <int NT, int PASS>
 __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4AttnParams p) {
   using C = QaCfg<NT>;
   constexpr int QT = C::QT;
+  constexpr int END = PASS == kAttnPrefix ? kAttnPrefix : kAttnAll;
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING);          // [warp][stage]
   int* base = reinterpret_cast<int*>(bars + C::WARPS * C::STAGES);       // [n + 1] first tile of each request
+  // Passes over shared and own rows weigh an item's start and end as well, QA_ITEM
+  // tiles, where there are items for every warp: an item is then that many units
+  // followed by its tiles, and runs are cut by units.
+  int W = PASS == kAttnAll ? 0 : QA_ITEM;
+  int* ubase = base + p.n + 1;                                           // [n] first unit of each request
   __shared__ int wtot[C::WARPS];
   __shared__ int slot_item[2 * C::WARPS];   // unit at which the partial's item starts, or -1
   __shared__ Item slot_info[2 * C::WARPS];
@@ -164,15 +172,8 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
   griddep_wait();
   griddep_launch_dependents();
   // tiles of every request, added up (kPagedMaxSeqs / C::THREADS passes at most)
-  int total = 0;
-  for (int i0 = 0; i0 < p.n; i0 += C::THREADS) {
-    const int i = i0 + threadIdx.x;
-    int v = 0;
-    if (i < p.n) {
-      const Item it = load_item<QA_TILE, QT>(p, i);
-      v = it.ntile * it.groups * p.nkv;
-      if (blockIdx.x == 0 && p.status && !rows_fit(p, i)) atomicOr(p.status, kPagedRows);
-    }
+  int total = 0, units = 0;
+  auto add_up = [&](int i, int v, int* first, int& total) {
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -188,9 +189,22 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
       if (w < warp) before = tiles_sum(before, wtot[w]);
       total = tiles_sum(total, wtot[w]);
     }
-    if (i < p.n) base[i] = tiles_sum(before, x - v);
+    if (i < p.n) first[i] = tiles_sum(before, x - v);
+  };
+  for (int i0 = 0; i0 < p.n; i0 += C::THREADS) {
+    const int i = i0 + threadIdx.x;
+    int v = 0, w = 0;
+    if (i < p.n) {
+      const Item it = load_item<QA_TILE, QT>(p, i);
+      v = it.ntile * it.groups * p.nkv;
+      w = (it.ntile + W) * it.groups * p.nkv;
+      if (blockIdx.x == 0 && p.status && !rows_fit(p, i)) atomicOr(p.status, kPagedRows);
+    }
+    add_up(i, v, base, total);
+    if (W > 0) add_up(i, w, ubase, units);
   }
-  if (total == kTilesFull) total = 0;
+  if (total == kTilesFull || units == kTilesFull) total = units = 0;
+  if (PASS != kAttnAll && units - total < QA_ITEM * (int)gridDim.x * C::WARPS) W = 0;
   if (threadIdx.x == 0) base[p.n] = total;
   __syncthreads();
 
@@ -200,10 +214,26 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     zero_rows<PASS>(p, threadIdx.x, C::THREADS);
     return;
   }
-  const Runs runs(total, ctas);
-  const int c0 = runs.start(cta), c1 = runs.start(cta + 1);
-  const Runs mine(c1 - c0, C::WARPS);
-  const int u0 = c0 + mine.start(warp), u1 = c0 + mine.start(warp + 1);
+  const Runs runs(W > 0 ? units : total, ctas);
+  // the first tile at or behind a unit
+  auto tile_at = [&](int unit) {
+    if (W == 0) return unit;
+    if (unit >= units) return total;
+    int lo = 0, hi = p.n - 1;
+    while (lo < hi) {   // last request whose first unit is at most that
+      const int mid = (lo + hi + 1) >> 1;
+      if (ubase[mid] <= unit) lo = mid; else hi = mid - 1;
+    }
+    const int nt = load_item<QA_TILE, QT>(p, lo).ntile, k = (unit - ubase[lo]) / (nt + W);
+    return base[lo] + k * nt + max(unit - ubase[lo] - k * (nt + W) - W, 0);
+  };
+  // the unit of an item's first tile
+  auto unit_of = [&](const Item& it, int item0) {
+    return W == 0 ? item0 : ubase[it.seq] + (item0 - base[it.seq]) / it.ntile * (it.ntile + W) + W;
+  };
+  const int cta_unit = runs.start(cta), c0 = tile_at(cta_unit), c1 = tile_at(runs.start(cta + 1));
+  const Runs mine(runs.start(cta + 1) - cta_unit, C::WARPS);
+  const int u0 = tile_at(cta_unit + mine.start(warp)), u1 = tile_at(cta_unit + mine.start(warp + 1));
 
   if (u0 < u1) {
     uint8_t* ring = smem + warp * C::STAGES * QA_STAGE;
@@ -308,6 +338,32 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[t][nt][x] = 0.f;
+        if (PASS == kAttnOwn && cur.j == 0 && has_prefix<PASS>(p, cur.it.seq)) {
+          // the item's first tile goes on from what the pass over its group's rows left
+          // (joined at the item's end instead, 256 requests of 512 rows took 97 us, not 62)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int r = r0 + nt * 8 + 2 * c + x, j = p.by_g.of(r);
+              if (j >= cur.it.rows) continue;
+              const size_t at = (size_t)(cur.it.row0 + j) * p.nq + head0 + r - j * G;
+              const float2 ml = __ldcg(p.pre_ml + at);
+              const float* src = p.pre_o + at * 128 + 16 * g;
+#pragma unroll
+              for (int t = 0; t < 8; t += 2) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(src + 2 * t));
+                o[t][nt][x] = v.x;
+                o[t][nt][2 + x] = v.y;
+                o[t + 1][nt][x] = v.z;
+                o[t + 1][nt][2 + x] = v.w;
+              }
+              if (ml.x != -INFINITY) {
+                negm[nt][x] = -ml.x / qscale[nt][x];
+                l[nt][x] = g == 0 ? ml.y : 0.f;
+              }
+            }
+        }
       }
 
       const uint32_t have = (loaded >> (4 * stage)) & 15u;
@@ -469,17 +525,16 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
           for (int x = 0; x < 2; ++x) {
             const float sum = col_sum(l[nt][x]);
             const int q = nt * 8 + 2 * c + x, r = r0 + q, j = p.by_g.of(r);
-            const float m = PASS == kAttnAll ? 0.f : partial_max(negm[nt][x], qscale[nt][x]);
+            const float m = PASS != kAttnPrefix ? 0.f : partial_max(negm[nt][x], qscale[nt][x]);
             Finish f{1.f, 0.f};
-            if (whole && j < cur.it.rows)
-              f = finish<PASS>(p, has_prefix<PASS>(p, cur.it.seq), (size_t)(cur.it.row0 + j) * p.nq + G0 + r - j * G, m, sum);
+            if (whole && j < cur.it.rows) f = finish<END>(p, false, 0, m, sum);
 #pragma unroll
             for (int t = 0; t < 8; t += 2) {
               const float v[4] = {o[t][nt][x], o[t][nt][2 + x], o[t + 1][nt][x], o[t + 1][nt][2 + x]};
               if (!whole)
                 *reinterpret_cast<float4*>(part + q * 128 + 16 * g + 2 * t) = make_float4(v[0], v[1], v[2], v[3]);
               else if (j < cur.it.rows)
-                finish4<PASS>(p, cur.it.row0 + j, G0 + r - j * G, 16 * g + 2 * t, v, f, m, sum);
+                finish4<END>(p, cur.it.row0 + j, G0 + r - j * G, 16 * g + 2 * t, v, f, m, sum);
             }
             if (!whole && g == 0) {
               part[QT * 128 + q] = partial_max(negm[nt][x], qscale[nt][x]);
@@ -522,8 +577,8 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
         __syncwarp();
         if (lane == 0) {
           // CTAs that hold part of the item: counted at the one holding its first tile
-          const int from = runs.of(item0);
-          const int to = runs.of(item0 + it.ntile - 1);
+          const int from = runs.of(unit_of(it, item0));
+          const int to = runs.of(unit_of(it, item0) + it.ntile - 1);
           if (atomicAdd(&p.counters[from], 1) == to - from) {
             p.counters[from] = 0;   // for the next call
             __threadfence();
@@ -540,7 +595,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
     __threadfence();
     const int item0 = slot_item[first], sub = slot_sub[first];
     const Item it = slot_info[first];
-    const int from = runs.of(item0), to = runs.of(item0 + it.ntile - 1);
+    const int from = runs.of(unit_of(it, item0)), to = runs.of(unit_of(it, item0) + it.ntile - 1);
     // the first CTA holds the item's start, at its right border; the others have it at their left one
 #pragma unroll 1
     for (int q = warp; q < QT; q += C::WARPS) {
@@ -550,8 +605,8 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
       merge_query(to - from + 1, [&](int k) { return cta_part + ((size_t)(from + k) * 2 + (k == 0 ? 1 : 0)) * C::SLOT; }, QT,
                   q, lane, v, &m, &l);
       const int head = (sub - grp * p.nkv) * G + r - j * G;
-      const Finish f = finish<PASS>(p, has_prefix<PASS>(p, it.seq), (size_t)(it.row0 + j) * p.nq + head, m, l);
-      finish4<PASS>(p, it.row0 + j, head, 4 * lane, v, f, m, l);
+      const Finish f = finish<END>(p, false, 0, m, l);
+      finish4<END>(p, it.row0 + j, head, 4 * lane, v, f, m, l);
     }
   }
   zero_rows<PASS>(p, threadIdx.x, C::THREADS);
@@ -567,7 +622,7 @@ size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms) {
 
 template <int NT, int PASS>
 static cudaError_t launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
-  const size_t smem = QaCfg<NT>::RING + QaCfg<NT>::WARPS * QaCfg<NT>::STAGES * 8 + ((size_t)p.n + 1) * 4;
+  const size_t smem = QaCfg<NT>::RING + QaCfg<NT>::WARPS * QaCfg<NT>::STAGES * 8 + ((size_t)p.n + 1) * (PASS == kAttnAll ? 4 : 8);
   DFL_TRY(cudaFuncSetAttribute(q4_attn_kernel<NT, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   return launch_pdl(q4_attn_kernel<NT, PASS>, dim3(num_sms), dim3(QaCfg<NT>::THREADS), smem, st, p);
 }

@@ -54,6 +54,7 @@ constexpr int QB_BLK = kQ4Block + 32;      // a row block's stride in shared mem
 constexpr int QB_STAGE = QB_TILE / kQ4Rows * QB_BLK;
 constexpr int QB_SEEN = 256;               // flag of a tile that every query of the item sees whole
 constexpr int QB_PREFIX = 1 << 16;         // beside an item's number of CTAs: there are sums over its group's rows
+constexpr int QB_ITEM = 6;                 // what an item's start and end cost beside its tiles, in tiles (9 to 11 us, 5 at 32 columns)
 constexpr int QB_SLACK = 6;
 constexpr float QB_RAISE = 8.f;
 
@@ -322,6 +323,13 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     return tiles_sum(before, x - v);
   };
   const int grid = gridDim.x;
+  // Passes over shared and own rows weigh an item's start and end as well, QB_ITEM
+  // tiles, where there are items for every CTA: an item is then that many units
+  // followed by its tiles, and runs are cut by units.  (Own rows of 64 requests, 16
+  // to 1,024 of them: 190 us by tiles, 88 by units; one group of 8 x 2,048 rows: 14
+  // by tiles, 20 by units.)
+  constexpr int W = PASS == kAttnAll ? 0 : QB_ITEM;
+  int units = 0, c1_unit = 0;   // of all items; where the CTA's run ends
   int total = 0, c0 = 0, c1 = 0, items = 0, ntile = 0, first = 0;   // (the last three of request threadIdx.x)
 #pragma unroll 1
   for (int i0 = 0; i0 < p.n; i0 += QB_THREADS) {
@@ -336,8 +344,13 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     int sum;
     first = scan(items * ntile, &sum);
     total = tiles_sum(total, sum);
+    if (W > 0) {
+      scan(items * (ntile + W), &sum);
+      units = tiles_sum(units, sum);
+    }
   }
-  if (total == kTilesFull) total = 0;
+  if (total == kTilesFull || units == kTilesFull) total = units = 0;
+  const bool weigh = W > 0 && units - total >= W * grid;
   // With few items, whole CTAs to each: a run that crosses from one item into the
   // next pays the start and the end of an item (6 to 8 us together) twice.  An
   // item takes a CTA for every `quota` of its tiles, the least number with which
@@ -367,6 +380,37 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       ms.run[1] = item0 + runs.start(part + 1);
       ms.share = parts;
     }
+  } else if (weigh) {
+    const Runs runs(units, min(grid, total));
+    const int u0 = runs.start(min((int)blockIdx.x, min(grid, total))), u1 = runs.start(min((int)blockIdx.x + 1, min(grid, total)));
+    c1_unit = u1;
+    int tiles_before = 0, units_before = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < p.n; i0 += QB_THREADS) {
+      const int i = i0 + threadIdx.x;
+      int m = 0, nt = 0, sum;
+      if (i < p.n) {
+        const Item it = load_item<QB_TILE, N>(p, i);
+        nt = it.ntile;
+        m = it.groups * p.nkv;
+      }
+      const int t = tiles_before + scan(m * nt, &sum);
+      tiles_before += sum;
+      const int u = units_before + scan(m * (nt + W), &sum);
+      units_before += sum;
+      auto tile_of = [&](int unit) {   // the first tile at or behind a unit of this request
+        const int k = (unit - u) / (nt + W);
+        return t + k * nt + max(unit - u - k * (nt + W) - W, 0);
+      };
+      if (u <= u0 && u0 < u + m * (nt + W)) {
+        ms.where[0] = i;
+        ms.where[1] = t;
+        ms.run[0] = tile_of(u0);
+      }
+      if (u <= u1 && u1 < u + m * (nt + W)) ms.run[1] = tile_of(u1);
+      if (u1 == units && threadIdx.x == 0) ms.run[1] = total;
+      if (u0 == units && threadIdx.x == 0) ms.run[0] = total;
+    }
   } else {
     const int ctas = min(grid, total);
     const Runs runs(total, ctas);
@@ -395,7 +439,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ms.tmem;
-  if (quota > 0) {
+  if (quota > 0 || weigh) {
     c0 = ms.run[0];
     c1 = ms.run[1];
   }
@@ -403,6 +447,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   // number of CTAs that hold an item of ntile tiles, the first of them tile item0 and in this CTA
   auto sharers = [&](int item0, int ntile) {
     if (quota > 0) return ms.share;
+    if (weigh)   // (the run ends inside the item's tiles)
+      return Runs(units, min(grid, total)).of(c1_unit + item0 + ntile - c1 - 1) - (int)blockIdx.x + 1;
     const Runs runs(total, min(grid, total));
     return runs.of(item0 + ntile - 1) - runs.of(item0) + 1;
   };
@@ -626,6 +672,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
 
       // ---- the item's run is over: sums over the lanes, then both sides' O
       const bool whole = bad || (j0 == 0 && nt == it.ntile);
+      const bool prefix = !bad && has_prefix<PASS>(p, it.seq);
       const int border = sg.item0 < c0 ? 0 : 1;
       const int last = t0 + nt - 1;   // the other side's last tile is last - 1
       qb_wait(&ms.pvdone[last & 1], (last >> 1) & 1, dead);
@@ -664,7 +711,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         Finish fin{1.f, 0.f};
         const float top = PASS == kAttnAll && whole ? 0.f : partial_max(-m, p.factor);
         if (whole && ms.coff[gt] >= 0) {
-          fin = finish<PASS>(p, has_prefix<PASS>(p, it.seq), ms.coff[gt], top, sum);
+          fin = finish<PASS>(p, prefix, ms.coff[gt], top, sum);
           if (PASS == kAttnPrefix) p.pre_ml[ms.coff[gt]] = make_float2(top, sum);
         }
         ms.fac[0][gt] = wa * fin.own;
@@ -711,13 +758,14 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
             if (to >= 0) p.pre_o[(size_t)to * 128 + row] = __uint_as_float(oa[i]);
           }
         } else {
-          if (PASS == kAttnOwn) {
+          if (PASS == kAttnOwn && prefix) {
+            // (16 loads together: one after another they took 10 us an item)
+            float a[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float f = ms.pre[16 * c + i];
-              if (f != 0.f)
-                oa[i] = __float_as_uint(fmaf(__ldcg(p.pre_o + (size_t)ms.coff[16 * c + i] * 128 + row), f, __uint_as_float(oa[i])));
-            }
+            for (int i = 0; i < 16; ++i) a[i] = __ldcg(p.pre_o + (size_t)max(ms.coff[16 * c + i], 0) * 128 + row);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (ms.pre[16 * c + i] != 0.f) oa[i] = __float_as_uint(fmaf(a[i], ms.pre[16 * c + i], __uint_as_float(oa[i])));
           }
           if (p.bf16) {
 #pragma unroll
@@ -742,7 +790,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         // (merged by the item's first CTA's entry; the others' partials follow its own)
         if (threadIdx.x == 0 && border == 1)
           ms.shared = make_int4(it.row0, it.rows, sg.sub,
-                                sharers(sg.item0, it.ntile) + (has_prefix<PASS>(p, it.seq) ? QB_PREFIX : 0));
+                                sharers(sg.item0, it.ntile) + (prefix ? QB_PREFIX : 0));
       }
       t0 += nt;
     }
