@@ -370,8 +370,13 @@ int dflash_paged_prefix_plan(const int32_t* table, int64_t table_ld, int max_pag
 size_t dflash_q4_prefix_workspace_size(int rows, int max_rows, int max_group, int nq, int nkv) {
   if (rows < 0 || max_rows < 1 || max_group < 1 || (long long)max_rows * max_group > DFLASH_Q4_MAX_ROWS) return 0;
   const size_t own = dflash_q4_attention_workspace_size(max_rows, nq, nkv);
-  const size_t group = dflash_q4_attention_workspace_size(max_rows * max_group, nq, nkv);
+  size_t group = dflash_q4_attention_workspace_size(max_rows * max_group, nq, nkv);
   if (own == 0 || group == 0 || (long long)rows * nq > INT32_MAX) return 0;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const size_t wide = kCounterBytes + q4_attn_tc_group_floats(max_rows * max_group, nq, nkv, sms) * sizeof(float);
+  if (group < wide) group = wide;
   return ((own > group ? own : group) + 15) / 16 * 16 + (size_t)rows * nq * 130 * sizeof(float);
 }
 

@@ -176,6 +176,7 @@ size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms);
 cudaError_t q4_attn_launch(const Q4AttnParams& p, int pass, int num_sms, cudaStream_t st);
 // the same for blocks of query rows (q4_attention_tc.cu)
 size_t q4_attn_tc_part_floats(int max_rows, int nq, int nkv, int num_sms);
+size_t q4_attn_tc_group_floats(int max_rows, int nq, int nkv, int num_sms);   // of a group's pass
 cudaError_t q4_attn_tc_launch(const Q4AttnParams& p, int pass, int num_sms, cudaStream_t st);
 // Query rows of a kv head (rows of a request times G) up to which the first
 // kernel runs; it takes them 16 at a time and decodes the cache for each group.

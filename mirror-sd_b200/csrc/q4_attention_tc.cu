@@ -60,21 +60,25 @@ constexpr float QB_RAISE = 8.f;
 
 template <int N_>
 struct QbCfg {
-  static constexpr int N = N_, CH = N / 16;
+  static constexpr int N = N_;
+  // Wide: each side takes half of every tile's columns, in place of all columns of
+  // every other tile; one decoded tile then serves 128 columns.
+  static constexpr bool WIDE = N > 80;
+  static constexpr int HN = WIDE ? N / 2 : N, CH = HN / 16;   // columns of a side
   // Query buffers and packed stages.  With 80 columns shared memory holds two and
   // two or one and three (8 requests of 16,384 rows, 160 query rows: 167 and 166 us).
   static constexpr int QB = N <= 64 ? 2 : 1;
-  static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S)
+  static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, HN for each side's O, N for each S)
   static constexpr int NS = N <= 64 ? 4 : 3;
-  static constexpr bool AHEAD = N <= 64;        // registers for the next 16 scores
-  static constexpr int SEGS = 8;                // ring of item records
+  static constexpr bool AHEAD = HN <= 64;       // registers for the next 16 scores
+  static constexpr int SEGS = WIDE ? 4 : 8;     // ring of item records (items run ahead by an S buffer each, and one)
   static constexpr int P_BYTES = (N + 63) / 64 * 16384;       // 64-column chunks of [128 rows][128 B]
   static constexpr int V_OFF = 0, V_BYTES = 32768;
   static constexpr int P_OFF = V_OFF + 2 * V_BYTES;
   static constexpr int Q_OFF = P_OFF + 2 * P_BYTES, Q_BYTES = N * 256;
   static constexpr int RING_OFF = Q_OFF + QB * Q_BYTES;
   static constexpr int MISC_OFF = RING_OFF + NS * QB_STAGE;
-  static constexpr uint32_t K_COL = 0, O_COL = 128, S_COL = 128 + 2 * N;   // 2 x 64 for K, N for each O and S
+  static constexpr uint32_t K_COL = 0, O_COL = 128, S_COL = 128 + 2 * HN;   // 2 x 64 for K, HN for each O, N for each S
   static constexpr int SLOT = N * 130;          // floats of a partial: O [N][128], m [N], l [N]
 };
 // warps: softmax of even tiles 0-3, of odd tiles 4-7, then (all in whole
@@ -104,13 +108,13 @@ struct QbMisc {
   int2 tile[16];                  // row blocks copied and QB_SEEN, rows below the request's end
   QbSeg seg[C::SEGS];
   alignas(16) float qf[C::SEGS][C::N];        // score factors
-  alignas(16) float negm[2][C::N];            // minus the columns' references, of either side
-  alignas(16) float fac[2][C::N];             // rescale factors; at the end what O is multiplied by
+  alignas(16) float negm[2][C::HN];           // minus the columns' references, of either side
+  alignas(16) float fac[2][C::HN];            // rescale factors; at the end what O is multiplied by
   alignas(16) float pre[C::N];                // and what the sums over the group's rows are (kAttnOwn)
-  int cmax[2][C::N];                 // column maxima as ordered integers
+  int cmax[2][C::HN];                // column maxima as ordered integers
   alignas(16) int cend[C::N];                 // where each column's keys end
   alignas(16) int coff[C::N];                 // output row of each column, or -1
-  float lsum[8][C::N];
+  float lsum[8][C::HN];
   int4 shared;                    // the item that starts here and reaches past the last tile (q4_tc_shared)
 };
 
@@ -284,11 +288,11 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ms.kready[i], 4); mbar_init(&ms.kfree[i], 1);
       mbar_init(&ms.vready[i], 4); mbar_init(&ms.pvdone[i], 1);
-      mbar_init(&ms.p_ready[i], 4);
+      mbar_init(&ms.p_ready[i], C::WIDE ? 8 : 4);
       mbar_init(&ms.q_ready[i], 1); mbar_init(&ms.q_free[i], 1);
     }
     mbar_init(&ms.o_free, 8);
-    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], 4); }
+    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], C::WIDE ? 8 : 4); }
     ms.abort = 0;
     ms.shared = make_int4(0, 0, 0, 0);
     ms.run[0] = ms.run[1] = 0;
@@ -300,7 +304,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     tmem_alloc(&ms.tmem, 512);
     tmem_relinquish();
   }
-  for (int i = threadIdx.x; i < 2 * N; i += QB_THREADS) ms.cmax[0][i] = float_key(-INFINITY);
+  for (int i = threadIdx.x; i < 2 * C::HN; i += QB_THREADS) ms.cmax[0][i] = float_key(-INFINITY);
 
   // The CTA's run of tiles [c0, c1), from the lengths.
   auto scan = [&](int v, int* sum) {   // what the threads before hold, and the sum of all
@@ -464,20 +468,23 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   // (registers go from the roles that move data to the two that compute)
   if (warp < QB_KDEC) {
     set_registers<QB_SOFT_REGS, true>();
-    // ---- softmax of the tiles t with t & 1 == x; thread = cached row, and channel at the end
+    // ---- softmax of the tiles t with t & 1 == x (wide: of columns 64 x .. of every
+    // tile); thread = cached row, and channel at the end
     const int x = warp >> 2, gt = threadIdx.x & 127;
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t o_t = tmem + C::O_COL + x * N + lanes;
+    constexpr int HN = C::HN;
+    const int col0 = C::WIDE ? x * HN : 0;   // the side's first column of the item
+    const uint32_t o_t = tmem + C::O_COL + x * HN + lanes;
     const int window = p.window > 0 ? p.window : 1 << 30;   // no cache is longer
     float* negm = ms.negm[x];
     float* facs = ms.fac[x];
-    uint8_t* pr = smem + C::P_OFF + x * C::P_BYTES + row * 128;
+    uint8_t* const stage_at = smem + C::P_OFF + x * (C::WIDE ? 16384 : C::P_BYTES);   // (of this side's P, tile 0)
     int u = c0, t0 = 0;   // the item's first tile, counted in the CTA
 #pragma unroll 1
     for (int seg = 0; u < c1; ++seg) {
       // S of the item's first tile is only issued once its record is there
-      if ((t0 & 1) == x) qb_wait(&ms.s_ready[t0 % C::SB], (t0 / C::SB) & 1, dead);
+      if (C::WIDE || (t0 & 1) == x) qb_wait(&ms.s_ready[t0 % C::SB], (t0 / C::SB) & 1, dead);
       const QbSeg& sg = ms.seg[seg % C::SEGS];
       // after an expired wait there may be no record: run to the end, writing nothing
       const bool bad = named_bar_or<256>(3, *dead);
@@ -487,27 +494,30 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       const float* qf = ms.qf[seg % C::SEGS];
       const bool uniform = sg.uniform;
       const float f = p.factor;
-      if (gt < N) {
-        const int r = sg.q0 + gt, j = p.by_g.of(r);
+      if (gt < HN) {
+        const int r = sg.q0 + col0 + gt, j = p.by_g.of(r);
         const bool real = j < it.rows;
         negm[gt] = real ? kUnset : 0.f;
-        if (x == 0) {
-          ms.cend[gt] = real ? (p.causal ? it.L - it.rows + j + 1 : it.L) : 0;
-          ms.coff[gt] = real ? (it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;
+        if (C::WIDE || x == 0) {
+          ms.cend[col0 + gt] = real ? (p.causal ? it.L - it.rows + j + 1 : it.L) : 0;
+          ms.coff[col0 + gt] = real ? (it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;
         }
       }
       named_bar_sync(3, 256);
-      float2 l[N / 2];
+      float2 l[HN / 2];
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) l[i] = make_float2(0.f, 0.f);
+      for (int i = 0; i < HN / 2; ++i) l[i] = make_float2(0.f, 0.f);
 
 #pragma unroll 1
-      for (int k = (t0 & 1) == x ? 0 : 1; k < nt; k += 2) {
+      for (int k = C::WIDE || (t0 & 1) == x ? 0 : 1; k < nt; k += C::WIDE ? 1 : 2) {
         const int t = t0 + k;
-        const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + lanes;
-        // P of this side is read, and its O holds the tiles before t
+        const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + col0 + lanes;
+        // this tile's P (wide: one of two) and, with two sides, O
+        uint8_t* const p_at = C::WIDE ? stage_at + (t & 1) * C::P_BYTES : stage_at;
+        uint8_t* const pr = p_at + row * 128;
+        // P is read, and this side's O holds the tiles before t (wide: before t - 1)
         auto wait_pv = [&]() {
-          if (t >= 2) qb_wait(&ms.pvdone[x], ((t >> 1) - 1) & 1, dead);
+          if (t >= 2) qb_wait(&ms.pvdone[t & 1], ((t >> 1) - 1) & 1, dead);
         };
         if (k > 0) qb_wait(&ms.s_ready[t % C::SB], (t / C::SB) & 1, dead);
         tc_fence_after();
@@ -531,12 +541,12 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           } else {
             const float inv = 1.f / f;
 #pragma unroll 1
-            for (int c = 0; c < N; c += 4) {
+            for (int c = 0; c < HN; c += 4) {
               uint32_t s[4];
               tmem_ld4(s_t + c, s);
               tmem_ld_wait();
-              const int4 e = *reinterpret_cast<const int4*>(&ms.cend[c]);
-              const float4 w = *reinterpret_cast<const float4*>(&qf[c]);
+              const int4 e = *reinterpret_cast<const int4*>(&ms.cend[col0 + c]);
+              const float4 w = *reinterpret_cast<const float4*>(&qf[col0 + c]);
               auto one = [&](uint32_t v, int end, float by) {
                 const bool seen = (key < end) & ((key < p.sink) | (key >= end - window));   // (no branch)
                 return seen ? __float_as_uint(__uint_as_float(v) * (by * inv)) : 0xff800000u;
@@ -593,7 +603,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         };
         // One round; a second one with new references if the first finds a score
         // that passes its column's by more than 2^8.
-        bool raise = k < 2;   // this side's first tile of the item
+        bool raise = k < (C::WIDE ? 1 : 2);   // this side's first tile of the item
         int done = 0;
 #pragma unroll 1
         for (int round = 0; round < 2; ++round) {
@@ -601,7 +611,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
             // Column maxima of the tile over the lanes, 16 columns at a time through
             // this side's P (its last reader is done), then over the warps.
             wait_pv();
-            float* stage = reinterpret_cast<float*>(smem + C::P_OFF + x * C::P_BYTES) + (warp & 3) * (16 * 36);
+            float* stage = reinterpret_cast<float*>(p_at) + (warp & 3) * (16 * 36);
 #pragma unroll 1
             for (int c = 0; c < C::CH; ++c) {
               uint32_t s[16];
@@ -623,7 +633,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               __syncwarp();
             }
             named_bar_sync(1 + x, 128);
-            if (gt < N) {
+            if (gt < HN) {
               const float nm = negm[gt], top = key_float(ms.cmax[x][gt]);
               const float rise = (top + nm) * p.factor;
               float fac = 1.f;
@@ -635,7 +645,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               ms.cmax[x][gt] = float_key(-INFINITY);
             }
             named_bar_sync(1 + x, 128);
-            if (k >= 2) {
+            if (k >= (C::WIDE ? 1 : 2)) {
+              if (C::WIDE) qb_wait(&ms.pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1, dead);   // O holds all tiles before t
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < C::CH; ++c) {
@@ -648,7 +659,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               }
               tmem_st_wait();
 #pragma unroll
-              for (int i = 0; i < N / 2; ++i) {
+              for (int i = 0; i < HN / 2; ++i) {
                 const float2 fac = *reinterpret_cast<const float2*>(&facs[2 * i]);
                 l[i].x *= fac.x;
                 l[i].y *= fac.y;
@@ -666,7 +677,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         tc_fence_before();
         warp_arrive(&ms.s_free[t % C::SB], lane);
         fence_proxy_async_smem();
-        warp_arrive(&ms.p_ready[x], lane);
+        warp_arrive(&ms.p_ready[t & 1], lane);
       }
       u += nt;
 
@@ -680,7 +691,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       {
         // 16 columns at a time through this side's P (its last reader is done):
         // lane i of the warp then adds half of column i / 2
-        float* stage = reinterpret_cast<float*>(smem + C::P_OFF + x * C::P_BYTES) + (warp & 3) * (16 * 36);
+        float* stage = reinterpret_cast<float*>(stage_at) + (warp & 3) * (16 * 36);
 #pragma unroll
         for (int c = 0; c < C::CH; ++c) {
 #pragma unroll
@@ -702,7 +713,23 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       }
       named_bar_sync(3, 256);
       float* part = p.part + ((size_t)blockIdx.x * 2 + border) * C::SLOT;
-      if (x == 0 && gt < N) {
+      if (C::WIDE && gt < HN) {
+        const int col = col0 + gt;
+        const float sum = (ms.lsum[4 * x][gt] + ms.lsum[4 * x + 1][gt]) + (ms.lsum[4 * x + 2][gt] + ms.lsum[4 * x + 3][gt]);
+        const float top = partial_max(negm[gt], p.factor);
+        Finish fin{1.f, 0.f};
+        if (whole && ms.coff[col] >= 0) {
+          fin = finish<PASS>(p, prefix, ms.coff[col], top, sum);
+          if (PASS == kAttnPrefix) p.pre_ml[ms.coff[col]] = make_float2(top, sum);
+        }
+        facs[gt] = fin.own;
+        if (PASS == kAttnOwn) ms.pre[col] = fin.pre;
+        if (!whole) {
+          part[N * 128 + col] = top;
+          part[N * 129 + col] = sum;
+        }
+      }
+      if (!C::WIDE && x == 0 && gt < HN) {
         // a side without a tile (one-tile run) or a column without a key has sum 0 and counts nothing
         const float ma = -ms.negm[0][gt], mb = -ms.negm[1][gt], m = fmaxf(ma, mb);
         const float wa = ma == -kUnset ? 0.f : exp2_fast((ma - m) * p.factor), wb = mb == -kUnset ? 0.f : exp2_fast((mb - m) * p.factor);
@@ -729,23 +756,33 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       uint8_t* out = static_cast<uint8_t*>(p.out) + 2 * row;
       // (a side without a tile has factor 0; its O may hold anything, so the
       // other side's is read in its place)
+      // (wide: each its own columns)
       const uint32_t o_all = tmem + C::O_COL + lanes;
-      const uint32_t o_a = nt > 1 || (t0 & 1) == 0 ? o_all : o_all + N, o_b = nt > 1 || (t0 & 1) == 1 ? o_all + N : o_all;
+      const uint32_t o_a = nt > 1 || (t0 & 1) == 0 ? o_all : o_all + HN, o_b = nt > 1 || (t0 & 1) == 1 ? o_all + HN : o_all;
 #pragma unroll 1
-      for (int c = x; c < C::CH; c += 2) {
-        uint32_t oa[16], ob[16];
+      for (int c0 = C::WIDE ? 0 : x; c0 < C::CH; c0 += C::WIDE ? 1 : 2) {
+        const int c = c0 + (C::WIDE ? x * C::CH : 0);   // 16 columns of the item
+        uint32_t oa[16];
         __syncwarp();
-        tmem_ld16(o_a + 16 * c, oa);
-        tmem_ld16(o_b + 16 * c, ob);
-        tmem_ld_wait();
+        if constexpr (C::WIDE) {
+          tmem_ld16(o_t + 16 * c0, oa);
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 fa = *reinterpret_cast<const float4*>(&ms.fac[0][16 * c + i]);
-          const float4 fb = *reinterpret_cast<const float4*>(&ms.fac[1][16 * c + i]);
-          const float wa[4] = {fa.x, fa.y, fa.z, fa.w}, wb[4] = {fb.x, fb.y, fb.z, fb.w};
+          for (int i = 0; i < 16; ++i) oa[i] = __float_as_uint(__uint_as_float(oa[i]) * facs[16 * c0 + i]);
+        } else {
+          uint32_t ob[16];
+          tmem_ld16(o_a + 16 * c, oa);
+          tmem_ld16(o_b + 16 * c, ob);
+          tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            oa[i + k] = __float_as_uint(fmaf(__uint_as_float(oa[i + k]), wa[k], __uint_as_float(ob[i + k]) * wb[k]));
+          for (int i = 0; i < 16; i += 4) {
+            const float4 fa = *reinterpret_cast<const float4*>(&ms.fac[0][16 * c + i]);
+            const float4 fb = *reinterpret_cast<const float4*>(&ms.fac[1][16 * c + i]);
+            const float wa[4] = {fa.x, fa.y, fa.z, fa.w}, wb[4] = {fb.x, fb.y, fb.z, fb.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              oa[i + k] = __float_as_uint(fmaf(__uint_as_float(oa[i + k]), wa[k], __uint_as_float(ob[i + k]) * wb[k]));
+          }
         }
         if (!whole) {
           float* dst = part + 16 * c * 128 + row;
@@ -1075,7 +1112,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         }
       }
     } else if (warp == QB_MMA2 && T > 0) {
-      // ---- O(side of t) += V^T(t) P^T(t)
+      // ---- O(side of t; wide: of both) += V^T(t) P^T(t)
       const uint32_t idesc = umma_idesc_f16(128, N, 0) | (1u << 16);   // B (P^T) with the columns contiguous
       const uint64_t vd = umma_desc_sw128(smem_u32(smem + C::V_OFF)), pd = desc_sw128_mn(smem_u32(smem + C::P_OFF), 16384);
       int seg = 0, k = 0, nt = 0;
@@ -1092,7 +1129,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           const uint64_t v = vd + (t & 1) * (C::V_BYTES >> 4), pp = pd + (t & 1) * (C::P_BYTES >> 4);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)   // (a side's first tile of the item starts its O)
-            umma_f16(tmem + C::O_COL + (t & 1) * N, v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc, k > 1 || ks > 0);
+            umma_f16(tmem + C::O_COL + (C::WIDE ? 0 : (t & 1) * N), v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc,
+                     k > (C::WIDE ? 0 : 1) || ks > 0);
           umma_commit(&ms.pvdone[t & 1]);
         }
         __syncwarp();
@@ -1161,11 +1199,20 @@ static cudaError_t launch_tc(const Q4AttnParams& p, int num_sms, cudaStream_t st
   static_assert(smem <= 227 * 1024, "shared memory");
   DFL_TRY(cudaFuncSetAttribute(q4_attn_tc_kernel<N, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   DFL_TRY(launch_pdl(q4_attn_tc_kernel<N, PASS>, dim3(num_sms), dim3(QB_THREADS), smem, st, p));
-  return launch_pdl(q4_attn_tc_merge_kernel<PASS>, dim3(num_sms, C::CH), dim3(256), 0, st, p, N);
+  return launch_pdl(q4_attn_tc_merge_kernel<PASS>, dim3(num_sms, N / 16), dim3(256), 0, st, p, N);
+}
+
+// Query rows of a group's pass past 80 of a kv head: 128 columns, wide.
+static bool wide_pass(int max_rows, int nq, int nkv) { return (long long)max_rows * (nq / nkv) > 80; }
+
+size_t q4_attn_tc_group_floats(int max_rows, int nq, int nkv, int num_sms) {
+  const size_t n = wide_pass(max_rows, nq, nkv) ? 128 : 80;
+  return (size_t)num_sms * (2 * n * 130 + sizeof(int4) / sizeof(float));
 }
 
 template <int PASS>
 static cudaError_t launch_pass(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
+  if (PASS == kAttnPrefix && wide_pass(p.max_rows, p.nq, p.nkv)) return launch_tc<128, kAttnPrefix>(p, num_sms, st);
   switch (q4_attn_tc_columns(p.max_rows, p.nq, p.nkv)) {
     case 32: return launch_tc<32, PASS>(p, num_sms, st);
     case 48: return launch_tc<48, PASS>(p, num_sms, st);
