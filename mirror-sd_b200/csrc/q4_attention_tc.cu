@@ -61,14 +61,16 @@ constexpr float QB_RAISE = 8.f;
 template <int N_>
 struct QbCfg {
   static constexpr int N = N_;
-  // Wide: each side takes half of every tile's columns, in place of all columns of
-  // every other tile; one decoded tile then serves 128 columns.
+  // Wide: four sides take a quarter of every tile's columns each, in place of all
+  // columns of every other tile; one decoded tile then serves 128 columns.  (Two
+  // sides of 64 columns: 3,840 cycles a tile.)
   static constexpr bool WIDE = N > 80;
-  static constexpr int HN = WIDE ? N / 2 : N, CH = HN / 16;   // columns of a side
+  static constexpr int SIDES = WIDE ? 4 : 2;                  // of 4 softmax warps each
+  static constexpr int HN = WIDE ? N / SIDES : N, CH = HN / 16;   // columns of a side
   // Query buffers and packed stages.  With 80 columns shared memory holds two and
   // two or one and three (8 requests of 16,384 rows, 160 query rows: 167 and 166 us).
   static constexpr int QB = N <= 64 ? 2 : 1;
-  static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, HN for each side's O, N for each S)
+  static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S)
   static constexpr int NS = N <= 64 ? 4 : 3;
   static constexpr bool AHEAD = HN <= 64;       // registers for the next 16 scores
   static constexpr int SEGS = WIDE ? 4 : 8;     // ring of item records (items run ahead by an S buffer each, and one)
@@ -78,16 +80,15 @@ struct QbCfg {
   static constexpr int Q_OFF = P_OFF + 2 * P_BYTES, Q_BYTES = N * 256;
   static constexpr int RING_OFF = Q_OFF + QB * Q_BYTES;
   static constexpr int MISC_OFF = RING_OFF + NS * QB_STAGE;
-  static constexpr uint32_t K_COL = 0, O_COL = 128, S_COL = 128 + 2 * HN;   // 2 x 64 for K, HN for each O, N for each S
+  static constexpr uint32_t K_COL = 0, O_COL = 128, S_COL = 128 + (WIDE ? N : 2 * N);   // 2 x 64 for K, N for each O and S
   static constexpr int SLOT = N * 130;          // floats of a partial: O [N][128], m [N], l [N]
+  // warps: softmax, side by side (even tiles 0-3, odd tiles 4-7), then the others, all
+  // in whole warpgroups, whose registers are dealt out anew after the common start
+  static constexpr int KDEC = 4 * SIDES, VDEC = KDEC + 4, MMA = VDEC + 4, LOAD = MMA + 1, QUERY = MMA + 2, MMA2 = MMA + 3;
+  static constexpr int THREADS = 32 * (MMA + 4), SOFT = 128 * SIDES;
+  // registers a thread at the start: 96, 640 * 96 = 256 * 144 + 384 * 64 (wide: 72, 896 * 72 > 512 * 88 + 384 * 48)
+  static constexpr int SOFT_REGS = WIDE ? 88 : 144, REST_REGS = WIDE ? 48 : 64;
 };
-// warps: softmax of even tiles 0-3, of odd tiles 4-7, then (all in whole
-// warpgroups, whose registers are dealt out anew after the common start)
-constexpr int QB_KDEC = 8, QB_VDEC = 12, QB_MMA = 16, QB_LOAD = 17, QB_QUERY = 18, QB_MMA2 = 19;
-constexpr int QB_THREADS = 640;
-// 96 registers a thread at the start: 640 * 96 = 256 * 144 + 384 * 64
-constexpr int QB_SOFT_REGS = 144, QB_REST_REGS = 64;
-
 struct QbSeg {          // a run of tiles of one item
   Item it;
   int sub, q0, head0;   // first query row (row * G + head) and head of the item
@@ -104,17 +105,17 @@ struct QbMisc {
   int abort;
   int where[2];                   // request of the CTA's first tile, and that request's first tile
   int run[2], share;              // whole CTAs to an item: this one's tiles, and their number
-  int wtot[QB_THREADS / 32];
+  int wtot[C::THREADS / 32];
   int2 tile[16];                  // row blocks copied and QB_SEEN, rows below the request's end
   QbSeg seg[C::SEGS];
   alignas(16) float qf[C::SEGS][C::N];        // score factors
-  alignas(16) float negm[2][C::HN];           // minus the columns' references, of either side
-  alignas(16) float fac[2][C::HN];            // rescale factors; at the end what O is multiplied by
+  alignas(16) float negm[C::SIDES][C::HN];           // minus the columns' references, of either side
+  alignas(16) float fac[C::SIDES][C::HN];            // rescale factors; at the end what O is multiplied by
   alignas(16) float pre[C::N];                // and what the sums over the group's rows are (kAttnOwn)
-  int cmax[2][C::HN];                // column maxima as ordered integers
+  int cmax[C::SIDES][C::HN];                // column maxima as ordered integers
   alignas(16) int cend[C::N];                 // where each column's keys end
   alignas(16) int coff[C::N];                 // output row of each column, or -1
-  float lsum[8][C::HN];
+  float lsum[4 * C::SIDES][C::HN];
   int4 shared;                    // the item that starts here and reaches past the last tile (q4_tc_shared)
 };
 
@@ -247,6 +248,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// largest value of a warp's lanes
+__device__ __forceinline__ float redux_max(float v) {
+  float d;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
+}
 // order-preserving map of floats to ints (-inf lowest)
 __device__ __forceinline__ int float_key(float f) {
   const int i = __float_as_int(f);
@@ -272,7 +279,7 @@ __host__ __device__ __forceinline__ int4* q4_tc_shared(float* part, int n, int g
 }
 
 template <int N, int PASS>
-__global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnParams p) {
+__global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const Q4AttnParams p) {
   using C = QbCfg<N>;
   constexpr int NS = C::NS;
   extern __shared__ uint8_t smem_raw[];
@@ -288,11 +295,11 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ms.kready[i], 4); mbar_init(&ms.kfree[i], 1);
       mbar_init(&ms.vready[i], 4); mbar_init(&ms.pvdone[i], 1);
-      mbar_init(&ms.p_ready[i], C::WIDE ? 8 : 4);
+      mbar_init(&ms.p_ready[i], C::WIDE ? 4 * C::SIDES : 4);
       mbar_init(&ms.q_ready[i], 1); mbar_init(&ms.q_free[i], 1);
     }
-    mbar_init(&ms.o_free, 8);
-    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], C::WIDE ? 8 : 4); }
+    mbar_init(&ms.o_free, 4 * C::SIDES);
+    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], C::WIDE ? 4 * C::SIDES : 4); }
     ms.abort = 0;
     ms.shared = make_int4(0, 0, 0, 0);
     ms.run[0] = ms.run[1] = 0;
@@ -300,11 +307,11 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   }
   griddep_wait();
   griddep_launch_dependents();
-  if (warp == QB_MMA) {
+  if (warp == C::MMA) {
     tmem_alloc(&ms.tmem, 512);
     tmem_relinquish();
   }
-  for (int i = threadIdx.x; i < 2 * C::HN; i += QB_THREADS) ms.cmax[0][i] = float_key(-INFINITY);
+  for (int i = threadIdx.x; i < C::SIDES * C::HN; i += C::THREADS) ms.cmax[0][i] = float_key(-INFINITY);
 
   // The CTA's run of tiles [c0, c1), from the lengths.
   auto scan = [&](int v, int* sum) {   // what the threads before hold, and the sum of all
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < QB_THREADS / 32; ++w) {
+    for (int w = 0; w < C::THREADS / 32; ++w) {
       if (w < warp) before = tiles_sum(before, ms.wtot[w]);
       all = tiles_sum(all, ms.wtot[w]);
     }
@@ -336,7 +343,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   int units = 0, c1_unit = 0;   // of all items; where the CTA's run ends
   int total = 0, c0 = 0, c1 = 0, items = 0, ntile = 0, first = 0;   // (the last three of request threadIdx.x)
 #pragma unroll 1
-  for (int i0 = 0; i0 < p.n; i0 += QB_THREADS) {
+  for (int i0 = 0; i0 < p.n; i0 += C::THREADS) {
     const int i = i0 + threadIdx.x;
     items = ntile = 0;
     if (i < p.n) {
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   // runs would have.  (8 items of 64 tiles 26.8 us in equal runs, 23.9 in whole
   // CTAs; 16 of 257 tiles, 160 query rows, 59.9 and 56.6.)
   int quota = 0;
-  if (p.n <= QB_THREADS && total > grid) {
+  if (p.n <= C::THREADS && total > grid) {
     int lo = (total + grid - 1) / grid, hi = lo + QB_SLACK + 1, sum;
 #pragma unroll 1
     while (lo < hi) {
@@ -390,7 +397,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     c1_unit = u1;
     int tiles_before = 0, units_before = 0;
 #pragma unroll 1
-    for (int i0 = 0; i0 < p.n; i0 += QB_THREADS) {
+    for (int i0 = 0; i0 < p.n; i0 += C::THREADS) {
       const int i = i0 + threadIdx.x;
       int m = 0, nt = 0, sum;
       if (i < p.n) {
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     }
     int before = 0;
 #pragma unroll 1
-    for (int i0 = 0; i0 < p.n; i0 += QB_THREADS) {
+    for (int i0 = 0; i0 < p.n; i0 += C::THREADS) {
       const int i = i0 + threadIdx.x;
       int v = 0, sum;
       if (i < p.n) {
@@ -466,9 +473,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   };
 
   // (registers go from the roles that move data to the two that compute)
-  if (warp < QB_KDEC) {
-    set_registers<QB_SOFT_REGS, true>();
-    // ---- softmax of the tiles t with t & 1 == x (wide: of columns 64 x .. of every
+  if (warp < C::KDEC) {
+    set_registers<C::SOFT_REGS, true>();
+    // ---- softmax of the tiles t with t & 1 == x (wide: of columns 32 x .. of every
     // tile); thread = cached row, and channel at the end
     const int x = warp >> 2, gt = threadIdx.x & 127;
     const int row = 32 * (warp & 3) + lane;
@@ -479,7 +486,6 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     const int window = p.window > 0 ? p.window : 1 << 30;   // no cache is longer
     float* negm = ms.negm[x];
     float* facs = ms.fac[x];
-    uint8_t* const stage_at = smem + C::P_OFF + x * (C::WIDE ? 16384 : C::P_BYTES);   // (of this side's P, tile 0)
     int u = c0, t0 = 0;   // the item's first tile, counted in the CTA
 #pragma unroll 1
     for (int seg = 0; u < c1; ++seg) {
@@ -487,7 +493,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       if (C::WIDE || (t0 & 1) == x) qb_wait(&ms.s_ready[t0 % C::SB], (t0 / C::SB) & 1, dead);
       const QbSeg& sg = ms.seg[seg % C::SEGS];
       // after an expired wait there may be no record: run to the end, writing nothing
-      const bool bad = named_bar_or<256>(3, *dead);
+      const bool bad = named_bar_or<C::SOFT>(1 + C::SIDES, *dead);
       Item it{};
       if (!bad) it = sg.it;
       const int nt = bad ? c1 - u : sg.nt, j0 = bad ? 0 : sg.j0;
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           ms.coff[col0 + gt] = real ? (it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;
         }
       }
-      named_bar_sync(3, 256);
+      named_bar_sync(1 + C::SIDES, C::SOFT);
       float2 l[HN / 2];
 #pragma unroll
       for (int i = 0; i < HN / 2; ++i) l[i] = make_float2(0.f, 0.f);
@@ -512,8 +518,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       for (int k = C::WIDE || (t0 & 1) == x ? 0 : 1; k < nt; k += C::WIDE ? 1 : 2) {
         const int t = t0 + k;
         const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + col0 + lanes;
-        // this tile's P (wide: one of two) and, with two sides, O
-        uint8_t* const p_at = C::WIDE ? stage_at + (t & 1) * C::P_BYTES : stage_at;
+        // (of two sides, each has a P of its own)
+        uint8_t* const p_at = smem + C::P_OFF + (t & 1) * C::P_BYTES;
         uint8_t* const pr = p_at + row * 128;
         // P is read, and this side's O holds the tiles before t (wide: before t - 1)
         auto wait_pv = [&]() {
@@ -595,9 +601,10 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
               w[i] = pack_f16x2(y[i].x, y[i].y);
             }
             if (c == 0) wait_pv();
-            uint8_t* d = pr + (c >> 2) * 16384;
-            *reinterpret_cast<uint4*>(d + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(d + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            const int cc = C::WIDE ? x * C::CH + c : c;   // 16 columns of the item
+            uint8_t* d = pr + (cc >> 2) * 16384;
+            *reinterpret_cast<uint4*>(d + (((2 * (cc & 3)) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(d + (((2 * (cc & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
           }
           return C::CH;
         };
@@ -611,26 +618,42 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
             // Column maxima of the tile over the lanes, 16 columns at a time through
             // this side's P (its last reader is done), then over the warps.
             wait_pv();
-            float* stage = reinterpret_cast<float*>(p_at) + (warp & 3) * (16 * 36);
+            if constexpr (C::WIDE) {   // (the sides' columns of P interleave; a side has 32, one a lane)
+              float mine = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < C::CH; ++c) {
-              uint32_t s[16];
-              tmem_ld16(s_t + 16 * c, s);
-              tmem_ld_wait();
+              for (int c = 0; c < C::CH; ++c) {
+                uint32_t s[16];
+                tmem_ld16(s_t + 16 * c, s);
+                tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) stage[i * 36 + lane] = __uint_as_float(s[i]);
-              __syncwarp();
-              float top = -INFINITY, top2 = -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float4 v = *reinterpret_cast<const float4*>(stage + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * i);
-                top = max3(top, v.x, v.y);
-                top2 = max3(top2, v.z, v.w);
+                for (int i = 0; i < 16; ++i) {
+                  const float top = redux_max(__uint_as_float(s[i]));
+                  if (lane == 16 * c + i) mine = top;
+                }
               }
-              top = fmaxf(top, top2);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-              if (!(lane & 1)) atomicMax(&ms.cmax[x][16 * c + (lane >> 1)], float_key(top));
-              __syncwarp();
+              atomicMax(&ms.cmax[x][lane], float_key(mine));
+            } else {
+              float* stage = reinterpret_cast<float*>(p_at) + (warp & 3) * (16 * 36);
+  #pragma unroll 1
+              for (int c = 0; c < C::CH; ++c) {
+                uint32_t s[16];
+                tmem_ld16(s_t + 16 * c, s);
+                tmem_ld_wait();
+  #pragma unroll
+                for (int i = 0; i < 16; ++i) stage[i * 36 + lane] = __uint_as_float(s[i]);
+                __syncwarp();
+                float top = -INFINITY, top2 = -INFINITY;
+  #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float4 v = *reinterpret_cast<const float4*>(stage + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * i);
+                  top = max3(top, v.x, v.y);
+                  top2 = max3(top2, v.z, v.w);
+                }
+                top = fmaxf(top, top2);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                if (!(lane & 1)) atomicMax(&ms.cmax[x][16 * c + (lane >> 1)], float_key(top));
+                __syncwarp();
+              }
             }
             named_bar_sync(1 + x, 128);
             if (gt < HN) {
@@ -688,10 +711,26 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       const int last = t0 + nt - 1;   // the other side's last tile is last - 1
       qb_wait(&ms.pvdone[last & 1], (last >> 1) & 1, dead);
       if (nt > 1) qb_wait(&ms.pvdone[(last - 1) & 1], ((last - 1) >> 1) & 1, dead);
-      {
+      if constexpr (C::WIDE) {
+        // lane i ends with the sum of column i: halves of the columns go to the lanes that keep them
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          v[2 * i] = l[i].x;
+          v[2 * i + 1] = l[i].y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2)
+#pragma unroll
+          for (int i = 0; i < o; ++i) {
+            const float give = lane & o ? v[i] : v[i + o], keep = lane & o ? v[i + o] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+        ms.lsum[warp][lane] = v[0];
+      } else {
         // 16 columns at a time through this side's P (its last reader is done):
         // lane i of the warp then adds half of column i / 2
-        float* stage = reinterpret_cast<float*>(stage_at) + (warp & 3) * (16 * 36);
+        float* stage = reinterpret_cast<float*>(smem + C::P_OFF + x * C::P_BYTES) + (warp & 3) * (16 * 36);
 #pragma unroll
         for (int c = 0; c < C::CH; ++c) {
 #pragma unroll
@@ -711,9 +750,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           __syncwarp();
         }
       }
-      named_bar_sync(3, 256);
+      named_bar_sync(1 + C::SIDES, C::SOFT);
       float* part = p.part + ((size_t)blockIdx.x * 2 + border) * C::SLOT;
-      if (C::WIDE && gt < HN) {
+      if (C::WIDE && gt < HN) {   // (the side's first warp)
         const int col = col0 + gt;
         const float sum = (ms.lsum[4 * x][gt] + ms.lsum[4 * x + 1][gt]) + (ms.lsum[4 * x + 2][gt] + ms.lsum[4 * x + 3][gt]);
         const float top = partial_max(negm[gt], p.factor);
@@ -749,7 +788,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           part[N * 129 + gt] = sum;
         }
       }
-      named_bar_sync(3, 256);
+      named_bar_sync(1 + C::SIDES, C::SOFT);
       tc_fence_after();
       // thread = channel: 32 lanes write 64 (128) contiguous bytes of a row;
       // the two groups of warps take every other 16 columns
@@ -833,10 +872,10 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     }
 
     if (threadIdx.x == 0) q4_tc_shared(p.part, N, grid)[blockIdx.x] = ms.shared;
-  } else if (warp < QB_VDEC) {
-    set_registers<QB_REST_REGS, false>();
+  } else if (warp < C::VDEC) {
+    set_registers<C::REST_REGS, false>();
     // ---- K codes to f16: thread = cached row
-    const int dt = threadIdx.x - 32 * QB_KDEC;
+    const int dt = threadIdx.x - 32 * C::KDEC;
     const uint32_t kt = tmem + C::K_COL + ((uint32_t)(32 * (warp & 3)) << 16);
 #pragma unroll 1
     for (int t = 0; t < T; ++t) {
@@ -871,10 +910,10 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
         if (lane == 0) mbar_arrive(&ms.empty[s]);
       }
     }
-  } else if (warp < QB_MMA) {
-    set_registers<QB_REST_REGS, false>();
+  } else if (warp < C::MMA) {
+    set_registers<C::REST_REGS, false>();
     // ---- V codes to f16, channels as rows: thread = 8 cached rows x 16 channels
-    const int dt = threadIdx.x - 32 * QB_VDEC;
+    const int dt = threadIdx.x - 32 * C::VDEC;
     const int oct = dt & 7, g = (dt >> 3) & 7, chunk = dt >> 6;
 #pragma unroll 1
     for (int t = 0; t < T; ++t) {
@@ -928,8 +967,8 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       }
     }
   } else {
-    set_registers<QB_REST_REGS, false>();
-    if (warp == QB_LOAD && T > 0) {
+    set_registers<C::REST_REGS, false>();
+    if (warp == C::LOAD && T > 0) {
     // ---- packed tiles, four at a time: lane 8 i + b looks after row block b of
     // tile i.  (One tile at a time, page number and addresses took this warp
     // about 1,700 cycles a tile, as long as a tile takes the other roles.)
@@ -989,9 +1028,9 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
     if (t < T)
       for (int i = max(t - NS, 0); i < t; ++i) mbar_wait(&ms.full[i % NS], (i / NS) & 1, nullptr, nullptr);
     zero_rows<PASS>(p, lane, 32);
-    } else if (warp == QB_LOAD) {
+    } else if (warp == C::LOAD) {
       zero_rows<PASS>(p, lane, 32);
-    } else if (warp == QB_QUERY && T > 0) {
+    } else if (warp == C::QUERY && T > 0) {
     // ---- query rows, as f16 with the factor that their scores take
     Cursor cur;
     first_cursor(cur);
@@ -1079,7 +1118,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
       cur.j += nt - 1;
       if (u < c1) cursor_next<QB_TILE, N>(p, cur);
     }
-    } else if (warp == QB_MMA && T > 0) {
+    } else if (warp == C::MMA && T > 0) {
       // ---- S(t) = K(t) Q^T, as soon as K is there and the softmax has read the buffer's last S
       const uint32_t idesc = umma_idesc_f16(128, N, 0);
       const uint64_t qd = umma_desc_sw128(smem_u32(smem + C::Q_OFF));
@@ -1111,7 +1150,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
           ++seg;
         }
       }
-    } else if (warp == QB_MMA2 && T > 0) {
+    } else if (warp == C::MMA2 && T > 0) {
       // ---- O(side of t; wide: of both) += V^T(t) P^T(t)
       const uint32_t idesc = umma_idesc_f16(128, N, 0) | (1u << 16);   // B (P^T) with the columns contiguous
       const uint64_t vd = umma_desc_sw128(smem_u32(smem + C::V_OFF)), pd = desc_sw128_mn(smem_u32(smem + C::P_OFF), 16384);
@@ -1144,7 +1183,7 @@ __global__ void __launch_bounds__(QB_THREADS, 1) q4_attn_tc_kernel(const Q4AttnP
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && ms.abort && p.status) atomicOr(p.status, kPagedTimeout);
-  if (warp == QB_MMA) {
+  if (warp == C::MMA) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -1198,7 +1237,7 @@ static cudaError_t launch_tc(const Q4AttnParams& p, int num_sms, cudaStream_t st
   constexpr size_t smem = C::MISC_OFF + sizeof(QbMisc<C>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
   DFL_TRY(cudaFuncSetAttribute(q4_attn_tc_kernel<N, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  DFL_TRY(launch_pdl(q4_attn_tc_kernel<N, PASS>, dim3(num_sms), dim3(QB_THREADS), smem, st, p));
+  DFL_TRY(launch_pdl(q4_attn_tc_kernel<N, PASS>, dim3(num_sms), dim3(C::THREADS), smem, st, p));
   return launch_pdl(q4_attn_tc_merge_kernel<PASS>, dim3(num_sms, N / 16), dim3(256), 0, st, p, N);
 }
 
