@@ -487,7 +487,9 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
  * The plan, once a step for all layers, compares the members' block tables: their
  * prefix is the pages that the rows of all members with query rows begin with
  * alike, as far as every query row sees them whole (starts, max_rows and causal as
- * in dflash_q4_attention; lens [n]).  Written: group_starts [num_groups + 1],
+ * in dflash_q4_attention; lens [n]).  Where that would spare fewer than `least`
+ * cached rows from being read, over all groups, nothing is shared: a pass over
+ * shared rows costs about as much as reading 32,768 rows of 8 kv heads.  Written: group_starts [num_groups + 1],
  * prefix [num_groups] (rows), row_of [num_groups], skip [n] (pages), own_lens [n].
  *
  * The attention gives what dflash_q4_attention gives without a window, up to the
@@ -498,7 +500,7 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
  * bytes, as for dflash_q4_attention. */
 int dflash_paged_prefix_plan(const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens, const int32_t* starts,
                              int n, int max_rows, int page_size, const int32_t* groups, int num_groups, int causal,
-                             int32_t* group_starts, int32_t* prefix, int32_t* row_of, int32_t* skip, int32_t* own_lens,
+                             int64_t least, int32_t* group_starts, int32_t* prefix, int32_t* row_of, int32_t* skip, int32_t* own_lens,
                              void* stream);
 size_t dflash_q4_prefix_workspace_size(int rows, int max_rows, int max_group, int nq, int nkv);
 int dflash_q4_prefix_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16, const uint8_t* pool, int num_pages,

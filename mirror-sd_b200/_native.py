@@ -154,7 +154,7 @@ EXPORTS = {
                                       c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p,
                                                                                   c_void_p, c_size_t, c_void_p]),
     "dflash_paged_prefix_plan": (c_int32, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
-                                           c_int] + [c_void_p] * 6),
+                                           c_int, c_int64] + [c_void_p] * 6),
     "dflash_q4_prefix_workspace_size": (c_size_t, [c_int] * 5),
     "dflash_q4_prefix_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_int,
                                              c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,

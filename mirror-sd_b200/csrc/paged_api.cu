@@ -349,7 +349,7 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
 
 int dflash_paged_prefix_plan(const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens, const int32_t* starts,
                              int n, int max_rows, int page_size, const int32_t* groups, int num_groups, int causal,
-                             int32_t* group_starts, int32_t* prefix, int32_t* row_of, int32_t* skip, int32_t* own_lens,
+                             int64_t least, int32_t* group_starts, int32_t* prefix, int32_t* row_of, int32_t* skip, int32_t* own_lens,
                              void* stream) {
   if (!table || !lens || !groups || !group_starts || !prefix || !row_of || !skip || !own_lens)
     return fail(DFLASH_ERR_INVALID, "NULL pointer");
@@ -358,10 +358,12 @@ int dflash_paged_prefix_plan(const int32_t* table, int64_t table_ld, int max_pag
     return fail(DFLASH_ERR_INVALID, "max_rows %d outside [1, %d]", max_rows, DFLASH_Q4_MAX_ROWS);
   if (num_groups < 1 || num_groups > DFLASH_PAGED_MAX_SEQS)
     return fail(DFLASH_ERR_INVALID, "%d groups outside [1, %d]", num_groups, DFLASH_PAGED_MAX_SEQS);
+  if (least < 0) return fail(DFLASH_ERR_INVALID, "least %lld", (long long)least);
   if (own_lens == lens) return fail(DFLASH_ERR_INVALID, "own_lens must not be lens");
   PrefixPlanParams p{};
   p.table = table; p.lens = lens; p.starts = starts; p.groups = groups; p.table_ld = table_ld;
   p.n = n; p.g = num_groups; p.max_rows = max_rows; p.page_size = page_size; p.max_pages = max_pages; p.causal = causal != 0;
+  p.least = least;
   p.group_starts = group_starts; p.prefix = prefix; p.row_of = row_of; p.skip = skip; p.own_lens = own_lens;
   CK(prefix_plan_launch(p, static_cast<cudaStream_t>(stream)));
   return DFLASH_OK;

@@ -325,7 +325,7 @@ PyObject* attention(PyObject* const* a) {
   return a[10] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[10]);
 }
 
-// (table, lens, starts, max_rows, page_size, groups, causal) -> (group_starts, prefix, row_of, skip, own_lens)
+// (table, lens, starts, max_rows, page_size, groups, causal, least) -> (group_starts, prefix, row_of, skip, own_lens)
 PyObject* prefix_plan(PyObject* const* a) {
   const at::Tensor& lens = tensor(a[1], "lens");
   const int dev = cuda_index(lens);
@@ -340,7 +340,7 @@ PyObject* prefix_plan(PyObject* const* a) {
   const at::Tensor out = empty({3 * g + 1 + 2 * n}, at::kInt, dev);   // [group_starts | prefix | row_of | skip | own_lens]
   int32_t* o = out.data_ptr<int32_t>();
   call("dflash_paged_prefix_plan", lib.prefix_plan, dev, t.data, t.ld, t.width, l, starts, (int)n, int32(a[3], "max_rows"),
-       int32(a[4], "page_size"), groups, (int)g, (int)boolean(a[6]), o, o + g + 1, o + 2 * g + 1, o + 3 * g + 1, o + 3 * g + 1 + n);
+       int32(a[4], "page_size"), groups, (int)g, (int)boolean(a[6]), (int64_t)integer(a[7]), o, o + g + 1, o + 2 * g + 1, o + 3 * g + 1, o + 3 * g + 1 + n);
   return tuple(slice(out, 0, g + 1), slice(out, g + 1, g), slice(out, 2 * g + 1, g), slice(out, 3 * g + 1, n),
                slice(out, 3 * g + 1 + n, n));
 }
@@ -612,7 +612,7 @@ PyMethodDef methods[] = {
     method<reserve_forked, 11>("reserve_forked"),
     method<release_forked, 8>("release_forked"),
     method<copy_pages, 2>("copy_pages"),
-    method<prefix_plan, 7>("prefix_plan"),
+    method<prefix_plan, 8>("prefix_plan"),
     method<prefix_attention, 16>("prefix_attention"),
     method<rope, 10>("rope"),
     method<verify, 6>("verify"),

@@ -12,36 +12,67 @@ namespace dfl {
 constexpr int PP_THREADS = 512;
 
 __global__ void __launch_bounds__(PP_THREADS) prefix_plan_kernel(const PrefixPlanParams p) {
-  __shared__ int from, upto, first, members, limit;   // the group's requests; of those with query rows: first, number; pages
+  extern __shared__ int sm[];
+  int* bound = sm;                // [g + 1] where the groups begin, never falling
+  int* limits = bound + p.g + 1;  // [g] pages at most that members with query rows can share
+  int* counts = limits + p.g;     // [g] their number
+  __shared__ int first, limit, warp_top[PP_THREADS / 32];
+  __shared__ unsigned long long spared;
   const int k = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    from = 0;
     first = INT32_MAX;
-    members = 0;
-    limit = p.max_pages;
+    spared = 0;
   }
   griddep_wait();
   griddep_launch_dependents();
+  // groups[] as boundaries that never fall (device data that the host has not seen): running maxima
+  int carry = 0;
+  for (int i0 = 0; i0 <= p.g; i0 += PP_THREADS) {
+    const int i = i0 + threadIdx.x;
+    int v = i <= p.g ? min(max(__ldg(p.groups + i), 0), p.n) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = max(v, x);
+    }
+    __syncthreads();
+    if (lane == 31) warp_top[warp] = v;
+    __syncthreads();
+    v = max(v, carry);
+    for (int w = 0; w < PP_THREADS / 32; ++w) {
+      if (w < warp) v = max(v, warp_top[w]);
+      carry = max(carry, warp_top[w]);
+    }
+    if (i <= p.g) bound[i] = v;
+    if (i < p.g) {
+      limits[i] = p.max_pages;
+      counts[i] = 0;
+    }
+  }
   __syncthreads();
-  // groups[] as boundaries that never fall (device data that the host has not seen)
-  for (int i = threadIdx.x; i <= k; i += PP_THREADS) atomicMax(&from, min(max(__ldg(p.groups + i), 0), p.n));
-  __syncthreads();
-  if (threadIdx.x == 0) upto = max(from, min(max(__ldg(p.groups + k + 1), 0), p.n));
-  __syncthreads();
-  const int a = from, b = upto;
+  const int a = bound[k], b = bound[k + 1];
   auto start = [&](int i) { return p.starts ? __ldg(p.starts + i) : i * p.max_rows; };
   auto rows = [&](int i) { return start(i + 1) - start(i); };
   auto length = [&](int i) { return (int)min((long long)max(__ldg(p.lens + i), 0), (long long)p.max_pages * p.page_size); };
-  for (int i = a + threadIdx.x; i < b; i += PP_THREADS) {
+  // What sharing could spare, of all groups together: every CTA adds it up for itself.
+  for (int i = bound[0] + threadIdx.x; i < bound[p.g]; i += PP_THREADS) {
     const int m = rows(i);
     if (m <= 0) continue;
+    int lo = 0, hi = p.g - 1;
+    while (lo < hi) {   // the last group that begins at or before the request
+      const int mid = (lo + hi + 1) >> 1;
+      if (bound[mid] <= i) lo = mid; else hi = mid - 1;
+    }
     const int seen = max(length(i) - (p.causal ? m - 1 : 0), 0);   // keys that all its query rows see
-    atomicMin(&first, i);
-    atomicAdd(&members, 1);
-    atomicMin(&limit, seen / p.page_size);
+    atomicMin(&limits[lo], seen / p.page_size);
+    atomicAdd(&counts[lo], 1);
+    if (lo == k) atomicMin(&first, i);
   }
   __syncthreads();
-  if (threadIdx.x == 0 && members < 2) limit = 0;
+  for (int i = threadIdx.x; i < p.g; i += PP_THREADS)
+    if (counts[i] > 1) atomicAdd(&spared, (unsigned long long)(counts[i] - 1) * limits[i] * p.page_size);
+  __syncthreads();
+  if (threadIdx.x == 0) limit = counts[k] < 2 || spared < (unsigned long long)p.least ? 0 : limits[k];
   __syncthreads();
   const int ref = first == INT32_MAX ? a : first;
   const int32_t* one = p.table + (size_t)ref * p.table_ld;
@@ -82,7 +113,7 @@ __global__ void __launch_bounds__(PP_THREADS) prefix_plan_kernel(const PrefixPla
 
 cudaError_t prefix_plan_launch(const PrefixPlanParams& p, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs || p.g < 1 || p.g > kPagedMaxSeqs) return cudaErrorInvalidValue;
-  return launch_pdl(prefix_plan_kernel, dim3(p.g), dim3(PP_THREADS), 0, st, p);
+  return launch_pdl(prefix_plan_kernel, dim3(p.g), dim3(PP_THREADS), ((size_t)3 * p.g + 1) * sizeof(int), st, p);
 }
 
 }  // namespace dfl

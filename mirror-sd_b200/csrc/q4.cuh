@@ -106,6 +106,7 @@ struct PrefixPlanParams {
   const int32_t *table, *lens, *starts, *groups;   // starts NULL: max_rows rows each; groups [g + 1]
   long long table_ld;
   int n, g, max_rows, page_size, max_pages, causal;
+  long long least;                                 // cached rows that it must spare, of all groups, to share any
   int32_t *group_starts, *prefix, *row_of;         // [g + 1], [g] rows, [g]
   int32_t *skip, *own_lens;                        // [n] columns, [n]
 };

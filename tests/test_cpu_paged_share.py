@@ -118,8 +118,8 @@ def test_restatement_keeps_rows_apart():
 
 
 def test_prefix_attention_refuses_bad_arguments(pkg, lib):
-    def plan(table=P, ld=8, lens=P, n=4, max_rows=1, page=16, groups=P, g=2, own=Q):
-        return lib.dflash_paged_prefix_plan(table, ld, 8, lens, None, n, max_rows, page, groups, g, 1, P, P, P, P, own, None)
+    def plan(table=P, ld=8, lens=P, n=4, max_rows=1, page=16, groups=P, g=2, own=Q, least=0):
+        return lib.dflash_paged_prefix_plan(table, ld, 8, lens, None, n, max_rows, page, groups, g, 1, least, P, P, P, P, own, None)
 
     for kw in (dict(table=None), dict(lens=None), dict(groups=None), dict(own=None)):
         _refused(pkg, plan(**kw), "NULL")
@@ -130,6 +130,7 @@ def test_prefix_attention_refuses_bad_arguments(pkg, lib):
     _refused(pkg, plan(g=0), "groups")
     _refused(pkg, plan(g=2049), "groups")
     _refused(pkg, plan(own=P), "own_lens")
+    _refused(pkg, plan(least=-1), "least")
 
     size = lib.dflash_q4_prefix_workspace_size
     assert size(100, 1, 8, 32, 8) >= 100 * 32 * 130 * 4 + lib.dflash_q4_attention_workspace_size(8, 32, 8)

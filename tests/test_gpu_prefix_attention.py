@@ -46,7 +46,7 @@ class Groups:
 
     def attend(self, pkg, causal, scale=None, **kw):
         plan = pkg.paged_prefix_plan(self.d_table, self.d_lens, kw.pop("sizes", self.sizes), self.page, self.starts,
-                                     max(max(self.rows), 1), causal, kw.pop("max_group", None))
+                                     max(max(self.rows), 1), causal, kw.pop("max_group", None), kw.pop("least", 0))
         status = torch.zeros(1, dtype=torch.int32, device="cuda")
         out = pkg.q4_prefix_attention(self.q, self.pool, self.d_table, plan, scale, status=status, **kw)
         return out, plan, int(status)
@@ -119,14 +119,21 @@ def test_members_that_sit_out_or_hold_other_pages(pkg):
     assert float((out.double() - plain.double()).abs().max()) <= 2e-2 * float(plain.abs().max())
 
 
+def test_what_spares_little_is_not_shared(pkg):
+    d = Groups(pkg, [(160, [10, 20, 30], [1, 1, 2]), (96, [5, 5], [1, 1])], 16, 8, 2, seed=9)
+    for least, want in ((0, [160, 96]), (2 * 160 + 96, [160, 96]), (2 * 160 + 97, [0, 0]), (1 << 40, [0, 0])):
+        assert d.check(pkg, True, least=least).prefix.tolist() == want
+
+
 def test_requests_of_no_group_and_groups_on_the_device(pkg):
     d = Groups(pkg, [(0, [50], [1]), (160, [10, 20, 30], [1, 1, 2]), (0, [33], [2])], 16, 8, 2, seed=4)
     i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
     assert d.check(pkg, True, sizes=i32([1, 4]), max_group=3).prefix.tolist() == [160]
     assert d.check(pkg, True, sizes=i32([-3, 1, 4, 2, 99]), max_group=3).prefix.tolist() == [0, 160, 0, 0]   # kept ascending
     assert d.check(pkg, True, sizes=[5]).prefix.tolist() == [0]
-    _, _, status = d.attend(pkg, True, sizes=i32([1, 4]), max_group=1)
+    _, _, status = d.attend(pkg, True, sizes=i32([0, 5]), max_group=2)
     assert status == 64                                   # more query rows in a group than promised
+    assert not d.attend(pkg, True, sizes=i32([1, 4]), max_group=1)[1].shares
 
 
 @pytest.mark.parametrize("strength,scale", [(1.0, None), (300.0, None), (30.0, 1.0), (1.0, 1e-20), (3e4, 3e4)])
@@ -147,14 +154,14 @@ def test_without_starts_and_with_strided_queries(pkg):
     want, _, _ = d.attend(pkg, True)
     wide = torch.zeros(12, 20, 128, dtype=torch.float16, device="cuda")
     wide[:, 3:15] = d.q
-    plan = pkg.paged_prefix_plan(d.d_table, d.d_lens, [4], 32, max_rows=3, causal=True)
+    plan = pkg.paged_prefix_plan(d.d_table, d.d_lens, [4], 32, max_rows=3, causal=True, least=0)
     assert torch.equal(pkg.q4_prefix_attention(wide[:, 3:15], d.pool, d.d_table, plan), want)
     out = torch.empty_like(want)
     ws = pkg.q4_prefix_workspace(50, 5, 9, 12, 4)        # a larger one serves
     for _ in range(3):
         assert pkg.q4_prefix_attention(d.q, d.pool, d.d_table, plan, out=out, workspace=ws) is out
         assert torch.equal(out, want)
-    empty = pkg.paged_prefix_plan(d.d_table, d.d_lens, [4], 32, torch.zeros(5, dtype=torch.int32).cuda(), 3, True)
+    empty = pkg.paged_prefix_plan(d.d_table, d.d_lens, [4], 32, torch.zeros(5, dtype=torch.int32).cuda(), 3, True, least=0)
     assert pkg.q4_prefix_attention(d.q[:0], d.pool, d.d_table, empty).shape == (0, 12, 128)
 
 
@@ -173,7 +180,7 @@ def test_a_run_of_forked_requests_through_the_cache(pkg):
     cache.fork([0, 0, 3, 3], [1, 2, 4, 5], [333, 320, 100, 100])
     for new in ([1] * 6, [4, 4, 0, 3, 2, 4]):
         step = cache.reserve(new)
-        plan = cache.prefix_plan(step, [3, 3], max(new))
+        plan = cache.prefix_plan(step, [3, 3], max(new), least=0)
         assert plan.prefix.tolist() == [320, 96]
         for l in range(2):
             cache.append(l, pkg.apply_rope(rows(sum(new), 2), rope, step), rows(sum(new), 2), step)
@@ -202,7 +209,7 @@ def test_streams_and_graphs(pkg):
     groups, ws = torch.tensor([0, 4], dtype=torch.int32).cuda(), pkg.q4_prefix_workspace(10, 3, 4, 8, 2)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        plan = pkg.paged_prefix_plan(d.d_table, d.d_lens, groups, 16, d.starts, 3, True, max_group=4)
+        plan = pkg.paged_prefix_plan(d.d_table, d.d_lens, groups, 16, d.starts, 3, True, max_group=4, least=0)
         out = pkg.q4_prefix_attention(d.q, d.pool, d.d_table, plan, workspace=ws)
         with pytest.raises(ValueError, match="graph"):
             pkg.paged_prefix_plan(d.d_table, d.d_lens, [4], 16, d.starts, 3, True)
