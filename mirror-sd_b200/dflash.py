@@ -130,12 +130,20 @@ def context_layers(hidden_states, layer_ids):
     return [hidden_states[lid + 1] for lid in layer_ids]
 
 
-def sample(logits: torch.Tensor, temperature: float = 0.0) -> torch.Tensor:
-    """Greedy argmax, first index on ties (dflash.py:133-136).  Sampling with
-    temperature is part of the target-side loop and is not on this path."""
+def sample(logits: torch.Tensor, temperature: float = 0.0, uniforms: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Greedy argmax, first index on ties; from 1e-5 on a sample of softmax(logits /
+    temperature) (dflash.py:133-136), drawn on the device with ``uniforms``, one
+    number in [0, 1) for each row of logits (by default torch's)."""
     if temperature < 1e-5:
         return torch.argmax(logits, dim=-1)
-    raise NotImplementedError("temperature sampling is outside the draft forward")
+    if not logits.is_cuda:
+        raise NotImplementedError("sampling with a temperature runs on a CUDA device")
+    from .sampling import sample_tokens
+    rows = logits.reshape(-1, logits.shape[-1])
+    rows = rows if rows.dtype in (torch.float16, torch.bfloat16, torch.float32) else rows.float()
+    if uniforms is None:
+        uniforms = torch.rand(rows.shape[0], device=logits.device)
+    return sample_tokens(rows, uniforms.reshape(-1), temperature).to(torch.int64).reshape(logits.shape[:-1])
 
 
 # ----------------------------------------------------------------------------

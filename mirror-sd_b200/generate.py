@@ -1,4 +1,4 @@
-"""Greedy speculative decoding around the device draft model (the block-draft
+"""Speculative decoding around the device draft model (the block-draft
 loop of mirror_sd/generate.py:591-789).
 
 Per step:
@@ -14,7 +14,8 @@ Per step:
 
 With greedy sampling the output equals the target's own greedy decode,
 whatever the draft proposes; the draft only changes how many target calls
-that takes.
+that takes.  With a temperature, step 4 accepts drafts by their probability
+(``verify_drafts``) and the output is distributed as the target's own samples.
 
 The target is any object with
     embed(ids [1, n] int64) -> [1, n, H] bf16 on the draft's device
@@ -31,7 +32,8 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from .dflash import DFlashDraftModel, accept
+from .dflash import DFlashDraftModel, accept, sample
+from .sampling import verify_drafts
 
 
 @dataclass
@@ -64,8 +66,12 @@ class SpecDecodeStats:
 def spec_generate(target, draft: DFlashDraftModel, input_ids: Sequence[int], max_new_tokens: int,
                   stop_token_ids: Optional[Sequence[int]] = None,
                   sink_size: int = 64, window_size: int = 1024,
-                  soft_anchor: bool = False, anchor_top_k: int = 8) -> Tuple[List[int], SpecDecodeStats]:
-    """Greedy speculative generation.  Returns (prompt + generated ids, stats).
+                  soft_anchor: bool = False, anchor_top_k: int = 8, temperature: float = 0.0,
+                  generator: Optional[torch.Generator] = None) -> Tuple[List[int], SpecDecodeStats]:
+    """Speculative generation.  Returns (prompt + generated ids, stats).
+
+    Greedy below a ``temperature`` of 1e-5; above, tokens are sampled at it with
+    random numbers from ``generator`` (of the draft's device; by default torch's).
 
     ``soft_anchor``: from the second step on, the draft embeds block row 0 as
     the softmax-weighted sum of the top ``anchor_top_k`` tokens under the
@@ -78,6 +84,11 @@ def spec_generate(target, draft: DFlashDraftModel, input_ids: Sequence[int], max
     stats = SpecDecodeStats()
     dev = draft.device
     stop = set(stop_token_ids or [])
+    greedy = temperature < 1e-5
+
+    def numbers(n):
+        return torch.rand(1, n, device=dev, generator=generator)
+
     out = [int(t) for t in input_ids]
     n_prompt = len(out)
     t0 = time.perf_counter()
@@ -85,7 +96,7 @@ def spec_generate(target, draft: DFlashDraftModel, input_ids: Sequence[int], max
     # prefill: the prompt's logits give the first token, its features the first context
     tcache = target.make_cache()
     logits, feats = target.forward(torch.tensor([out], device=dev), tcache)
-    out.append(int(torch.argmax(logits[0, -1]).item()))
+    out.append(int(sample(logits[0, -1], temperature, None if greedy else numbers(1)).item()))
     target_hidden = feats
     stats.prefill_time = time.perf_counter() - t0
 
@@ -105,8 +116,12 @@ def spec_generate(target, draft: DFlashDraftModel, input_ids: Sequence[int], max
         verify_ids = torch.cat([torch.tensor([[anchor]], device=dev, dtype=torch.int64),
                                 drafts.to(torch.int64)], dim=1)
         logits, feats = target.forward(verify_ids, tcache)
-        posterior = torch.argmax(logits, dim=-1).to(torch.int32)         # [1, B]
-        acc, corr = accept(drafts, posterior)
+        if greedy:
+            posterior = torch.argmax(logits, dim=-1).to(torch.int32)     # [1, B]
+            acc, corr = accept(drafts, posterior)
+        else:
+            scores = logits if logits.dtype in (torch.float16, torch.bfloat16, torch.float32) else logits.float()
+            acc, corr = verify_drafts(scores, drafts.to(torch.int32), numbers(B), temperature)
         a = int(acc[0].item())                                            # one host sync per step
         new = drafts[0, :a].tolist() + [int(corr[0].item())]
         tcache.trim(B - (a + 1))                                          # rejected positions
