@@ -119,12 +119,7 @@ __device__ __forceinline__ void merge_slots(const Q4AttnParams& p, uint32_t mask
   }
   constexpr int END = PASS == kAttnPrefix ? kAttnPrefix : kAttnAll;   // (own rows went on from the group's)
   const int grp = p.by_nkv.of(sub), head0 = (sub - grp * p.nkv) * p.by_g.d;
-  Finish fin{0.f, 0.f};
-  if (whole) {
-    const int r = grp * QT + q, j = p.by_g.of(r);
-    if (j < it.rows)
-      fin = finish<END>(p, false, 0, M, l);
-  }
+  const Finish fin = finish<END>(p, false, 0, M, l);
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     if (whole) {
@@ -527,7 +522,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
             const int q = nt * 8 + 2 * c + x, r = r0 + q, j = p.by_g.of(r);
             const float m = PASS != kAttnPrefix ? 0.f : partial_max(negm[nt][x], qscale[nt][x]);
             Finish f{1.f, 0.f};
-            if (whole && j < cur.it.rows) f = finish<END>(p, false, 0, m, sum);
+            if (whole) f = finish<END>(p, false, 0, m, sum);
 #pragma unroll
             for (int t = 0; t < 8; t += 2) {
               const float v[4] = {o[t][nt][x], o[t][nt][2 + x], o[t + 1][nt][x], o[t + 1][nt][2 + x]};
