@@ -547,7 +547,7 @@ int dflash_rope(const void* x, int64_t x_row, int64_t x_head, int type, int rows
  *     place (p without the draft itself where there are no probs; p where nothing
  *     is left), from p behind the last draft: the first token whose running sum, in
  *     vocabulary order, passes uniforms[block - 1] times the whole sum.
- * NaN logits count as -inf (probability 0), others as clamped to +-1e30; a row
+ * vocab <= 2^22.  NaN logits count as -inf (probability 0), others as clamped to +-1e30; a row
  * with nothing above -inf refuses its draft, and its token is -1.  Rows behind
  * the first refused draft are not read. */
 int dflash_verify_drafts(const void* logits, int64_t seq_stride, int64_t row_stride, int type, int n, int block, int vocab,

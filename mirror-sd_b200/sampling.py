@@ -31,7 +31,7 @@ def verify_drafts(logits, drafts, uniforms, temperature: Union[float, torch.Tens
     running sum passes it.  num_drafts [n] int32: how many of its drafts a
     request uses, where not all.
 
-    NaN logits count as -inf; a row that leaves no token refuses its draft and
+    V is 2^22 at most.  NaN logits count as -inf; a row that leaves no token refuses its draft and
     gives token -1."""
     return N.load_paged().verify(logits, drafts, uniforms, temperature, draft_probs, num_drafts)
 

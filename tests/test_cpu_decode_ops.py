@@ -60,7 +60,7 @@ def test_verify_refuses_bad_arguments(pkg, lib):
     _refused(pkg, verify(u=None), "NULL")
     _refused(pkg, verify(out=None), "NULL")
     _refused(pkg, verify(type=-1), "type")
-    for kw in (dict(n=-1), dict(block=0), dict(vocab=0), dict(vocab=2 ** 31 - 1), dict(n=2 ** 28)):
+    for kw in (dict(n=-1), dict(block=0), dict(vocab=0), dict(vocab=2 ** 31 - 1), dict(vocab=2 ** 22 + 1), dict(n=2 ** 28)):
         _refused(pkg, verify(**kw), "block")
     for t in (-0.1, math.nan, math.inf):
         _refused(pkg, verify(temp=t), "temperature")

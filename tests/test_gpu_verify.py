@@ -139,6 +139,18 @@ def test_masked_rows(pkg, dtype):
     check(pkg, x, d, u, [1e-5, 1e-4, 50.0, 1e6, float("inf"), 0.9e-5, -1.0, float("nan"), 3e38, float("inf"), 2e-5, 1e10])
 
 
+def test_the_largest_vocabulary(pkg):
+    # rows that have no usable reference are read entry by entry, while the other warps wait
+    vocab = 2 ** 22
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(2, 3, vocab, generator=g).to(torch.float16)
+    x[0, 0, vocab - 2] = x[0, 1, 77] = float("inf")
+    x[0, 2, 5] = float("nan")
+    d = torch.tensor([[vocab - 2, 77], [vocab - 1, 0]], dtype=torch.int32)
+    u = torch.rand(2, 3, generator=g)
+    check(pkg, x.cuda(), d.cuda(), u.cuda(), [1.0, 0.7])
+
+
 def test_random_numbers_at_their_ends(pkg):
     x, d, _ = inputs(4, 3, 300, "f32", 15, keep=1.0)
     for v in (0.0, 1.0 - 2.0 ** -24, 1.0):
