@@ -162,6 +162,7 @@ struct Q4AttnParams {
   const int32_t* skip;               // kAttnOwn: columns of each request's table row that its group's pass covers
   float* pre_o;                      // what that pass leaves: [T, NQ, 128] sums, and their (m, l) [T, NQ]
   float2* pre_ml;
+  int weigh;                         // whether the few-rows kernel weighs items (q4_attention.cu)
 };
 // An ordinary call; the query rows of groups of requests over the rows that each
 // group shares, which leaves sums and statistics; the requests' own rows, joined

@@ -54,6 +54,7 @@ constexpr int QA_STAGE = QA_TILE / kQ4Rows * kQ4Block;
 constexpr int QA_LEAST = 4;
 constexpr int QA_ITEM = 3;                           // what an item's start and end cost beside its tiles, in tiles
 constexpr float QA_RAISE = 8.f;
+constexpr size_t QA_SMEM = 225 * 1024;               // dynamic shared memory at most, beside the kernel's static 1.3 KB
 
 // ---- fragments
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -146,8 +147,8 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
   // Passes over shared and own rows weigh an item's start and end as well, QA_ITEM
   // tiles, where there are items for every warp: an item is then that many units
   // followed by its tiles, and runs are cut by units.
-  int W = PASS == kAttnAll ? 0 : QA_ITEM;
-  int* ubase = base + p.n + 1;                                           // [n] first unit of each request
+  int W = PASS == kAttnAll || !p.weigh ? 0 : QA_ITEM;
+  int* ubase = base + p.n + 1;                                           // [n] first unit of each request, if weighed
   __shared__ int wtot[C::WARPS];
   __shared__ int slot_item[2 * C::WARPS];   // unit at which the partial's item starts, or -1
   __shared__ Item slot_info[2 * C::WARPS];
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(QaCfg<NT>::THREADS, 1) q4_attn_kernel(const Q4
             for (int x = 0; x < 4; ++x) o[t][nt][x] = 0.f;
         if (PASS == kAttnOwn && cur.j == 0 && has_prefix<PASS>(p, cur.it.seq)) {
           // the item's first tile goes on from what the pass over its group's rows left
-          // (joined at the item's end instead, 256 requests of 512 rows took 97 us, not 62)
+          // (joined at the item's end instead, 256 requests of 512 rows took 74 us, not 62)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -616,8 +617,12 @@ size_t q4_attn_part_floats(int max_rows, int nq, int nkv, int num_sms) {
 }
 
 template <int NT, int PASS>
-static cudaError_t launch(const Q4AttnParams& p, int num_sms, cudaStream_t st) {
-  const size_t smem = QaCfg<NT>::RING + QaCfg<NT>::WARPS * QaCfg<NT>::STAGES * 8 + ((size_t)p.n + 1) * (PASS == kAttnAll ? 4 : 8);
+static cudaError_t launch(Q4AttnParams p, int num_sms, cudaStream_t st) {
+  size_t smem = QaCfg<NT>::RING + QaCfg<NT>::WARPS * QaCfg<NT>::STAGES * 8 + ((size_t)p.n + 1) * sizeof(int);
+  // (beside the ring there is room for the units of about a thousand requests, which have items enough for
+  // even runs without)
+  p.weigh = PASS != kAttnAll && smem + (size_t)p.n * sizeof(int) <= QA_SMEM;
+  if (p.weigh) smem += (size_t)p.n * sizeof(int);
   DFL_TRY(cudaFuncSetAttribute(q4_attn_kernel<NT, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   return launch_pdl(q4_attn_kernel<NT, PASS>, dim3(num_sms), dim3(QaCfg<NT>::THREADS), smem, st, p);
 }

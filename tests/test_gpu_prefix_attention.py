@@ -136,6 +136,15 @@ def test_requests_of_no_group_and_groups_on_the_device(pkg):
     assert not d.attend(pkg, True, sizes=i32([1, 4]), max_group=1)[1].shares
 
 
+@pytest.mark.parametrize("nq,nkv,rows", [(2, 1, 1), (12, 1, 1), (4, 1, 9)])
+def test_as_many_requests_as_there_may_be(pkg, nq, nkv, rows):
+    # 2,048 requests in 64 groups, and in 1,024 pairs
+    d = Groups(pkg, [(16, [i % 3 for i in range(32)], [rows] * 32)] * 64, 16, nq, nkv, seed=13)
+    assert d.check(pkg, False).prefix.tolist() == [16] * 64
+    d = Groups(pkg, [(32, [1, 2], [rows, rows])] * 1024, 16, nq, nkv, seed=14)
+    assert d.check(pkg, False).prefix.tolist() == [32] * 1024
+
+
 @pytest.mark.parametrize("strength,scale", [(1.0, None), (300.0, None), (30.0, 1.0), (1.0, 1e-20), (3e4, 3e4)])
 def test_large_and_small_scores(pkg, strength, scale):
     """Weights that live on one side, on both, on one key, or on none in particular.  (Where scores pass 2^24 a
