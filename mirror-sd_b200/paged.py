@@ -233,9 +233,11 @@ def paged_prefix_plan(table, lens, groups, page_size: int, starts=None, max_rows
     elif max_group is None:
         raise ValueError("max_group is needed with groups on the device")
     else:
-        others = lens.numel() - (groups.numel() - 1)
-    # (known on the host where the table itself is too narrow for `least` rows to be spared)
+        others = lens.numel() - 1                 # at most: device groups may be empty
+    # (known on the host where the table itself is too narrow for `least` rows to be spared; the device, whose groups
+    # may not be what the host takes them for, is then told to share nothing either)
     shares = max_group > 1 and others * table.shape[1] * page_size >= max(least, 1)
+    least = least if shares else 1 << 62
     return PrefixPlan(*N.load_paged().prefix_plan(table, lens, starts, max_rows, page_size, groups, causal, least), starts,
                       max_rows, max_group, page_size, bool(causal), shares)
 

@@ -136,6 +136,17 @@ def test_requests_of_no_group_and_groups_on_the_device(pkg):
     assert not d.attend(pkg, True, sizes=i32([1, 4]), max_group=1)[1].shares
 
 
+def test_groups_on_the_device_that_the_host_rule_misjudges(pkg):
+    # one group of three beside empty ones, and groups of three that the caller states as groups of one
+    d = Groups(pkg, [(128, [30, 1, 70], [2, 2, 2])], 64, 8, 2, seed=12)
+    bounds = torch.tensor([0, 0, 0, 3, 3], dtype=torch.int32, device="cuda")
+    assert d.check(pkg, True, sizes=bounds, max_group=3).prefix.tolist()[2] == 128
+    assert d.check(pkg, True, sizes=bounds, max_group=3, least=256).prefix.tolist()[2] == 128
+    assert d.check(pkg, True, sizes=bounds, max_group=3, least=257).prefix.tolist() == [0] * 4
+    whole = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    assert d.check(pkg, True, sizes=whole, max_group=1).prefix.tolist() == [0]
+
+
 @pytest.mark.parametrize("nq,nkv,rows", [(2, 1, 1), (12, 1, 1), (4, 1, 9)])
 def test_as_many_requests_as_there_may_be(pkg, nq, nkv, rows):
     # 2,048 requests in 64 groups, and in 1,024 pairs
