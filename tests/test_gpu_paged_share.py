@@ -159,6 +159,15 @@ def test_page_copies(pkg, page, nkv, layers):
         assert torch.equal(p, w)
 
 
+def test_copies_of_pages_beyond_4_gb(pkg):
+    pool = torch.zeros(16000, 8, 16, 2304, dtype=torch.uint8, device="cuda")
+    pool[3] = torch.randint(0, 256, (8, 16, 2304), device="cuda", dtype=torch.uint8)
+    pkg.q4_copy_pages([pool], torch.tensor([[3, 15999, 256], [-1, -1, 0]], dtype=torch.int32).cuda())
+    pkg.q4_copy_pages([pool], torch.tensor([[15999, 7, 100]], dtype=torch.int32).cuda())
+    assert pool.nbytes > 1 << 32 and torch.equal(pool[15999], pool[3])
+    assert torch.equal(pool[7, :, :7], pool[3, :, :7]) and not bool(pool[7, :, 7:].any()) and not bool(pool[15998].any())
+
+
 @pytest.mark.parametrize("capturable", [False, True])
 @pytest.mark.parametrize("page,seed", [(16, 0), (64, 1)])
 def test_lives_of_forked_requests_keep_their_rows(pkg, capturable, page, seed):

@@ -13,15 +13,15 @@ class Groups:
     """Requests in groups: (rows shared, [rows of their own], [query rows]) each, on shuffled pages.  Shared rows are
     whole pages plus, where `prefix` is none, rows that the members hold alike on pages of their own."""
 
-    def __init__(self, pkg, groups, page, nq, nkv, dtype=torch.float16, seed=0, strength=1.0):
+    def __init__(self, pkg, groups, page, nq, nkv, dtype=torch.float16, seed=0, strength=1.0, base=0):
         rng, g = np.random.default_rng(seed), torch.Generator().manual_seed(seed)
         self.page, self.nq, self.nkv, self.sizes = page, nq, nkv, [len(own) for _, own, _ in groups]
         cdiv = lambda a: -(-a // page)
         self.lens = [p + o for p, own, _ in groups for o in own]
         self.rows = [r for _, _, rows in groups for r in rows]
         pages = sum(cdiv(p) + sum(cdiv(p + o) - p // page for o in own) for p, own, _ in groups)
-        perm = iter(rng.permutation(pages + 5).astype(np.int32).tolist())
-        self.pool = pkg.q4_pool(pages + 5, nkv, page)
+        perm = iter((base + rng.permutation(pages + 5)).astype(np.int32).tolist())
+        self.pool = pkg.q4_pool(base + pages + 5, nkv, page)
         self.table = np.full((len(self.lens), max(1, max(map(cdiv, self.lens)))), -1, np.int32)
         self.ks, self.vs, i = [], [], 0
         make = lambda n: [(torch.randn(n, nkv, 128, generator=g) * s).to(dtype) for s in (strength, 0.5)]
@@ -35,7 +35,7 @@ class Groups:
                 self.table[i, :len(mine)] = mine
                 if p + o:
                     pos = np.arange(p + o)
-                    slots = torch.from_numpy((np.array(mine)[pos // page] * page + pos % page).astype(np.int32)).cuda()
+                    slots = torch.from_numpy((np.array(mine, np.int64)[pos // page] * page + pos % page).astype(np.int32)).cuda()
                     pkg.q4_append(k.cuda(), v.cuda(), slots, self.pool)
                 self.ks.append(U.q4_values(k))
                 self.vs.append(U.q4_values(v))
@@ -145,6 +145,24 @@ def test_groups_on_the_device_that_the_host_rule_misjudges(pkg):
     assert d.check(pkg, True, sizes=bounds, max_group=3, least=257).prefix.tolist() == [0] * 4
     whole = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
     assert d.check(pkg, True, sizes=whole, max_group=1).prefix.tolist() == [0]
+
+
+@pytest.mark.parametrize("rows", [1, 5, 33])
+def test_pages_beyond_4_gb(pkg, rows):
+    d = Groups(pkg, [(512, [3, 100, 64], [rows] * 3)], 256, 16, 8, seed=15, base=16000)
+    assert d.pool.nbytes > 1 << 32
+    # whole pages that the first member's first row sees: of 515 - (rows - 1) rows
+    assert d.check(pkg, True).prefix.tolist() == [(516 - rows) // 256 * 256]
+
+
+def test_no_rows_and_nobody_with_rows(pkg):
+    d = Groups(pkg, [(64, [3, 5], [0, 0]), (64, [2, 2], [0, 0])], 64, 4, 2, seed=16)
+    plan = pkg.paged_prefix_plan(d.d_table, d.d_lens, d.sizes, 64, d.starts, 4, True, least=0)
+    assert plan.prefix.tolist() == [0, 0] and plan.own_lens.tolist() == d.lens
+    assert pkg.q4_prefix_attention(d.q, d.pool, d.d_table, plan).shape == (0, 4, 128)
+    out = torch.full((3, 4, 128), 5.0, dtype=torch.float16, device="cuda")     # rows that no request owns
+    pkg.q4_prefix_attention(torch.zeros_like(out), d.pool, d.d_table, plan, out=out)
+    assert bool((out == 5).all())
 
 
 @pytest.mark.parametrize("nq,nkv,rows", [(2, 1, 1), (12, 1, 1), (4, 1, 9)])

@@ -151,6 +151,22 @@ def test_the_largest_vocabulary(pkg):
     check(pkg, x.cuda(), d.cuda(), u.cuda(), [1.0, 0.7])
 
 
+def test_rows_past_32_bits(pkg):
+    n, block, vocab = 3, 3, 1001
+    x, d, u = inputs(n, block, vocab, "f16", 12)
+    wide = torch.empty(n * block, 1 << 28, dtype=torch.float16, device="cuda").view(n, block, -1)     # 4.8 GB
+    wide[:, :, 7:7 + vocab] = x
+    view = wide[:, :, 7:7 + vocab]
+    assert check(pkg, view, d, u, [1.0, 0.7, 0.0]) == check(pkg, x, d, u, [1.0, 0.7, 0.0])
+
+
+def test_no_requests(pkg):
+    none = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="cuda")
+    accepted, tokens = pkg.verify_drafts(none(0, 4, 100), none(0, 3, dtype=torch.int32), none(0, 4))
+    assert accepted.shape == tokens.shape == (0,)
+    assert pkg.sample_tokens(none(0, 100), none(0)).shape == (0,)
+
+
 def test_random_numbers_at_their_ends(pkg):
     x, d, _ = inputs(4, 3, 300, "f32", 15, keep=1.0)
     for v in (0.0, 1.0 - 2.0 ** -24, 1.0):
