@@ -61,33 +61,31 @@ constexpr float QB_RAISE = 8.f;
 template <int N_>
 struct QbCfg {
   static constexpr int N = N_;
-  // Wide: four sides take a quarter of every tile's columns each, in place of all
-  // columns of every other tile; one decoded tile then serves 128 columns.  (Two
-  // sides of 64 columns: 3,840 cycles a tile.)
+  // Wide: query rows as the instruction's rows, cached rows as its columns (below)
   static constexpr bool WIDE = N > 80;
-  static constexpr int SIDES = WIDE ? 4 : 2;                  // of 4 softmax warps each
-  static constexpr int HN = WIDE ? N / SIDES : N, CH = HN / 16;   // columns of a side
+  static constexpr int CH = N / 16;
   // Query buffers and packed stages.  With 80 columns shared memory holds two and
   // two or one and three (8 requests of 16,384 rows, 160 query rows: 167 and 166 us).
   static constexpr int QB = N <= 64 ? 2 : 1;
   static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S)
   static constexpr int NS = N <= 64 ? 4 : 3;
-  static constexpr bool AHEAD = HN <= 64;       // registers for the next 16 scores
+  static constexpr bool AHEAD = N <= 64;        // registers for the next 16 scores
   static constexpr int SEGS = WIDE ? 4 : 8;     // ring of item records (items run ahead by an S buffer each, and one)
-  static constexpr int P_BYTES = (N + 63) / 64 * 16384;       // 64-column chunks of [128 rows][128 B]
+  static constexpr int P_BYTES = (N + 63) / 64 * 16384;       // 64-column chunks of [128 rows][128 B] (wide: of K)
   static constexpr int V_OFF = 0, V_BYTES = 32768;
   static constexpr int P_OFF = V_OFF + 2 * V_BYTES;
   static constexpr int Q_OFF = P_OFF + 2 * P_BYTES, Q_BYTES = N * 256;
   static constexpr int RING_OFF = Q_OFF + QB * Q_BYTES;
   static constexpr int MISC_OFF = RING_OFF + NS * QB_STAGE;
-  static constexpr uint32_t K_COL = 0, O_COL = 128, S_COL = 128 + (WIDE ? N : 2 * N);   // 2 x 64 for K, N for each O and S
+  // 2 x 64 for K, N for each O and S (wide: N for each S, which P takes the place of, and each O)
+  static constexpr uint32_t K_COL = 0, O_COL = WIDE ? 2 * N : 128, S_COL = WIDE ? 0 : 128 + 2 * N;
   static constexpr int SLOT = N * 130;          // floats of a partial: O [N][128], m [N], l [N]
   // warps: softmax, side by side (even tiles 0-3, odd tiles 4-7), then the others, all
   // in whole warpgroups, whose registers are dealt out anew after the common start
-  static constexpr int KDEC = 4 * SIDES, VDEC = KDEC + 4, MMA = VDEC + 4, LOAD = MMA + 1, QUERY = MMA + 2, MMA2 = MMA + 3;
-  static constexpr int THREADS = 32 * (MMA + 4), SOFT = 128 * SIDES;
-  // registers a thread at the start: 96, 640 * 96 = 256 * 144 + 384 * 64 (wide: 72, 896 * 72 > 512 * 88 + 384 * 48)
-  static constexpr int SOFT_REGS = WIDE ? 88 : 144, REST_REGS = WIDE ? 48 : 64;
+  static constexpr int KDEC = 8, VDEC = 12, MMA = 16, LOAD = 17, QUERY = 18, MMA2 = 19;
+  static constexpr int THREADS = 640;
+  // registers a thread at the start: 96, 640 * 96 = 256 * 144 + 384 * 64
+  static constexpr int SOFT_REGS = 144, REST_REGS = 64;
 };
 struct QbSeg {          // a run of tiles of one item
   Item it;
@@ -109,13 +107,13 @@ struct QbMisc {
   int2 tile[16];                  // row blocks copied and QB_SEEN, rows below the request's end
   QbSeg seg[C::SEGS];
   alignas(16) float qf[C::SEGS][C::N];        // score factors
-  alignas(16) float negm[C::SIDES][C::HN];           // minus the columns' references, of either side
-  alignas(16) float fac[C::SIDES][C::HN];            // rescale factors; at the end what O is multiplied by
+  alignas(16) float negm[2][C::N];            // minus the columns' references, of either side
+  alignas(16) float fac[2][C::N];             // rescale factors; at the end what O is multiplied by
   alignas(16) float pre[C::N];                // and what the sums over the group's rows are (kAttnOwn)
-  int cmax[C::SIDES][C::HN];                // column maxima as ordered integers
+  int cmax[2][C::N];                          // column maxima as ordered integers
   alignas(16) int cend[C::N];                 // where each column's keys end
   alignas(16) int coff[C::N];                 // output row of each column, or -1
-  float lsum[4 * C::SIDES][C::HN];
+  float lsum[C::WIDE ? 2 : 8][C::N];
   int4 shared;                    // the item that starts here and reaches past the last tile (q4_tc_shared)
 };
 
@@ -248,12 +246,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// largest value of a warp's lanes
-__device__ __forceinline__ float redux_max(float v) {
-  float d;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
-  return d;
-}
 // order-preserving map of floats to ints (-inf lowest)
 __device__ __forceinline__ int float_key(float f) {
   const int i = __float_as_int(f);
@@ -278,6 +270,167 @@ __host__ __device__ __forceinline__ int4* q4_tc_shared(float* part, int n, int g
   return reinterpret_cast<int4*>(part + (size_t)grid * 2 * n * 130);
 }
 
+// ---- softmax of the wide form: of the tiles t with t & 1 == x; thread = query row.
+// A row's scores lie in one lane, so its reference and sum are the thread's own:
+// no votes and no exchange between lanes.  P, as f16, takes the place of the scores
+// that are read.
+template <class C, class Sharers>
+__device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& ms, uint32_t tmem, int c0, int c1,
+                                             volatile int* dead, Sharers sharers) {
+  constexpr int N = C::N;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = warp >> 2, row = threadIdx.x & (N - 1), G = p.by_g.d;
+  const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+  const uint32_t s_t = tmem + C::S_COL + x * N + lanes, o_all = tmem + C::O_COL + lanes, o_t = o_all + x * N;
+  int u = c0, t0 = 0;   // the item's first tile, counted in the CTA
+#pragma unroll 1
+  for (int seg = 0; u < c1; ++seg) {
+    // S of the item's first tile is only issued once its record is there
+    if ((t0 & 1) == x) qb_wait(&ms.s_ready[x], (t0 >> 1) & 1, dead);
+    const QbSeg& sg = ms.seg[seg % C::SEGS];
+    // after an expired wait there may be no record: run to the end, writing nothing
+    const bool bad = named_bar_or<256>(3, *dead);
+    Item it{};
+    if (!bad) it = sg.it;
+    const int nt = bad ? c1 - u : sg.nt, j0 = bad ? 0 : sg.j0, sub = sg.sub, item0 = sg.item0;
+    const int r = sg.q0 + row, j = p.by_g.of(r);
+    const long long at = j < it.rows ? (long long)(it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;   // row of the sums
+    const float f = score_factor(ms.qf[seg % C::SEGS][row]);
+    float negm = kUnset;   // minus the reference
+    float2 l = make_float2(0.f, 0.f);
+
+#pragma unroll 1
+    for (int k = (t0 & 1) == x ? 0 : 1; k < nt; k += 2) {
+      const int t = t0 + k;
+      if (k > 0) qb_wait(&ms.s_ready[x], (t >> 1) & 1, dead);
+      tc_fence_after();
+      const int2 info = ms.tile[t & 15];
+      if (!(info.x & QB_SEEN)) {   // some key is hidden: its scores to -inf, where they lie
+#pragma unroll 1
+        for (int c = 0; c < C::CH; ++c) {
+          const int left = (info.x >> c & 1) ? info.y - 16 * c : 0;
+          if (left >= 16) continue;
+          uint32_t s[16];
+          tmem_ld16(s_t + 16 * c, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = i < left ? s[i] : 0xff800000u;
+          tmem_st16(s_t + 16 * c, s);
+        }
+        tmem_st_wait();
+      }
+      uint32_t s[2][32];
+      tmem_ld32(s_t, s[0]);
+      float top = -INFINITY, top2 = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait();
+        if (c < 3) tmem_ld32(s_t + 32 * (c + 1), s[(c + 1) & 1]);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          top = max3(top, __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
+          top2 = max3(top2, __uint_as_float(s[c & 1][i + 2]), __uint_as_float(s[c & 1][i + 3]));
+        }
+      }
+      tmem_ld32(s_t, s[0]);
+      top = fmaxf(top, top2);
+      const float rise = (top + negm) * f;
+      if (__any_sync(0xffffffffu, rise > QB_RAISE)) {   // (a row without a reference: any visible key)
+        float fac = 1.f;
+        if (rise > QB_RAISE) {
+          fac = exp2_fast(-rise);
+          negm = -top;
+        }
+        l.x *= fac;
+        l.y *= fac;
+        if (k >= 2) {   // O holds this side's tiles before t
+          tmem_ld_wait();
+#pragma unroll 1
+          for (int c = 0; c < C::CH; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_t + 16 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fac);
+            tmem_st16(o_t + 16 * c, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float2 nm = make_float2(negm, negm), ff = make_float2(f, f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait();
+        if (c < 3) tmem_ld32(s_t + 32 * (c + 1), s[(c + 1) & 1]);
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float2 y = mul2(add2(make_float2(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), nm), ff);
+          y.x = exp2_fast(y.x);
+          y.y = exp2_fast(y.y);
+          l = add2(l, y);
+          w[i] = pack_f16x2(y.x, y.y);
+        }
+        tmem_st16(s_t + 16 * c, w);   // (over scores that this warp has read)
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&ms.p_ready[x], lane);
+    }
+    u += nt;
+
+    // ---- the item's run is over: both sides' sums and O, half the channels each
+    const bool whole = bad || (j0 == 0 && nt == it.ntile);
+    const int border = item0 < c0 ? 0 : 1;
+    const int last = t0 + nt - 1;   // the other side's last tile is last - 1
+    ms.negm[x][row] = negm;
+    ms.lsum[x][row] = l.x + l.y;
+    qb_wait(&ms.pvdone[last & 1], (last >> 1) & 1, dead);
+    if (nt > 1) qb_wait(&ms.pvdone[(last - 1) & 1], ((last - 1) >> 1) & 1, dead);
+    named_bar_sync(3, 256);
+    tc_fence_after();
+    // (a side without a tile, or a row without a key, has the sum 0 and counts nothing)
+    const float ma = -ms.negm[0][row], mb = -ms.negm[1][row], m = fmaxf(ma, mb);
+    const float wa = ma == -kUnset ? 0.f : exp2_fast((ma - m) * f), wb = mb == -kUnset ? 0.f : exp2_fast((mb - m) * f);
+    const float sum = wa * ms.lsum[0][row] + wb * ms.lsum[1][row], top = partial_max(-m, f);
+    float* part = p.part + ((size_t)blockIdx.x * 2 + border) * C::SLOT;
+    float* to = whole ? p.pre_o + at * 128 : part + row * 128;
+    const bool write = !whole || at >= 0;
+    if (x == 0) {
+      if (!whole) {
+        part[N * 128 + row] = top;
+        part[N * 129 + row] = sum;
+      } else if (at >= 0) {
+        p.pre_ml[at] = make_float2(top, sum);
+      }
+    }
+    // (the O of a side without a tile may hold anything: the other's is read in its place)
+    const uint32_t o_a = nt > 1 || (t0 & 1) == 0 ? o_all : o_all + N, o_b = nt > 1 || (t0 & 1) == 1 ? o_all + N : o_all;
+#pragma unroll 1
+    for (int c = 4 * x; c < 4 * x + 4; ++c) {
+      uint32_t oa[16], ob[16];
+      __syncwarp();
+      tmem_ld16(o_a + 16 * c, oa);
+      tmem_ld16(o_b + 16 * c, ob);
+      tmem_ld_wait();
+      if (write) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(__uint_as_float(oa[i + e]), wa, __uint_as_float(ob[i + e]) * wb);
+          *reinterpret_cast<float4*>(to + 16 * c + i) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+    }
+    tc_fence_before();
+    warp_arrive(&ms.o_free, lane);
+    // (merged by the item's first CTA's entry; the others' partials follow its own)
+    if (!whole && threadIdx.x == 0 && border == 1) ms.shared = make_int4(it.row0, it.rows, sub, sharers(item0, it.ntile));
+    t0 += nt;
+  }
+  if (threadIdx.x == 0) q4_tc_shared(p.part, N, gridDim.x)[blockIdx.x] = ms.shared;
+}
+
 template <int N, int PASS>
 __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const Q4AttnParams p) {
   using C = QbCfg<N>;
@@ -295,11 +448,11 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ms.kready[i], 4); mbar_init(&ms.kfree[i], 1);
       mbar_init(&ms.vready[i], 4); mbar_init(&ms.pvdone[i], 1);
-      mbar_init(&ms.p_ready[i], C::WIDE ? 4 * C::SIDES : 4);
+      mbar_init(&ms.p_ready[i], 4);
       mbar_init(&ms.q_ready[i], 1); mbar_init(&ms.q_free[i], 1);
     }
-    mbar_init(&ms.o_free, 4 * C::SIDES);
-    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], C::WIDE ? 4 * C::SIDES : 4); }
+    mbar_init(&ms.o_free, 8);
+    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], 4); }
     ms.abort = 0;
     ms.shared = make_int4(0, 0, 0, 0);
     ms.run[0] = ms.run[1] = 0;
@@ -311,7 +464,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     tmem_alloc(&ms.tmem, 512);
     tmem_relinquish();
   }
-  for (int i = threadIdx.x; i < C::SIDES * C::HN; i += C::THREADS) ms.cmax[0][i] = float_key(-INFINITY);
+  for (int i = threadIdx.x; i < 2 * N; i += C::THREADS) ms.cmax[0][i] = float_key(-INFINITY);
 
   // The CTA's run of tiles [c0, c1), from the lengths.
   auto scan = [&](int v, int* sum) {   // what the threads before hold, and the sum of all
@@ -475,14 +628,14 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
   // (registers go from the roles that move data to the two that compute)
   if (warp < C::KDEC) {
     set_registers<C::SOFT_REGS, true>();
-    // ---- softmax of the tiles t with t & 1 == x (wide: of columns 32 x .. of every
-    // tile); thread = cached row, and channel at the end
+    if constexpr (C::WIDE) {
+      wide_softmax<C>(p, ms, tmem, c0, c1, dead, sharers);
+    } else {
+    // ---- softmax of the tiles t with t & 1 == x; thread = cached row, and channel at the end
     const int x = warp >> 2, gt = threadIdx.x & 127;
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    constexpr int HN = C::HN;
-    const int col0 = C::WIDE ? x * HN : 0;   // the side's first column of the item
-    const uint32_t o_t = tmem + C::O_COL + x * HN + lanes;
+    const uint32_t o_t = tmem + C::O_COL + x * N + lanes;
     const int window = p.window > 0 ? p.window : 1 << 30;   // no cache is longer
     float* negm = ms.negm[x];
     float* facs = ms.fac[x];
@@ -490,38 +643,37 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
 #pragma unroll 1
     for (int seg = 0; u < c1; ++seg) {
       // S of the item's first tile is only issued once its record is there
-      if (C::WIDE || (t0 & 1) == x) qb_wait(&ms.s_ready[t0 % C::SB], (t0 / C::SB) & 1, dead);
+      if ((t0 & 1) == x) qb_wait(&ms.s_ready[t0 % C::SB], (t0 / C::SB) & 1, dead);
       const QbSeg& sg = ms.seg[seg % C::SEGS];
       // after an expired wait there may be no record: run to the end, writing nothing
-      const bool bad = named_bar_or<C::SOFT>(1 + C::SIDES, *dead);
+      const bool bad = named_bar_or<256>(3, *dead);
       Item it{};
       if (!bad) it = sg.it;
       const int nt = bad ? c1 - u : sg.nt, j0 = bad ? 0 : sg.j0;
       const float* qf = ms.qf[seg % C::SEGS];
       const bool uniform = sg.uniform;
       const float f = p.factor;
-      if (gt < HN) {
-        const int r = sg.q0 + col0 + gt, j = p.by_g.of(r);
+      if (gt < N) {
+        const int r = sg.q0 + gt, j = p.by_g.of(r);
         const bool real = j < it.rows;
         negm[gt] = real ? kUnset : 0.f;
-        if (C::WIDE || x == 0) {
-          ms.cend[col0 + gt] = real ? (p.causal ? it.L - it.rows + j + 1 : it.L) : 0;
-          ms.coff[col0 + gt] = real ? (it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;
+        if (x == 0) {
+          ms.cend[gt] = real ? (p.causal ? it.L - it.rows + j + 1 : it.L) : 0;
+          ms.coff[gt] = real ? (it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;
         }
       }
-      named_bar_sync(1 + C::SIDES, C::SOFT);
-      float2 l[HN / 2];
+      named_bar_sync(3, 256);
+      float2 l[N / 2];
 #pragma unroll
-      for (int i = 0; i < HN / 2; ++i) l[i] = make_float2(0.f, 0.f);
+      for (int i = 0; i < N / 2; ++i) l[i] = make_float2(0.f, 0.f);
 
 #pragma unroll 1
-      for (int k = C::WIDE || (t0 & 1) == x ? 0 : 1; k < nt; k += C::WIDE ? 1 : 2) {
+      for (int k = (t0 & 1) == x ? 0 : 1; k < nt; k += 2) {
         const int t = t0 + k;
-        const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + col0 + lanes;
-        // (of two sides, each has a P of its own)
-        uint8_t* const p_at = smem + C::P_OFF + (t & 1) * C::P_BYTES;
+        const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + lanes;
+        uint8_t* const p_at = smem + C::P_OFF + x * C::P_BYTES;
         uint8_t* const pr = p_at + row * 128;
-        // P is read, and this side's O holds the tiles before t (wide: before t - 1)
+        // P is read, and this side's O holds the tiles before t
         auto wait_pv = [&]() {
           if (t >= 2) qb_wait(&ms.pvdone[t & 1], ((t >> 1) - 1) & 1, dead);
         };
@@ -547,12 +699,12 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           } else {
             const float inv = 1.f / f;
 #pragma unroll 1
-            for (int c = 0; c < HN; c += 4) {
+            for (int c = 0; c < N; c += 4) {
               uint32_t s[4];
               tmem_ld4(s_t + c, s);
               tmem_ld_wait();
-              const int4 e = *reinterpret_cast<const int4*>(&ms.cend[col0 + c]);
-              const float4 w = *reinterpret_cast<const float4*>(&qf[col0 + c]);
+              const int4 e = *reinterpret_cast<const int4*>(&ms.cend[c]);
+              const float4 w = *reinterpret_cast<const float4*>(&qf[c]);
               auto one = [&](uint32_t v, int end, float by) {
                 const bool seen = (key < end) & ((key < p.sink) | (key >= end - window));   // (no branch)
                 return seen ? __float_as_uint(__uint_as_float(v) * (by * inv)) : 0xff800000u;
@@ -601,16 +753,15 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
               w[i] = pack_f16x2(y[i].x, y[i].y);
             }
             if (c == 0) wait_pv();
-            const int cc = C::WIDE ? x * C::CH + c : c;   // 16 columns of the item
-            uint8_t* d = pr + (cc >> 2) * 16384;
-            *reinterpret_cast<uint4*>(d + (((2 * (cc & 3)) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(d + (((2 * (cc & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            uint8_t* d = pr + (c >> 2) * 16384;
+            *reinterpret_cast<uint4*>(d + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(d + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
           }
           return C::CH;
         };
         // One round; a second one with new references if the first finds a score
         // that passes its column's by more than 2^8.
-        bool raise = k < (C::WIDE ? 1 : 2);   // this side's first tile of the item
+        bool raise = k < 2;   // this side's first tile of the item
         int done = 0;
 #pragma unroll 1
         for (int round = 0; round < 2; ++round) {
@@ -618,45 +769,29 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
             // Column maxima of the tile over the lanes, 16 columns at a time through
             // this side's P (its last reader is done), then over the warps.
             wait_pv();
-            if constexpr (C::WIDE) {   // (the sides' columns of P interleave; a side has 32, one a lane)
-              float mine = -INFINITY;
+            float* stage = reinterpret_cast<float*>(p_at) + (warp & 3) * (16 * 36);
 #pragma unroll 1
-              for (int c = 0; c < C::CH; ++c) {
-                uint32_t s[16];
-                tmem_ld16(s_t + 16 * c, s);
-                tmem_ld_wait();
+            for (int c = 0; c < C::CH; ++c) {
+              uint32_t s[16];
+              tmem_ld16(s_t + 16 * c, s);
+              tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float top = redux_max(__uint_as_float(s[i]));
-                  if (lane == 16 * c + i) mine = top;
-                }
+              for (int i = 0; i < 16; ++i) stage[i * 36 + lane] = __uint_as_float(s[i]);
+              __syncwarp();
+              float top = -INFINITY, top2 = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(stage + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * i);
+                top = max3(top, v.x, v.y);
+                top2 = max3(top2, v.z, v.w);
               }
-              atomicMax(&ms.cmax[x][lane], float_key(mine));
-            } else {
-              float* stage = reinterpret_cast<float*>(p_at) + (warp & 3) * (16 * 36);
-  #pragma unroll 1
-              for (int c = 0; c < C::CH; ++c) {
-                uint32_t s[16];
-                tmem_ld16(s_t + 16 * c, s);
-                tmem_ld_wait();
-  #pragma unroll
-                for (int i = 0; i < 16; ++i) stage[i * 36 + lane] = __uint_as_float(s[i]);
-                __syncwarp();
-                float top = -INFINITY, top2 = -INFINITY;
-  #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float4 v = *reinterpret_cast<const float4*>(stage + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * i);
-                  top = max3(top, v.x, v.y);
-                  top2 = max3(top2, v.z, v.w);
-                }
-                top = fmaxf(top, top2);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                if (!(lane & 1)) atomicMax(&ms.cmax[x][16 * c + (lane >> 1)], float_key(top));
-                __syncwarp();
-              }
+              top = fmaxf(top, top2);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+              if (!(lane & 1)) atomicMax(&ms.cmax[x][16 * c + (lane >> 1)], float_key(top));
+              __syncwarp();
             }
             named_bar_sync(1 + x, 128);
-            if (gt < HN) {
+            if (gt < N) {
               const float nm = negm[gt], top = key_float(ms.cmax[x][gt]);
               const float rise = (top + nm) * p.factor;
               float fac = 1.f;
@@ -668,8 +803,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
               ms.cmax[x][gt] = float_key(-INFINITY);
             }
             named_bar_sync(1 + x, 128);
-            if (k >= (C::WIDE ? 1 : 2)) {
-              if (C::WIDE) qb_wait(&ms.pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1, dead);   // O holds all tiles before t
+            if (k >= 2) {
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < C::CH; ++c) {
@@ -682,7 +816,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
               }
               tmem_st_wait();
 #pragma unroll
-              for (int i = 0; i < HN / 2; ++i) {
+              for (int i = 0; i < N / 2; ++i) {
                 const float2 fac = *reinterpret_cast<const float2*>(&facs[2 * i]);
                 l[i].x *= fac.x;
                 l[i].y *= fac.y;
@@ -711,23 +845,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
       const int last = t0 + nt - 1;   // the other side's last tile is last - 1
       qb_wait(&ms.pvdone[last & 1], (last >> 1) & 1, dead);
       if (nt > 1) qb_wait(&ms.pvdone[(last - 1) & 1], ((last - 1) >> 1) & 1, dead);
-      if constexpr (C::WIDE) {
-        // lane i ends with the sum of column i: halves of the columns go to the lanes that keep them
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          v[2 * i] = l[i].x;
-          v[2 * i + 1] = l[i].y;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2)
-#pragma unroll
-          for (int i = 0; i < o; ++i) {
-            const float give = lane & o ? v[i] : v[i + o], keep = lane & o ? v[i + o] : v[i];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-          }
-        ms.lsum[warp][lane] = v[0];
-      } else {
+      {
         // 16 columns at a time through this side's P (its last reader is done):
         // lane i of the warp then adds half of column i / 2
         float* stage = reinterpret_cast<float*>(smem + C::P_OFF + x * C::P_BYTES) + (warp & 3) * (16 * 36);
@@ -750,25 +868,9 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           __syncwarp();
         }
       }
-      named_bar_sync(1 + C::SIDES, C::SOFT);
+      named_bar_sync(3, 256);
       float* part = p.part + ((size_t)blockIdx.x * 2 + border) * C::SLOT;
-      if (C::WIDE && gt < HN) {   // (the side's first warp)
-        const int col = col0 + gt;
-        const float sum = (ms.lsum[4 * x][gt] + ms.lsum[4 * x + 1][gt]) + (ms.lsum[4 * x + 2][gt] + ms.lsum[4 * x + 3][gt]);
-        const float top = partial_max(negm[gt], p.factor);
-        Finish fin{1.f, 0.f};
-        if (whole && ms.coff[col] >= 0) {
-          fin = finish<PASS>(p, prefix, ms.coff[col], top, sum);
-          if (PASS == kAttnPrefix) p.pre_ml[ms.coff[col]] = make_float2(top, sum);
-        }
-        facs[gt] = fin.own;
-        if (PASS == kAttnOwn) ms.pre[col] = fin.pre;
-        if (!whole) {
-          part[N * 128 + col] = top;
-          part[N * 129 + col] = sum;
-        }
-      }
-      if (!C::WIDE && x == 0 && gt < HN) {
+      if (x == 0 && gt < N) {
         // a side without a tile (one-tile run) or a column without a key has sum 0 and counts nothing
         const float ma = -ms.negm[0][gt], mb = -ms.negm[1][gt], m = fmaxf(ma, mb);
         const float wa = ma == -kUnset ? 0.f : exp2_fast((ma - m) * p.factor), wb = mb == -kUnset ? 0.f : exp2_fast((mb - m) * p.factor);
@@ -788,28 +890,20 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           part[N * 129 + gt] = sum;
         }
       }
-      named_bar_sync(1 + C::SIDES, C::SOFT);
+      named_bar_sync(3, 256);
       tc_fence_after();
       // thread = channel: 32 lanes write 64 (128) contiguous bytes of a row;
       // the two groups of warps take every other 16 columns
       uint8_t* out = static_cast<uint8_t*>(p.out) + 2 * row;
       // (a side without a tile has factor 0; its O may hold anything, so the
       // other side's is read in its place)
-      // (wide: each its own columns)
       const uint32_t o_all = tmem + C::O_COL + lanes;
-      const uint32_t o_a = nt > 1 || (t0 & 1) == 0 ? o_all : o_all + HN, o_b = nt > 1 || (t0 & 1) == 1 ? o_all + HN : o_all;
+      const uint32_t o_a = nt > 1 || (t0 & 1) == 0 ? o_all : o_all + N, o_b = nt > 1 || (t0 & 1) == 1 ? o_all + N : o_all;
 #pragma unroll 1
-      for (int c0 = C::WIDE ? 0 : x; c0 < C::CH; c0 += C::WIDE ? 1 : 2) {
-        const int c = c0 + (C::WIDE ? x * C::CH : 0);   // 16 columns of the item
-        uint32_t oa[16];
+      for (int c = x; c < C::CH; c += 2) {
+        uint32_t oa[16], ob[16];
         __syncwarp();
-        if constexpr (C::WIDE) {
-          tmem_ld16(o_t + 16 * c0, oa);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) oa[i] = __float_as_uint(__uint_as_float(oa[i]) * facs[16 * c0 + i]);
-        } else {
-          uint32_t ob[16];
+        {
           tmem_ld16(o_a + 16 * c, oa);
           tmem_ld16(o_b + 16 * c, ob);
           tmem_ld_wait();
@@ -872,11 +966,13 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     }
 
     if (threadIdx.x == 0) q4_tc_shared(p.part, N, grid)[blockIdx.x] = ms.shared;
+    }
   } else if (warp < C::VDEC) {
     set_registers<C::REST_REGS, false>();
     // ---- K codes to f16: thread = cached row
     const int dt = threadIdx.x - 32 * C::KDEC;
     const uint32_t kt = tmem + C::K_COL + ((uint32_t)(32 * (warp & 3)) << 16);
+    uint8_t* const ks = smem + C::P_OFF + dt * 128;   // (wide: 64 channels of a row in 128 bytes)
 #pragma unroll 1
     for (int t = 0; t < T; ++t) {
       const int s = t % NS;
@@ -902,10 +998,21 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
             out[4 * i + 2] = dequant<2>(w[i], sp, ns);
             out[4 * i + 3] = dequant<3>(w[i], sp, ns);
           }
-          tmem_st16(kt + (t & 1) * 64 + 16 * c, out);
+          if constexpr (C::WIDE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(ks + (t & 1) * C::P_BYTES + (c >> 1) * 16384 + ((((4 * c + i) & 7) ^ (dt & 7)) << 4)) =
+                  make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
+          } else {
+            tmem_st16(kt + (t & 1) * 64 + 16 * c, out);
+          }
         }
-        tmem_st_wait();
-        tc_fence_before();
+        if constexpr (C::WIDE) {
+          fence_proxy_async_smem();
+        } else {
+          tmem_st_wait();
+          tc_fence_before();
+        }
         warp_arrive(&ms.kready[t & 1], lane);
         if (lane == 0) mbar_arrive(&ms.empty[s]);
       }
@@ -1120,8 +1227,9 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     }
     } else if (warp == C::MMA && T > 0) {
       // ---- S(t) = K(t) Q^T, as soon as K is there and the softmax has read the buffer's last S
+      // (wide: Q K(t)^T, and P(t - 2), which took its place, is read)
       const uint32_t idesc = umma_idesc_f16(128, N, 0);
-      const uint64_t qd = umma_desc_sw128(smem_u32(smem + C::Q_OFF));
+      const uint64_t qd = umma_desc_sw128(smem_u32(smem + C::Q_OFF)), kd = umma_desc_sw128(smem_u32(smem + C::P_OFF));
       int seg = 0, k = 0, nt = 0;
 #pragma unroll 1
       for (int t = 0; t < T; ++t) {
@@ -1130,7 +1238,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           qb_wait(&ms.q_ready[qb], (seg / C::QB) & 1, dead);
           nt = ms.seg[seg % C::SEGS].nt;
         }
-        if (t >= C::SB) qb_wait(&ms.s_free[t % C::SB], (t / C::SB - 1) & 1, dead);
+        if (t >= C::SB) qb_wait(C::WIDE ? &ms.pvdone[t & 1] : &ms.s_free[t % C::SB], (t / C::SB - 1) & 1, dead);
         qb_wait(&ms.kready[t & 1], (t >> 1) & 1, dead);
         const bool last = ++k == nt;
         if (elect_one()) {
@@ -1139,7 +1247,11 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           const uint64_t q = qd + qb * (C::Q_BYTES >> 4);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            umma_ts(d, ka + ks * 8, q + ((ks >> 2) * (N * 128) >> 4) + 2 * (ks & 3), idesc, ks > 0);
+            if constexpr (C::WIDE)
+              umma_f16(d, q + (ks >> 2) * 1024 + 2 * (ks & 3), kd + (t & 1) * (C::P_BYTES >> 4) + (ks >> 2) * 1024 + 2 * (ks & 3),
+                       idesc, ks > 0);
+            else
+              umma_ts(d, ka + ks * 8, q + ((ks >> 2) * (N * 128) >> 4) + 2 * (ks & 3), idesc, ks > 0);
           umma_commit(&ms.s_ready[t % C::SB]);
           umma_commit(&ms.kfree[t & 1]);
           if (last) umma_commit(&ms.q_free[qb]);
@@ -1151,8 +1263,8 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
         }
       }
     } else if (warp == C::MMA2 && T > 0) {
-      // ---- O(side of t; wide: of both) += V^T(t) P^T(t)
-      const uint32_t idesc = umma_idesc_f16(128, N, 0) | (1u << 16);   // B (P^T) with the columns contiguous
+      // ---- O(side of t) += V^T(t) P^T(t) (wide: P(t) V(t), P from TMEM)
+      const uint32_t idesc = umma_idesc_f16(128, N, 0) | (C::WIDE ? 0 : 1u << 16);   // B (P^T) with the columns contiguous
       const uint64_t vd = umma_desc_sw128(smem_u32(smem + C::V_OFF)), pd = desc_sw128_mn(smem_u32(smem + C::P_OFF), 16384);
       int seg = 0, k = 0, nt = 0;
 #pragma unroll 1
@@ -1168,8 +1280,11 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           const uint64_t v = vd + (t & 1) * (C::V_BYTES >> 4), pp = pd + (t & 1) * (C::P_BYTES >> 4);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)   // (a side's first tile of the item starts its O)
-            umma_f16(tmem + C::O_COL + (C::WIDE ? 0 : (t & 1) * N), v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc,
-                     k > (C::WIDE ? 0 : 1) || ks > 0);
+            if constexpr (C::WIDE)
+              umma_ts(tmem + C::O_COL + (t & 1) * N, tmem + C::S_COL + (t & 1) * N + ks * 8, v + (ks >> 2) * 1024 + 2 * (ks & 3),
+                      idesc, k > 1 || ks > 0);
+            else
+              umma_f16(tmem + C::O_COL + (t & 1) * N, v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc, k > 1 || ks > 0);
           umma_commit(&ms.pvdone[t & 1]);
         }
         __syncwarp();
