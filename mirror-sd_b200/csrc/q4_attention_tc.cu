@@ -82,10 +82,11 @@ struct QbCfg {
   static constexpr int SLOT = N * 130;          // floats of a partial: O [N][128], m [N], l [N]
   // warps: softmax, side by side (even tiles 0-3, odd tiles 4-7), then the others, all
   // in whole warpgroups, whose registers are dealt out anew after the common start
-  static constexpr int KDEC = 8, VDEC = 12, MMA = 16, LOAD = 17, QUERY = 18, MMA2 = 19;
-  static constexpr int THREADS = 640;
-  // registers a thread at the start: 96, 640 * 96 = 256 * 144 + 384 * 64
-  static constexpr int SOFT_REGS = 144, REST_REGS = 64;
+  // (wide: two warps to a side's 32 rows, half the columns each)
+  static constexpr int KDEC = WIDE ? 16 : 8, VDEC = KDEC + 4, MMA = VDEC + 4, LOAD = MMA + 1, QUERY = MMA + 2, MMA2 = MMA + 3;
+  static constexpr int THREADS = 32 * (MMA + 4);
+  // registers a thread at the start: 96, 640 * 96 = 256 * 144 + 384 * 64 (wide: 72, 896 * 72 > 512 * 80 + 384 * 56)
+  static constexpr int SOFT_REGS = WIDE ? 80 : 144, REST_REGS = WIDE ? 56 : 64;
 };
 struct QbSeg {          // a run of tiles of one item
   Item it;
@@ -98,22 +99,23 @@ struct QbSeg {          // a run of tiles of one item
 template <class C>
 struct QbMisc {
   uint64_t full[4], empty[4], kready[2], kfree[2], vready[2], pvdone[2], s_ready[4], s_free[4], p_ready[2];
-  uint64_t q_ready[2], q_free[2], o_free;
+  uint64_t q_ready[2], q_free[2], o_free, rec_ready[4];
   uint32_t tmem;
   int abort;
+  int started;                    // items that the softmax warps have begun (wide)
   int where[2];                   // request of the CTA's first tile, and that request's first tile
   int run[2], share;              // whole CTAs to an item: this one's tiles, and their number
   int wtot[C::THREADS / 32];
   int2 tile[16];                  // row blocks copied and QB_SEEN, rows below the request's end
   QbSeg seg[C::SEGS];
-  alignas(16) float qf[C::SEGS][C::N];        // score factors
+  alignas(16) float qf[C::WIDE ? 2 : C::SEGS][C::N];   // score factors
   alignas(16) float negm[2][C::N];            // minus the columns' references, of either side
-  alignas(16) float fac[2][C::N];             // rescale factors; at the end what O is multiplied by
+  alignas(16) float fac[2][C::WIDE ? 2 * C::N : C::N];             // rescale factors; at the end what O is multiplied by
   alignas(16) float pre[C::N];                // and what the sums over the group's rows are (kAttnOwn)
   int cmax[2][C::N];                          // column maxima as ordered integers
   alignas(16) int cend[C::N];                 // where each column's keys end
   alignas(16) int coff[C::N];                 // output row of each column, or -1
-  float lsum[C::WIDE ? 2 : 8][C::N];
+  float lsum[C::WIDE ? 4 : 8][C::N];
   int4 shared;                    // the item that starts here and reaches past the last tile (q4_tc_shared)
 };
 
@@ -167,6 +169,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 // A warp's wait for a phase, bounded: when it expires (or once another wait has)
 // the flag is set and every later wait returns at once.  All lanes poll: one
@@ -270,31 +277,91 @@ __host__ __device__ __forceinline__ int4* q4_tc_shared(float* part, int n, int g
   return reinterpret_cast<int4*>(part + (size_t)grid * 2 * n * 130);
 }
 
-// ---- softmax of the wide form: of the tiles t with t & 1 == x; thread = query row.
-// A row's scores lie in one lane, so its reference and sum are the thread's own:
-// no votes and no exchange between lanes.  P, as f16, takes the place of the scores
-// that are read.
+// 16 bytes of a bf16 query row, the row's others in 15 neighbouring lanes, as f16.
+// A row whose largest magnitude lies in [2^-3, 2^15] is rounded to f16 as it is (what
+// is below 2^-14 loses bits, 2^-22 of that largest at most); any other row is scaled
+// by a power of two first, whose exponent is returned (0: none).
+__device__ __forceinline__ int query_f16(uint4* at, int lane) {
+  const uint32_t half = lane < 16 ? 0xffffu : 0xffff0000u;   // the lanes of this lane's row
+  const uint4 w = *at;
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  float x[8], a = 0.f;
+  int e = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[2 * k] = __uint_as_float(u[k] << 16);
+    x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+    a = fmaxf(a, fmaxf(fabsf(x[2 * k]), fabsf(x[2 * k + 1])));
+  }
+  const uint32_t big = __ballot_sync(0xffffffffu, a >= 0.125f), nonzero = __ballot_sync(0xffffffffu, a > 0.f);
+  const bool plain = (!(nonzero & half) || (big & half)) && a <= 32768.f;
+  if (!__all_sync(0xffffffffu, plain)) {
+#pragma unroll 1
+    for (int o = 1; o < 16; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if (a != 0.f && !(a >= 0.125f && a <= 32768.f)) {
+      e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
+      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= down;
+    }
+  }
+  *at = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+  return e;
+}
+__device__ __forceinline__ float scaled_factor(float f, int e) { return fminf(f * __uint_as_float((uint32_t)e << 23), 3e38f); }
+
+// ---- softmax of the wide form: of the tiles t with t & 1 == x; thread = query row,
+// half of the tile's columns.  Scores of a row lie in two lanes, so its reference and
+// its sums are those threads' own, and all that two warps have to tell each other is
+// whether a score passes a reference.  P, as f16, takes the place of the scores that
+// are read.
 template <class C, class Sharers>
-__device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& ms, uint32_t tmem, int c0, int c1,
+__device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& ms, uint8_t* q_smem, uint32_t tmem, int c0, int c1,
                                              volatile int* dead, Sharers sharers) {
-  constexpr int N = C::N;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = warp >> 2, row = threadIdx.x & (N - 1), G = p.by_g.d;
+  constexpr int N = C::N, SOFT = 32 * C::KDEC;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = warp >> 3, half = warp >> 2 & 1;
+  const int row = 32 * (warp & 3) + lane, pair = 4 + 4 * x + (warp & 3), G = p.by_g.d;   // barrier of the two warps
   const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-  const uint32_t s_t = tmem + C::S_COL + x * N + lanes, o_all = tmem + C::O_COL + lanes, o_t = o_all + x * N;
+  const uint32_t s_t = tmem + C::S_COL + x * N + 64 * half + lanes, o_all = tmem + C::O_COL + lanes, o_t = o_all + x * N + 64 * half;
+  // Query rows: 8 a warp, two at a time (lanes 0-15, 16-31), on their way while the
+  // item before is finished.  (One warp for all 128: 8 us an item, 15 in bf16.)
+  const float base_f = 16.f * p.scale_log2;
+  const int piece = lane & 15, q_row0 = 8 * warp + (lane >> 4);
+  uint8_t* const q_dst = q_smem + (piece >> 3) * (N * 128) + q_row0 * 128;
+  auto query_at = [&](int i) { return q_dst + 2 * i * 128 + (((piece & 7) ^ (q_row0 + 2 * i & 7)) << 4); };
+  auto load_queries = [&](int seg) {
+    qb_wait(&ms.rec_ready[seg & 3], (seg >> 2) & 1, dead);
+    if (__any_sync(0xffffffffu, *dead)) return;   // (there may be no record)
+    const QbSeg& sg = ms.seg[seg % C::SEGS];
+    const uint16_t* q = static_cast<const uint16_t*>(p.q) + (size_t)sg.it.row0 * p.q_row + 8 * piece;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = sg.q0 + q_row0 + 2 * i, j = p.by_g.of(r);
+      const bool real = j < sg.it.rows;
+      cp_async16_zfill(smem_u32(query_at(i)), real ? q + (size_t)j * p.q_row + (size_t)(sg.head0 + r - j * G) * p.q_head : p.q, real);
+    }
+    cp_async_commit();
+  };
+  if (c0 < c1) load_queries(0);
   int u = c0, t0 = 0;   // the item's first tile, counted in the CTA
 #pragma unroll 1
   for (int seg = 0; u < c1; ++seg) {
-    // S of the item's first tile is only issued once its record is there
+    cp_async_wait<0>();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = p.bf16 ? query_f16(reinterpret_cast<uint4*>(query_at(i)), lane) : 0;
+      if (piece == 0) ms.qf[seg & 1][q_row0 + 2 * i] = e ? scaled_factor(base_f, e) : base_f;
+    }
+    fence_proxy_async_smem();
+    warp_arrive(&ms.q_ready[0], lane);
     if ((t0 & 1) == x) qb_wait(&ms.s_ready[x], (t0 >> 1) & 1, dead);
     const QbSeg& sg = ms.seg[seg % C::SEGS];
     // after an expired wait there may be no record: run to the end, writing nothing
-    const bool bad = named_bar_or<256>(3, *dead);
-    Item it{};
-    if (!bad) it = sg.it;
-    const int nt = bad ? c1 - u : sg.nt, j0 = bad ? 0 : sg.j0, sub = sg.sub, item0 = sg.item0;
-    const int r = sg.q0 + row, j = p.by_g.of(r);
-    const long long at = j < it.rows ? (long long)(it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;   // row of the sums
-    const float f = score_factor(ms.qf[seg % C::SEGS][row]);
+    const bool bad = named_bar_or<SOFT>(3, *dead);
+    const int nt = bad ? c1 - u : sg.nt;
+    const float f = score_factor(ms.qf[seg & 1][row]);
+    if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(&ms.started) = seg + 1;
     float negm = kUnset;   // minus the reference
     float2 l = make_float2(0.f, 0.f);
 
@@ -306,8 +373,8 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
       const int2 info = ms.tile[t & 15];
       if (!(info.x & QB_SEEN)) {   // some key is hidden: its scores to -inf, where they lie
 #pragma unroll 1
-        for (int c = 0; c < C::CH; ++c) {
-          const int left = (info.x >> c & 1) ? info.y - 16 * c : 0;
+        for (int c = 0; c < 4; ++c) {
+          const int left = (info.x >> (4 * half + c) & 1) ? info.y - 64 * half - 16 * c : 0;
           if (left >= 16) continue;
           uint32_t s[16];
           tmem_ld16(s_t + 16 * c, s);
@@ -318,39 +385,41 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
         }
         tmem_st_wait();
       }
-      uint32_t s[2][32];
-      tmem_ld32(s_t, s[0]);
+      uint32_t s[2][16];
+      tmem_ld16(s_t, s[0]);
       float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         tmem_ld_wait();
-        if (c < 3) tmem_ld32(s_t + 32 * (c + 1), s[(c + 1) & 1]);
+        tmem_ld16(s_t + 16 * ((c + 1) & 3), s[(c + 1) & 1]);   // (at last the first ones again)
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
+        for (int i = 0; i < 16; i += 4) {
           top = max3(top, __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
           top2 = max3(top2, __uint_as_float(s[c & 1][i + 2]), __uint_as_float(s[c & 1][i + 3]));
         }
       }
-      tmem_ld32(s_t, s[0]);
       top = fmaxf(top, top2);
-      const float rise = (top + negm) * f;
-      if (__any_sync(0xffffffffu, rise > QB_RAISE)) {   // (a row without a reference: any visible key)
-        float fac = 1.f;
+      if (named_bar_or<64>(pair, (top + negm) * f > QB_RAISE)) {   // (a row without a reference: any visible key)
+        ms.fac[x][row + half * N] = top;
+        named_bar_sync(pair, 64);
+        top = fmaxf(top, ms.fac[x][row + (half ^ 1) * N]);
+        const float rise = (top + negm) * f;
+        float by = 1.f;
         if (rise > QB_RAISE) {
-          fac = exp2_fast(-rise);
+          by = exp2_fast(-rise);
           negm = -top;
         }
-        l.x *= fac;
-        l.y *= fac;
-        if (k >= 2) {   // O holds this side's tiles before t
+        l.x *= by;
+        l.y *= by;
+        if (k >= 2) {   // O holds this side's tiles before t: half of its channels
           tmem_ld_wait();
 #pragma unroll 1
-          for (int c = 0; c < C::CH; ++c) {
+          for (int c = 0; c < 4; ++c) {
             uint32_t o[16];
             tmem_ld16(o_t + 16 * c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fac);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
             tmem_st16(o_t + 16 * c, o);
           }
           tmem_st_wait();
@@ -360,42 +429,50 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         tmem_ld_wait();
-        if (c < 3) tmem_ld32(s_t + 32 * (c + 1), s[(c + 1) & 1]);
-        uint32_t w[16];
+        if (c < 3) tmem_ld16(s_t + 16 * (c + 1), s[(c + 1) & 1]);
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 8; ++i) {
           float2 y = mul2(add2(make_float2(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), nm), ff);
           y.x = exp2_fast(y.x);
           y.y = exp2_fast(y.y);
           l = add2(l, y);
           w[i] = pack_f16x2(y.x, y.y);
         }
-        tmem_st16(s_t + 16 * c, w);   // (over scores that this warp has read)
+        tmem_st8(s_t + 8 * c, w);   // (over scores that this warp has read)
       }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&ms.p_ready[x], lane);
     }
     u += nt;
+    if (u < c1) {
+      qb_wait(&ms.q_free[0], seg & 1, dead);
+      load_queries(seg + 1);
+    }
 
-    // ---- the item's run is over: both sides' sums and O, half the channels each
-    const bool whole = bad || (j0 == 0 && nt == it.ntile);
-    const int border = item0 < c0 ? 0 : 1;
+    // ---- the item's run is over: both sides' sums and O, a quarter of the channels each
     const int last = t0 + nt - 1;   // the other side's last tile is last - 1
-    ms.negm[x][row] = negm;
-    ms.lsum[x][row] = l.x + l.y;
+    if (half == 0) ms.negm[x][row] = negm;
+    ms.lsum[2 * x + half][row] = l.x + l.y;
     qb_wait(&ms.pvdone[last & 1], (last >> 1) & 1, dead);
     if (nt > 1) qb_wait(&ms.pvdone[(last - 1) & 1], ((last - 1) >> 1) & 1, dead);
-    named_bar_sync(3, 256);
+    named_bar_sync(3, SOFT);
     tc_fence_after();
+    Item it{};
+    if (!bad) it = sg.it;
+    const bool whole = bad || (sg.j0 == 0 && nt == it.ntile);
+    const int border = sg.item0 < c0 ? 0 : 1, r = sg.q0 + row, j = p.by_g.of(r);
+    const long long at = j < it.rows ? (long long)(it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;   // row of the sums
     // (a side without a tile, or a row without a key, has the sum 0 and counts nothing)
     const float ma = -ms.negm[0][row], mb = -ms.negm[1][row], m = fmaxf(ma, mb);
     const float wa = ma == -kUnset ? 0.f : exp2_fast((ma - m) * f), wb = mb == -kUnset ? 0.f : exp2_fast((mb - m) * f);
-    const float sum = wa * ms.lsum[0][row] + wb * ms.lsum[1][row], top = partial_max(-m, f);
     float* part = p.part + ((size_t)blockIdx.x * 2 + border) * C::SLOT;
     float* to = whole ? p.pre_o + at * 128 : part + row * 128;
     const bool write = !whole || at >= 0;
-    if (x == 0) {
+    if (x == 0 && half == 0) {
+      const float sum = wa * (ms.lsum[0][row] + ms.lsum[1][row]) + wb * (ms.lsum[2][row] + ms.lsum[3][row]);
+      const float top = partial_max(-m, f);
       if (!whole) {
         part[N * 128 + row] = top;
         part[N * 129 + row] = sum;
@@ -406,7 +483,7 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
     // (the O of a side without a tile may hold anything: the other's is read in its place)
     const uint32_t o_a = nt > 1 || (t0 & 1) == 0 ? o_all : o_all + N, o_b = nt > 1 || (t0 & 1) == 1 ? o_all + N : o_all;
 #pragma unroll 1
-    for (int c = 4 * x; c < 4 * x + 4; ++c) {
+    for (int c = 2 * (warp >> 2); c < 2 * (warp >> 2) + 2; ++c) {
       uint32_t oa[16], ob[16];
       __syncwarp();
       tmem_ld16(o_a + 16 * c, oa);
@@ -422,10 +499,11 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
         }
       }
     }
+    // (merged by the item's first CTA's entry; the others' partials follow its own)
+    if (!whole && threadIdx.x == 0 && border == 1)
+      ms.shared = make_int4(it.row0, it.rows, sg.sub, sharers(sg.item0, it.ntile));
     tc_fence_before();
     warp_arrive(&ms.o_free, lane);
-    // (merged by the item's first CTA's entry; the others' partials follow its own)
-    if (!whole && threadIdx.x == 0 && border == 1) ms.shared = make_int4(it.row0, it.rows, sub, sharers(item0, it.ntile));
     t0 += nt;
   }
   if (threadIdx.x == 0) q4_tc_shared(p.part, N, gridDim.x)[blockIdx.x] = ms.shared;
@@ -448,12 +526,13 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ms.kready[i], 4); mbar_init(&ms.kfree[i], 1);
       mbar_init(&ms.vready[i], 4); mbar_init(&ms.pvdone[i], 1);
-      mbar_init(&ms.p_ready[i], 4);
-      mbar_init(&ms.q_ready[i], 1); mbar_init(&ms.q_free[i], 1);
+      mbar_init(&ms.p_ready[i], C::WIDE ? 8 : 4);
+      mbar_init(&ms.q_ready[i], C::WIDE ? C::KDEC : 1); mbar_init(&ms.q_free[i], 1);
     }
-    mbar_init(&ms.o_free, 8);
+    mbar_init(&ms.o_free, C::KDEC);
+    for (int i = 0; i < 4; ++i) mbar_init(&ms.rec_ready[i], 1);
     for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], 4); }
-    ms.abort = 0;
+    ms.abort = ms.started = 0;
     ms.shared = make_int4(0, 0, 0, 0);
     ms.run[0] = ms.run[1] = 0;
     fence_mbar_init();
@@ -629,7 +708,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
   if (warp < C::KDEC) {
     set_registers<C::SOFT_REGS, true>();
     if constexpr (C::WIDE) {
-      wide_softmax<C>(p, ms, tmem, c0, c1, dead, sharers);
+      wide_softmax<C>(p, ms, smem + C::Q_OFF, tmem, c0, c1, dead, sharers);
     } else {
     // ---- softmax of the tiles t with t & 1 == x; thread = cached row, and channel at the end
     const int x = warp >> 2, gt = threadIdx.x & 127;
@@ -984,7 +1063,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
         const int rr = dt & 15;
         const uint8_t* blk = st + (dt >> 4) * QB_BLK;
         const uint2 sc = *reinterpret_cast<const uint2*>(blk + kQ4KS + rr * 8);
-#pragma unroll 1
+#pragma unroll C::WIDE ? 4 : 1
         for (int c = 0; c < 4; ++c) {   // 32 channels: groups 2c and 2c + 1
           const uint4 w4 = *reinterpret_cast<const uint4*>(blk + q4_k_piece(rr, c));
           const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
@@ -1048,7 +1127,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           ns[jj] = scale_shift(sp[jj]);
         }
         uint8_t* vt = smem + C::V_OFF + (t & 1) * C::V_BYTES + chunk * 16384 + g * 2048;
-#pragma unroll 1
+#pragma unroll C::WIDE ? 2 : 1
         for (int h = 0; h < 2; ++h) {   // 8 channels: words 2h and 2h + 1 of each piece
           uint2 w[4];
 #pragma unroll
@@ -1147,13 +1226,21 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     for (int seg = 0; u < c1; ++seg) {
       const int qb = seg % C::QB;
       const int nt = min(cur.it.ntile - cur.j, c1 - u);
-      if (seg >= C::QB) qb_wait(&ms.q_free[qb], ((seg / C::QB) - 1) & 1, dead);
+      if constexpr (C::WIDE) {   // the softmax warps bring the rows; records run ahead of them, while there is room
+        for (uint32_t i = 0; *reinterpret_cast<volatile int*>(&ms.started) < seg - (C::SEGS - 2) && !*dead; ++i) {
+          if (i == kSpinLimit) *dead = 1;
+          __nanosleep(100);
+        }
+        __syncwarp();
+      } else if (seg >= C::QB) {
+        qb_wait(&ms.q_free[qb], ((seg / C::QB) - 1) & 1, dead);
+      }
       uint8_t* qs = smem + C::Q_OFF + qb * C::Q_BYTES;
-      float* qf = ms.qf[seg % C::SEGS];
+      float* qf = ms.qf[C::WIDE ? 0 : seg % C::SEGS];
       const int grp = p.by_nkv.of(cur.sub), q0 = grp * N, head0 = (cur.sub - grp * p.nkv) * G;
       // every 16-byte piece of the rows at once (2 rows an instruction), then the
       // bf16 ones to f16 in place
-      {
+      if (!C::WIDE) {
         const int piece = lane & 15;
         const int r = q0 + (lane >> 4);
         int j = p.by_g.of(r), h = r - j * G;
@@ -1173,42 +1260,19 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
         __syncwarp();
       }
       bool uniform = true;
-      for (int i = lane; i < N; i += 32) qf[i] = base_f;
+      if (!C::WIDE)
+        for (int i = lane; i < N; i += 32) qf[i] = base_f;
       __syncwarp();
-      if (p.bf16) {
-        // A row whose largest magnitude lies in [2^-3, 2^15] is rounded to f16
-        // as it is (what is below 2^-14 loses bits, 2^-22 of that largest at
-        // most); any other row is scaled by a power of two first.
+      if (!C::WIDE && p.bf16) {
         const int piece = lane & 15;
         uint8_t* src = qs + (piece >> 3) * (N * 128);
-        const uint32_t half = lane < 16 ? 0xffffu : 0xffff0000u;   // the lanes of this lane's row
 #pragma unroll 4
         for (int i = lane >> 4; i < N; i += 2) {
-          uint4* at = reinterpret_cast<uint4*>(src + i * 128 + (((piece & 7) ^ (i & 7)) << 4));
-          const uint4 w = *at;
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          float x[8], a = 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[2 * k] = __uint_as_float(u[k] << 16);
-            x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-            a = fmaxf(a, fmaxf(fabsf(x[2 * k]), fabsf(x[2 * k + 1])));
+          const int e = query_f16(reinterpret_cast<uint4*>(src + i * 128 + (((piece & 7) ^ (i & 7)) << 4)), lane);
+          if (e) {
+            if (piece == 0) qf[i] = scaled_factor(base_f, e);
+            uniform = false;
           }
-          const uint32_t big = __ballot_sync(0xffffffffu, a >= 0.125f), nonzero = __ballot_sync(0xffffffffu, a > 0.f);
-          const bool plain = (!(nonzero & half) || (big & half)) && a <= 32768.f;
-          if (!__all_sync(0xffffffffu, plain)) {
-#pragma unroll 1
-            for (int o = 1; o < 16; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-            if (a != 0.f && !(a >= 0.125f && a <= 32768.f)) {
-              const int e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
-              const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) x[k] *= down;
-              if (piece == 0) qf[i] = fminf(base_f * __uint_as_float((uint32_t)e << 23), 3e38f);
-              uniform = false;
-            }
-          }
-          *at = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
         }
         uniform = __all_sync(0xffffffffu, uniform);
       }
@@ -1220,7 +1284,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ms.q_ready[qb]);
+      if (lane == 0) mbar_arrive(C::WIDE ? &ms.rec_ready[seg & 3] : &ms.q_ready[qb]);
       u += nt;
       cur.j += nt - 1;
       if (u < c1) cursor_next<QB_TILE, N>(p, cur);
@@ -1281,7 +1345,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)   // (a side's first tile of the item starts its O)
             if constexpr (C::WIDE)
-              umma_ts(tmem + C::O_COL + (t & 1) * N, tmem + C::S_COL + (t & 1) * N + ks * 8, v + (ks >> 2) * 1024 + 2 * (ks & 3),
+              umma_ts(tmem + C::O_COL + (t & 1) * N, tmem + C::S_COL + (t & 1) * N + (ks >> 2) * 64 + (ks & 3) * 8, v + (ks >> 2) * 1024 + 2 * (ks & 3),
                       idesc, k > 1 || ks > 0);
             else
               umma_f16(tmem + C::O_COL + (t & 1) * N, v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc, k > 1 || ks > 0);
