@@ -67,7 +67,7 @@ struct QbCfg {
   // Query buffers and packed stages.  With 80 columns shared memory holds two and
   // two or one and three (8 requests of 16,384 rows, 160 query rows: 167 and 166 us).
   static constexpr int QB = N <= 64 ? 2 : 1;
-  static constexpr int SB = N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S)
+  static constexpr int SB = WIDE ? 3 : N <= 64 ? 4 : 2;    // S buffers (TMEM: 128 for K, N for each O and S; wide: 4 N)
   static constexpr int NS = N <= 64 ? 4 : 3;
   static constexpr bool AHEAD = N <= 64;        // registers for the next 16 scores
   static constexpr int SEGS = WIDE ? 4 : 8;     // ring of item records (items run ahead by an S buffer each, and one)
@@ -77,8 +77,8 @@ struct QbCfg {
   static constexpr int Q_OFF = P_OFF + 2 * P_BYTES, Q_BYTES = N * 256;
   static constexpr int RING_OFF = Q_OFF + QB * Q_BYTES;
   static constexpr int MISC_OFF = RING_OFF + NS * QB_STAGE;
-  // 2 x 64 for K, N for each O and S (wide: N for each S, which P takes the place of, and each O)
-  static constexpr uint32_t K_COL = 0, O_COL = WIDE ? 2 * N : 128, S_COL = WIDE ? 0 : 128 + 2 * N;
+  // 2 x 64 for K, N for each O and S (wide: N for each S, which P takes the place of, and one O)
+  static constexpr uint32_t K_COL = 0, O_COL = WIDE ? SB * N : 128, S_COL = WIDE ? 0 : 128 + 2 * N;
   static constexpr int SLOT = N * 130;          // floats of a partial: O [N][128], m [N], l [N]
   // warps: softmax, side by side (even tiles 0-3, odd tiles 4-7), then the others, all
   // in whole warpgroups, whose registers are dealt out anew after the common start
@@ -99,7 +99,7 @@ struct QbSeg {          // a run of tiles of one item
 template <class C>
 struct QbMisc {
   uint64_t full[4], empty[4], kready[2], kfree[2], vready[2], pvdone[2], s_ready[4], s_free[4], p_ready[2];
-  uint64_t q_ready[2], q_free[2], o_free, rec_ready[4];
+  uint64_t q_ready[2], q_free[2], o_free, rec_ready[4], decided[2][4];
   uint32_t tmem;
   int abort;
   int started;                    // items that the softmax warps have begun (wide)
@@ -311,10 +311,13 @@ __device__ __forceinline__ int query_f16(uint4* at, int lane) {
 __device__ __forceinline__ float scaled_factor(float f, int e) { return fminf(f * __uint_as_float((uint32_t)e << 23), 3e38f); }
 
 // ---- softmax of the wide form: of the tiles t with t & 1 == x; thread = query row,
-// half of the tile's columns.  Scores of a row lie in two lanes, so its reference and
-// its sums are those threads' own, and all that two warps have to tell each other is
-// whether a score passes a reference.  P, as f16, takes the place of the scores that
-// are read.
+// half of the tile's columns.  Both sides add to one O, so a row has one reference,
+// which each tile may raise after the tile before has: the sides hand it on in the
+// order of the tiles (`decided`), early in a tile's work, and a raise waits for the
+// products that O still takes.  P, as f16, takes the place of the scores that are
+// read; with a third buffer S of the next tile is there when a side comes to it.
+// (Sides with an O each leave room for two buffers, so that a tile's S waits for PV
+// of the tile two before: 2,200 cycles a tile, of which the hand-overs alone are 950.)
 template <class C, class Sharers>
 __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& ms, uint8_t* q_smem, uint32_t tmem, int c0, int c1,
                                              volatile int* dead, Sharers sharers) {
@@ -322,7 +325,7 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = warp >> 3, half = warp >> 2 & 1;
   const int row = 32 * (warp & 3) + lane, pair = 4 + 4 * x + (warp & 3), G = p.by_g.d;   // barrier of the two warps
   const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-  const uint32_t s_t = tmem + C::S_COL + x * N + 64 * half + lanes, o_all = tmem + C::O_COL + lanes, o_t = o_all + x * N + 64 * half;
+  const uint32_t o_all = tmem + C::O_COL + lanes, o_t = o_all + 64 * half;
   // Query rows: 8 a warp, two at a time (lanes 0-15, 16-31), on their way while the
   // item before is finished.  (One warp for all 128: 8 us an item, 15 in bf16.)
   const float base_f = 16.f * p.scale_log2;
@@ -355,7 +358,7 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
     }
     fence_proxy_async_smem();
     warp_arrive(&ms.q_ready[0], lane);
-    if ((t0 & 1) == x) qb_wait(&ms.s_ready[x], (t0 >> 1) & 1, dead);
+    if ((t0 & 1) == x) qb_wait(&ms.s_ready[t0 % C::SB], (t0 / C::SB) & 1, dead);
     const QbSeg& sg = ms.seg[seg % C::SEGS];
     // after an expired wait there may be no record: run to the end, writing nothing
     const bool bad = named_bar_or<SOFT>(3, *dead);
@@ -368,7 +371,8 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
 #pragma unroll 1
     for (int k = (t0 & 1) == x ? 0 : 1; k < nt; k += 2) {
       const int t = t0 + k;
-      if (k > 0) qb_wait(&ms.s_ready[x], (t >> 1) & 1, dead);
+      const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + 64 * half + lanes;
+      if (k > 0) qb_wait(&ms.s_ready[t % C::SB], (t / C::SB) & 1, dead);
       tc_fence_after();
       const int2 info = ms.tile[t & 15];
       if (!(info.x & QB_SEEN)) {   // some key is hidden: its scores to -inf, where they lie
@@ -399,6 +403,16 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
         }
       }
       top = fmaxf(top, top2);
+      if (k > 0) {
+        qb_wait(&ms.decided[x ^ 1][warp & 3], ((t - 1) >> 1) & 1, dead);
+        const float now = ms.negm[0][row];
+        if (__any_sync(0xffffffffu, now != negm)) {
+          const float by = now == negm ? 1.f : exp2_fast((now - negm) * f);   // (0 for a row without a reference before)
+          l.x *= by;
+          l.y *= by;
+          negm = now;
+        }
+      }
       if (named_bar_or<64>(pair, (top + negm) * f > QB_RAISE)) {   // (a row without a reference: any visible key)
         ms.fac[x][row + half * N] = top;
         named_bar_sync(pair, 64);
@@ -411,7 +425,9 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
         }
         l.x *= by;
         l.y *= by;
-        if (k >= 2) {   // O holds this side's tiles before t: half of its channels
+        if (k > 0) {   // O, once it holds all tiles before t: half of its channels
+          qb_wait(&ms.pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1, dead);
+          tc_fence_after();
           tmem_ld_wait();
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
@@ -424,7 +440,11 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
           }
           tmem_st_wait();
         }
+        if (half == 0) ms.negm[0][row] = negm;
+      } else if (k == 0 && half == 0) {
+        ms.negm[0][row] = negm;
       }
+      warp_arrive(&ms.decided[x][warp & 3], lane);
       const float2 nm = make_float2(negm, negm), ff = make_float2(f, f);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -452,11 +472,17 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
     }
 
     // ---- the item's run is over: both sides' sums and O, a quarter of the channels each
-    const int last = t0 + nt - 1;   // the other side's last tile is last - 1
-    if (half == 0) ms.negm[x][row] = negm;
+    const int last = t0 + nt - 1;
+    // (the row's reference is that of the side with the last tile; the other's sums may have an older one)
+    if ((last & 1) != x) {
+      qb_wait(&ms.decided[x ^ 1][warp & 3], (last >> 1) & 1, dead);
+      const float now = ms.negm[0][row], by = now == negm ? 1.f : exp2_fast((now - negm) * f);
+      l.x *= by;
+      l.y *= by;
+      negm = now;
+    }
     ms.lsum[2 * x + half][row] = l.x + l.y;
     qb_wait(&ms.pvdone[last & 1], (last >> 1) & 1, dead);
-    if (nt > 1) qb_wait(&ms.pvdone[(last - 1) & 1], ((last - 1) >> 1) & 1, dead);
     named_bar_sync(3, SOFT);
     tc_fence_after();
     Item it{};
@@ -464,15 +490,12 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
     const bool whole = bad || (sg.j0 == 0 && nt == it.ntile);
     const int border = sg.item0 < c0 ? 0 : 1, r = sg.q0 + row, j = p.by_g.of(r);
     const long long at = j < it.rows ? (long long)(it.row0 + j) * p.nq + sg.head0 + r - j * G : -1;   // row of the sums
-    // (a side without a tile, or a row without a key, has the sum 0 and counts nothing)
-    const float ma = -ms.negm[0][row], mb = -ms.negm[1][row], m = fmaxf(ma, mb);
-    const float wa = ma == -kUnset ? 0.f : exp2_fast((ma - m) * f), wb = mb == -kUnset ? 0.f : exp2_fast((mb - m) * f);
     float* part = p.part + ((size_t)blockIdx.x * 2 + border) * C::SLOT;
     float* to = whole ? p.pre_o + at * 128 : part + row * 128;
     const bool write = !whole || at >= 0;
     if (x == 0 && half == 0) {
-      const float sum = wa * (ms.lsum[0][row] + ms.lsum[1][row]) + wb * (ms.lsum[2][row] + ms.lsum[3][row]);
-      const float top = partial_max(-m, f);
+      const float sum = (ms.lsum[0][row] + ms.lsum[1][row]) + (ms.lsum[2][row] + ms.lsum[3][row]);
+      const float top = partial_max(negm, f);
       if (!whole) {
         part[N * 128 + row] = top;
         part[N * 129 + row] = sum;
@@ -480,23 +503,15 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
         p.pre_ml[at] = make_float2(top, sum);
       }
     }
-    // (the O of a side without a tile may hold anything: the other's is read in its place)
-    const uint32_t o_a = nt > 1 || (t0 & 1) == 0 ? o_all : o_all + N, o_b = nt > 1 || (t0 & 1) == 1 ? o_all + N : o_all;
 #pragma unroll 1
     for (int c = 2 * (warp >> 2); c < 2 * (warp >> 2) + 2; ++c) {
-      uint32_t oa[16], ob[16];
+      uint32_t o[16];
       __syncwarp();
-      tmem_ld16(o_a + 16 * c, oa);
-      tmem_ld16(o_b + 16 * c, ob);
+      tmem_ld16(o_all + 16 * c, o);
       tmem_ld_wait();
       if (write) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(__uint_as_float(oa[i + e]), wa, __uint_as_float(ob[i + e]) * wb);
-          *reinterpret_cast<float4*>(to + 16 * c + i) = make_float4(v[0], v[1], v[2], v[3]);
-        }
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(to + 16 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
       }
     }
     // (merged by the item's first CTA's entry; the others' partials follow its own)
@@ -531,7 +546,8 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     }
     mbar_init(&ms.o_free, C::KDEC);
     for (int i = 0; i < 4; ++i) mbar_init(&ms.rec_ready[i], 1);
-    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], 4); }
+    for (int i = 0; i < 8; ++i) mbar_init(&ms.decided[i >> 2][i & 3], 2);
+    for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], C::WIDE ? 1 : 4); }
     ms.abort = ms.started = 0;
     ms.shared = make_int4(0, 0, 0, 0);
     ms.run[0] = ms.run[1] = 0;
@@ -1291,7 +1307,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     }
     } else if (warp == C::MMA && T > 0) {
       // ---- S(t) = K(t) Q^T, as soon as K is there and the softmax has read the buffer's last S
-      // (wide: Q K(t)^T, and P(t - 2), which took its place, is read)
+      // (wide: Q K(t)^T, and the P that took its place is read)
       const uint32_t idesc = umma_idesc_f16(128, N, 0);
       const uint64_t qd = umma_desc_sw128(smem_u32(smem + C::Q_OFF)), kd = umma_desc_sw128(smem_u32(smem + C::P_OFF));
       int seg = 0, k = 0, nt = 0;
@@ -1302,7 +1318,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           qb_wait(&ms.q_ready[qb], (seg / C::QB) & 1, dead);
           nt = ms.seg[seg % C::SEGS].nt;
         }
-        if (t >= C::SB) qb_wait(C::WIDE ? &ms.pvdone[t & 1] : &ms.s_free[t % C::SB], (t / C::SB - 1) & 1, dead);
+        if (t >= C::SB) qb_wait(&ms.s_free[t % C::SB], (t / C::SB - 1) & 1, dead);
         qb_wait(&ms.kready[t & 1], (t >> 1) & 1, dead);
         const bool last = ++k == nt;
         if (elect_one()) {
@@ -1327,7 +1343,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
         }
       }
     } else if (warp == C::MMA2 && T > 0) {
-      // ---- O(side of t) += V^T(t) P^T(t) (wide: P(t) V(t), P from TMEM)
+      // ---- O(side of t) += V^T(t) P^T(t) (wide: O += P(t) V(t), P from TMEM)
       const uint32_t idesc = umma_idesc_f16(128, N, 0) | (C::WIDE ? 0 : 1u << 16);   // B (P^T) with the columns contiguous
       const uint64_t vd = umma_desc_sw128(smem_u32(smem + C::V_OFF)), pd = desc_sw128_mn(smem_u32(smem + C::P_OFF), 16384);
       int seg = 0, k = 0, nt = 0;
@@ -1345,11 +1361,12 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)   // (a side's first tile of the item starts its O)
             if constexpr (C::WIDE)
-              umma_ts(tmem + C::O_COL + (t & 1) * N, tmem + C::S_COL + (t & 1) * N + (ks >> 2) * 64 + (ks & 3) * 8, v + (ks >> 2) * 1024 + 2 * (ks & 3),
-                      idesc, k > 1 || ks > 0);
+              umma_ts(tmem + C::O_COL, tmem + C::S_COL + (t % C::SB) * N + (ks >> 2) * 64 + (ks & 3) * 8,
+                      v + (ks >> 2) * 1024 + 2 * (ks & 3), idesc, k > 0 || ks > 0);
             else
               umma_f16(tmem + C::O_COL + (t & 1) * N, v + (ks >> 2) * 1024 + 2 * (ks & 3), pp + ks * 128, idesc, k > 1 || ks > 0);
           umma_commit(&ms.pvdone[t & 1]);
+          if (C::WIDE) umma_commit(&ms.s_free[t % C::SB]);
         }
         __syncwarp();
         if (++k == nt) {
