@@ -9,6 +9,23 @@
 // cached row is one TMEM lane: the thread that decodes its 64 bytes stores it
 // as the A operand without passing through shared memory.
 //
+// The pass of a group's query rows over the rows that it shares (kAttnPrefix) has
+// the wide form where there are more than 64 of them a kv head: 128 query rows are
+// the instruction's rows, so a thread has a query row's scores and forms its maximum
+// and its sum alone, P goes back to TMEM, and one decoded tile serves 128 rows:
+//
+//   S[128 query rows, 128] = Q K^T      both from shared memory
+//   O[128 query rows, 128] += P V       P from TMEM, V^T from shared memory
+//
+// (There one O serves both sides, 16 warps share the softmax, and K goes to shared
+// memory; see wide_softmax.)  1,360 query rows a kv head on 2 groups of 16,384 rows
+// take 182 us, in the transposed form 270, 12 of them the start (lengths, query rows,
+// first tiles) and 5 the end; 1,024 on 4,096 rows 38.  A tile takes 1,900 cycles, of
+// which the MMAs need 1,024 and shared memory moves bytes for 1,570 (64 KB for QK^T,
+// 32 for PV, 64 of decoded K and V written, 36 of codes in and out).  What would pay
+// next: Q as the operand in TMEM with scores of 64 cached rows at a time (bytes for
+// 1,310), or pairs of CTAs that decode half of a tile each.
+//
 // Work: the tiles of 128 cached rows of all items, end to end, in equal runs
 // of one CTA per SM (q4_attn.cuh).  The CTAs that share an item write partial
 // results, which a second small kernel merges.  No CTA waits for another:
@@ -85,8 +102,9 @@ struct QbCfg {
   // (wide: two warps to a side's 32 rows, half the columns each)
   static constexpr int KDEC = WIDE ? 16 : 8, VDEC = KDEC + 4, MMA = VDEC + 4, LOAD = MMA + 1, QUERY = MMA + 2, MMA2 = MMA + 3;
   static constexpr int THREADS = 32 * (MMA + 4);
-  // registers a thread at the start: 96, 640 * 96 = 256 * 144 + 384 * 64 (wide: 72, 896 * 72 > 512 * 80 + 384 * 56)
-  static constexpr int SOFT_REGS = WIDE ? 80 : 144, REST_REGS = WIDE ? 56 : 64;
+  // registers a thread at the start: 96, 640 * 96 = 256 * 144 + 384 * 64 (wide: 72, and
+  // all keep them; 80 and 56: 266 us where 72 and 72 take 260)
+  static constexpr int SOFT_REGS = WIDE ? 72 : 144, REST_REGS = WIDE ? 72 : 64;
 };
 struct QbSeg {          // a run of tiles of one item
   Item it;
@@ -545,8 +563,10 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
       mbar_init(&ms.q_ready[i], C::WIDE ? C::KDEC : 1); mbar_init(&ms.q_free[i], 1);
     }
     mbar_init(&ms.o_free, C::KDEC);
-    for (int i = 0; i < 4; ++i) mbar_init(&ms.rec_ready[i], 1);
-    for (int i = 0; i < 8; ++i) mbar_init(&ms.decided[i >> 2][i & 3], 2);
+    if (C::WIDE) {
+      for (int i = 0; i < 4; ++i) mbar_init(&ms.rec_ready[i], 1);
+      for (int i = 0; i < 8; ++i) mbar_init(&ms.decided[i >> 2][i & 3], 2);
+    }
     for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], C::WIDE ? 1 : 4); }
     ms.abort = ms.started = 0;
     ms.shared = make_int4(0, 0, 0, 0);
@@ -1143,7 +1163,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
           ns[jj] = scale_shift(sp[jj]);
         }
         uint8_t* vt = smem + C::V_OFF + (t & 1) * C::V_BYTES + chunk * 16384 + g * 2048;
-#pragma unroll C::WIDE ? 2 : 1
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {   // 8 channels: words 2h and 2h + 1 of each piece
           uint2 w[4];
 #pragma unroll
@@ -1437,8 +1457,10 @@ static cudaError_t launch_tc(const Q4AttnParams& p, int num_sms, cudaStream_t st
   return launch_pdl(q4_attn_tc_merge_kernel<PASS>, dim3(num_sms, N / 16), dim3(256), 0, st, p, N);
 }
 
-// Query rows of a group's pass past 80 of a kv head: 128 columns, wide.
-static bool wide_pass(int max_rows, int nq, int nkv) { return (long long)max_rows * (nq / nkv) > 80; }
+// Query rows of a group's pass past 64 of a kv head: the wide form (us, wide / not:
+// 64 rows on 8 groups of 8,192 rows 71 / 66 in f16 and 72 / 71 in bf16, 80 rows 73 / 78
+// and 74 / 86; 32 groups of 4,096 rows 139 / 126 and 141 / 146).
+static bool wide_pass(int max_rows, int nq, int nkv) { return (long long)max_rows * (nq / nkv) > 64; }
 
 size_t q4_attn_tc_group_floats(int max_rows, int nq, int nkv, int num_sms) {
   const size_t n = wide_pass(max_rows, nq, nkv) ? 128 : 80;
