@@ -751,6 +751,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t o_t = tmem + C::O_COL + x * N + lanes;
+    uint8_t* pr = smem + C::P_OFF + x * C::P_BYTES + row * 128;
     const int window = p.window > 0 ? p.window : 1 << 30;   // no cache is longer
     float* negm = ms.negm[x];
     float* facs = ms.fac[x];
@@ -786,11 +787,9 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
       for (int k = (t0 & 1) == x ? 0 : 1; k < nt; k += 2) {
         const int t = t0 + k;
         const uint32_t s_t = tmem + C::S_COL + (t % C::SB) * N + lanes;
-        uint8_t* const p_at = smem + C::P_OFF + x * C::P_BYTES;
-        uint8_t* const pr = p_at + row * 128;
         // P is read, and this side's O holds the tiles before t
         auto wait_pv = [&]() {
-          if (t >= 2) qb_wait(&ms.pvdone[t & 1], ((t >> 1) - 1) & 1, dead);
+          if (t >= 2) qb_wait(&ms.pvdone[x], ((t >> 1) - 1) & 1, dead);
         };
         if (k > 0) qb_wait(&ms.s_ready[t % C::SB], (t / C::SB) & 1, dead);
         tc_fence_after();
@@ -884,7 +883,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
             // Column maxima of the tile over the lanes, 16 columns at a time through
             // this side's P (its last reader is done), then over the warps.
             wait_pv();
-            float* stage = reinterpret_cast<float*>(p_at) + (warp & 3) * (16 * 36);
+            float* stage = reinterpret_cast<float*>(smem + C::P_OFF + x * C::P_BYTES) + (warp & 3) * (16 * 36);
 #pragma unroll 1
             for (int c = 0; c < C::CH; ++c) {
               uint32_t s[16];
@@ -949,7 +948,7 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
         tc_fence_before();
         warp_arrive(&ms.s_free[t % C::SB], lane);
         fence_proxy_async_smem();
-        warp_arrive(&ms.p_ready[t & 1], lane);
+        warp_arrive(&ms.p_ready[x], lane);
       }
       u += nt;
 
@@ -1018,19 +1017,17 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
       for (int c = x; c < C::CH; c += 2) {
         uint32_t oa[16], ob[16];
         __syncwarp();
-        {
-          tmem_ld16(o_a + 16 * c, oa);
-          tmem_ld16(o_b + 16 * c, ob);
-          tmem_ld_wait();
+        tmem_ld16(o_a + 16 * c, oa);
+        tmem_ld16(o_b + 16 * c, ob);
+        tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 fa = *reinterpret_cast<const float4*>(&ms.fac[0][16 * c + i]);
-            const float4 fb = *reinterpret_cast<const float4*>(&ms.fac[1][16 * c + i]);
-            const float wa[4] = {fa.x, fa.y, fa.z, fa.w}, wb[4] = {fb.x, fb.y, fb.z, fb.w};
+        for (int i = 0; i < 16; i += 4) {
+          const float4 fa = *reinterpret_cast<const float4*>(&ms.fac[0][16 * c + i]);
+          const float4 fb = *reinterpret_cast<const float4*>(&ms.fac[1][16 * c + i]);
+          const float wa[4] = {fa.x, fa.y, fa.z, fa.w}, wb[4] = {fb.x, fb.y, fb.z, fb.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              oa[i + k] = __float_as_uint(fmaf(__uint_as_float(oa[i + k]), wa[k], __uint_as_float(ob[i + k]) * wb[k]));
-          }
+          for (int k = 0; k < 4; ++k)
+            oa[i + k] = __float_as_uint(fmaf(__uint_as_float(oa[i + k]), wa[k], __uint_as_float(ob[i + k]) * wb[k]));
         }
         if (!whole) {
           float* dst = part + 16 * c * 128 + row;
