@@ -13,7 +13,7 @@ class Groups:
     """Requests in groups: (rows shared, [rows of their own], [query rows]) each, on shuffled pages.  Shared rows are
     whole pages plus, where `prefix` is none, rows that the members hold alike on pages of their own."""
 
-    def __init__(self, pkg, groups, page, nq, nkv, dtype=torch.float16, seed=0, strength=1.0, base=0):
+    def __init__(self, pkg, groups, page, nq, nkv, dtype=torch.float16, seed=0, strength=1.0, base=0, growth=None):
         rng, g = np.random.default_rng(seed), torch.Generator().manual_seed(seed)
         self.page, self.nq, self.nkv, self.sizes = page, nq, nkv, [len(own) for _, own, _ in groups]
         cdiv = lambda a: -(-a // page)
@@ -31,6 +31,8 @@ class Groups:
             for o in own:
                 k1, v1 = make(o)
                 k, v = torch.cat([k0, k1]), torch.cat([v0, v1])
+                if growth:
+                    k = (k.double() * growth(torch.arange(p + o).double())[:, None, None]).to(dtype)
                 mine = common + [next(perm) for _ in range(cdiv(p + o) - p // page)]
                 self.table[i, :len(mine)] = mine
                 if p + o:
@@ -185,6 +187,41 @@ def test_large_and_small_scores(pkg, strength, scale):
         out, _, _ = d.attend(pkg, True, scale)
         plain = pkg.q4_attention(d.q, d.pool, d.d_table, d.d_lens, d.starts, 3, True, scale=scale)
         assert torch.equal(out, plain) and bool(torch.isfinite(out).all())
+
+
+GROWTH = {"up": lambda pos: 1 + pos / 40, "down": lambda pos: 40 / (1 + pos / 40), "steps": lambda pos: 1 + 30 * (pos // 128 % 3)}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("growth", GROWTH)
+@pytest.mark.parametrize("members,nq,nkv", [(20, 4, 1), (33, 16, 2), (70, 4, 1), (3, 4, 1)])
+def test_scores_that_grow_or_fall_along_the_cache(pkg, dtype, growth, members, nq, nkv):
+    # (every tile of shared rows passes the references of the tiles before, or none does)
+    d = Groups(pkg, [(1424, [1 + i % 7 for i in range(members)], [1 + i % 3 for i in range(members)])], 16, nq, nkv, dtype,
+               seed=21, growth=GROWTH[growth])
+    assert d.check(pkg, False).prefix.tolist() == [1424]
+
+
+@pytest.mark.parametrize("rows", [1, 3, 5, 9])
+def test_query_rows_of_all_magnitudes_in_bf16(pkg, rows):
+    d = Groups(pkg, [(700, [5] * 30, [rows] * 30)], 64, 8, 2, torch.bfloat16, seed=22)
+    size = torch.arange(d.q.shape[0], device="cuda") % 7 - 3
+    d.q *= (2.0 ** (14 * size))[:, None, None].to(torch.bfloat16)
+    d.q[0] = 0
+    d.check(pkg, False)
+
+
+def test_shared_pages_that_are_not_there(pkg):
+    # entries outside the pool hide their rows, as in q4_attention
+    d = Groups(pkg, [(1024, [9] * 40, [1] * 40)], 32, 16, 4, seed=23)
+    hidden = [0, 5, 17, 31]
+    d.d_table[:, hidden] = torch.tensor([-1, 10 ** 6, -7, 2 ** 30], dtype=torch.int32, device="cuda")
+    out, plan, status = d.attend(pkg, False)
+    assert plan.prefix.tolist() == [1024]
+    keep = torch.tensor([p // 32 not in hidden for p in range(1024 + 9)])
+    want, bound = U.attention(d.q, [k[keep] for k in d.ks], [v[keep] for v in d.vs], d.rows, U.scale_of(128), False)
+    tol = U.attention_tolerance(want, bound, out.dtype) + bound[0] * 2.0 ** -18
+    assert bool(((out.double().cpu() - want).abs() <= tol).all())
 
 
 def test_without_starts_and_with_strided_queries(pkg):
