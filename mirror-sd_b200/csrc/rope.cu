@@ -11,7 +11,7 @@
 // operations a pair, and the angles, shared by all heads of a row, are made once
 // a row into shared memory while the first elements are on their way.  65,521 rows
 // of 40 heads in bf16 are 1.34 GB in and out, 204 us at the rate of a copy; they
-// take 202.  256 rows take a launch.
+// take 206.  256 rows take a launch.
 #include "decode.cuh"
 
 namespace dfl {
