@@ -592,14 +592,15 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     __syncthreads();
     if (lane == 31) ms.wtot[warp] = x;
     __syncthreads();
-    int before = 0, all = 0;
+    int w = lane < C::THREADS / 32 ? ms.wtot[lane] : 0;
 #pragma unroll
-    for (int w = 0; w < C::THREADS / 32; ++w) {
-      if (w < warp) before = tiles_sum(before, ms.wtot[w]);
-      all = tiles_sum(all, ms.wtot[w]);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w = tiles_sum(w, y);
     }
-    *sum = all;
-    return tiles_sum(before, x - v);
+    *sum = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+    return tiles_sum(warp > 0 ? before : 0, x - v);
   };
   const int grid = gridDim.x;
   // Passes over shared and own rows weigh an item's start and end as well, QB_ITEM
