@@ -292,3 +292,42 @@ def test_streams_and_graphs(pkg):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, d.attend(pkg, True)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("count", [5, 40])
+def test_groups_of_many_rows_and_all_lengths(pkg, dtype, count):
+    # several items a CTA, of one tile to ten, with 65 to 300 query rows a kv head
+    lens = [16, 128, 144, 384, 640, 1280, 256]
+    d = Groups(pkg, [(lens[i % 7], [1 + (i + j) % 5 for j in range(17 + i % 4 * 19)], [1] * (17 + i % 4 * 19)) for i in range(count)],
+               16, 8, 2, dtype, seed=31)
+    plan = d.check(pkg, True)
+    assert plan.prefix.tolist() == [lens[i % 7] for i in range(count)]
+
+
+def test_large_groups_on_two_streams_and_in_graphs(pkg):
+    d = Groups(pkg, [(2048, [1 + i % 9 for i in range(40)], [1] * 40), (1000, [3] * 70, [1] * 70)], 16, 16, 4, torch.bfloat16, seed=32)
+    want = d.attend(pkg, True)[0]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(d.attend(pkg, True)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    groups = torch.tensor([0, 40, 110], dtype=torch.int32, device="cuda")
+    graphs = []
+    for _ in range(2):       # (two graphs that share a workspace, one after the other)
+        ws = graphs[0][2] if graphs else pkg.q4_prefix_workspace(110, 1, 70, 16, 4)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan = pkg.paged_prefix_plan(d.d_table, d.d_lens, groups, 16, d.starts, 1, True, max_group=70, least=0)
+            graphs.append((graph, pkg.q4_prefix_attention(d.q, d.pool, d.d_table, plan, workspace=ws), ws))
+    d.q.mul_(0.5)
+    want = d.attend(pkg, True)[0]
+    for _ in range(3):
+        for graph, _, _ in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, out, _ in graphs)
