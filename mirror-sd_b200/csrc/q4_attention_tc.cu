@@ -295,35 +295,33 @@ __host__ __device__ __forceinline__ int4* q4_tc_shared(float* part, int n, int g
   return reinterpret_cast<int4*>(part + (size_t)grid * 2 * n * 130);
 }
 
-// 16 bytes of a bf16 query row, the row's others in 15 neighbouring lanes, as f16.
-// A row whose largest magnitude lies in [2^-3, 2^15] is rounded to f16 as it is (what
-// is below 2^-14 loses bits, 2^-22 of that largest at most); any other row is scaled
-// by a power of two first, whose exponent is returned (0: none).
-__device__ __forceinline__ int query_f16(uint4* at, int lane) {
-  const uint32_t half = lane < 16 ? 0xffffu : 0xffff0000u;   // the lanes of this lane's row
-  const uint4 w = *at;
+// 16 bytes of bf16 as floats; returns the largest magnitude.
+__device__ __forceinline__ float query_floats(const uint4& w, float (&x)[8]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-  float x[8], a = 0.f;
-  int e = 0;
+  float a = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     x[2 * k] = __uint_as_float(u[k] << 16);
     x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
     a = fmaxf(a, fmaxf(fabsf(x[2 * k]), fabsf(x[2 * k + 1])));
   }
-  const uint32_t big = __ballot_sync(0xffffffffu, a >= 0.125f), nonzero = __ballot_sync(0xffffffffu, a > 0.f);
-  const bool plain = (!(nonzero & half) || (big & half)) && a <= 32768.f;
-  if (!__all_sync(0xffffffffu, plain)) {
-#pragma unroll 1
-    for (int o = 1; o < 16; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if (a != 0.f && !(a >= 0.125f && a <= 32768.f)) {
-      e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
-      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+  return a;
+}
+// 16 bytes of a bf16 query row, the row's others in 15 neighbouring lanes, as f16.
+// A row whose largest magnitude lies in [2^-3, 2^15] is rounded to f16 as it is (what
+// is below 2^-14 loses bits, 2^-22 of that largest at most); any other row is scaled
+// by a power of two first, whose exponent is returned (0: none).  All lanes take part;
+// rows without `mine` stay as they are.
+__device__ __forceinline__ int query_f16(uint4* at, bool mine, int lane) {
+  float x[8];
+  const float a = __uint_as_float(   // (not negative: ordered as integers)
+      __reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, __float_as_uint(query_floats(*at, x))));
+  const bool scaled = mine && a != 0.f && !(a >= 0.125f && a <= 32768.f);
+  const int e = scaled ? min(max((int)(__float_as_uint(a) >> 23), 1), 253) : 0;
+  const float down = scaled ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] *= down;
-    }
-  }
-  *at = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+  for (int k = 0; k < 8; ++k) x[k] *= down;
+  if (mine) *at = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
   return e;
 }
 __device__ __forceinline__ float scaled_factor(float f, int e) { return fminf(f * __uint_as_float((uint32_t)e << 23), 3e38f); }
@@ -371,7 +369,7 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int e = p.bf16 ? query_f16(reinterpret_cast<uint4*>(query_at(i)), lane) : 0;
+      const int e = p.bf16 ? query_f16(reinterpret_cast<uint4*>(query_at(i)), true, lane) : 0;
       if (piece == 0) ms.qf[seg & 1][q_row0 + 2 * i] = e ? scaled_factor(base_f, e) : base_f;
     }
     fence_proxy_async_smem();
@@ -1272,40 +1270,63 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
       uint8_t* qs = smem + C::Q_OFF + qb * C::Q_BYTES;
       float* qf = ms.qf[C::WIDE ? 0 : seg % C::SEGS];
       const int grp = p.by_nkv.of(cur.sub), q0 = grp * N, head0 = (cur.sub - grp * p.nkv) * G;
-      // every 16-byte piece of the rows at once (2 rows an instruction), then the
-      // bf16 ones to f16 in place
-      if (!C::WIDE) {
-        const int piece = lane & 15;
-        const int r = q0 + (lane >> 4);
-        int j = p.by_g.of(r), h = r - j * G;
-        const uint16_t* q = static_cast<const uint16_t*>(p.q) + (size_t)cur.it.row0 * p.q_row + 8 * piece;
-        uint8_t* dst = qs + (piece >> 3) * (N * 128);
-#pragma unroll 4
-        for (int i = lane >> 4; i < N; i += 2) {
-          const bool real = j < cur.it.rows;
-          cp_async16_zfill(smem_u32(dst + i * 128 + (((piece & 7) ^ (i & 7)) << 4)),
-                           real ? q + (size_t)j * p.q_row + (size_t)(head0 + h) * p.q_head : p.q, real);
-          h += 2;
-          if (h >= G) { h -= G; ++j; }
-          if (h >= G) { h -= G; ++j; }   // (one head a kv head)
+      bool uniform = true;
+      if constexpr (!C::WIDE) {
+        // Every 16-byte piece of the rows at once, 2 rows an instruction.  (One warp does
+        // it all: what a row costs is its chain of instructions, so addresses are added
+        // up, four rows' under way together.)
+        const int piece = lane & 15, side = lane >> 4;
+        uint8_t* const dst = qs + (piece >> 3) * (N * 128) + side * 128;
+        int j = p.by_g.of(q0 + side), h = q0 + side - j * G;
+        const uint16_t* at = static_cast<const uint16_t*>(p.q) + (size_t)(cur.it.row0 + j) * p.q_row + (size_t)(head0 + h) * p.q_head + 8 * piece;
+        const long long wrap = p.q_row - G * p.q_head;
+#pragma unroll 1
+        for (int i = 0; i < N; i += 8) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const bool real = j < cur.it.rows;
+            cp_async16_zfill(smem_u32(dst + (i + e) * 128 + (((piece & 7) ^ (e + side)) << 4)), real ? at : p.q, real);
+            h += 2;
+            at += 2 * p.q_head;
+            if (h >= G) { h -= G; ++j; at += wrap; }
+            if (h >= G) { h -= G; ++j; at += wrap; }   // (one head a kv head)
+          }
         }
         cp_async_commit();
+        for (int i = lane; i < N; i += 32) qf[i] = base_f;
         cp_async_wait<0>();
         __syncwarp();
-      }
-      bool uniform = true;
-      if (!C::WIDE)
-        for (int i = lane; i < N; i += 32) qf[i] = base_f;
-      __syncwarp();
-      if (!C::WIDE && p.bf16) {
-        const int piece = lane & 15;
-        uint8_t* src = qs + (piece >> 3) * (N * 128);
-#pragma unroll 4
-        for (int i = lane >> 4; i < N; i += 2) {
-          const int e = query_f16(reinterpret_cast<uint4*>(src + i * 128 + (((piece & 7) ^ (i & 7)) << 4)), lane);
-          if (e) {
-            if (piece == 0) qf[i] = scaled_factor(base_f, e);
-            uniform = false;
+        if (p.bf16) {
+          // To f16 in place, the rows that have to be scaled behind the others: votes are
+          // cheaper than maxima (256 requests of 16 x 4 rows 212 us, all rows by maxima 245).
+          const uint32_t half = side == 0 ? 0xffffu : 0xffff0000u;   // the lanes of this lane's row
+          uint64_t left = 0;
+#pragma unroll 1
+          for (int i = 0; i < N; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              uint4* const to = reinterpret_cast<uint4*>(dst + (i + e) * 128 + (((piece & 7) ^ (e + side)) << 4));
+              float x[8];
+              const float a = query_floats(*to, x);
+              const uint32_t big = __ballot_sync(0xffffffffu, a >= 0.125f), nonzero = __ballot_sync(0xffffffffu, a > 0.f),
+                             over = __ballot_sync(0xffffffffu, a > 32768.f);
+              if (!(over & half) && (!(nonzero & half) || (big & half)))
+                *to = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+              else
+                left |= 1ull << ((i + e) / 2);
+            }
+          }
+          if (__any_sync(0xffffffffu, left != 0)) {
+#pragma unroll 1
+            for (int i = 0; i < N; i += 8) {
+#pragma unroll
+              for (int k = 0; k < 8; k += 2) {
+                const bool mine = left >> ((i + k) / 2) & 1;
+                const int e = query_f16(reinterpret_cast<uint4*>(dst + (i + k) * 128 + (((piece & 7) ^ (k + side)) << 4)), mine, lane);
+                if (e && piece == 0) qf[i + k + side] = scaled_factor(base_f, e);
+                uniform = uniform && e == 0;
+              }
+            }
           }
         }
         uniform = __all_sync(0xffffffffu, uniform);
