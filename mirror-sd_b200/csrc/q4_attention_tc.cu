@@ -19,8 +19,8 @@
 //
 // (There one O serves both sides, 16 warps share the softmax, and K goes to shared
 // memory; see wide_softmax.)  1,360 query rows a kv head on 2 groups of 16,384 rows
-// take 182 us, in the transposed form 270, 12 of them the start (lengths, query rows,
-// first tiles) and 5 the end; 1,024 on 4,096 rows 38.  A tile takes 1,900 cycles, of
+// take 178 us, in the transposed form 270, 10 of them the start (lengths, query rows,
+// first tiles) and 5 the end; 1,024 on 4,096 rows 35.  A tile takes 1,900 cycles, of
 // which the MMAs need 1,024 and shared memory moves bytes for 1,570 (64 KB for QK^T,
 // 32 for PV, 64 of decoded K and V written, 36 of codes in and out).  What would pay
 // next: Q as the operand in TMEM with scores of 64 cached rows at a time (bytes for
