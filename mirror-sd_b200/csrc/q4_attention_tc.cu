@@ -117,10 +117,9 @@ struct QbSeg {          // a run of tiles of one item
 template <class C>
 struct QbMisc {
   uint64_t full[4], empty[4], kready[2], kfree[2], vready[2], pvdone[2], s_ready[4], s_free[4], p_ready[2];
-  uint64_t q_ready[2], q_free[2], o_free, rec_ready[4], decided[2][4];
+  uint64_t q_ready[2], q_free[2], o_free, rec_ready[4], begun[4], decided[2][4];
   uint32_t tmem;
   int abort;
-  int started;                    // items that the softmax warps have begun (wide)
   int where[2];                   // request of the CTA's first tile, and that request's first tile
   int run[2], share;              // whole CTAs to an item: this one's tiles, and their number
   int wtot[C::THREADS / 32];
@@ -380,7 +379,7 @@ __device__ __forceinline__ void wide_softmax(const Q4AttnParams& p, QbMisc<C>& m
     const bool bad = named_bar_or<SOFT>(3, *dead);
     const int nt = bad ? c1 - u : sg.nt;
     const float f = score_factor(ms.qf[seg & 1][row]);
-    if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(&ms.started) = seg + 1;
+    if (threadIdx.x == 0) mbar_arrive(&ms.begun[seg & 3]);
     float negm = kUnset;   // minus the reference
     float2 l = make_float2(0.f, 0.f);
 
@@ -562,11 +561,11 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
     }
     mbar_init(&ms.o_free, C::KDEC);
     if (C::WIDE) {
-      for (int i = 0; i < 4; ++i) mbar_init(&ms.rec_ready[i], 1);
+      for (int i = 0; i < 4; ++i) { mbar_init(&ms.rec_ready[i], 1); mbar_init(&ms.begun[i], 1); }
       for (int i = 0; i < 8; ++i) mbar_init(&ms.decided[i >> 2][i & 3], 2);
     }
     for (int i = 0; i < C::SB; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.s_free[i], C::WIDE ? 1 : 4); }
-    ms.abort = ms.started = 0;
+    ms.abort = 0;
     ms.shared = make_int4(0, 0, 0, 0);
     ms.run[0] = ms.run[1] = 0;
     fence_mbar_init();
@@ -1259,11 +1258,8 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
       const int qb = seg % C::QB;
       const int nt = min(cur.it.ntile - cur.j, c1 - u);
       if constexpr (C::WIDE) {   // the softmax warps bring the rows; records run ahead of them, while there is room
-        for (uint32_t i = 0; *reinterpret_cast<volatile int*>(&ms.started) < seg - (C::SEGS - 2) && !*dead; ++i) {
-          if (i == kSpinLimit) *dead = 1;
-          __nanosleep(100);
-        }
-        __syncwarp();
+        // (that of item seg - 4 is no longer read once item seg - 3 has begun)
+        if (seg >= 3) qb_wait(&ms.begun[(seg - 3) & 3], ((seg - 3) >> 2) & 1, dead);
       } else if (seg >= C::QB) {
         qb_wait(&ms.q_free[qb], ((seg / C::QB) - 1) & 1, dead);
       }
