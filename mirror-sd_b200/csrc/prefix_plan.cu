@@ -79,7 +79,9 @@ __global__ void __launch_bounds__(PP_THREADS) prefix_plan_kernel(const PrefixPla
   for (int i = a + warp; i < b; i += PP_THREADS / 32) {
     if (i == ref || rows(i) <= 0) continue;
     const int32_t* other = p.table + (size_t)i * p.table_ld;
-    int most = *reinterpret_cast<volatile int*>(&limit);
+    int most = 0;   // (read by one lane: the votes below need the whole warp, and other warps lower it meanwhile)
+    if (lane == 0) most = *reinterpret_cast<volatile int*>(&limit);
+    most = __shfl_sync(0xffffffffu, most, 0);
 #pragma unroll 4
     for (int c0 = 0; c0 < most; c0 += 32) {
       const int c = c0 + lane;

@@ -1,0 +1,55 @@
+"""Plans of shared prefixes on the GPU, against their definition on the host."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(v):
+    return torch.tensor(np.array(v), dtype=torch.int32).cuda()
+
+
+def definition(table, lens, rows, bounds, page, causal, least):
+    """(prefix of each group, skip and own rows of each request)."""
+    prefix, spared = [], 0
+    for a, b in zip(bounds, bounds[1:]):
+        mine = [i for i in range(a, b) if rows[i] > 0]
+        pages = 0
+        if len(mine) > 1:
+            pages = min(max(lens[i] - (rows[i] - 1 if causal else 0), 0) // page for i in mine)
+            same = (table[mine, :pages] == table[mine[0], :pages]).all(0)
+            pages = pages if same.all() else int(np.argmin(same))
+            spared += (len(mine) - 1) * pages * page
+        prefix.append(pages * page)
+    if spared < least:
+        prefix = [0] * len(prefix)
+    skip = [0] * len(lens)
+    for k, (a, b) in enumerate(zip(bounds, bounds[1:])):
+        for i in range(a, b):
+            skip[i] = prefix[k] // page if rows[i] > 0 else 0
+    return prefix, skip, [n - s * page for n, s in zip(lens, skip)]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,g,columns,page", [(40, 1, 700, 16), (40, 5, 300, 32), (300, 17, 65, 64), (2048, 600, 33, 16),
+                                              (2048, 1, 40, 16), (2, 1, 1, 256)])
+def test_plans_match_the_definition(pkg, n, g, columns, page, causal):
+    """Members that differ at random columns, in the order that makes each of them shorten the prefix of those before it,
+    and in others: many warps compare while the limit falls."""
+    rng = np.random.default_rng(n + g + columns)
+    for trial in range(8):
+        bounds = [0] + sorted(rng.integers(0, n + 1, g).tolist()) if g > 1 else [0, n]
+        table = np.zeros((n, columns), np.int32)
+        for a, b in zip(bounds, bounds[1:]):
+            table[a:b] = rng.integers(0, 1 << 20, columns)
+            at = rng.integers(0, 3 * columns, max(b - a, 1))
+            at = np.sort(at)[::-1] if trial % 2 else at
+            for i, c in zip(range(a + 1, b), at):
+                table[i, c:] += 1 + i
+        lens = (rng.integers(0, columns * page + 1, n) if trial % 3 == 0 else np.full(n, columns * page)).tolist()
+        rows = rng.integers(0, 4, n).tolist()
+        starts = i32(np.concatenate([[0], np.cumsum(rows)]))
+        plan = pkg.paged_prefix_plan(i32(table), i32(lens), i32(bounds), page, starts, 3, causal, n, 0)
+        got = plan.prefix.tolist(), plan.skip.tolist(), plan.own_lens.tolist()
+        assert got == definition(table, lens, rows, bounds, page, causal, 0), trial
