@@ -424,10 +424,11 @@ __device__ __forceinline__ int drafts_of(const VerifyParams& p, int seq) {
 __device__ __forceinline__ float temperature_of(const VerifyParams& p, int seq) { return p.temps ? __ldg(p.temps + seq) : p.temp; }
 __device__ __forceinline__ bool is_greedy(float temp) { return !(temp >= 1e-5f); }
 
-struct Part {   // of a row, by a warp
-  float m;      // reference, or the largest entry
-  int s;        // bits of the sum, or the entry's place
+struct alignas(8) Part {   // of a row, by a warp (stored as 64 bits)
+  float m;                 // reference, or the largest entry
+  int s;                   // bits of the sum, or the entry's place
 };
+static_assert(sizeof(Part) == 8 && alignof(Part) == 8, "st_cluster_u64 stores it whole");
 // What a cluster's CTAs know of their request: rows whose drafts are accepted so
 // far, or -1 - stop once that is known, and the bits of the last decided row's
 // reference (its first largest entry, where the request is greedy).
