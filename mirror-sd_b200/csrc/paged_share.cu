@@ -93,9 +93,9 @@ __global__ void __launch_bounds__(PG_THREADS) paged_fork_kernel(const ForkParams
 // the one that ends up keeping it: after the first that finds too few, it is
 // turned away too, for one before it may still hold the page.
 __global__ void __launch_bounds__(PG_THREADS) paged_reserve_forked_kernel(const ReserveParams p, int32_t* holders, int32_t* copies) {
-  extern __shared__ int sm[];
+  extern __shared__ __align__(16) int words[];
   const int n = p.n, n4 = (n + 3) & ~3;
-  int* tail = sm;                   // [n4] page written into, -1: it is the request's own
+  int* tail = words;                // [n4] page written into, -1: it is the request's own (read 16 bytes at a time)
   int* first_row = tail + n4;       // [n]
   int* first_need = first_row + n;  // [n]
   int* len = first_need + n;        // [n]
