@@ -487,8 +487,8 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
  * The plan, once a step for all layers, compares the members' block tables: their
  * prefix is the pages that the rows of all members with query rows begin with
  * alike, as far as every query row sees them whole (starts, max_rows and causal as
- * in dflash_q4_attention; lens [n]).  Where that would spare fewer than `least`
- * cached rows from being read, over all groups, nothing is shared: a pass over
+ * in dflash_q4_attention; lens [n]).  Where the pages found alike spare fewer than
+ * `least` cached rows from being read, over all groups, nothing is shared: a pass over
  * shared rows costs about as much as reading 32,768 rows of 8 kv heads.  Written: group_starts [num_groups + 1],
  * prefix [num_groups] (rows), row_of [num_groups], skip [n] (pages), own_lens [n].
  *

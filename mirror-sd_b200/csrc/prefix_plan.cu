@@ -3,8 +3,11 @@
 // those that every query row sees whole.  Once a step, for all layers.
 //
 // One CTA a group; a warp compares a member's table row with the first member's,
-// 32 columns at a time, up to the first difference that any warp has found.  Few
-// numbers, so what it takes is latency.
+// 32 columns at a time, up to the first difference that any warp has found.  Nothing
+// is compared where the lengths alone leave fewer rows to spare than are asked for.
+// What the tables spare is known once all groups are compared: one group's CTA sees
+// that for itself, several groups' is added up by a second kernel.  Few numbers, so
+// what both take is latency.
 #include "q4.cuh"
 
 namespace dfl {
@@ -54,7 +57,7 @@ __global__ void __launch_bounds__(PP_THREADS) prefix_plan_kernel(const PrefixPla
   auto start = [&](int i) { return p.starts ? __ldg(p.starts + i) : i * p.max_rows; };
   auto rows = [&](int i) { return start(i + 1) - start(i); };
   auto length = [&](int i) { return (int)min((long long)max(__ldg(p.lens + i), 0), (long long)p.max_pages * p.page_size); };
-  // What sharing could spare, of all groups together: every CTA adds it up for itself.
+  // What sharing could spare at most, by the lengths, of all groups together: every CTA adds it up for itself.
   for (int i = bound[0] + threadIdx.x; i < bound[p.g]; i += PP_THREADS) {
     const int m = rows(i);
     if (m <= 0) continue;
@@ -94,7 +97,8 @@ __global__ void __launch_bounds__(PP_THREADS) prefix_plan_kernel(const PrefixPla
     }
   }
   __syncthreads();
-  const int pages = limit;
+  int pages = limit;
+  if (p.g == 1 && (counts[0] - 1ll) * pages * p.page_size < p.least) pages = 0;
   auto plan = [&](int i, int skip) {
     p.skip[i] = skip;
     p.own_lens[i] = max(length(i) - skip * p.page_size, 0);
@@ -113,9 +117,35 @@ __global__ void __launch_bounds__(PP_THREADS) prefix_plan_kernel(const PrefixPla
     for (int i = b + threadIdx.x; i < p.n; i += PP_THREADS) plan(i, 0);
 }
 
+// A plan that spares fewer than `least` rows (each sharing member's shared rows, less
+// once a group) shares nothing.
+__global__ void __launch_bounds__(PP_THREADS) prefix_least_kernel(const PrefixPlanParams p) {
+  __shared__ long long part[PP_THREADS / 32];
+  griddep_wait();
+  griddep_launch_dependents();
+  long long spared = 0;
+  for (int i = threadIdx.x; i < p.n; i += PP_THREADS) spared += (long long)p.skip[i] * p.page_size;
+  for (int k = threadIdx.x; k < p.g; k += PP_THREADS) spared -= p.prefix[k];
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) spared += __shfl_xor_sync(0xffffffffu, spared, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = spared;
+  __syncthreads();
+  spared = 0;
+  for (int w = 0; w < PP_THREADS / 32; ++w) spared += part[w];
+  if (spared >= p.least) return;
+  for (int i = threadIdx.x; i < p.n; i += PP_THREADS) {
+    p.own_lens[i] += p.skip[i] * p.page_size;
+    p.skip[i] = 0;
+  }
+  for (int k = threadIdx.x; k < p.g; k += PP_THREADS) p.prefix[k] = 0;
+}
+
 cudaError_t prefix_plan_launch(const PrefixPlanParams& p, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs || p.g < 1 || p.g > kPagedMaxSeqs) return cudaErrorInvalidValue;
-  return launch_pdl(prefix_plan_kernel, dim3(p.g), dim3(PP_THREADS), ((size_t)3 * p.g + 1) * sizeof(int), st, p);
+  DFL_TRY(launch_pdl(prefix_plan_kernel, dim3(p.g), dim3(PP_THREADS), ((size_t)3 * p.g + 1) * sizeof(int), st, p));
+  // (nothing spares 2^42 rows, 2,048 requests of 2^31: the first kernel has then shared nothing)
+  if (p.g == 1 || p.least <= 0 || p.least > 1ll << 42) return cudaSuccess;
+  return launch_pdl(prefix_least_kernel, dim3(1), dim3(PP_THREADS), 0, st, p);
 }
 
 }  // namespace dfl

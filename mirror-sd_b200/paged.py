@@ -216,8 +216,8 @@ def paged_prefix_plan(table, lens, groups, page_size: int, starts=None, max_rows
     boundaries [g + 1] with ``max_group``, the requests of a group at most.  Requests
     of no group are on their own, and where sharing would spare fewer than ``least``
     cached rows from being read, over all groups, all of them are (8 samples of 2,048
-    rows each take 18 us on their own, 29 shared).  lens, starts, max_rows and causal
-    as for ``q4_attention``."""
+    rows each take 18 us on their own, 29 shared).  What is spared is counted in the
+    pages found alike.  lens, starts, max_rows and causal as for ``q4_attention``."""
     if not torch.is_tensor(groups):
         sizes = [int(s) for s in groups]
         if not sizes or any(s < 1 for s in sizes) or sum(sizes) > lens.numel():

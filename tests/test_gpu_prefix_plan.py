@@ -50,6 +50,9 @@ def test_plans_match_the_definition(pkg, n, g, columns, page, causal):
         lens = (rng.integers(0, columns * page + 1, n) if trial % 3 == 0 else np.full(n, columns * page)).tolist()
         rows = rng.integers(0, 4, n).tolist()
         starts = i32(np.concatenate([[0], np.cumsum(rows)]))
-        plan = pkg.paged_prefix_plan(i32(table), i32(lens), i32(bounds), page, starts, 3, causal, n, 0)
-        got = plan.prefix.tolist(), plan.skip.tolist(), plan.own_lens.tolist()
-        assert got == definition(table, lens, rows, bounds, page, causal, 0), trial
+        want = definition(table, lens, rows, bounds, page, causal, 0)[0]
+        total = sum((sum(r > 0 for r in rows[a:b]) - 1) * p for a, b, p in zip(bounds, bounds[1:], want) if p)
+        for least in (0, total, total + 1):
+            plan = pkg.paged_prefix_plan(i32(table), i32(lens), i32(bounds), page, starts, 3, causal, n, least)
+            got = plan.prefix.tolist(), plan.skip.tolist(), plan.own_lens.tolist()
+            assert got == definition(table, lens, rows, bounds, page, causal, least), (trial, least)
