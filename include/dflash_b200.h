@@ -495,9 +495,10 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
  * The attention gives what dflash_q4_attention gives without a window, up to the
  * rounding of one more join in fp32: the group's query rows over its prefix, then
  * each request's over its own rows, joined.  max_group: requests of a group at
- * most (more set DFLASH_PAGED_ROWS, and their rows are undefined); max_rows *
- * max_group <= DFLASH_Q4_MAX_ROWS.  workspace: dflash_q4_prefix_workspace_size()
- * bytes, as for dflash_q4_attention. */
+ * most (a group of more query rows than max_rows * max_group sets
+ * DFLASH_PAGED_ROWS; they are right all the same); max_rows * max_group <=
+ * DFLASH_Q4_MAX_ROWS.  workspace: dflash_q4_prefix_workspace_size() bytes, as for
+ * dflash_q4_attention. */
 int dflash_paged_prefix_plan(const int32_t* table, int64_t table_ld, int max_pages, const int32_t* lens, const int32_t* starts,
                              int n, int max_rows, int page_size, const int32_t* groups, int num_groups, int causal,
                              int64_t least, int32_t* group_starts, int32_t* prefix, int32_t* row_of, int32_t* skip, int32_t* own_lens,

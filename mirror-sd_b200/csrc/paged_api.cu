@@ -1,5 +1,6 @@
 // C ABI of the paged 4-bit K/V cache (include/dflash_b200.h): argument checks
 // and launches of paged.cu, q4_cache.cu and q4_attention.cu.
+#include <algorithm>
 #include <cmath>
 
 #include "api_error.cuh"
@@ -106,7 +107,7 @@ int attention_params(const uint16_t* q, int64_t q_row, int64_t q_head, int bf16,
   p = Q4AttnParams{};
   p.q = q; p.q_row = q_row; p.q_head = q_head; p.bf16 = bf16 != 0; p.pool = pool;
   p.table = table; p.lens = lens; p.starts = starts; p.table_ld = table_ld;
-  p.n = n; p.T = rows; p.max_rows = max_rows; p.nq = nq; p.nkv = nkv;
+  p.n = n; p.T = rows; p.max_rows = p.most_rows = max_rows; p.nq = nq; p.nkv = nkv;
   p.by_g = Divisor(G); p.by_nkv = Divisor(nkv);
   p.page_shift = log2_of(page_size);
   p.max_pages = max_pages; p.num_pages = num_pages; p.causal = causal != 0; p.sink = sink; p.window = window;
@@ -415,6 +416,12 @@ int dflash_q4_prefix_attention(const uint16_t* q, int64_t q_row, int64_t q_head,
   group.pre_ml = own.pre_ml = reinterpret_cast<float2*>(group.pre_o + (size_t)rows * nq * 128);
   group.row_of = row_of;
   group.table_rows = n;
+  // The own pass joins what the group pass leaves for every row, so a group of more rows than the caller said (on the
+  // device, where nobody has looked) is taken whole: max_rows and max_group choose the kernel, any number of rows runs
+  // through it.  The bounds are those of the divisions by G and nkv, x * d < 2^32: millions of rows.
+  const double G = nq / nkv, columns = few_group ? q4_attn_columns(group.max_rows, nq, nkv) : q4_attn_tc_columns(group.max_rows, nq, nkv);
+  const double by_g = (4294967295.0 / G - 128) / G, by_nkv = (4e9 / ((double)nkv * nkv) - 1) * columns / G;
+  group.most_rows = std::max(group.most_rows, (int)std::min({by_g, by_nkv, (double)rows}));
   own.skip = skip;
   if (int rc = attention_launch(group, few_group, kAttnPrefix, workspace, stream)) return rc;
   return attention_launch(own, few_own, kAttnOwn, workspace, stream);

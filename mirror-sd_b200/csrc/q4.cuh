@@ -156,6 +156,7 @@ struct Q4AttnParams {
   int* counters;                     // [2 * num_sms], zero between calls
   float* part;                       // partial results
   int32_t* status;                   // or NULL
+  int most_rows;                     // query rows of a request that are taken (kAttnPrefix: of a group); more are cut off
   // passes over rows that several requests share (AttnPass)
   const int32_t* row_of;             // kAttnPrefix: the table row of each group, of table_rows
   int table_rows;

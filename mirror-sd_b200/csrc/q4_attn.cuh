@@ -42,7 +42,7 @@ __device__ __forceinline__ int seq_rows(const Q4AttnParams& p, int i, int* row0)
   a = min(max(a, 0), p.T);
   b = min(max(b, a), p.T);
   *row0 = a;
-  return min(b - a, p.max_rows);
+  return min(b - a, p.most_rows);
 }
 // Whether they are the rows that the caller meant; the host has not seen starts,
 // so what does not fit is cut off above and reported.

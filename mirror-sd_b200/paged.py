@@ -213,7 +213,8 @@ def paged_prefix_plan(table, lens, groups, page_size: int, starts=None, max_rows
     their rows of the block table on the device: whole pages that all members with
     query rows begin with and whose rows all their query rows see.  groups: the
     sizes of consecutive runs of requests, or an int32 device tensor of their
-    boundaries [g + 1] with ``max_group``, the requests of a group at most.  Requests
+    boundaries [g + 1] with ``max_group``, the requests of a group at most (where one
+    has more, the attention's ``status`` says so, its rows are right).  Requests
     of no group are on their own, and where sharing would spare fewer than ``least``
     cached rows from being read, over all groups, all of them are (8 samples of 2,048
     rows each take 18 us on their own, 29 shared).  What is spared is counted in the
