@@ -30,6 +30,7 @@ from . import _native as N
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIM = 128
+MAX_GROUP_ROWS = 65536              # query rows that one pass of the attention takes of a request or a group
 BLOCK_BYTES = 2304                   # 16 rows of one kv head, K and V with their scales
 STATUS_BITS = {1: "too few free pages", 2: "a request outgrew its row of the block table",
                4: "more new rows than slots", 8: "more pages came back than were lent",
@@ -243,9 +244,23 @@ def paged_prefix_plan(table, lens, groups, page_size: int, starts=None, max_rows
                       max_rows, max_group, page_size, bool(causal), shares)
 
 
+def _prefix_group(max_rows: int, max_group: int) -> int:
+    """The requests of max_rows rows each that one pass takes of a group of max_group."""
+    return min(max_group, max(MAX_GROUP_ROWS // max(max_rows, 1), 1))
+
+
+def _shared_group(plan: Optional[PrefixPlan], rows: int) -> int:
+    """The max_group with which prefix attention takes a plan's groups, 0 where it does not: nothing is shared, or a group
+    may have more of the step's rows than one pass takes."""
+    if plan is None or not plan.shares:
+        return 0
+    group = _prefix_group(plan.max_rows, plan.max_group)
+    return group if plan.max_rows * group >= min(rows, plan.max_rows * plan.max_group) else 0
+
+
 def _prefix_workspace_size(rows, max_rows, max_group, num_heads, num_kv_heads, device) -> int:
     with torch.cuda.device(device):
-        size = N.load().dflash_q4_prefix_workspace_size(rows, max_rows, max_group, num_heads, num_kv_heads)
+        size = N.load().dflash_q4_prefix_workspace_size(rows, max_rows, _prefix_group(max_rows, max_group), num_heads, num_kv_heads)
     if size == 0:
         raise ValueError(f"no such attention: {rows} rows, groups of {max_group} x {max_rows}, {num_heads} / {num_kv_heads} heads")
     return size
@@ -265,18 +280,20 @@ def q4_prefix_workspace(rows: int, max_rows: int, max_group: int, num_heads: int
 def q4_prefix_attention(q, pool, table, plan: PrefixPlan, scale: Optional[float] = None, out=None, status=None, workspace=None):
     """``q4_attention`` (without a window) of the requests that ``plan`` was made
     for: the rows that a group shares are read once for all its query rows, each
-    request's own rows for its own, and both are joined in fp32."""
+    request's own rows for its own, and both are joined in fp32.  Where max_rows *
+    max_group and the rows of q both pass 65,536, every request is read on its own."""
     if pool.dim() != 4 or q.dim() != 3:
         raise ValueError("q must be [rows, heads, 128] and pool a tensor from q4_pool()")
     if pool.shape[2] * 16 != plan.page_size:
         raise ValueError(f"the plan is for pages of {plan.page_size} rows, the pool's have {pool.shape[2] * 16}")
+    group = _shared_group(plan, q.shape[0])
+    if not group:
+        lens = plan.own_lens + plan.skip * plan.page_size if plan.shares else plan.own_lens
+        return q4_attention(q, pool, table, lens, plan.starts, plan.max_rows, plan.causal, 0, 0, scale, out, status, workspace)
     if workspace is None:
-        workspace = q4_prefix_workspace(q.shape[0], plan.max_rows, plan.max_group, q.shape[1], pool.shape[1], pool.device)
-    if not plan.shares:
-        return N.load_paged().attention(q, pool, table, plan.own_lens, plan.starts, plan.max_rows, plan.causal, 0, 0,
-                                        HEAD_DIM ** -0.5 if scale is None else scale, out, status, workspace)
+        workspace = q4_prefix_workspace(q.shape[0], plan.max_rows, group, q.shape[1], pool.shape[1], pool.device)
     return N.load_paged().prefix_attention(q, pool, table, plan.starts, plan.max_rows, plan.group_starts, plan.prefix, plan.row_of,
-                                           plan.max_group, plan.skip, plan.own_lens, plan.causal,
+                                           group, plan.skip, plan.own_lens, plan.causal,
                                            HEAD_DIM ** -0.5 if scale is None else scale, out, status, workspace)
 
 
@@ -437,13 +454,13 @@ class PagedKVCacheQ4:
         stream = self._enter()
         if plan is not None and (sink or window or max_rows != plan.max_rows or bool(causal) != plan.causal):
             raise ValueError("a plan goes with the max_rows and causal that it was made for, and without a window")
+        group = _shared_group(plan, q.shape[0])
         if workspace is None:
             # (prefix attention keeps sums of every row: sizes by the next power of two)
-            key = (max_rows, q.shape[1]) if plan is None else (1 << max(q.shape[0] - 1, 0).bit_length(), max_rows, plan.max_group,
-                                                               q.shape[1])
+            key = (1 << max(q.shape[0] - 1, 0).bit_length(), max_rows, group, q.shape[1]) if group else (max_rows, q.shape[1])
             size = self._sizes.get(key)
             if size is None:
-                of = _workspace_size if plan is None else _prefix_workspace_size
+                of = _prefix_workspace_size if group else _workspace_size
                 size = self._sizes[key] = of(*key, self.nkv, self.device)
             # A graph may be replayed on any stream, beside eager calls and other graphs, and long after a larger
             # workspace has taken this one's place: it shares none with them.
