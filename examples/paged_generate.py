@@ -101,6 +101,8 @@ def generate(target, draft, prompts, max_new_tokens, temperature=0.0, generator=
     for i, t in enumerate(sd.sample(logits[0, ends.to(dev)], temperature, numbers(n)).tolist()):
         out[i].append(t)
     cache.check()
+    if min(o[-1] for o in out) < 0:
+        raise RuntimeError("the target's logits leave a request no token")
     rows, fresh = [len(p) for p in prompts], True       # context rows that each request brings
     active = list(range(n))
     while active:
@@ -123,6 +125,8 @@ def generate(target, draft, prompts, max_new_tokens, temperature=0.0, generator=
         cache.trim(torch.zeros(n, dtype=torch.int32, device=dev).index_copy(0, where, B - 1 - acc.int()))
         a, c, d = acc.tolist(), corr.tolist(), drafts.tolist()      # the step's one host synchronisation
         cache.check()                                               # a request without pages ends the run
+        if min(a + c) < 0:                                          # and so does one that verify_drafts could not serve
+            raise RuntimeError("drafts could not be verified, or the target's logits leave a request no token")
         accepted.append(a)
         for k, i in enumerate(active):
             out[i] += d[k][:a[k]] + [c[k]]

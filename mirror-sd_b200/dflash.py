@@ -133,7 +133,8 @@ def context_layers(hidden_states, layer_ids):
 def sample(logits: torch.Tensor, temperature: float = 0.0, uniforms: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Greedy argmax, first index on ties; from 1e-5 on a sample of softmax(logits /
     temperature) (dflash.py:133-136), drawn on the device with ``uniforms``, one
-    number in [0, 1) for each row of logits (by default torch's)."""
+    number in [0, 1) for each row of logits (by default torch's); -1 for a row of
+    NaN and -inf, which leaves no token."""
     if temperature < 1e-5:
         return torch.argmax(logits, dim=-1)
     if not logits.is_cuda:

@@ -89,6 +89,13 @@ def spec_generate(target, draft: DFlashDraftModel, input_ids: Sequence[int], max
     def numbers(n):
         return torch.rand(1, n, device=dev, generator=generator)
 
+    def usable(accepted, token):          # (before either is a slice's end or an index)
+        if accepted < 0:
+            raise RuntimeError("the drafts could not be verified: a device-side wait expired")
+        if token < 0:
+            raise RuntimeError("the target's logits leave no token: a row of NaN and -inf")
+        return token
+
     out = [int(t) for t in input_ids]
     n_prompt = len(out)
     t0 = time.perf_counter()
@@ -96,7 +103,7 @@ def spec_generate(target, draft: DFlashDraftModel, input_ids: Sequence[int], max
     # prefill: the prompt's logits give the first token, its features the first context
     tcache = target.make_cache()
     logits, feats = target.forward(torch.tensor([out], device=dev), tcache)
-    out.append(int(sample(logits[0, -1], temperature, None if greedy else numbers(1)).item()))
+    out.append(usable(0, int(sample(logits[0, -1], temperature, None if greedy else numbers(1)).item())))
     target_hidden = feats
     stats.prefill_time = time.perf_counter() - t0
 
@@ -123,7 +130,8 @@ def spec_generate(target, draft: DFlashDraftModel, input_ids: Sequence[int], max
             scores = logits if logits.dtype in (torch.float16, torch.bfloat16, torch.float32) else logits.float()
             acc, corr = verify_drafts(scores, drafts.to(torch.int32), numbers(B), temperature)
         a = int(acc[0].item())                                            # one host sync per step
-        new = drafts[0, :a].tolist() + [int(corr[0].item())]
+        token = usable(a, int(corr[0].item()))
+        new = drafts[0, :a].tolist() + [token]
         tcache.trim(B - (a + 1))                                          # rejected positions
         target_hidden = ([f[:, :a + 1, :] for f in feats] if isinstance(feats, (list, tuple))
                          else feats[:, :a + 1, :])

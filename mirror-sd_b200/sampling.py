@@ -32,13 +32,14 @@ def verify_drafts(logits, drafts, uniforms, temperature: Union[float, torch.Tens
     request uses, where not all.
 
     V is 2^22 at most.  NaN logits count as -inf; a row that leaves no token refuses its draft and
-    gives token -1."""
+    gives token -1.  accepted -1 (and token -1) means that a bounded wait on the device expired and
+    nothing is known of the request: check both before they become slices and indices."""
     return N.load_paged().verify(logits, drafts, uniforms, temperature, draft_probs, num_drafts)
 
 
 def sample_tokens(logits, uniforms, temperature: Union[float, torch.Tensor] = 1.0):
     """One token a row of logits [n, V], each from its random number in
-    uniforms [n]: ``verify_drafts`` without drafts."""
+    uniforms [n]: ``verify_drafts`` without drafts.  -1 for a row that leaves none."""
     if logits.dim() != 2:
         raise ValueError(f"logits must be [n, V], got {tuple(logits.shape)}")
     none = torch.empty(logits.shape[0], 0, dtype=torch.int32, device=logits.device)
