@@ -550,8 +550,10 @@ int dflash_rope(const void* x, int64_t x_row, int64_t x_head, int type, int rows
  *     vocabulary order, passes uniforms[block - 1] times the whole sum.
  * vocab <= 2^22.  NaN logits count as -inf (probability 0), others as clamped to +-1e30; a row
  * with nothing above -inf refuses its draft, and its token is -1.  accepted -1 and
- * token -1: a bounded wait on the device expired (nothing else reports it).  Rows
- * behind the first refused draft are not read. */
+ * token -1: a bounded wait on the device expired (nothing else reports it).
+ * Rows run ahead of the decisions, so all rows up to the one behind a request's
+ * last draft (and their distributions) may be read and must be there; those behind
+ * the first refused draft have no part in the result. */
 int dflash_verify_drafts(const void* logits, int64_t seq_stride, int64_t row_stride, int type, int n, int block, int vocab,
                          const int32_t* drafts, const float* uniforms, const float* temperatures, float temperature,
                          const float* probs, int64_t probs_seq_stride, int64_t probs_row_stride, const int32_t* num_drafts,

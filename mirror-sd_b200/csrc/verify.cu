@@ -12,10 +12,10 @@
 // bits, c = log2(e) / T, against a reference m of each thread that moves when a logit
 // passes it by 2^8 (so the exponents that matter are small, and exact to 2^-24 of
 // themselves).  One more warp joins the runs' parts of a row (in 64 bits) and decides
-// its draft, while the others are at work on the next row already: rows behind the
-// first refused draft need not be read, but waiting for each decision would take
-// 5 us a row (load latency, two exchanges, a decision) of which the bytes of a row
-// are 1 or 2.  How far the others may run ahead is `ahead` rows.
+// its draft, while the others are at work on the next rows already: rows behind the
+// first refused draft do not count, but waiting for each decision would take 5 us a
+// row (load latency, two exchanges, a decision) of which the bytes of a row are 1 or
+// 2.  So up to `ahead` of them are read all the same.
 //
 // 256 requests of up to 16 rows of 151,936 bf16 logits, 4.9 rows each on average:
 // 152 us, where the rows' bytes are 47 us of HBM (all rows of all requests: 200 us).

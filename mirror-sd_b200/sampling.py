@@ -29,7 +29,8 @@ def verify_drafts(logits, drafts, uniforms, temperature: Union[float, torch.Tens
     from max(p - q, 0) at the refused place, or from p behind the last draft,
     with the last random number: the first token in vocabulary order whose
     running sum passes it.  num_drafts [n] int32: how many of its drafts a
-    request uses, where not all.
+    request uses, where not all.  Rows behind a refused draft do not count, but
+    may be read: they must hold what they will hold when the call is made.
 
     V is 2^22 at most.  NaN logits count as -inf; a row that leaves no token refuses its draft and
     gives token -1.  accepted -1 (and token -1) means that a bounded wait on the device expired and
