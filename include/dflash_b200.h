@@ -548,7 +548,8 @@ int dflash_rope(const void* x, int64_t x_row, int64_t x_head, int type, int rows
  *     place (p without the draft itself where there are no probs; p where nothing
  *     is left), from p behind the last draft: the first token whose running sum, in
  *     vocabulary order, passes uniforms[block - 1] times the whole sum.
- * vocab <= 2^22.  NaN logits count as -inf (probability 0), others as clamped to +-1e30; a row
+ * vocab <= 2^22.  NaN logits count as -inf (probability 0), and for a sampled request
+ * others as clamped to +-1e30 (a greedy one compares them as they are); a row
  * with nothing above -inf refuses its draft, and its token is -1.  accepted -1 and
  * token -1: a bounded wait on the device expired (nothing else reports it).
  * Rows run ahead of the decisions, so all rows up to the one behind a request's

@@ -31,7 +31,8 @@
 // 2^-22 of themselves move running sums by more than an unlikely token weighs.
 //
 // Logits: NaN counts as -inf, a weight of 0; what lies beyond +-1e30 counts as
-// that.  A row that leaves no token refuses its draft and gives token -1.
+// that, but for greedy requests (T < 1e-5), which compare logits as they are, as an
+// argmax does.  A row that leaves no token refuses its draft and gives token -1.
 #include <algorithm>
 
 #include "decode.cuh"
@@ -96,7 +97,7 @@ struct Logits {
   }
 };
 
-// a logit as the definition takes it: NaN is -inf, and finite ones (and +inf) lie within +-1e30
+// a logit as a sampled request takes it: NaN is -inf, and finite ones (and +inf) lie within +-1e30
 __device__ __forceinline__ float clean(float x) {
   if (!(x > -INFINITY)) return -INFINITY;
   return fminf(fmaxf(x, -VF_BIG), VF_BIG);

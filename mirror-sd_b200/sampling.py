@@ -20,7 +20,8 @@ def verify_drafts(logits, drafts, uniforms, temperature: Union[float, torch.Tens
     positions, row j those of the token behind [anchor, drafts][j]; drafts
     [n, block - 1] int32; uniforms [n, block] f32, random numbers in [0, 1).
     temperature: a number or [n] f32 on the device; below 1e-5 a request is
-    greedy and gives what ``accept`` gives.
+    greedy and gives what ``accept`` gives for the first largest logits, compared
+    as they are.  (Sampled requests take logits beyond +-1e30 for that.)
 
     Draft j is accepted while uniforms[j] * q(draft) < p_j(draft) with p_j =
     softmax(logits_j / temperature) and q its probability in ``draft_probs``
