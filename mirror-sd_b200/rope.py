@@ -86,19 +86,48 @@ class Rope:
         self.turns = (freq / (2 * math.pi)).to(device)
 
 
+class _Turned(torch.autograd.Function):
+    """Rows turned; their gradient is that of the result turned back (and again, so it has one itself)."""
+
+    @staticmethod
+    def forward(ctx, x, rope, positions, inverse):
+        step = isinstance(positions, PagedStep)
+        ctx.rope, ctx.inverse, ctx.step = rope, not inverse, positions if step else None
+        ctx.save_for_backward(*(positions[:1] + positions[2:3] if step else (positions,)))   # (changed in place meanwhile: an error)
+        # (rows of no request of a step are left unwritten: as a gradient they are zero)
+        out = torch.zeros_like(x, memory_format=torch.contiguous_format) if step else None
+        return _turn(x, rope, positions, out, inverse)
+
+    @staticmethod
+    def backward(ctx, grad):
+        saved = ctx.saved_tensors
+        positions = saved[0] if ctx.step is None else ctx.step._replace(starts=saved[0], lens=saved[1])
+        return _Turned.apply(grad, ctx.rope, positions, ctx.inverse), None, None, None
+
+
+def _turn(x, rope, positions, out, inverse):
+    starts = lens = None
+    if isinstance(positions, PagedStep):
+        starts, lens, positions = positions.starts, positions.lens, None
+    return N.load_paged().rope(x, rope.turns, rope.factor, rope.rotary_dim, rope.interleaved, inverse, positions, starts, lens,
+                               out)
+
+
 def apply_rope(x, rope: Rope, positions: Union[torch.Tensor, PagedStep], out=None, inverse: bool = False):
     """x [rows, heads, head_dim] (f16, bf16 or f32; strided rows and heads) with
     its rows turned to their positions, in a new tensor or in ``out`` (x itself,
     or memory apart from x).  positions: int32 or int64 [rows], or the
     ``PagedStep`` whose packed rows x holds (rows of no request are then left
     unwritten).  inverse: turned back, which is also the gradient of x from that
-    of the result.  Angles are formed in 64 bits; the result is rounded once."""
+    of the result, and what autograd gets where x requires one (then without
+    ``out``, and rows of no request are zeros).  Angles are formed in 64 bits; the
+    result is rounded once."""
     if x.dim() == 3 and x.shape[2] != rope.head_dim:
         raise ValueError(f"x has heads of {x.shape[2]} channels, the positions are for {rope.head_dim}")
-    starts = lens = None
-    if isinstance(positions, PagedStep):
-        starts, lens, positions = positions.starts, positions.lens, None
-    elif positions is None:
+    if positions is None:
         raise ValueError("positions must be a tensor or a PagedStep")
-    return N.load_paged().rope(x, rope.turns, rope.factor, rope.rotary_dim, rope.interleaved, inverse, positions, starts, lens,
-                               out)
+    if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
+        if out is not None:
+            raise ValueError("apply_rope writes to out without a gradient: leave it to a new tensor, or use torch.no_grad()")
+        return _Turned.apply(x, rope, positions, inverse)
+    return _turn(x, rope, positions, out, inverse)
