@@ -1293,35 +1293,40 @@ __global__ void __launch_bounds__(QbCfg<N>::THREADS, 1) q4_attn_tc_kernel(const 
         cp_async_wait<0>();
         __syncwarp();
         if (p.bf16) {
-          // To f16 in place, the rows that have to be scaled behind the others: votes are
-          // cheaper than maxima (256 requests of 16 x 4 rows 212 us, all rows by maxima 245).
+          // To f16 in place.  Votes are cheaper than maxima (256 requests of 16 x 4 rows
+          // 210 us, all rows by maxima 245), but rows that have to be scaled need these: behind
+          // 8 rows of which some were scaled the next 8 go there at once (all scaled: 317 us,
+          // with votes first 348).
           const uint32_t half = side == 0 ? 0xffffu : 0xffff0000u;   // the lanes of this lane's row
-          uint64_t left = 0;
+          bool scaling = false;
 #pragma unroll 1
           for (int i = 0; i < N; i += 8) {
+            uint32_t left = scaling ? 15u : 0u;
+            if (!scaling) {
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              uint4* const to = reinterpret_cast<uint4*>(dst + (i + e) * 128 + (((piece & 7) ^ (e + side)) << 4));
-              float x[8];
-              const float a = query_floats(*to, x);
-              const uint32_t big = __ballot_sync(0xffffffffu, a >= 0.125f), nonzero = __ballot_sync(0xffffffffu, a > 0.f),
-                             over = __ballot_sync(0xffffffffu, a > 32768.f);
-              if (!(over & half) && (!(nonzero & half) || (big & half)))
-                *to = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
-              else
-                left |= 1ull << ((i + e) / 2);
+              for (int e = 0; e < 8; e += 2) {
+                uint4* const to = reinterpret_cast<uint4*>(dst + (i + e) * 128 + (((piece & 7) ^ (e + side)) << 4));
+                float x[8];
+                const float a = query_floats(*to, x);
+                const uint32_t big = __ballot_sync(0xffffffffu, a >= 0.125f), nonzero = __ballot_sync(0xffffffffu, a > 0.f),
+                               over = __ballot_sync(0xffffffffu, a > 32768.f);
+                if (!(over & half) && (!(nonzero & half) || (big & half)))
+                  *to = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+                else
+                  left |= 1u << (e / 2);
+              }
             }
-          }
-          if (__any_sync(0xffffffffu, left != 0)) {
-#pragma unroll 1
-            for (int i = 0; i < N; i += 8) {
+            if (__any_sync(0xffffffffu, left != 0)) {
+              bool any = false;
 #pragma unroll
               for (int k = 0; k < 8; k += 2) {
-                const bool mine = left >> ((i + k) / 2) & 1;
+                const bool mine = left >> (k / 2) & 1;
                 const int e = query_f16(reinterpret_cast<uint4*>(dst + (i + k) * 128 + (((piece & 7) ^ (k + side)) << 4)), mine, lane);
                 if (e && piece == 0) qf[i + k + side] = scaled_factor(base_f, e);
-                uniform = uniform && e == 0;
+                any = any || e != 0;
               }
+              scaling = __any_sync(0xffffffffu, any);
+              uniform = uniform && !scaling;
             }
           }
         }
