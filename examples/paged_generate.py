@@ -34,7 +34,7 @@ class PagedTarget:
     embedding.  ``forward`` takes the packed new tokens of all requests."""
 
     def __init__(self, vocab, hidden, layers, heads, kv_heads, inter, features, max_seqs=1, max_len=4096,
-                 num_pages=None, page_size=64, rope_theta=1e4, seed=0, device="cuda", samples=1, least=32768):
+                 num_pages=None, page_size=64, rope_theta=1e4, seed=0, device="cuda", samples=1, least=None):
         g = torch.Generator().manual_seed(seed)
         w = lambda o, i, gain=1.0: (torch.randn(o, i, generator=g) * gain * i ** -0.5).to(device, torch.float16)
         self.device, self.heads, self.kv_heads = torch.device(device), heads, kv_heads

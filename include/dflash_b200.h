@@ -488,9 +488,10 @@ int dflash_q4_attention(const uint16_t* q, int64_t q_row, int64_t q_head, int bf
  * prefix is the pages that the rows of all members with query rows begin with
  * alike, as far as every query row sees them whole (starts, max_rows and causal as
  * in dflash_q4_attention; lens [n]).  Where the pages found alike spare fewer than
- * `least` cached rows from being read, over all groups, nothing is shared: a pass over
- * shared rows costs about as much as reading 32,768 rows of 8 kv heads.  Written: group_starts [num_groups + 1],
- * prefix [num_groups] (rows), row_of [num_groups], skip [n] (pages), own_lens [n].
+ * `least` cached rows from being read, over all groups, nothing is shared: a pass
+ * over shared rows pays from about 2^20 / nkv rows on.  Written: group_starts
+ * [num_groups + 1], prefix [num_groups] (rows), row_of [num_groups], skip [n]
+ * (pages), own_lens [n].
  *
  * The attention gives what dflash_q4_attention gives without a window, up to the
  * rounding of one more join in fp32: the group's query rows over its prefix, then

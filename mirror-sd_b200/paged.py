@@ -30,6 +30,10 @@ from . import _native as N
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIM = 128
+# Cached rows, times kv heads, that sharing has to spare to pay for its two more launches.  1 to 8 kv heads, groups of 2 to
+# 256 requests of 1 to 16 rows, us shared / on their own: at 2^19 of them 34 shapes of 39 lose (64 requests on 8 kv heads 36 /
+# 32, on one 49 / 29), at 2^20 32 of 37 gain (64 requests on 8 kv heads 37 / 47, 16 groups of 16 on one 41 / 50).
+LEAST_SPARED = 1 << 20
 MAX_GROUP_ROWS = 65536              # query rows that one pass of the attention takes of a request or a group
 BLOCK_BYTES = 2304                   # 16 rows of one kv head, K and V with their scales
 STATUS_BITS = {1: "too few free pages", 2: "a request outgrew its row of the block table",
@@ -209,7 +213,7 @@ class PrefixPlan(NamedTuple):
 
 
 def paged_prefix_plan(table, lens, groups, page_size: int, starts=None, max_rows: int = 1, causal: bool = False,
-                      max_group: Optional[int] = None, least: int = 32768) -> PrefixPlan:
+                      max_group: Optional[int] = None, least: int = LEAST_SPARED // 8) -> PrefixPlan:
     """Which cached rows the requests of each group share, found by comparing
     their rows of the block table on the device: whole pages that all members with
     query rows begin with and whose rows all their query rows see.  groups: the
@@ -218,8 +222,9 @@ def paged_prefix_plan(table, lens, groups, page_size: int, starts=None, max_rows
     has more, the attention's ``status`` says so, its rows are right).  Requests
     of no group are on their own, and where sharing would spare fewer than ``least``
     cached rows from being read, over all groups, all of them are (8 samples of 2,048
-    rows each take 18 us on their own, 29 shared).  What is spared is counted in the
-    pages found alike.  lens, starts, max_rows and causal as for ``q4_attention``."""
+    rows each take 18 us on their own, 28 shared).  What is spared is counted in the
+    pages found alike; the default is for 8 kv heads, with others 2 ** 20 over their
+    number.  lens, starts, max_rows and causal as for ``q4_attention``."""
     if not torch.is_tensor(groups):
         sizes = [int(s) for s in groups]
         if not sizes or any(s < 1 for s in sizes) or sum(sizes) > lens.numel():
@@ -436,13 +441,13 @@ class PagedKVCacheQ4:
         q4_append(k, v, step.slots, self.pools[layer], self.status)
 
     def prefix_plan(self, step: PagedStep, groups: Union[torch.Tensor, Sequence[int]], max_rows: int, causal: bool = True,
-                    max_group: Optional[int] = None, least: int = 32768) -> PrefixPlan:
+                    max_group: Optional[int] = None, least: Optional[int] = None) -> PrefixPlan:
         """For ``attend``, once a step: the rows that consecutive requests share
         (``paged_prefix_plan``; groups are their numbers, as forks of one prompt lie
         side by side)."""
         self._enter()
         return paged_prefix_plan(self.table, self.lens, groups, self.page_size, step.starts, max_rows, causal, max_group,
-                                 least)
+                                 LEAST_SPARED // self.nkv if least is None else least)
 
     def attend(self, layer: int, q, step: PagedStep, max_rows: int, causal: bool = True, sink: int = 0,
                window: int = 0, scale: Optional[float] = None, out=None, workspace=None, plan: Optional[PrefixPlan] = None):

@@ -56,3 +56,15 @@ def test_plans_match_the_definition(pkg, n, g, columns, page, causal):
             plan = pkg.paged_prefix_plan(i32(table), i32(lens), i32(bounds), page, starts, 3, causal, n, least)
             got = plan.prefix.tolist(), plan.skip.tolist(), plan.own_lens.tolist()
             assert got == definition(table, lens, rows, bounds, page, causal, least), (trial, least)
+
+
+@pytest.mark.parametrize("nkv,members,shares", [(64, 9, True), (64, 8, False), (8, 9, False), (128, 5, True), (128, 4, False)])
+def test_a_plan_of_the_cache_asks_for_rows_by_its_kv_heads(pkg, nkv, members, shares):
+    """2^20 rows times kv heads spared, of 2,048 rows that 4 to 9 requests share."""
+    cache = pkg.PagedKVCacheQ4(1, 30, nkv, members, 2304, 256, forkable=True)
+    cache.reserve([2048] + [0] * (members - 1))
+    cache.fork(0, list(range(1, members)))
+    step = cache.reserve([1] * members)
+    assert cache.prefix_plan(step, [members], 1).prefix.tolist() == [2048 if shares else 0]
+    assert cache.prefix_plan(step, [members], 1, least=1).prefix.tolist() == [2048]
+    cache.check()
