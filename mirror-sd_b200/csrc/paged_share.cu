@@ -12,9 +12,10 @@
 // Release returns a page when its last holder gives it up, in the order of (request,
 // column) of that.
 //
-// All but the copies is latency: reserve and release run as one cluster of 8 CTAs, whose
-// barrier (0.3 us) separates reading the tables and counts from changing them,
-// where a second launch would cost 2 us.  The copies stream: 2304 bytes for
+// All but the copies is latency, of searches, table entries and counts that wait for
+// one another (512 requests: reserve and release 9 us each, 16 with cold tables):
+// they run as one cluster of 8 CTAs, whose barrier (0.3 us) separates reading the
+// tables and counts from changing them, where a second launch would cost 2 us.  The copies stream: 2304 bytes for
 // every 16 rows of a kv head, of all layers in one launch, and only the row
 // blocks that hold rows.
 #include "paged_scan.cuh"
@@ -345,8 +346,8 @@ __global__ void __launch_bounds__(PG_THREADS) paged_release_forked_kernel(const 
 
 // ---- copies: the CTAs share the (copy, layer) pairs out evenly.  A page that many
 // requests fork from is read by many copies, from L2 (plain loads), and what is written
-// leaves the caches first: 480 copies from 32 pages over 16 layers, 283 MB written, take
-// 54 us (5.3 TB/s), with streaming loads 72, with ordinary stores 69, with both 75.
+// leaves the caches first: 480 copies from 32 pages over 16 layers, 323 MB written, take
+// 63 us (5.1 TB/s), with streaming loads 65, with ordinary stores 66, with both 72.
 constexpr int CP_THREADS = 256, CP_FLY = 4;
 __global__ void __launch_bounds__(CP_THREADS) q4_copy_kernel(const __grid_constant__ CopyParams p) {
   __shared__ int list[kPagedMaxSeqs];   // the copies to make, in order
@@ -418,7 +419,7 @@ cudaError_t paged_release_forked_launch(const ReleaseParams& p, int32_t* holders
 cudaError_t q4_copy_launch(const CopyParams& p, int num_sms, cudaStream_t st) {
   if (p.n < 1 || p.n > kPagedMaxSeqs || p.layers < 1 || p.layers > kCopyPools) return cudaErrorInvalidValue;
   const long long units = (long long)p.n * p.layers;
-  // (16 CTAs an SM in all: 8 take 57 us, 64 the same)
+  // (16 CTAs an SM in all: 8 take 68 us, 64 65)
   return launch_pdl(q4_copy_kernel, dim3((int)(units < 16 * num_sms ? units : 16 * num_sms)), dim3(CP_THREADS), 0, st, p);
 }
 

@@ -18,12 +18,13 @@
 // 2.  So up to `ahead` of them are read all the same.
 //
 // 256 requests of up to 16 rows of 151,936 bf16 logits, 4.9 rows each on average:
-// 152 us, where the rows' bytes are 47 us of HBM (all rows of all requests: 200 us).
+// 150 us, where the rows' bytes are 47 us of HBM (all rows of all requests: 200 us).
 // What bounds it is the longest chains: a request whose drafts are all accepted
 // takes 16 rows one after another, each 4 to 8 us while others share its SMs, and the
-// token costs 10 to 25 us.  One request: 24 us, all of it such a chain.  (Rounds of a
-// few rows of all requests, a launch each: 188 us; each such launch costs 12 us beside
-// its bytes.  Rings filled by bulk copies in place of 8 loads a lane: 180 us.)
+// token costs 10 to 25 us.  One request: 17 to 25 us, all of it such a chain.  (Rounds of a
+// few rows of all requests, a launch each, when this took 180 us: 188; each such launch
+// costs 12 us beside its bytes.  Rings filled by bulk copies in place of 8 loads a lane,
+// when it took 155: 180.)
 //
 // The row that the token comes from is read once more, from L2, with weights to 2^-31
 // of themselves and sums in 64 bits: u times the sum must fall between the same two
@@ -807,12 +808,20 @@ __global__ void __launch_bounds__(VF_THREADS, VF_CTAS) verify_kernel(const Verif
 template <int TYPE>
 static cudaError_t launch(const VerifyParams& p, int num_sms, cudaStream_t st) {
   // CTAs of a request: 8 KB of a row each at least, and at most twice as many CTAs
-  // in all as are resident together (256 requests: 2 CTAs 166 us, 4 154, 8 199).
+  // in all as are resident together.  us with 1 / 2 / 4 / 8 / 16 CTAs, the rule's in brackets:
+  //   256 requests, 16 rows of 151,936   247 / 154 / [150] / 180 / 255
+  //   256 requests, 16 rows of 32,003     80 /  72 /  [75] / 110 / 215
+  //    64 requests, 16 rows of 151,936   200 / 101 /  76 / 71 / [75]
+  //    64 requests, 8 rows of 32,003      40 /  31 / [28] / 33 / 55
+  //   512 requests, 8 rows of 32,003      84 / [92] / 113 / 187 / 395
+  // 1,024 requests, 4 rows of 8,192      [47] / 70 / 124 / 240 / 563
+  //     1 request, 16 rows of 151,936     83 /  46 /  34 / 28 / [23]
   const long long bytes = (long long)p.vocab * elem_bytes(p.type);
   int ctas = VF_CLUSTER;
   while (ctas > 1 && (p.n * (long long)ctas > 2 * VF_CTAS * num_sms || bytes / ctas < 8192)) ctas /= 2;
-  // Rows to run ahead: one where the requests fill the GPU (two: the same; none:
-  // 194 against 180 us), as many as there is room for where they do not.
+  // Rows to run ahead: one where the requests fill the GPU, as many as there is room
+  // for where they do not (none / one / two / seven: 256 requests of 151,936 156 / 150 /
+  // 151 / 152 us, of 32,003 78 / 75 / 76 / 76, 16 requests of 151,936 54 / 48 / 48 / 47).
   const int ahead = p.n * (long long)ctas > VF_CTAS * num_sms ? 1 : VF_DEPTH - 1;
   DFL_TRY(cudaFuncSetAttribute(verify_kernel<TYPE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   return launch_pdl_cluster(verify_kernel<TYPE>, dim3(p.n * ctas), dim3(VF_THREADS), ctas, st, p, ctas, ahead);
