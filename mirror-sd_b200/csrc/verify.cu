@@ -29,7 +29,9 @@
 // The row that the token comes from is read once more, from L2, with weights to 2^-31
 // of themselves and sums in 64 bits: u times the sum must fall between the same two
 // of up to 150,000 running sums, whatever order they are added up in, and weights to
-// 2^-22 of themselves move running sums by more than an unlikely token weighs.
+// 2^-22 of themselves move running sums by more than an unlikely token weighs.  (Where p
+// and q agree to 2^-30 of p everywhere, what is left of p is rounding, and so is its
+// token; a draft that q proposes is refused there once in 2^30 times at most.)
 //
 // Logits: NaN counts as -inf, a weight of 0; what lies beyond +-1e30 counts as
 // that, but for greedy requests (T < 1e-5), which compare logits as they are, as an
